@@ -1,13 +1,16 @@
 /*
  * tmac.h — C ABI of the TitanMAC sparse hot path for MI355X (gfx950).
  *
- * Two operations live behind this boundary:
+ * Behind this boundary live
  *   - the Block-ELL block-sparse GEMM (forward Y = X·W, dX = dY·Wᵀ, and the
  *     dW SDDMM restricted to W's non-zero blocks), which replaces the dense
  *     nn.Linear calls of the TitanMAC MLP;
  *   - windowed + persistent-token attention computed tile-sparsely, which
  *     replaces the masked F.scaled_dot_product_attention call of
- *     WindowedAttention.
+ *     WindowedAttention;
+ *   - the ops around them (convolution, norm, projections, the memory's update);
+ *   - the model's two ends: the token embedding, and the log probabilities of
+ *     given tokens.
  *
  * The reference (bigwolfeman/TitanMAC-Standalone) is pure Python and has no
  * FFI of its own; each entry point below cites the reference call it stands in
@@ -38,7 +41,7 @@
 extern "C" {
 #endif
 
-#define TMAC_ABI_VERSION 8
+#define TMAC_ABI_VERSION 9
 #define TMAC_BLOCK 64
 
 typedef enum {
@@ -673,6 +676,67 @@ int tmac_linear_dx(const void* d_dY, int64_t lddy, const void* d_W, int64_t ldw,
 int tmac_linear_wgrad_workspace(int M, int N, int K, size_t* ws_bytes);
 int tmac_linear_wgrad(const void* d_dY, int64_t lddy, const void* d_X, int64_t ldx, void* d_dW,
                       void* d_ws, size_t ws_bytes, int M, int N, int K, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Token embedding: the lookups in front of the blocks (models/titanmac.py:183-190).
+ * ------------------------------------------------------------------------ */
+
+/* out [B, n_prefix + T, d], contiguous:
+ *   out[b, p]            = prefix[p]                                     p < n_prefix
+ *   out[b, n_prefix + t] = scale · W[ids[b, t]] + P[pos(b, t)],          pos = t without d_pos
+ * in fp32, rounded once. ids, pos: int64 [B, T], contiguous. W [V, d], P [n_pos, d] (nullable: no term) and
+ * prefix [n_prefix, d] have row pitches ldw, ldp, ldpre. An id (position) outside its table reads
+ * nothing and gives a row of NaN. Any d; 16-byte accesses where d, pitches and pointers allow.
+ * B·(n_prefix + T), V, n_pos <= 2^30; d <= 2^20. */
+int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_W, int64_t ldw, const void* d_P,
+                   int64_t ldp, const void* d_prefix, int64_t ldpre, void* d_out, int B, int T, int n_prefix, int d,
+                   int64_t V, int64_t n_pos, float scale, int dtype, void* stream);
+
+/* dW[v] = scale · Σ_{ids[b, t] = v} g[b, n_prefix + t], dense [V, d] and contiguous, rows without a token
+ * zero; g: the [B, n_prefix + T, d] gradient as rows of pitch ldg. fp32 sums in ascending order of (b, t)
+ * (deterministic), rounded once. ids outside [0, V) count nowhere. Also the gradient of P for given positions
+ * (ids = pos, V = n_pos, scale = 1). d_ws: tmac_embed_grad_workspace(B·T, V, d) bytes, 16-byte aligned. */
+int tmac_embed_grad_workspace(int64_t n_tokens, int64_t V, int d, size_t* ws_bytes);
+int tmac_embed_grad(const int64_t* d_ids, const void* d_g, int64_t ldg, void* d_dW, void* d_ws, size_t ws_bytes,
+                    int B, int T, int n_prefix, int d, int64_t V, float scale, int dtype, void* stream);
+
+/* dprefix[p] = Σ_b g[b, p] (nullable) and, for positions 0 .. T - 1, dP[t] = Σ_b g[b, n_prefix + t] with rows
+ * [T, n_pos) zero (nullable); both contiguous. */
+int tmac_embed_pos_grad(const void* d_g, int64_t ldg, void* d_dprefix, void* d_dP, int B, int T, int n_prefix, int d,
+                        int64_t n_pos, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Log probabilities of given tokens (F.cross_entropy of models/titanmac.py:666-680 by row, and what a
+ * server reports of a decoded token).
+ * ------------------------------------------------------------------------ */
+
+#define TMAC_LOGPROB_MAX_TOP 64
+
+/* For each of the B·T rows z [V] at z + b·stride_b + t·stride_t (any alignment):
+ *   lp    = z[target] − lse(z); 0 where target == ignore_index, NaN for another target outside [0, V)
+ *   H     = −Σ p ln p                                                    (d_entropy nullable)
+ *   top_k <= TMAC_LOGPROB_MAX_TOP largest values' indices and log probabilities, ties to the lower index
+ *   stats = {m, s}: the row's maximum and Σ e^{z − m}, for the backward; {0, 0} for a row of −inf
+ * fp32 throughout. −inf is probability 0. A row without a distribution (a NaN, +inf, nothing but −inf)
+ * gives NaN and top ids −1. With neither entropy nor top_k, rows to be ignored are not read. top_k <= V <= 2^28. */
+int tmac_logprob_workspace(int B, int T, int64_t V, int top_k, int dtype, size_t* ws_bytes);
+int tmac_logprob_fwd(const void* d_z, int64_t stride_b, int64_t stride_t, const int64_t* d_targets,
+                     int64_t ignore_index, float* d_lp, float* d_entropy, int top_k, int64_t* d_top_ids,
+                     float* d_top_lp, float* d_stats, void* d_ws, size_t ws_bytes, int B, int T, int64_t V, int dtype,
+                     void* stream);
+
+/* dz[b, t, j] = g_lp (δ_{j,target} − p_j) − g_H p_j (ln p_j + H), contiguous [B, T, V] in dtype, from the
+ * forward's stats and entropy. g_lp, g_entropy (nullable): fp32, one per row at the given stride (0: one
+ * value for all). Rows of which nothing was asked are zeros, and not read. */
+int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t stride_t, const int64_t* d_targets,
+                     int64_t ignore_index, const float* d_stats, const float* d_entropy, const float* d_g_lp,
+                     int64_t g_lp_stride, const float* d_g_entropy, int64_t g_entropy_stride, void* d_dz, int B, int T,
+                     int64_t V, int dtype, void* stream);
+
+/* loss (one value of dtype) = −Σ lp / n over the n rows whose target is not ignore_index (NaN for none),
+ * neg_inv = −1 / n. */
+int tmac_logprob_mean(const float* d_lp, const int64_t* d_targets, int64_t ignore_index, int rows, void* d_loss,
+                      int dtype, float* d_neg_inv, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ from pathlib import Path
 
 import torch  # the HIP runtime torch loads (libamdhip64.so.7) also serves libtmac.so
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 F32, BF16, F16 = 0, 1, 2
 EPI_NONE, EPI_GELU = 0, 1
@@ -100,6 +100,15 @@ SIGNATURES = {
                         ctypes.c_float, _i, _vp, _vp, _sz, _i, _vp],
     "tmac_silu_bwd": [_vp, _vp, _vp, _i64, _i, _vp],
     "tmac_mse_grad": [_vp, _vp, _vp, _i64, ctypes.c_float, _i, _vp],
+    "tmac_embed_fwd": [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _i64, _i64,
+                       ctypes.c_float, _i, _vp],
+    "tmac_embed_grad_workspace": [_i64, _i64, _i, ctypes.POINTER(_sz)],
+    "tmac_embed_grad": [_vp, _vp, _i64, _vp, _vp, _sz, _i, _i, _i, _i, _i64, ctypes.c_float, _i, _vp],
+    "tmac_embed_pos_grad": [_vp, _i64, _vp, _vp, _i, _i, _i, _i, _i64, _i, _vp],
+    "tmac_logprob_workspace": [_i, _i, _i64, _i, _i, ctypes.POINTER(_sz)],
+    "tmac_logprob_fwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _i, _i, _i64, _i, _vp],
+    "tmac_logprob_bwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i, _vp],
+    "tmac_logprob_mean": [_vp, _vp, _i64, _i, _vp, _i, _vp, _vp],
 }
 
 

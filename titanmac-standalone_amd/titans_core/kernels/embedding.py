@@ -1,0 +1,202 @@
+"""Token embedding in front of the blocks (HIP kernels for gfx950).
+
+The model looks its tokens up, adds the rows of their positions and puts the persistent tokens in front
+(models/titanmac.py:183-190):
+
+    out[b, p]      = prefix[p]                                     p < Np
+    out[b, Np + t] = scale * weight[ids[b, t]] + pos_weight[position(b, t)]
+
+``token_embedding`` does that in one launch. Its gradients are dense, as ``nn.Embedding``'s: the tokens are
+sorted by id and each row's sum is formed in order (deterministic, fp32) and written once.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .norm import _rows
+
+_INDEX = (torch.int64, torch.int32)
+
+
+def _table(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A table whose rows the kernels can read (copied only if they cannot be)."""
+    if t is None or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
+        return t
+    return t.contiguous()
+
+
+def _pitch(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else max(t.stride(0), t.shape[1])
+
+
+def _check(ids, weight, pos_weight, positions, prefix) -> None:
+    if ids.dim() != 2:
+        raise ValueError(f"token_embedding: ids must be [B, T], got {tuple(ids.shape)}")
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"token_embedding: weight must be [V, d], got {tuple(weight.shape)}")
+    for name, t in (("ids", ids), ("positions", positions)):
+        if t is not None and t.dtype not in _INDEX:
+            raise TypeError(f"token_embedding: {name} must be int64 or int32, got {t.dtype}")
+    for name, t in (("pos_weight", pos_weight), ("prefix", prefix)):
+        if t is None:
+            continue
+        if t.dim() != 2 or t.shape[1] != weight.shape[1]:
+            raise ValueError(f"token_embedding: {name} must be [n, {weight.shape[1]}], got {tuple(t.shape)}")
+        if t.dtype != weight.dtype:
+            raise TypeError(f"token_embedding: {name} dtype {t.dtype} != weight dtype {weight.dtype}")
+    if positions is not None:
+        if pos_weight is None:
+            raise ValueError("token_embedding: positions need pos_weight")
+        if tuple(positions.shape) not in (tuple(ids.shape), (ids.shape[1],)):
+            raise ValueError(f"token_embedding: positions must be {tuple(ids.shape)} or ({ids.shape[1]},), got "
+                             f"{tuple(positions.shape)}")
+    if pos_weight is not None:
+        if pos_weight.shape[0] == 0:
+            raise ValueError("token_embedding: pos_weight has no rows")
+        if positions is None and ids.shape[1] > pos_weight.shape[0]:
+            raise ValueError(f"token_embedding: {ids.shape[1]} positions, but pos_weight has "
+                             f"{pos_weight.shape[0]} rows")
+
+
+def _index(t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
+    return None if t is None else t.expand(like.shape).to(torch.int64).contiguous()
+
+
+def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor],
+                     positions: Optional[torch.Tensor], prefix: Optional[torch.Tensor],
+                     scale: float) -> torch.Tensor:
+    """[B, Np + T, d] in weight's dtype."""
+    _check(ids, weight, pos_weight, positions, prefix)
+    code = _lib.dtype_code(weight.dtype)
+    dev = _lib.require_device(*(t for t in (weight, ids, pos_weight, positions, prefix) if t is not None),
+                              what="token_embedding")
+    (B, T), (V, d) = ids.shape, weight.shape
+    n_prefix = 0 if prefix is None else prefix.shape[0]
+    out = torch.empty((B, n_prefix + T, d), dtype=weight.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    i, q, w, p, f = _index(ids, ids), _index(positions, ids), _table(weight), _table(pos_weight), _table(prefix)
+    with _lib.device_guard(dev):
+        rc = _lib.lib().tmac_embed_fwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(w), _pitch(w), _lib.ptr(p), _pitch(p),
+                                       _lib.ptr(f), _pitch(f), _lib.ptr(out), B, T, n_prefix, d, V,
+                                       0 if p is None else p.shape[0], scale, code, _lib.stream_ptr(dev))
+    _lib.check(rc, "tmac_embed_fwd")
+    return out
+
+
+token_embedding_fwd = torch.library.custom_op("titanmac::token_embedding", mutates_args=())(_token_embedding)
+
+
+@token_embedding_fwd.register_fake
+def _(ids, weight, pos_weight, positions, prefix, scale):
+    n_prefix = 0 if prefix is None else prefix.shape[0]
+    return weight.new_empty((ids.shape[0], n_prefix + ids.shape[1], weight.shape[1]))
+
+
+def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optional[torch.Tensor], n_prefix: int,
+                         V: int, n_pos: int, scale: float, need_w: bool, need_p: bool,
+                         need_f: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of weight [V, d], pos_weight [n_pos, d] and prefix [n_prefix, d] in grad's dtype; empty where
+    not needed."""
+    dev = _lib.require_device(*(t for t in (grad, ids, positions) if t is not None), what="token_embedding backward")
+    (B, T), d = ids.shape, int(grad.shape[-1])
+    code, L = _lib.dtype_code(grad.dtype), _lib.lib()
+    g = _rows(grad)
+    dw, dp, df = (grad.new_empty((n if need else 0, d))
+                  for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
+
+    def by_sorted(index, out, factor):
+        nb = ctypes.c_size_t(0)
+        _lib.check(L.tmac_embed_grad_workspace(B * T, out.shape[0], d, ctypes.byref(nb)), "tmac_embed_grad_workspace")
+        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev)
+        _lib.check(L.tmac_embed_grad(_lib.ptr(index), _lib.ptr(g), max(g.stride(0), d), _lib.ptr(out), _lib.ptr(ws),
+                                     nb.value, B, T, n_prefix, d, out.shape[0], factor, code,
+                                     _lib.stream_ptr(dev)), "tmac_embed_grad")
+
+    with _lib.device_guard(dev):
+        if need_w:
+            by_sorted(_index(ids, ids), dw, scale)
+        if need_p and positions is not None:
+            by_sorted(_index(positions, ids), dp, 1.0)
+        by_sum = need_p and positions is None
+        if by_sum or need_f:
+            _lib.check(L.tmac_embed_pos_grad(_lib.ptr(g), max(g.stride(0), d), _lib.ptr(df) if need_f else 0,
+                                             _lib.ptr(dp) if by_sum else 0, B, T, n_prefix, d,
+                                             n_pos if by_sum else 0, code, _lib.stream_ptr(dev)),
+                       "tmac_embed_pos_grad")
+    return dw, dp, df
+
+
+token_embedding_bwd = torch.library.custom_op("titanmac::token_embedding_bwd",
+                                              mutates_args=())(_token_embedding_bwd)
+
+
+@token_embedding_bwd.register_fake
+def _(grad, ids, positions, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
+    d = grad.shape[-1]
+    return tuple(grad.new_empty((n if need else 0, d))
+                 for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
+
+
+def _setup(ctx, inputs, output):
+    ids, weight, pos_weight, positions, prefix, scale = inputs
+    ctx.save_for_backward(ids, positions)
+    ctx.sizes = (0 if prefix is None else prefix.shape[0], weight.shape[0],
+                 0 if pos_weight is None else pos_weight.shape[0], scale)
+
+
+def _composed(grad, ids, positions, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
+    """The gradients in torch's operations, for a backward that is itself differentiated."""
+    g = grad[:, n_prefix:].float()
+
+    def scatter(index, n, factor):
+        ok = (index >= 0) & (index < n)
+        rows = torch.where(ok.unsqueeze(-1), g, 0.0).reshape(-1, g.shape[-1]) * factor
+        out = torch.zeros((n, g.shape[-1]), dtype=torch.float32, device=g.device)
+        return out.index_add(0, torch.where(ok, index, 0).reshape(-1).long(), rows).to(grad.dtype)
+
+    if positions is None:
+        positions = torch.arange(ids.shape[1], device=ids.device)
+    return (scatter(ids, V, scale) if need_w else None,
+            scatter(positions.expand(ids.shape), n_pos, 1.0) if need_p else None,
+            grad[:, :n_prefix].float().sum(0).to(grad.dtype) if need_f else None)
+
+
+def _backward(ctx, grad):
+    ids, positions = ctx.saved_tensors
+    need = [ctx.needs_input_grad[i] for i in (1, 2, 4)]
+    args = (grad, ids, positions, *ctx.sizes, *need)
+    if torch.is_grad_enabled() and grad.requires_grad:
+        dw, dp, df = _composed(*args)
+    else:
+        op = _token_embedding_bwd if _lib.direct_backward(grad, ids) else token_embedding_bwd
+        dw, dp, df = op(*args)
+    return (None, dw if need[0] else None, dp if need[1] else None, None, df if need[2] else None, None)
+
+
+token_embedding_fwd.register_autograd(_backward, setup_context=_setup)
+_native = _lib.native_function(_token_embedding, _setup, _backward)
+
+
+def token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor] = None, *,
+                    positions: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None,
+                    scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[ids] + pos_weight[positions], behind the rows of prefix: [B, Np + T, d].
+
+    ids: int64 or int32 [B, T]; weight [V, d], pos_weight [n_pos, d] and prefix [Np, d] of one dtype
+    (float32, bfloat16, float16), any d. positions: [B, T] or [T], by default 0 .. T - 1. The sum is formed in
+    fp32 and rounded once. Nothing is copied to the host to look at the ids: one outside [0, V), or a
+    position outside its table, gives a row of NaN and adds to no gradient.
+
+    Differentiable in the three tables (a second time too)."""
+    args = (ids, weight, pos_weight, positions, prefix, float(scale))
+    tables = (ids, weight, pos_weight, positions, prefix)
+    if _lib.direct_call(*tables):
+        return _token_embedding(*args)
+    if _lib.eager_native(*tables):
+        return _native(*args)
+    return token_embedding_fwd(*args)

@@ -1,0 +1,267 @@
+"""Log probabilities of given tokens (HIP kernels for gfx950).
+
+The model's loss is the mean of -log softmax(logits)[target] over the tokens (models/titanmac.py:666-680),
+a server wants the same number for each token, with the entropy of its distribution and the most probable
+alternatives, and a policy update the gradients of both:
+
+    lp = z[target] - lse(z),   H = -sum p ln p,   dz = g_lp (delta - p) - g_H p (ln p + H)
+
+``token_logprobs`` reads the logits once, whatever is asked, and once more for their gradient;
+``token_cross_entropy`` is the loss. All sums and results are fp32; the gradient has the logits' dtype.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+MAX_TOP = 64
+_INDEX = (torch.int64, torch.int32)
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns; None for what was not asked."""
+    logprobs: torch.Tensor
+    entropy: Optional[torch.Tensor] = None
+    top_ids: Optional[torch.Tensor] = None
+    top_logprobs: Optional[torch.Tensor] = None
+
+
+def _check(logits: torch.Tensor, targets: torch.Tensor, what: str) -> None:
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"{what}: logits must be [..., V], got {tuple(logits.shape)}")
+    if targets.shape != logits.shape[:-1]:
+        raise ValueError(f"{what}: targets must be {tuple(logits.shape[:-1])} for logits {tuple(logits.shape)}, got "
+                         f"{tuple(targets.shape)}")
+    if targets.dtype not in _INDEX:
+        raise TypeError(f"{what}: targets must be int64 or int32, got {targets.dtype}")
+
+
+def _rows3(z: torch.Tensor):
+    """(z as [B, T, V] whose rows the kernels can read, B, T, V): a view, copied only if its rows' values are not
+    neighbours or more than two strides lead to them."""
+    V = z.shape[-1]
+    z = z.reshape(1, 1, V) if z.dim() == 1 else z.unsqueeze(0) if z.dim() == 2 else z
+    if z.dim() > 3:
+        z = z.reshape(1, -1, V) if z.numel() else z.reshape(0, 0, V)
+    if V > 1 and z.stride(2) != 1:
+        z = z.contiguous()
+    return z, int(z.shape[0]), int(z.shape[1]), int(V)
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    return t.to(torch.int64).contiguous()
+
+
+def _fwd(logits, targets, entropy, top_k, ignore_index, dev):
+    z, B, T, V = _rows3(logits)
+    lead, n = targets.shape, B * T
+    new = lambda shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=dev)  # noqa: E731
+    lp, stats = new(lead), new((n, 2))
+    ent = new(lead if entropy else (0,))
+    ids, top = new((*lead, top_k) if top_k else (0,), torch.int64), new((*lead, top_k) if top_k else (0,))
+    if n:
+        L, nb = _lib.lib(), ctypes.c_size_t(0)
+        code, tg = _lib.dtype_code(z.dtype), _flat(targets)
+        _lib.check(L.tmac_logprob_workspace(B, T, V, top_k, code, ctypes.byref(nb)), "tmac_logprob_workspace")
+        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev) if nb.value else None
+        with _lib.device_guard(dev):
+            rc = L.tmac_logprob_fwd(_lib.ptr(z), z.stride(0), z.stride(1), _lib.ptr(tg), ignore_index, _lib.ptr(lp),
+                                    _lib.ptr(ent) if entropy else 0, top_k, _lib.ptr(ids) if top_k else 0,
+                                    _lib.ptr(top) if top_k else 0, _lib.ptr(stats), _lib.ptr(ws), nb.value, B, T, V,
+                                    code, _lib.stream_ptr(dev))
+        _lib.check(rc, "tmac_logprob_fwd")
+    return lp, ent, ids, top, stats
+
+
+def _logprob_fwd(logits: torch.Tensor, targets: torch.Tensor, entropy: bool, top_k: int, ignore_index: int
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(logprobs, entropy, top_ids, top_logprobs, stats fp32 [rows, 2]); empty tensors for what is not asked."""
+    _check(logits, targets, "token_logprobs")
+    _lib.dtype_code(logits.dtype)
+    if not 0 <= top_k <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top_k must be in [0, {min(MAX_TOP, logits.shape[-1])}], got {top_k}")
+    dev = _lib.require_device(logits, targets, what="token_logprobs")
+    return _fwd(logits, targets, entropy, top_k, ignore_index, dev)
+
+
+logprob_fwd = torch.library.custom_op("titanmac::token_logprobs", mutates_args=())(_logprob_fwd)
+
+
+@logprob_fwd.register_fake
+def _(logits, targets, entropy, top_k, ignore_index):
+    lead = logits.shape[:-1]
+    n = 1
+    for s in lead:
+        n *= s
+    f = lambda shape, dt=torch.float32: logits.new_empty(shape, dtype=dt)  # noqa: E731
+    return (f(lead), f(lead if entropy else (0,)), f((*lead, top_k) if top_k else (0,), torch.int64),
+            f((*lead, top_k) if top_k else (0,)), f((n, 2)))
+
+
+def _row_grad(g: Optional[torch.Tensor]):
+    """(fp32 values of a per-row gradient, stride): stride 0 for one value for all rows."""
+    if g is None:
+        return None, 0
+    g = g.to(torch.float32)
+    if all(s == 0 for s, n in zip(g.stride(), g.shape) if n > 1):
+        return g, 0
+    return g.contiguous(), 1
+
+
+def _logprob_bwd(g_lp: Optional[torch.Tensor], g_ent: Optional[torch.Tensor], logits: torch.Tensor,
+                 targets: torch.Tensor, stats: torch.Tensor, entropy: torch.Tensor, ignore_index: int) -> torch.Tensor:
+    """The gradient of the logits; g_lp, g_ent: per row, or one value for all."""
+    dev = _lib.require_device(*(t for t in (logits, targets, stats, entropy, g_lp, g_ent) if t is not None),
+                              what="token_logprobs backward")
+    z, B, T, V = _rows3(logits)
+    dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if dz.numel() == 0:
+        return dz
+    (gl, sl), (ge, se) = _row_grad(g_lp), _row_grad(g_ent)
+    tg = _flat(targets)
+    with _lib.device_guard(dev):
+        rc = _lib.lib().tmac_logprob_bwd(_lib.ptr(z), z.stride(0), z.stride(1), _lib.ptr(tg), ignore_index,
+                                         _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(gl), sl, _lib.ptr(ge), se,
+                                         _lib.ptr(dz), B, T, V, _lib.dtype_code(z.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "tmac_logprob_bwd")
+    return dz
+
+
+logprob_bwd = torch.library.custom_op("titanmac::token_logprobs_bwd", mutates_args=())(_logprob_bwd)
+
+
+@logprob_bwd.register_fake
+def _(g_lp, g_ent, logits, targets, stats, entropy, ignore_index):
+    return logits.new_empty(logits.shape)
+
+
+def _composed(g_lp, g_ent, logits, targets, ignore_index):
+    """The gradient in torch's operations, for a backward that is itself differentiated."""
+    logp = torch.log_softmax(logits.float(), dim=-1)
+    p = logp.exp()
+    dz = torch.zeros_like(p)
+    if g_lp is not None:
+        given = targets != ignore_index
+        g = (g_lp.float() * given).unsqueeze(-1)
+        at = torch.arange(p.shape[-1], device=p.device) == targets.unsqueeze(-1)
+        dz = dz + g * (at.to(p.dtype) - p)
+    if g_ent is not None:
+        some = torch.where(p > 0, logp, 0.0)
+        H = -(p * some).sum(-1, keepdim=True)
+        dz = dz - g_ent.float().unsqueeze(-1) * p * (some + H)
+    return dz.to(logits.dtype)
+
+
+def _gradient(g_lp, g_ent, logits, targets, stats, entropy, ignore_index):
+    if g_lp is None and g_ent is None:
+        return None
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (g_lp, g_ent, logits)):
+        return _composed(g_lp, g_ent, logits, targets, ignore_index)
+    direct = all(_lib.direct_backward(g, logits) for g in (g_lp, g_ent) if g is not None)
+    op = _logprob_bwd if direct else logprob_bwd
+    return op(g_lp, g_ent, logits, targets, stats, entropy, ignore_index)
+
+
+def _setup(ctx, inputs, output):
+    logits, targets, entropy, _top_k, ignore_index = inputs
+    ctx.save_for_backward(logits, targets, output[4], output[1])
+    ctx.with_entropy, ctx.ignore_index = entropy, ignore_index
+    ctx.set_materialize_grads(False)
+
+
+def _backward(ctx, g_lp, g_ent, _g_ids, _g_top, _g_stats):
+    dz = _gradient(g_lp, g_ent if ctx.with_entropy else None, *ctx.saved_tensors, ctx.ignore_index)
+    return dz, None, None, None, None
+
+
+logprob_fwd.register_autograd(_backward, setup_context=_setup)
+_native = _lib.native_function(_logprob_fwd, _setup, _backward, all_outputs=True)
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool = False, top_k: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of `targets` under softmax(logits), with what else is asked of each row.
+
+    logits [..., V] (float32, bfloat16, float16; any strides, read in place where a row's values are
+    neighbours), targets int64 or int32 [...]. Results, fp32:
+
+    - logprobs [...]: log softmax(logits)[target]; 0 where target == ignore_index, and NaN for any other
+      target outside [0, V) (nothing is copied to the host to look at them);
+    - entropy [...]: -sum p ln p in nats, of every row;
+    - top_ids, top_logprobs [..., top_k] (top_k <= 64): the most probable tokens in order, equal logits by
+      the lower index, of every row.
+
+    -inf is probability 0. A row with a NaN or +inf, or nothing but -inf, has no distribution: its values are
+    NaN and its top_ids -1. logprobs and entropy are differentiable (a second time too), top_logprobs is not."""
+    args = (logits, targets, bool(entropy), int(top_k), int(ignore_index))
+    if _lib.direct_call(logits, targets):
+        lp, ent, ids, top, _ = _logprob_fwd(*args)
+    elif _lib.eager_native(logits, targets):
+        lp, ent, ids, top, _ = _native(*args)
+    else:
+        lp, ent, ids, top, _ = logprob_fwd(*args)
+    return TokenLogprobs(lp, ent if entropy else None, ids if top_k else None, top.detach() if top_k else None)
+
+
+# ------------------------------------------------------------------ the loss
+
+def _cross_entropy_fwd(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, wide: bool
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(the mean of -lp over the given targets, in logits' dtype or (wide) fp32; fp32 -1 / their number; stats)."""
+    _check(logits, targets, "token_cross_entropy")
+    code = _lib.F32 if wide else _lib.dtype_code(logits.dtype)
+    _lib.dtype_code(logits.dtype)
+    dev = _lib.require_device(logits, targets, what="token_cross_entropy")
+    lp, _, _, _, stats = _fwd(logits, targets, False, 0, ignore_index, dev)
+    loss = torch.empty((), dtype=torch.float32 if wide else logits.dtype, device=dev)
+    inv = torch.empty((), dtype=torch.float32, device=dev)
+    tg = _flat(targets)
+    with _lib.device_guard(dev):
+        rc = _lib.lib().tmac_logprob_mean(_lib.ptr(lp), _lib.ptr(tg), ignore_index, lp.numel(), _lib.ptr(loss), code,
+                                          _lib.ptr(inv), _lib.stream_ptr(dev))
+    _lib.check(rc, "tmac_logprob_mean")
+    return loss, inv, stats
+
+
+cross_entropy_fwd = torch.library.custom_op("titanmac::token_cross_entropy", mutates_args=())(_cross_entropy_fwd)
+
+
+@cross_entropy_fwd.register_fake
+def _(logits, targets, ignore_index, wide):
+    n = 1
+    for s in logits.shape[:-1]:
+        n *= s
+    f = lambda shape, dt=torch.float32: logits.new_empty(shape, dtype=dt)  # noqa: E731
+    return f((), torch.float32 if wide else logits.dtype), f(()), f((n, 2))
+
+
+def _ce_setup(ctx, inputs, output):
+    logits, targets, ignore_index, _wide = inputs
+    ctx.save_for_backward(logits, targets, output[1], output[2])
+    ctx.ignore_index = ignore_index
+
+
+def _ce_backward(ctx, g_loss, *_):
+    logits, targets, inv, stats = ctx.saved_tensors
+    g_lp = (g_loss * inv).expand(targets.shape)
+    return _gradient(g_lp, None, logits, targets, stats, None, ctx.ignore_index), None, None, None
+
+
+cross_entropy_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)
+_ce_native = _lib.native_function(_cross_entropy_fwd, _ce_setup, _ce_backward)
+
+
+def token_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100) -> torch.Tensor:
+    """The mean of -log softmax(logits)[target] over the targets other than ignore_index (NaN where there are
+    none), as F.cross_entropy of [..., V] logits: in their dtype, or fp32 inside torch.autocast. Ignored
+    rows are not read and get zeros as gradient. Other targets outside [0, V) make it NaN."""
+    args = (logits, targets, int(ignore_index), torch.is_autocast_enabled("cuda"))
+    if _lib.direct_call(logits, targets):
+        return _cross_entropy_fwd(*args)[0]
+    if _lib.eager_native(logits, targets):
+        return _ce_native(*args)
+    return cross_entropy_fwd(*args)[0]
