@@ -738,6 +738,15 @@ int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t stride_t, const 
 int tmac_logprob_mean(const float* d_lp, const int64_t* d_targets, int64_t ignore_index, int rows, void* d_loss,
                       int dtype, float* d_neg_inv, void* stream);
 
+/* The same lp and H for the logits z = X · Wᵀ of the model's head (models/titanmac.py:126-128), which are
+ * not stored: X [M, K] and W [V, K] in 16 bit with pitches ldx, ldw, K a multiple of 64, pointers 16-byte
+ * aligned, pitches multiples of 8 up to 2^22. The logits are fp32 sums that are not rounded.
+ * d_ws: tmac_head_logprob_workspace bytes, 16-byte aligned. */
+int tmac_head_logprob_workspace(int M, int64_t V, int K, size_t* ws_bytes);
+int tmac_head_logprob(const void* d_X, int64_t ldx, const void* d_W, int64_t ldw, const int64_t* d_targets,
+                      int64_t ignore_index, float* d_lp, float* d_entropy, int M, int64_t V, int K, void* d_ws,
+                      size_t ws_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

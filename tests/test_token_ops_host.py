@@ -166,3 +166,31 @@ def test_differentiable_gradients_match_autograd():
 def test_exported_from_the_package():
     assert _lib.SIGNATURES["tmac_embed_fwd"] and set(tc.__all__) >= {
         "token_embedding", "token_logprobs", "token_cross_entropy", "TokenLogprobs"}
+
+
+def test_head_refusals_and_argument_errors(lib):
+    x, w, t = torch.zeros(2, 64).bfloat16(), torch.zeros(5, 64).bfloat16(), torch.zeros(2, dtype=torch.long)
+    with pytest.raises(RuntimeError, match="GPU"):
+        tc.head_logprobs(x, w, t)
+    with pytest.raises(RuntimeError, match="GPU"):
+        tc.head_logprobs(x.float(), w.float(), t)
+    for err, text, args in ((ValueError, "hidden must be", (x[:, :32], w, t)), (ValueError, "hidden must be", (x, w[:0], t)),
+                            (ValueError, "hidden must be", (x, w[0], t)), (TypeError, "weight dtype", (x, w.half(), t)),
+                            (ValueError, "targets must be", (x, w, t[:1])), (TypeError, "targets must be", (x, w, t.float()))):
+        with pytest.raises(err, match=text):
+            tc.head_logprobs(*args)
+    n = ctypes.c_size_t(0)
+    assert lib.tmac_head_logprob_workspace(300, 1000, 640, ctypes.byref(n)) == 0 and n.value >= 300 * 16
+    assert lib.tmac_head_logprob_workspace(300, 1000, 640, None) == -1
+    # X, ldx, W, ldw, targets, ignore, lp, ent, M, V, K, ws, ws_bytes, dtype, stream
+    ok = [FAKE, 640, FAKE, 640, FAKE, -100, FAKE, None, 300, 1000, 640, FAKE, n.value, 1, None]
+    for at, value, want in ((0, None, -1), (2, None, -1), (4, None, -1), (6, None, -1), (11, None, -6),
+                            (12, n.value - 1, -6), (11, FAKE + 8, -5), (0, FAKE + 8, -5), (2, FAKE + 2, -5), (1, 632, -2),
+                            (3, 644, -5), (1, (1 << 22) + 8, -2), (10, 600, -2), (10, 0, -2), (9, 0, -2),
+                            (9, (1 << 28) + 1, -2), (8, -1, -2), (13, 0, -4)):
+        bad = list(ok)
+        bad[at] = value
+        assert lib.tmac_head_logprob(*bad) == want, (at, value)
+    for M in (1, 64, 65, 8192, 1 << 30):
+        for V in (1, 129, 128000, 1 << 28):
+            assert lib.tmac_head_logprob_workspace(M, V, 64, ctypes.byref(n)) == 0 and n.value >= 16 * M

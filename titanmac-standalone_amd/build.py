@@ -37,7 +37,7 @@ HIP_FLAGS = [
 ]
 SOURCES = ["tmac_host.cpp", "bell_kernels.hip", "wattn_kernels.hip", "conv_kernels.hip",
            "norm_kernels.hip", "memory_kernels.hip", "linear_kernels.hip", "embed_kernels.hip",
-           "logprob_kernels.hip"]
+           "logprob_kernels.hip", "head_kernels.hip"]
 
 
 def _hipcc() -> str:

@@ -28,44 +28,8 @@ using namespace tmac;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kFar = -1e4f;  // differences are cut here in products with an exponential that is then 0
 constexpr int kMaxTop = 64;
 constexpr int kUnroll = 4;
-
-__device__ __forceinline__ float exp_d(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
-
-// Running softmax statistics. mu is m, or 0 while nothing above −inf was seen (so that −inf − mu is
-// −inf and not NaN); a NaN, or +inf (whose z − mu is NaN), makes s NaN.
-struct Stat {
-  float m, mu, s, h;
-};
-__device__ __forceinline__ Stat stat_none() { return Stat{-__builtin_inff(), 0.f, 0.f, 0.f}; }
-
-__device__ __forceinline__ void stat_raise(Stat& a, float m) {
-  if (m > a.m) {
-    const float d = fmaxf(a.m - m, kFar), f = exp_d(d);  // f = 0 for the first m
-    a.h = f * fmaf(a.s, d, a.h);
-    a.s *= f;
-    a.m = a.mu = m;
-  }
-}
-template <bool ENT>
-__device__ __forceinline__ void stat_add(Stat& a, float z) {
-  const float d = z - a.mu, e = exp_d(d);
-  a.s += e;
-  if (ENT) a.h = fmaf(e, fmaxf(d, kFar), a.h);
-}
-__device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
-  stat_raise(a, b.m);
-  // b's terms at a's maximum; where b has none above −inf it has s = h = 0 (or NaN)
-  const float d = b.m == -__builtin_inff() ? 0.f : fmaxf(b.m - a.mu, kFar), f = exp_d(d);
-  a.h = fmaf(f, fmaf(b.s, d, b.h), a.h);
-  a.s = fmaf(f, b.s, a.s);
-}
-__device__ __forceinline__ Stat stat_shfl(const Stat& a, int x) {
-  return Stat{__shfl_xor(a.m, x), __shfl_xor(a.mu, x), __shfl_xor(a.s, x), __shfl_xor(a.h, x)};
-}
 
 // (value, index) as one whole number: larger value first, then lower index; 0 is no entry.
 __device__ __forceinline__ uint64_t top_key(float z, int idx) {

@@ -1,6 +1,6 @@
 // Rows of values in global memory, shared by the kernels that stream them: N values at once as one
 // 16-byte access (N = kRowVec<DT>) or a single value (N = 1, rows that are not 16-byte aligned),
-// converted to and from fp32.
+// converted to and from fp32; and the running statistics of a row's softmax.
 #pragma once
 
 #include "tmac_device.h"
@@ -50,6 +50,43 @@ __device__ __forceinline__ void row_store(void* __restrict__ p, const float (&v)
     for (int i = 0; i < 4; ++i) x[i] = Mfma<DT>::pack2(v[2 * i], v[2 * i + 1]);
     *static_cast<u32x4*>(p) = x;
   }
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFar = -1e4f;  // differences are cut here in products with an exponential that is then 0
+
+__device__ __forceinline__ float exp_d(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// Running softmax statistics: m the maximum, s = Σ e^{z − m}, h = Σ e^{z − m} (z − m). mu is m, or 0 while nothing above −inf was seen (so that −inf − mu is
+// −inf and not NaN); a NaN, or +inf (whose z − mu is NaN), makes s NaN.
+struct Stat {
+  float m, mu, s, h;
+};
+__device__ __forceinline__ Stat stat_none() { return Stat{-__builtin_inff(), 0.f, 0.f, 0.f}; }
+
+__device__ __forceinline__ void stat_raise(Stat& a, float m) {
+  if (m > a.m) {
+    const float d = fmaxf(a.m - m, kFar), f = exp_d(d);  // f = 0 for the first m
+    a.h = f * fmaf(a.s, d, a.h);
+    a.s *= f;
+    a.m = a.mu = m;
+  }
+}
+template <bool ENT>
+__device__ __forceinline__ void stat_add(Stat& a, float z) {
+  const float d = z - a.mu, e = exp_d(d);
+  a.s += e;
+  if (ENT) a.h = fmaf(e, fmaxf(d, kFar), a.h);
+}
+__device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
+  stat_raise(a, b.m);
+  // b's terms at a's maximum; where b has none above −inf it has s = h = 0 (or NaN)
+  const float d = b.m == -__builtin_inff() ? 0.f : fmaxf(b.m - a.mu, kFar), f = exp_d(d);
+  a.h = fmaf(f, fmaf(b.s, d, b.h), a.h);
+  a.s = fmaf(f, b.s, a.s);
+}
+__device__ __forceinline__ Stat stat_shfl(const Stat& a, int x) {
+  return Stat{__shfl_xor(a.m, x), __shfl_xor(a.mu, x), __shfl_xor(a.s, x), __shfl_xor(a.h, x)};
 }
 
 inline bool row_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

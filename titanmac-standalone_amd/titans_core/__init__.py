@@ -13,8 +13,8 @@ from .attn import (BlockSparseAttention, WindowConfig, WindowedAttention, build_
                    create_block_sparse_attention)
 from .blocks import MLPBlock, RMSNorm, TitanBlock
 from .config import TITANS_VARIANTS, TitanMACConfig
-from .kernels import (BlockELLLinear, BlockELLPattern, TokenLogprobs, block_ell_mm, causal_dwconv, rms_norm,
-                      token_cross_entropy, token_embedding, token_logprobs, windowed_attention)
+from .kernels import (BlockELLLinear, BlockELLPattern, TokenLogprobs, block_ell_mm, causal_dwconv, head_logprobs,
+                      rms_norm, token_cross_entropy, token_embedding, token_logprobs, windowed_attention)
 from .memory import DecayGate, DeepMemoryMLP, ForgetGate, NeuralMemory
 from .models import TitanMAC
 
@@ -25,4 +25,5 @@ __all__ = ["TitanMACConfig", "TITANS_VARIANTS", "WindowedAttention", "WindowConf
            "RMSNorm", "TitanBlock", "BlockELLLinear", "BlockELLPattern", "block_ell_mm",
            "causal_dwconv", "rms_norm", "windowed_attention", "NeuralMemory", "ForgetGate",
            "DecayGate", "DeepMemoryMLP", "TitanMAC", "token_embedding", "token_logprobs",
-           "token_cross_entropy", "TokenLogprobs"]
+           "token_cross_entropy", "head_logprobs",
+           "TokenLogprobs"]

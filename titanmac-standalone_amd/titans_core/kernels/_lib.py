@@ -109,6 +109,8 @@ SIGNATURES = {
     "tmac_logprob_fwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _i, _i, _i64, _i, _vp],
     "tmac_logprob_bwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i, _vp],
     "tmac_logprob_mean": [_vp, _vp, _i64, _i, _vp, _i, _vp, _vp],
+    "tmac_head_logprob_workspace": [_i, _i64, _i, ctypes.POINTER(_sz)],
+    "tmac_head_logprob": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i64, _i, _vp, _sz, _i, _vp],
 }
 
 

@@ -7,7 +7,8 @@ alternatives, and a policy update the gradients of both:
     lp = z[target] - lse(z),   H = -sum p ln p,   dz = g_lp (delta - p) - g_H p (ln p + H)
 
 ``token_logprobs`` reads the logits once, whatever is asked, and once more for their gradient;
-``token_cross_entropy`` is the loss. All sums and results are fp32; the gradient has the logits' dtype.
+``token_cross_entropy`` is the loss; ``head_logprobs`` scores hidden states without storing their logits.
+All sums and results are fp32; gradients have their input's dtype.
 """
 from __future__ import annotations
 
@@ -15,8 +16,10 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+import torch.nn.functional as F
 
 from . import _lib
+from .linear import _HALF, _MAX_PITCH, _rows
 
 MAX_TOP = 64
 _INDEX = (torch.int64, torch.int32)
@@ -265,3 +268,68 @@ def token_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_i
     if _lib.eager_native(logits, targets):
         return _ce_native(*args)
     return cross_entropy_fwd(*args)[0]
+
+
+# ------------------------------------------------------------------ scores from the hidden states
+
+def _head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, entropy: bool,
+                   ignore_index: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(logprobs, entropy or an empty tensor) of 16-bit hidden [..., K] and weight [V, K], K a multiple of 64."""
+    _check_head(hidden, weight, targets)
+    dev = _lib.require_device(hidden, weight, targets, what="head_logprobs")
+    (V, K), lead, M = weight.shape, targets.shape, targets.numel()
+    lp = torch.empty(lead, dtype=torch.float32, device=dev)
+    ent = torch.empty(lead if entropy else (0,), dtype=torch.float32, device=dev)
+    if M:
+        L, nb = _lib.lib(), ctypes.c_size_t(0)
+        x, w, tg = _rows(hidden), _rows(weight), _flat(targets)
+        _lib.check(L.tmac_head_logprob_workspace(M, V, K, ctypes.byref(nb)), "tmac_head_logprob_workspace")
+        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev)
+        with _lib.device_guard(dev):
+            rc = L.tmac_head_logprob(_lib.ptr(x), x.stride(0), _lib.ptr(w), w.stride(0), _lib.ptr(tg), ignore_index,
+                                     _lib.ptr(lp), _lib.ptr(ent) if entropy else 0, M, V, K, _lib.ptr(ws), nb.value,
+                                     _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+        _lib.check(rc, "tmac_head_logprob")
+    return lp, ent
+
+
+head_logprobs_fwd = torch.library.custom_op("titanmac::head_logprobs", mutates_args=())(_head_logprobs)
+
+
+@head_logprobs_fwd.register_fake
+def _(hidden, weight, targets, entropy, ignore_index):
+    f = lambda shape: hidden.new_empty(shape, dtype=torch.float32)  # noqa: E731
+    return f(targets.shape), f(targets.shape if entropy else (0,))
+
+
+def _check_head(hidden, weight, targets) -> None:
+    if weight.dim() != 2 or weight.shape[0] == 0 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"head_logprobs: hidden must be [..., K] and weight [V, K], got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if weight.dtype != hidden.dtype:
+        raise TypeError(f"head_logprobs: weight dtype {weight.dtype} != hidden dtype {hidden.dtype}")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"head_logprobs: targets must be {tuple(hidden.shape[:-1])} for hidden "
+                         f"{tuple(hidden.shape)}, got {tuple(targets.shape)}")
+    if targets.dtype not in _INDEX:
+        raise TypeError(f"head_logprobs: targets must be int64 or int32, got {targets.dtype}")
+
+
+def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, entropy: bool = False,
+                  ignore_index: int = -100) -> TokenLogprobs:
+    """token_logprobs(F.linear(hidden, weight), targets) with logprobs and (if asked) entropy, the logits [..., V]
+    never stored: one kernel multiplies and keeps the running softmax statistics. The logits' fp32 sums are not
+    rounded on the way, so the scores are nearer to exact than those of 16-bit logits.
+
+    hidden [..., K] and weight [V, K] of one dtype, targets int64 or int32 [...]. Where the kernel does not
+    apply (fp32, K not a multiple of 64, a gradient is needed) the logits are formed by F.linear and scored by
+    token_logprobs, which has the gradient."""
+    _check_head(hidden, weight, targets)
+    K = weight.shape[1]
+    grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+    if grad or hidden.dtype not in _HALF or K == 0 or K % 64 or K > _MAX_PITCH or weight.stride(0) > _MAX_PITCH:
+        _lib.require_device(hidden, weight, targets, what="head_logprobs")
+        return token_logprobs(F.linear(hidden, weight), targets, entropy=entropy, ignore_index=ignore_index)
+    args = (hidden, weight, targets, bool(entropy), int(ignore_index))
+    lp, ent = _head_logprobs(*args) if _lib.direct_call(hidden, weight, targets) else head_logprobs_fwd(*args)
+    return TokenLogprobs(lp, ent if entropy else None)
