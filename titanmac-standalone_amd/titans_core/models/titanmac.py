@@ -13,8 +13,10 @@ Same constructor, submodules, parameters, buffers and state_dict keys as the ref
 - ``forward_mag`` (:315-432) and ``forward_mal`` (:434-547).
 
 Every block op runs on the HIP kernels (RMSNorm, depthwise conv, tile-sparse attention,
-Block-ELL MLP when configured), the neural memory's update on its HIP step, and the dense
-projections and the LM head on hipBLASLt.
+Block-ELL MLP when configured), the neural memory's update on its HIP step, the embeddings and the
+loss on theirs (``token_embedding``, ``token_cross_entropy``), and the dense projections and the LM
+head on hipBLASLt. ``score``, which the reference lacks, gives each token's log probability without
+storing the logits.
 
 One change of schedule, not of result: when the memory is read-only (eval mode without
 ``enable_test_time_memory``), ``forward_mac``'s segments do not depend on each other. The
@@ -36,7 +38,25 @@ from torch.utils.checkpoint import checkpoint
 from ..blocks.norms import RMSNorm
 from ..blocks.titan_block import TitanBlock
 from ..config import TitanMACConfig
+from ..kernels import _lib
+from ..kernels.embedding import token_embedding
+from ..kernels.logprobs import head_logprobs, token_cross_entropy, token_logprobs
 from ..memory.neural_memory import NeuralMemory
+
+
+_IGNORE = -100  # F.cross_entropy's ignore_index
+
+
+def _untouched(m: nn.Module, kind: type) -> bool:
+    """Whether calling m does just what `kind`'s own forward does: no subclass, replaced forward or hook."""
+    return (type(m) is kind and "forward" not in m.__dict__ and not m._forward_hooks and not m._forward_pre_hooks
+            and not m._backward_hooks and not m._backward_pre_hooks
+            and not torch.nn.modules.module._has_any_global_hook())
+
+
+def _plain_lookup(m: nn.Module) -> bool:
+    return (_untouched(m, nn.Embedding) and m.padding_idx is None and m.max_norm is None
+            and not m.scale_grad_by_freq and not m.sparse)
 
 
 class TitanMAC(nn.Module):
@@ -94,15 +114,28 @@ class TitanMAC(nn.Module):
 
     # ------------------------------------------------------------------ helpers
 
-    def _embed(self, input_ids: torch.Tensor) -> torch.Tensor:
-        T = input_ids.shape[1]
-        pos = torch.arange(T, device=input_ids.device)
-        return self.embed_tokens(input_ids) + self.embed_positions(pos).unsqueeze(0)
+    def _embed(self, input_ids: torch.Tensor, persistent: bool = False) -> torch.Tensor:
+        """Token plus position rows [B, T, d], behind the persistent tokens if asked (and there are any):
+        one kernel for plain embedding modules on the GPU, the modules themselves otherwise."""
+        B, T = input_ids.shape
+        tok, pos = self.embed_tokens, self.embed_positions
+        prefix = self.persistent_tokens if persistent and self.config.n_persistent > 0 else None
+        if _plain_lookup(tok) and _plain_lookup(pos) and T <= pos.num_embeddings:
+            tables = [t for t in (tok.weight, pos.weight, prefix) if t is not None]
+            if (input_ids.dtype in (torch.int64, torch.int32) and _lib.eager_native(input_ids, *tables)
+                    and all(t.is_cuda and t.device == input_ids.device and t.dtype == tok.weight.dtype
+                            and t.dtype in _lib._DTYPE_CODE for t in tables)):
+                return token_embedding(input_ids, tok.weight, pos.weight, prefix=prefix)
+        x = tok(input_ids) + pos(torch.arange(T, device=input_ids.device)).unsqueeze(0)
+        return x if prefix is None else torch.cat([prefix.unsqueeze(0).expand(B, -1, -1), x], dim=1)
 
     def _persistent(self, B: int) -> Optional[torch.Tensor]:
         if self.persistent_tokens is not None and self.config.n_persistent > 0:
             return self.persistent_tokens.unsqueeze(0).expand(B, -1, -1)
         return None
+
+    def _n_persistent(self) -> int:
+        return 0 if self.persistent_tokens is None else self.config.n_persistent
 
     def _blocks(self, y: torch.Tensor, layers=None) -> torch.Tensor:
         for layer in (self.layers if layers is None else layers):
@@ -178,15 +211,29 @@ class TitanMAC(nn.Module):
             return self.neural_memory.update(y)
         return self.neural_memory.compute_loss(y)
 
+    @staticmethod
+    def _next_tokens(labels: torch.Tensor) -> torch.Tensor:
+        """The token that each position is to predict; the last one's is ignored."""
+        return F.pad(labels[..., 1:], (0, 1), value=_IGNORE)
+
+    def _cross_entropy(self, logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+        """F.cross_entropy of the logits [B, T, V] against the next token: on its kernel (the logits read in
+        place, once) for plain GPU tensors."""
+        V = self.config.vocab_size
+        if (logits.is_cuda and labels.is_cuda and logits.device == labels.device and logits.dtype in _lib._DTYPE_CODE
+                and labels.dtype == torch.int64 and logits.shape == (*labels.shape, V) and labels.shape[-1] > 0
+                and _lib.eager_native(logits, labels)):
+            return token_cross_entropy(logits, self._next_tokens(labels), ignore_index=_IGNORE)
+        return F.cross_entropy(logits[..., :-1, :].contiguous().reshape(-1, V),
+                               labels[..., 1:].contiguous().reshape(-1), reduction="mean", ignore_index=_IGNORE)
+
     def _output(self, logits: torch.Tensor, labels: Optional[torch.Tensor],
                 memory_loss: Optional[torch.Tensor]) -> Dict[str, torch.Tensor]:
         out = {"logits": logits}
         if memory_loss is not None:
             out["memory_loss"] = memory_loss
         if labels is not None:
-            ce = F.cross_entropy(logits[..., :-1, :].contiguous().reshape(-1, self.config.vocab_size),
-                                 labels[..., 1:].contiguous().reshape(-1), reduction="mean",
-                                 ignore_index=-100)
+            ce = self._cross_entropy(logits, labels)
             if memory_loss is None:
                 out["loss"] = ce
             else:
@@ -221,6 +268,11 @@ class TitanMAC(nn.Module):
     def forward_mac(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                     attention_mask: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
         """Memory as Context (models/titanmac.py:160-313)."""
+        h, memory_loss = self._hidden_mac(input_ids)
+        return self._output(self.lm_head(h), labels, memory_loss)
+
+    def _hidden_mac(self, input_ids: torch.Tensor):
+        """(the head's input [B, T, d], memory loss) of forward_mac."""
         if self.neural_memory is None:
             raise ValueError("forward_mac requires use_neural_memory=True")
         B, T = input_ids.shape
@@ -259,47 +311,48 @@ class TitanMAC(nn.Module):
                 gate = torch.sigmoid(self.gate_proj(self.neural_memory.retrieve(ys)))
                 o[:, a:b] = ys * gate
             memory_loss = (acc / n_segments).squeeze()
-        logits = self.lm_head(self.norm(o))
-        return self._output(logits, labels, memory_loss)
+        return self.norm(o), memory_loss
 
     # ------------------------------------------------------------------ MAG / MAL
 
     def forward_mag(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                     attention_mask: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
         """Memory as Gate (models/titanmac.py:315-432): o = blocks(x̃) ⊙ sigmoid(gate_proj(M*(x̃)))."""
+        h, memory_loss = self._hidden_mag(input_ids)
+        return self._output(self.lm_head(h), labels, memory_loss)
+
+    def _hidden_mag(self, input_ids: torch.Tensor):
+        """(the head's input [B, T, d], memory loss) of forward_mag."""
         if self.neural_memory is None:
             raise ValueError("forward_mag requires use_neural_memory=True")
-        B = input_ids.shape[0]
-        x = self._embed(input_ids)
-        persistent = self._persistent(B)
-        xc = x if persistent is None else torch.cat([persistent, x], dim=1)
+        xc = self._embed(input_ids, persistent=True)
         gate = torch.sigmoid(self.gate_proj(self.neural_memory.retrieve(xc)))
         y = self._blocks(xc)
         o = y * gate
-        Np = 0 if persistent is None else self.config.n_persistent
+        Np = self._n_persistent()
         memory_loss = self._memory_step(y[:, Np:])
-        logits = self.lm_head(self.norm(o)[:, Np:])
-        return self._output(logits, labels, memory_loss)
+        return self.norm(o)[:, Np:], memory_loss
 
     def forward_mal(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                     attention_mask: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
         """Memory as Layer (models/titanmac.py:434-547): even layers are blocks, odd layers add
         memory_proj(M*(y))."""
+        h, memory_loss = self._hidden_mal(input_ids)
+        return self._output(self.lm_head(h), labels, memory_loss)
+
+    def _hidden_mal(self, input_ids: torch.Tensor):
+        """(the head's input [B, T, d], memory loss) of forward_mal."""
         if self.neural_memory is None:
             raise ValueError("forward_mal requires use_neural_memory=True")
-        B = input_ids.shape[0]
-        x = self._embed(input_ids)
-        persistent = self._persistent(B)
-        y = x if persistent is None else torch.cat([persistent, x], dim=1)
+        y = self._embed(input_ids, persistent=True)
         for i, layer in enumerate(self.layers):
             if i % 2 == 0:
                 y = self._blocks(y, [layer])
             else:
                 y = y + self.memory_proj(self.neural_memory.retrieve(y))
-        Np = 0 if persistent is None else self.config.n_persistent
+        Np = self._n_persistent()
         memory_loss = self._memory_step(y[:, Np:])
-        logits = self.lm_head(self.norm(y)[:, Np:])
-        return self._output(logits, labels, memory_loss)
+        return self.norm(y)[:, Np:], memory_loss
 
     def forward_with_memory(self, *args, **kwargs):
         """Alias of forward_mac (models/titanmac.py:550-552)."""
@@ -318,15 +371,46 @@ class TitanMAC(nn.Module):
             if variant == "MAL":
                 return self.forward_mal(input_ids, labels, attention_mask)
             raise ValueError(f"Unknown titans_variant: {variant}")
-        B = input_ids.shape[0]
-        x = self._embed(input_ids)
-        persistent = self._persistent(B)
-        if persistent is not None:
-            x = torch.cat([persistent, x], dim=1)
-        logits = self.lm_head(self.norm(self._blocks(x)))
-        if persistent is not None:
+        logits = self.lm_head(self.norm(self._blocks(self._embed(input_ids, persistent=True))))
+        if self._n_persistent():
             logits = logits[:, self.config.n_persistent:, :]
         return self._output(logits, labels, None)
+
+    # ------------------------------------------------------------------ scores
+
+    def score(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None, *, entropy: bool = False,
+              top_k: int = 0) -> Dict[str, torch.Tensor]:
+        """Per-token scores of a text: ``logprobs`` [B, T] fp32, at position t the log probability of
+        labels[:, t + 1] (labels defaults to input_ids) given the tokens up to t, 0 at the last position and
+        where that label is -100; on request ``entropy`` [B, T] and ``top_ids``, ``top_logprobs``
+        [B, T, top_k] of each position's distribution; with a neural memory its ``memory_loss``, and the
+        memory is updated exactly as by ``forward``.
+
+        Under ``torch.no_grad()`` in 16 bit and without top_k the logits are never stored (``head_logprobs``);
+        otherwise they are formed as in ``forward`` and read once (``token_logprobs``)."""
+        labels = input_ids if labels is None else labels
+        if labels.shape != input_ids.shape:
+            raise ValueError(f"score: labels must be {tuple(input_ids.shape)}, got {tuple(labels.shape)}")
+        memory_loss = None
+        if self.neural_memory is not None and self.config.use_neural_memory:
+            hidden = {"MAC": self._hidden_mac, "MAG": self._hidden_mag,
+                      "MAL": self._hidden_mal}.get(self.config.titans_variant)
+            if hidden is None:
+                raise ValueError(f"Unknown titans_variant: {self.config.titans_variant}")
+            h, memory_loss = hidden(input_ids)
+        else:
+            h = self.norm(self._blocks(self._embed(input_ids, persistent=True)))[:, self._n_persistent():]
+        targets = self._next_tokens(labels)[..., :labels.shape[-1]]
+        head = self.lm_head
+        if (top_k == 0 and _untouched(head, nn.Linear) and head.bias is None and head.weight.dtype == h.dtype
+                and not torch.is_autocast_enabled("cuda")):
+            r = head_logprobs(h, head.weight, targets, entropy=entropy, ignore_index=_IGNORE)
+        else:
+            r = token_logprobs(head(h), targets, entropy=entropy, top_k=top_k, ignore_index=_IGNORE)
+        out = {n: t for n, t in r._asdict().items() if t is not None}
+        if memory_loss is not None:
+            out["memory_loss"] = memory_loss
+        return out
 
     # ------------------------------------------------------------------ utilities
 
