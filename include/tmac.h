@@ -692,18 +692,17 @@ int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_W, 
                    int64_t ldp, const void* d_prefix, int64_t ldpre, void* d_out, int B, int T, int n_prefix, int d,
                    int64_t V, int64_t n_pos, float scale, int dtype, void* stream);
 
-/* dW[v] = scale · Σ_{ids[b, t] = v} g[b, n_prefix + t], dense [V, d] and contiguous, rows without a token
- * zero; g: the [B, n_prefix + T, d] gradient as rows of pitch ldg. fp32 sums in ascending order of (b, t)
- * (deterministic), rounded once. ids outside [0, V) count nowhere. Also the gradient of P for given positions
- * (ids = pos, V = n_pos, scale = 1). d_ws: tmac_embed_grad_workspace(B·T, V, d) bytes, 16-byte aligned. */
-int tmac_embed_grad_workspace(int64_t n_tokens, int64_t V, int d, size_t* ws_bytes);
-int tmac_embed_grad(const int64_t* d_ids, const void* d_g, int64_t ldg, void* d_dW, void* d_ws, size_t ws_bytes,
-                    int B, int T, int n_prefix, int d, int64_t V, float scale, int dtype, void* stream);
-
-/* dprefix[p] = Σ_b g[b, p] (nullable) and, for positions 0 .. T - 1, dP[t] = Σ_b g[b, n_prefix + t] with rows
- * [T, n_pos) zero (nullable); both contiguous. */
-int tmac_embed_pos_grad(const void* d_g, int64_t ldg, void* d_dprefix, void* d_dP, int B, int T, int n_prefix, int d,
-                        int64_t n_pos, int dtype, void* stream);
+/* Its gradients, each nullable, dense, contiguous and in dtype, of g [B, n_prefix + T, d] given as rows of pitch ldg:
+ *   dW[v] = scale · Σ_{ids[b, t] = v} g[b, n_prefix + t]    [V, d]
+ *   dP[q] = Σ_{pos(b, t) = q} g[b, n_prefix + t]            [n_pos, d]
+ *   dprefix[p] = Σ_b g[b, p]                                [n_prefix, d]
+ * Rows without a token are zeros, indices outside a table count nowhere. fp32 sums in ascending order of
+ * (b, t) (deterministic), rounded once. d_ws: 16-byte aligned, tmac_embed_bwd_workspace(B·T, V, n_pos, d) bytes with
+ * V = 0 without d_dW and n_pos = 0 without d_dP or d_pos; none where both are. */
+int tmac_embed_bwd_workspace(int64_t n_tokens, int64_t V, int64_t n_pos, int d, size_t* ws_bytes);
+int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_g, int64_t ldg, void* d_dW, void* d_dP,
+                   void* d_dprefix, void* d_ws, size_t ws_bytes, int B, int T, int n_prefix, int d, int64_t V,
+                   int64_t n_pos, float scale, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Log probabilities of given tokens (F.cross_entropy of models/titanmac.py:666-680 by row, and what a

@@ -90,23 +90,21 @@ def test_embedding_argument_errors(lib):
     empty[9] = 0
     assert lib.tmac_embed_fwd(*empty) == 0
     n = ctypes.c_size_t(0)
-    assert lib.tmac_embed_grad_workspace(1000, 50, 64, ctypes.byref(n)) == 0 and n.value >= 4 * (51 + 2000) + 2 * 16 * 64 * 4
-    assert lib.tmac_embed_grad_workspace(1000, 0, 64, ctypes.byref(n)) == -2
-    assert lib.tmac_embed_grad_workspace(1000, 50, 64, None) == -1
-    lib.tmac_embed_grad_workspace(6, 100, 64, ctypes.byref(n))
-    # ids, g, ldg, dW, ws, ws_bytes, B, T, n_prefix, d, V, scale, dtype, stream
-    ok = [FAKE, FAKE, 64, FAKE, FAKE, n.value, 2, 3, 4, 64, 100, 1.0, 1, None]
-    for at, value, want in ((0, None, -1), (1, None, -1), (3, None, -1), (4, None, -6), (5, n.value - 1, -6),
-                            (4, FAKE + 4, -5), (2, 63, -2), (10, 0, -2), (12, 9, -4)):
+    assert lib.tmac_embed_bwd_workspace(1000, 50, 0, 64, ctypes.byref(n)) == 0 and n.value >= 4 * (51 + 2000) + 2 * 16 * 64 * 4
+    assert lib.tmac_embed_bwd_workspace(1000, -1, 0, 64, ctypes.byref(n)) == -2
+    assert lib.tmac_embed_bwd_workspace(1000, 50, (1 << 30) + 1, 64, ctypes.byref(n)) == -2
+    assert lib.tmac_embed_bwd_workspace(1000, 50, 0, 64, None) == -1
+    lib.tmac_embed_bwd_workspace(6, 100, 50, 64, ctypes.byref(n))
+    # ids, pos, g, ldg, dW, dP, dprefix, ws, ws_bytes, B, T, n_prefix, d, V, n_pos, scale, dtype, stream
+    ok = [FAKE, FAKE, FAKE, 64, FAKE, FAKE, FAKE, FAKE, n.value, 2, 3, 4, 64, 100, 50, 1.0, 1, None]
+    for at, value, want in ((0, None, -1), (2, None, -1), (7, None, -6), (8, n.value - 1, -6), (7, FAKE + 4, -5),
+                            (3, 63, -2), (13, 0, -2), (14, 0, -2), (16, 9, -4), (12, 0, -2), (11, 0, -2), (9, -1, -2)):
         bad = list(ok)
         bad[at] = value
-        assert lib.tmac_embed_grad(*bad) == want, (at, value)
-    # g, ldg, dprefix, dP, B, T, n_prefix, d, n_pos, dtype, stream
-    ok = [FAKE, 64, FAKE, FAKE, 2, 3, 4, 64, 50, 1, None]
-    for at, value, want in ((0, None, -1), (1, 63, -2), (8, 2, -2), (9, 5, -4), (7, 0, -2)):
-        bad = list(ok)
-        bad[at] = value
-        assert lib.tmac_embed_pos_grad(*bad) == want, (at, value)
+        assert lib.tmac_embed_bwd(*bad) == want, (at, value)
+    bad = list(ok)
+    bad[1], bad[14] = None, 2  # fewer position rows than positions
+    assert lib.tmac_embed_bwd(*bad) == -2
 
 
 def test_logprob_argument_errors(lib):

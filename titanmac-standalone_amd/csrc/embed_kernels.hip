@@ -9,9 +9,10 @@
 // once, and the gradient, dense as nn.Embedding's, is written once, rows without a token as zeros.
 //
 // The gradient sums each row's tokens in ascending order of position (deterministic): a sort gives every
-// row of W its list of tokens; a list of up to 64 is summed where its row is written; longer ones (the
-// frequent tokens: a text's first hundred ids are half of it) are summed 64 tokens a workgroup into fp32
-// partial rows that a third kernel adds in order, so one frequent token does not hold one workgroup.
+// row of W its list of tokens; a list of up to 16 is summed where its row is written; longer ones (the
+// frequent tokens: a text's first hundred ids are half of it) are summed 16 tokens a workgroup into fp32
+// partial rows that a third kernel adds in order, so one frequent token does not hold one workgroup (lists
+// of up to 64 in one thread's chain of loads: 54 us of 30 for 32768 tokens of 640 bf16, V = 128000).
 
 #include "row_device.h"
 
@@ -21,14 +22,15 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Rows per workgroup: about `per` pieces (cpr of them a row) for each thread, more where the grid would
-// pass 2^22 workgroups.
-int rows_per_block(int64_t rows, int cpr, int per) {
-  int64_t rpb = kThreads * per > cpr ? kThreads * per / cpr : 1;
-  while ((rows + rpb - 1) / rpb > (1 << 22)) rpb *= 2;
-  return static_cast<int>(rpb);
-}
+constexpr int kMaxRowsPerBlock = 4 * kThreads;
+constexpr int kMaxGrid = 1 << 22;  // workgroups of a launch; they take turns beyond that
 
+// Rows per workgroup and turn: about `per` (at most 4) pieces, cpr of them a row, for each thread.
+int rows_per_block(int cpr, int per) { return kThreads * per > cpr ? kThreads * per / cpr : 1; }
+int grid(int64_t blocks) { return static_cast<int>(blocks < kMaxGrid ? blocks : kMaxGrid); }
+
+// One piece per thread and turn: two or four in flight measured 10 and 25 % slower (9.9 us against 10.9 and 12.8
+// for 4 x 4112 rows of 640 bf16: the registers cost more waves than the loads gain).
 template <int DT, int N>
 __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
     const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const uint8_t* __restrict__ W,
@@ -36,34 +38,34 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
     uint8_t* __restrict__ out, int rows, int T, int Np, int d, int64_t V, int64_t n_pos, float scale, int cpr,
     int rpb) {
   constexpr int E = kRowSize<DT>;
-  const int row0 = blockIdx.x * rpb;
-  const int n = min(rpb, rows - row0) * cpr;
   const int S = Np + T;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int r = i / cpr, c = (i - r * cpr) * N;
-    const int row = row0 + r;
-    const int b = row / S, s = row - b * S;
-    float v[N];
-    if (s < Np) {
-      row_load<DT, N>(prefix + (static_cast<int64_t>(s) * ldpre + c) * E, v);
-    } else {
-      const int64_t tok = static_cast<int64_t>(b) * T + (s - Np);
-      const int64_t id = ids[tok];
-      const int64_t p = pos ? pos[tok] : s - Np;
-      // an index outside its table reads nothing and gives a row of NaN
-      const bool ok = id >= 0 && id < V && (!P || (p >= 0 && p < n_pos));
-      if (ok) {
-        row_load<DT, N>(W + (id * ldw + c) * E, v);
-        float q[N];
-        if (P) row_load<DT, N>(P + (p * ldp + c) * E, q);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = P ? fmaf(scale, v[e], q[e]) : scale * v[e];
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rpb; row0 < rows; row0 += static_cast<int64_t>(gridDim.x) * rpb) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(rpb), rows - row0)) * cpr;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int r = i / cpr, c = (i - r * cpr) * N;
+      const int row = static_cast<int>(row0) + r;
+      const int b = row / S, s = row - b * S;
+      float v[N];
+      if (s < Np) {
+        row_load<DT, N>(prefix + (s * ldpre + c) * E, v);
       } else {
+        const int64_t tok = static_cast<int64_t>(b) * T + (s - Np);
+        const int64_t id = ids[tok];
+        const int64_t p = pos ? pos[tok] : s - Np;
+        // an index outside its table reads nothing and gives a row of NaN
+        if (id >= 0 && id < V && (!P || (p >= 0 && p < n_pos))) {
+          float q[N];
+          row_load<DT, N>(W + (id * ldw + c) * E, v);
+          if (P) row_load<DT, N>(P + (p * ldp + c) * E, q);
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = __builtin_nanf("");
+          for (int e = 0; e < N; ++e) v[e] = P ? fmaf(scale, v[e], q[e]) : scale * v[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = __builtin_nanf("");
+        }
       }
+      row_store<DT, N>(out + (static_cast<int64_t>(row) * d + c) * E, v);
     }
-    row_store<DT, N>(out + (static_cast<int64_t>(row) * d + c) * E, v);
   }
 }
 
@@ -81,29 +83,74 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
   return v;
 }
 
-// Stable counting sort of the tokens by id, without passes over digits: workgroup w owns the ids
-// [w R, (w + 1) R) and reads all of them twice (they stay in L2). The first time it counts, per wave, how
+// The ids of a workgroup of the sort: [0, 8), then eight ranges to an octave up to 8192, then 512 each.
+// Low ids are the frequent ones (token tables are made by frequency), and a narrow range is cheap where
+// every batch has some: the ids' bits are what the placing below counts instructions by.
+struct IdRange {
+  int lo, n;
+};
+__host__ __device__ inline IdRange id_range(int block) {
+  if (block == 0) return IdRange{0, 8};
+  const int o = (block - 1) >> 3, i = (block - 1) & 7;
+  if (o <= 9) return IdRange{(8 + i) << o, 1 << o};
+  return IdRange{(1 << 13) + (block - 81) * kMaxRange, kMaxRange};
+}
+int n_ranges(int64_t V) {
+  if (V > (1 << 13)) return static_cast<int>(81 + (V - (1 << 13) + kMaxRange - 1) / kMaxRange);
+  int n = 1;
+  while (id_range(n).lo < V) ++n;
+  return n;
+}
+
+// Stable counting sort of the tokens by id, without passes over digits: each workgroup owns a range of
+// ids and reads all of them twice (they stay in L2). The first time it counts, per wave, how
 // often each of its ids comes and how many ids come before its range, which is where its part of the list
 // begins; the second time each wave places its tokens behind those of the waves before it.
 // row_start[v]: where id v's tokens begin (row_start[V] their number); perm: the row of g of each, in
 // ascending order; key: its id. An id outside [0, V) is in no list.
-__global__ __launch_bounds__(64 * kSortWaves) void embed_sort_kernel(
-    const int64_t* __restrict__ ids, int n_tok, int T, int Np, int V, int R, int32_t* __restrict__ row_start,
+// HELD: batches of 64 ids that a wave keeps in registers between the two readings (all it has), or 0.
+template <int HELD>
+__global__ __launch_bounds__(64 * kSortWaves, 8) void embed_sort_kernel(
+    const int64_t* __restrict__ ids, int n_tok, int T, uint32_t T_inv, int Np, int V, int32_t* __restrict__ row_start,
     int32_t* __restrict__ perm, int32_t* __restrict__ key) {
   __shared__ int hist[kSortWaves * kMaxRange];
   __shared__ int s_tot[kSortWaves], s_below[kSortWaves];
+  constexpr int kAhead = HELD ? HELD : 8, kLoads = kAhead < 8 ? kAhead : 8;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int lo = blockIdx.x * R, hi = min(lo + R, V);
+  const IdRange range = id_range(blockIdx.x);
+  const int lo = range.lo, R = min(range.n, V - lo);  // lo < V
   const int per = (n_tok + 64 * kSortWaves - 1) / (64 * kSortWaves) * 64;
   const int begin = wave * per, end = min(begin + per, n_tok);
   int* const mine = hist + wave * R;
   for (int i = tid; i < kSortWaves * R; i += 64 * kSortWaves) hist[i] = 0;
-  __syncthreads();
+  // this lane's part of kAhead batches of ids from n0 on, relative to the range: −1 outside it
   int below = 0;
-  for (int n = begin + lane; n < end; n += 64) {
-    const int64_t id = ids[n];
-    if (id >= 0 && id < lo) ++below;
-    if (id >= lo && id < hi) atomicAdd(mine + static_cast<int>(id - lo), 1);
+  int rel[kAhead];
+  auto load = [&](int n0, bool count) {
+#pragma unroll
+    for (int u0 = 0; u0 < kAhead; u0 += kLoads) {
+      int64_t id[kLoads];
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int n = n0 + 64 * (u0 + u) + lane;
+        id[u] = n < end ? ids[n] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        // ids of 2^32 and more, and negative ones, to the largest unsigned value
+        const uint32_t x = static_cast<uint64_t>(id[u]) >> 32 ? ~0u : static_cast<uint32_t>(id[u]);
+        if (count) below += x < static_cast<uint32_t>(lo);
+        const uint32_t r = x - static_cast<uint32_t>(lo);
+        rel[u0 + u] = x != ~0u && r < static_cast<uint32_t>(R) ? static_cast<int>(r) : -1;
+      }
+    }
+  };
+  __syncthreads();
+  for (int n0 = begin; n0 < end; n0 += 64 * kAhead) {
+    load(n0, true);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (rel[u] >= 0) atomicAdd(mine + rel[u], 1);
   }
   below = wave_scan(below, lane);
   if (lane == 63) s_below[wave] = below;
@@ -116,7 +163,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort_kernel(
   __syncthreads();
   int run = inc - tot;
   for (int w = 0; w < kSortWaves; ++w) run += s_below[w] + (w < wave ? s_tot[w] : 0);
-  if (tid < R && lo + tid < V) {
+  if (tid < R) {
     row_start[lo + tid] = run;
     for (int w = 0; w < kSortWaves; ++w) {
       const int c = hist[w * R + tid];
@@ -126,36 +173,47 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort_kernel(
     if (lo + tid == V - 1) row_start[V] = run;
   }
   __syncthreads();
-  for (int n0 = begin; n0 < end; n0 += 64) {
-    const int n = n0 + lane;
-    const int64_t id = n < end ? ids[n] : -1;
-    const int rel = id >= lo && id < hi ? static_cast<int>(id - lo) : -1;
-    // the tokens of one id at a time, in the order of the lanes
-    for (uint64_t todo = __ballot(rel >= 0); todo;) {
-      const int r = __builtin_amdgcn_readlane(rel, __builtin_ctzll(todo));
-      const uint64_t same = __ballot(rel == r);
-      int at = 0;
-      if (lane == 0) at = atomicAdd(mine + r, __popcll(same));
-      at = __builtin_amdgcn_readfirstlane(at);
-      if (rel == r) {
-        const int slot = at + __popcll(same & ((1ull << lane) - 1));
-        perm[slot] = n + (n / T + 1) * Np;
-        key[slot] = static_cast<int>(id);
+  const int bits = 32 - __builtin_clz(R);
+  for (int n0 = begin; n0 < end; n0 += 64 * kAhead) {
+    if (!HELD) load(n0, false);  // HELD: there is one turn, and they are still here
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool in = rel[u] >= 0;
+      uint64_t same = __ballot(in);
+      if (!same) continue;
+      // the lanes with this lane's id; the first of them takes the places for all
+      uint32_t lo32 = static_cast<uint32_t>(same), hi32 = static_cast<uint32_t>(same >> 32);
+      for (int b = 0; b < bits; ++b) {
+        const uint32_t bit = rel[u] >> b & 1;
+        const uint64_t set = __ballot(bit);
+        lo32 &= ~(static_cast<uint32_t>(set) ^ (0u - bit));
+        hi32 &= ~(static_cast<uint32_t>(set >> 32) ^ (0u - bit));
       }
-      todo &= ~same;
+      same = static_cast<uint64_t>(hi32) << 32 | lo32;
+      const int n = n0 + 64 * u + lane, lead = in ? __builtin_ctzll(same) : lane;
+      int at = 0;
+      if (in && lane == lead) at = atomicAdd(mine + rel[u], __popcll(same));
+      at = __shfl(at, lead);
+      if (in) {
+        const int slot = at + __popcll(same & ((1ull << lane) - 1));
+        int b = T > 1 ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), T_inv)) : n;  // n / T, or one less
+        if (T > 1 && n - b * T >= T) ++b;
+        perm[slot] = n + (b + 1) * Np;
+        key[slot] = lo + rel[u];
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------ the sums
 
-constexpr int kList = 64;  // longest list that is summed in one piece; tokens per partial row
+constexpr int kList = 16;  // longest list that is summed in one piece; tokens per partial row
 
 // v += the rows perm[a .. b) of g at column c, in order
 template <int DT, int N>
 __device__ __forceinline__ void sum_rows(const uint8_t* __restrict__ g, int64_t ldg,
                                          const int32_t* __restrict__ perm, int a, int b, int c, float (&v)[N]) {
-  constexpr int E = kRowSize<DT>, U = 4;
+  constexpr int E = kRowSize<DT>, U = 8;
   for (; a + U <= b; a += U) {
     float x[U][N];
 #pragma unroll
@@ -173,119 +231,160 @@ __device__ __forceinline__ void sum_rows(const uint8_t* __restrict__ g, int64_t 
   }
 }
 
-// Workgroups [0, n_chunks): the part of each long list that lies in sorted tokens [64 j, 64 j + 64), into
-// part[j][0] (the list of the first of them) and part[j][1] (of the last, if another). Long lists have more
-// than 64 tokens, so no third one reaches into the chunk. The other workgroups: rpb rows of dW each.
+// What one launch of the gradients covers.
+struct Grad {
+  const uint8_t* g;  // rows of pitch ldg
+  int64_t ldg;
+  const int32_t *row_start, *perm, *key;  // the sorted lists
+  float* part;
+  uint8_t* dW;  // [V, d] by sorted tokens
+  int V, rpb, chunks, row_blocks;
+  float scale;
+  uint8_t *dprefix, *dP;  // rows [first, last) of [prefix | positions] by sums over the sequences
+  int B, T, Np, first, last, pos_blocks, pos_rpb;
+  int d, cpr;
+};
+
+// The part of each long list that lies in sorted tokens [16 j, 16 j + 16), into part[j][0] (the list of the
+// first of them) and part[j][1] (of the last, if another). Long lists have more than 16 tokens, so no third
+// one reaches into the chunk.
 template <int DT, int N>
-__global__ __launch_bounds__(kThreads) void embed_grad_kernel(
-    const uint8_t* __restrict__ g, int64_t ldg, const int32_t* __restrict__ row_start,
-    const int32_t* __restrict__ perm, const int32_t* __restrict__ key, float* __restrict__ part,
-    uint8_t* __restrict__ dW, int V, int d, float scale, int cpr, int rpb, int n_chunks) {
-  constexpr int E = kRowSize<DT>;
-  if (static_cast<int>(blockIdx.x) < n_chunks) {
-    const int j = blockIdx.x, n_valid = row_start[V];
-    const int a0 = kList * j, b0 = min(a0 + kList, n_valid);
-    if (a0 >= b0) return;
-    const int k0 = key[a0], k1 = key[b0 - 1];
-    for (int which = 0; which < (k0 == k1 ? 1 : 2); ++which) {
-      const int k = which ? k1 : k0;
-      const int s = row_start[k], e = row_start[k + 1];
-      if (e - s <= kList) continue;
-      const int a = max(a0, s), b = min(b0, e);
-      for (int c = threadIdx.x; c < cpr; c += kThreads) {
-        float v[N] = {};
-        sum_rows<DT, N>(g, ldg, perm, a, b, c * N, v);
-        float* const to = part + (static_cast<int64_t>(2 * j + which) * d + c * N);
+__device__ __forceinline__ void grad_chunk(const Grad& a, int j) {
+  const int n_valid = a.row_start[a.V];
+  const int a0 = kList * j, b0 = min(a0 + kList, n_valid);
+  if (a0 >= b0) return;
+  const int k0 = a.key[a0], k1 = a.key[b0 - 1];
+  for (int which = 0; which < (k0 == k1 ? 1 : 2); ++which) {
+    const int k = which ? k1 : k0;
+    const int s = a.row_start[k], e = a.row_start[k + 1];
+    if (e - s <= kList) continue;
+    for (int c = threadIdx.x; c < a.cpr; c += kThreads) {
+      float v[N] = {};
+      sum_rows<DT, N>(a.g, a.ldg, a.perm, max(a0, s), min(b0, e), c * N, v);
+      float* const to = a.part + (static_cast<int64_t>(2 * j + which) * a.d + c * N);
 #pragma unroll
-        for (int q = 0; q < N; ++q) to[q] = v[q];
-      }
+      for (int q = 0; q < N; ++q) to[q] = v[q];
     }
-    return;
-  }
-  const int row0 = (blockIdx.x - n_chunks) * rpb;
-  const int n = min(rpb, V - row0) * cpr;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int r = i / cpr, c = (i - r * cpr) * N;
-    const int a = row_start[row0 + r], b = row_start[row0 + r + 1];
-    if (b - a > kList) continue;
-    float v[N] = {};
-    sum_rows<DT, N>(g, ldg, perm, a, b, c, v);
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] *= scale;
-    row_store<DT, N>(dW + (static_cast<int64_t>(row0 + r) * d + c) * E, v);
   }
 }
 
-// The long list that begins in chunk j, if one does (it reaches the chunk's end, so at most one): its
-// partial rows, added in order by eight groups of threads and those groups' sums in order.
+// rpb rows of dW: their lists' ends first, so that the rows without a token (most of a large table) are
+// stores and nothing else.
 template <int DT, int N>
-__global__ __launch_bounds__(1024) void embed_grad_long_kernel(
-    const int32_t* __restrict__ row_start, const int32_t* __restrict__ key, const float* __restrict__ part,
-    uint8_t* __restrict__ dW, int V, int d, float scale, int cpr) {
-  constexpr int E = kRowSize<DT>, kGroups = 8, kWide = 1024 / kGroups;
-  __shared__ float sums[kGroups][kWide][N];
-  const int j = blockIdx.x, n_valid = row_start[V];
-  const int last = kList * j + kList - 1;  // a long list that begins here covers it
-  if (last >= n_valid) return;
-  const int k = key[last];
-  const int s = row_start[k], e = row_start[k + 1];
-  if (e - s <= kList || s < kList * j) return;
-  // chunks j .. j1 hold it: in chunk j it is the last list, in the others the first
-  const int j1 = (e - 1) / kList, n = j1 - j + 1, per = (n + kGroups - 1) / kGroups;
-  const int grp = threadIdx.x / kWide, t = threadIdx.x % kWide;
-  const int first = s == kList * j ? 0 : 1;
-  for (int c0 = 0; c0 < cpr; c0 += kWide) {
-    const int c = c0 + t;
+__device__ __forceinline__ void grad_rows(const Grad& a, int block) {
+  constexpr int E = kRowSize<DT>;
+  __shared__ int s_start[kMaxRowsPerBlock + 1];
+  const int row0 = block * a.rpb, rows = min(a.rpb, a.V - row0), n = rows * a.cpr;
+  for (int i = threadIdx.x; i <= rows; i += kThreads) s_start[i] = a.row_start[row0 + i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int r = i / a.cpr, c = (i - r * a.cpr) * N;
+    const int p = s_start[r], q = s_start[r + 1];
+    if (q - p > kList) continue;
     float v[N] = {};
-    if (c < cpr) {
-      const int end = min(n, (grp + 1) * per);
-#pragma unroll 8
-      for (int i = grp * per; i < end; ++i) {
-        const float* from = part + (static_cast<int64_t>(2 * (j + i) + (i ? 0 : first)) * d + c * N);
+    sum_rows<DT, N>(a.g, a.ldg, a.perm, p, q, c, v);
 #pragma unroll
-        for (int q = 0; q < N; ++q) v[q] += from[q];
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < N; ++q) sums[grp][t][q] = v[q];
-    __syncthreads();
-    if (grp == 0 && c < cpr) {
-      for (int o = 1; o < kGroups; ++o)
-#pragma unroll
-        for (int q = 0; q < N; ++q) v[q] += sums[o][t][q];
-#pragma unroll
-      for (int q = 0; q < N; ++q) v[q] *= scale;
-      row_store<DT, N>(dW + (static_cast<int64_t>(k) * d + c * N) * E, v);
-    }
-    __syncthreads();
+    for (int e = 0; e < N; ++e) v[e] *= a.scale;
+    row_store<DT, N>(a.dW + (static_cast<int64_t>(row0 + r) * a.d + c) * E, v);
   }
+  __syncthreads();
 }
 
-// Row s of [prefix | positions]: the sum over the sequences of g[b, s], zeros behind the last position.
+// Rows s of [prefix | positions]: the sum over the sequences of g[b, s], zeros behind the last position.
 template <int DT, int N>
-__global__ __launch_bounds__(kThreads) void embed_pos_grad_kernel(
-    const uint8_t* __restrict__ g, int64_t ldg, uint8_t* __restrict__ dprefix, uint8_t* __restrict__ dP, int B,
-    int T, int Np, int d, int row_first, int rows, int cpr, int rpb) {
+__device__ __forceinline__ void grad_positions(const Grad& a, int block) {
   constexpr int E = kRowSize<DT>;
-  const int S = Np + T;
-  const int row0 = row_first + blockIdx.x * rpb;
-  const int n = min(rpb, rows - row0) * cpr;
+  const int S = a.Np + a.T;
+  const int row0 = a.first + block * a.pos_rpb, n = min(a.pos_rpb, a.last - row0) * a.cpr;
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int r = i / cpr, c = (i - r * cpr) * N;
+    const int r = i / a.cpr, c = (i - r * a.cpr) * N;
     const int s = row0 + r;
     float v[N] = {};
     if (s < S) {
 #pragma unroll 4
-      for (int b = 0; b < B; ++b) {
+      for (int b = 0; b < a.B; ++b) {
         float x[N];
-        row_load<DT, N>(g + ((static_cast<int64_t>(b) * S + s) * ldg + c) * E, x);
+        row_load<DT, N>(a.g + ((static_cast<int64_t>(b) * S + s) * a.ldg + c) * E, x);
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] += x[e];
       }
     }
-    uint8_t* const to = s < Np ? dprefix + (static_cast<int64_t>(s) * d + c) * E
-                               : dP + (static_cast<int64_t>(s - Np) * d + c) * E;
-    row_store<DT, N>(to, v);
+    row_store<DT, N>(s < a.Np ? a.dprefix + (static_cast<int64_t>(s) * a.d + c) * E
+                              : a.dP + (static_cast<int64_t>(s - a.Np) * a.d + c) * E,
+                     v);
+  }
+}
+
+// The chunks of long lists first, whose sums the next launch waits for.
+template <int DT, int N>
+__global__ __launch_bounds__(kThreads) void embed_grad_kernel(Grad a) {
+  const int blocks = a.chunks + a.pos_blocks + a.row_blocks;
+  for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
+    if (b < a.chunks)
+      grad_chunk<DT, N>(a, b);
+    else if (b < a.chunks + a.pos_blocks)
+      grad_positions<DT, N>(a, b - a.chunks);
+    else
+      grad_rows<DT, N>(a, b - a.chunks - a.pos_blocks);
+  }
+}
+
+// The long lists that begin in this workgroup's chunks (one reaches its chunk's end, so there is at most one a
+// chunk): their partial rows, added in order by eight groups of threads and those groups' sums in order.
+constexpr int kLongChunks = 8;
+
+template <int DT, int N>
+__global__ __launch_bounds__(1024) void embed_grad_long_kernel(Grad a) {
+  constexpr int E = kRowSize<DT>, kGroups = 8, kWide = 1024 / kGroups;
+  __shared__ float sums[kGroups][kWide][N];
+  __shared__ int s_key[kLongChunks];
+  for (int base = blockIdx.x * kLongChunks; base < a.chunks; base += gridDim.x * kLongChunks) {
+    if (threadIdx.x < kLongChunks) {
+      const int j = base + threadIdx.x, last = kList * j + kList - 1;  // the entry that such a list covers
+      int k = -1;
+      if (last < a.row_start[a.V]) {
+        k = a.key[last];
+        const int s = a.row_start[k], e = a.row_start[k + 1];
+        if (e - s <= kList || s < kList * j) k = -1;
+      }
+      s_key[threadIdx.x] = k;
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < kLongChunks; ++i0) {
+      const int j = base + i0, k = s_key[i0];
+      if (k < 0) continue;
+      // chunks j .. j1 hold it: in chunk j it is the last list, in the others the first
+      const int s = a.row_start[k], e = a.row_start[k + 1];
+      const int j1 = (e - 1) / kList, n = j1 - j + 1, per = (n + kGroups - 1) / kGroups;
+      const int grp = threadIdx.x / kWide, t = threadIdx.x % kWide;
+      const int first = s == kList * j ? 0 : 1;
+      for (int c0 = 0; c0 < a.cpr; c0 += kWide) {
+        const int c = c0 + t;
+        float v[N] = {};
+        if (c < a.cpr) {
+          const int end = min(n, (grp + 1) * per);
+#pragma unroll 8
+          for (int i = grp * per; i < end; ++i) {
+            const float* from = a.part + (static_cast<int64_t>(2 * (j + i) + (i ? 0 : first)) * a.d + c * N);
+#pragma unroll
+            for (int q = 0; q < N; ++q) v[q] += from[q];
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < N; ++q) sums[grp][t][q] = v[q];
+        __syncthreads();
+        if (grp == 0 && c < a.cpr) {
+          for (int o = 1; o < kGroups; ++o)
+#pragma unroll
+            for (int q = 0; q < N; ++q) v[q] += sums[o][t][q];
+#pragma unroll
+          for (int q = 0; q < N; ++q) v[q] *= a.scale;
+          row_store<DT, N>(a.dW + (static_cast<int64_t>(k) * a.d + c * N) * E, v);
+        }
+        __syncthreads();
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -362,8 +461,9 @@ extern "C" int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const 
                     wide_rows(d_P, ldp, dtype) && (!n_prefix || wide_rows(d_prefix, ldpre, dtype));
   dispatch(dtype, wide, [&](auto dt, auto n) {
     constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
-    const int cpr = d / N, rpb = rows_per_block(rows, cpr, 1);
-    embed_fwd_kernel<DT, N><<<(rows + rpb - 1) / rpb, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+    const int cpr = d / N;
+    const int rpb = rows_per_block(cpr, 1);
+    embed_fwd_kernel<DT, N><<<grid((rows + rpb - 1) / rpb), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
         d_ids, d_pos, static_cast<const uint8_t*>(d_W), ldw, static_cast<const uint8_t*>(d_P), ldp,
         static_cast<const uint8_t*>(d_prefix), ldpre, static_cast<uint8_t*>(d_out), rows, T, n_prefix, d, V, n_pos,
         scale, cpr, rpb);
@@ -371,66 +471,93 @@ extern "C" int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const 
   return launch_status();
 }
 
-extern "C" int tmac_embed_grad_workspace(int64_t n_tokens, int64_t V, int d, size_t* ws_bytes) {
+extern "C" int tmac_embed_bwd_workspace(int64_t n_tokens, int64_t V, int64_t n_pos, int d, size_t* ws_bytes) {
   if (!ws_bytes) return TMAC_ERR_NULL;
-  if (n_tokens < 0 || n_tokens > kMaxRows || V <= 0 || V > kMaxRows || d <= 0 || d > kMaxD) return TMAC_ERR_SHAPE;
-  *ws_bytes = grad_ws(n_tokens, V, d).total;
+  if (n_tokens < 0 || n_tokens > kMaxRows || V < 0 || V > kMaxRows || n_pos < 0 || n_pos > kMaxRows || d <= 0 ||
+      d > kMaxD)
+    return TMAC_ERR_SHAPE;
+  *ws_bytes = grad_ws(n_tokens, V > n_pos ? V : n_pos, d).total;  // the two sorts take turns
   return TMAC_OK;
 }
 
-extern "C" int tmac_embed_grad(const int64_t* d_ids, const void* d_g, int64_t ldg, void* d_dW, void* d_ws,
-                               size_t ws_bytes, int B, int T, int n_prefix, int d, int64_t V, float scale,
-                               int dtype, void* stream) {
+extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_g, int64_t ldg, void* d_dW,
+                              void* d_dP, void* d_dprefix, void* d_ws, size_t ws_bytes, int B, int T, int n_prefix,
+                              int d, int64_t V, int64_t n_pos, float scale, int dtype, void* stream) {
   const int st = check_sizes(B, T, n_prefix, d, dtype);
   if (st != TMAC_OK) return st;
-  if (V <= 0 || V > kMaxRows || ldg < d) return TMAC_ERR_SHAPE;
+  const bool sums = d_dP && !d_pos;  // positions 0 .. T - 1: plain sums, no sort
+  if (ldg < d || (d_dW && (V <= 0 || V > kMaxRows)) || (d_dP && (n_pos <= 0 || n_pos > kMaxRows)) ||
+      (sums && n_pos < T) || (d_dprefix && !n_prefix))
+    return TMAC_ERR_SHAPE;
   const int n_tok = B * T;
-  if (!d_dW || (n_tok > 0 && (!d_ids || !d_g))) return TMAC_ERR_NULL;
-  const GradWs w = grad_ws(n_tok, V, d);
-  if (!d_ws || ws_bytes < w.total) return TMAC_ERR_WORKSPACE;
-  if (!row_aligned16(d_ws)) return TMAC_ERR_ALIGN;
+  if ((n_tok > 0 || (B > 0 && d_dprefix)) && !d_g) return TMAC_ERR_NULL;
+  if (d_dW && n_tok > 0 && !d_ids) return TMAC_ERR_NULL;
+  size_t need = 0;
+  if (d_dW || (d_dP && d_pos)) tmac_embed_bwd_workspace(n_tok, d_dW ? V : 0, d_dP && d_pos ? n_pos : 0, d, &need);
+  if (need && (!d_ws || ws_bytes < need)) return TMAC_ERR_WORKSPACE;
+  if (need && !row_aligned16(d_ws)) return TMAC_ERR_ALIGN;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  uint8_t* const ws = static_cast<uint8_t*>(d_ws);
-  int32_t* const row_start = reinterpret_cast<int32_t*>(ws);
-  int32_t* const perm = reinterpret_cast<int32_t*>(ws + w.perm);
-  int32_t* const key = reinterpret_cast<int32_t*>(ws + w.key);
-  float* const part = reinterpret_cast<float*>(ws + w.part);
-  const int n_v = static_cast<int>(V);
-  const int R = max(1, min(kMaxRange, (n_v + 511) / 512));
-  embed_sort_kernel<<<(n_v + R - 1) / R, 64 * kSortWaves, 0, s>>>(d_ids, n_tok, T, n_prefix, n_v, R, row_start,
-                                                                  perm, key);
-  const bool wide = d % (dtype == TMAC_F32 ? 4 : 8) == 0 && row_aligned16(d_dW) && wide_rows(d_g, ldg, dtype);
-  dispatch(dtype, wide, [&](auto dt, auto n) {
-    constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
-    const int cpr = d / N, rpb = rows_per_block(V, cpr, 4);
-    const int chunks = n_tok > kList ? (n_tok + kList - 1) / kList : 0;
-    embed_grad_kernel<DT, N><<<chunks + (n_v + rpb - 1) / rpb, kThreads, 0, s>>>(
-        static_cast<const uint8_t*>(d_g), ldg, row_start, perm, key, part, static_cast<uint8_t*>(d_dW), n_v, d,
-        scale, cpr, rpb, chunks);
-    if (chunks)
-      embed_grad_long_kernel<DT, N><<<chunks, 1024, 0, s>>>(row_start, key, part, static_cast<uint8_t*>(d_dW), n_v,
-                                                           d, scale, cpr);
-  });
-  return launch_status();
-}
+  const bool wide = d % (dtype == TMAC_F32 ? 4 : 8) == 0 && row_aligned16(d_dW) && row_aligned16(d_dP) &&
+                    row_aligned16(d_dprefix) && wide_rows(d_g, ldg, dtype);
 
-extern "C" int tmac_embed_pos_grad(const void* d_g, int64_t ldg, void* d_dprefix, void* d_dP, int B, int T,
-                                   int n_prefix, int d, int64_t n_pos, int dtype, void* stream) {
-  const int st = check_sizes(B, T, n_prefix, d, dtype);
-  if (st != TMAC_OK) return st;
-  if (n_pos < 0 || n_pos > kMaxRows || ldg < d || (d_dP && n_pos < T)) return TMAC_ERR_SHAPE;
-  // rows [first, last) of [prefix | positions]
-  const int first = d_dprefix ? 0 : n_prefix, last = n_prefix + (d_dP ? static_cast<int>(n_pos) : 0);
-  if (first >= last) return TMAC_OK;
-  if (B > 0 && !d_g) return TMAC_ERR_NULL;
-  const bool wide = d % (dtype == TMAC_F32 ? 4 : 8) == 0 && row_aligned16(d_dprefix) && row_aligned16(d_dP) &&
-                    wide_rows(d_g, ldg, dtype);
-  dispatch(dtype, wide, [&](auto dt, auto n) {
-    constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
-    const int cpr = d / N, rpb = rows_per_block(last - first, cpr, 1);
-    embed_pos_grad_kernel<DT, N><<<(last - first + rpb - 1) / rpb, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-        static_cast<const uint8_t*>(d_g), ldg, static_cast<uint8_t*>(d_dprefix), static_cast<uint8_t*>(d_dP), B, T,
-        n_prefix, d, first, last, cpr, rpb);
-  });
+  // three launches by sorted tokens (`out`), one for the sums alone
+  auto part = [&](const int64_t* index, void* out, int64_t n_rows, float factor, bool with_sums) {
+    Grad a{};
+    a.g = static_cast<const uint8_t*>(d_g);
+    a.ldg = ldg;
+    a.d = d;
+    a.B = B;
+    a.T = T;
+    a.Np = n_prefix;
+    if (with_sums) {
+      a.dprefix = static_cast<uint8_t*>(d_dprefix);
+      a.dP = sums ? static_cast<uint8_t*>(d_dP) : nullptr;
+      a.first = d_dprefix ? 0 : n_prefix;
+      a.last = n_prefix + (sums ? static_cast<int>(n_pos) : 0);
+    }
+    if (out) {
+      uint8_t* const ws = static_cast<uint8_t*>(d_ws);
+      const GradWs w = grad_ws(n_tok, n_rows, d);
+      int32_t* const row_start = reinterpret_cast<int32_t*>(ws);
+      int32_t* const perm = reinterpret_cast<int32_t*>(ws + w.perm);
+      int32_t* const key = reinterpret_cast<int32_t*>(ws + w.key);
+      a.row_start = row_start;
+      a.perm = perm;
+      a.key = key;
+      a.part = reinterpret_cast<float*>(ws + w.part);
+      a.dW = static_cast<uint8_t*>(out);
+      a.V = static_cast<int>(n_rows);
+      a.scale = factor;
+      a.chunks = n_tok > kList ? (n_tok + kList - 1) / kList : 0;
+      const uint32_t T_inv = T > 1 ? static_cast<uint32_t>((1ull << 32) / static_cast<uint32_t>(T)) : 0;
+      auto sort = [&](auto held) {
+        embed_sort_kernel<decltype(held)::value><<<n_ranges(a.V), 64 * kSortWaves, 0, s>>>(
+            index, n_tok, T, T_inv, n_prefix, a.V, row_start, perm, key);
+      };
+      if (n_tok <= 4 * 64 * kSortWaves)
+        sort(std::integral_constant<int, 4>{});
+      else
+        sort(std::integral_constant<int, 0>{});
+    }
+    dispatch(dtype, wide, [&](auto dt, auto n) {
+      constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
+      a.cpr = d / N;
+      a.rpb = rows_per_block(a.cpr, 4);
+      a.pos_rpb = rows_per_block(a.cpr, 1);
+      a.row_blocks = (a.V + a.rpb - 1) / a.rpb;
+      a.pos_blocks = a.last > a.first ? (a.last - a.first + a.pos_rpb - 1) / a.pos_rpb : 0;
+      const int64_t blocks = static_cast<int64_t>(a.chunks) + a.pos_blocks + a.row_blocks;
+      if (!blocks) return;
+      embed_grad_kernel<DT, N><<<grid(blocks), kThreads, 0, s>>>(a);
+      if (a.chunks)
+        embed_grad_long_kernel<DT, N><<<grid((a.chunks + kLongChunks - 1) / kLongChunks), 1024, 0, s>>>(a);
+    });
+  };
+  const bool any_sums = sums || d_dprefix;
+  if (d_dW)
+    part(d_ids, d_dW, V, scale, any_sums);
+  else if (any_sums)
+    part(nullptr, nullptr, 0, 1.f, true);
+  if (d_dP && d_pos) part(d_pos, d_dP, n_pos, 1.f, false);
   return launch_status();
 }

@@ -12,6 +12,7 @@ sorted by id and each row's sum is formed in order (deterministic, fp32) and wri
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -63,7 +64,9 @@ def _check(ids, weight, pos_weight, positions, prefix) -> None:
 
 
 def _index(t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
-    return None if t is None else t.expand(like.shape).to(torch.int64).contiguous()
+    if t is None or t.dtype == torch.int64 and t.shape == like.shape and t.is_contiguous():
+        return t
+    return t.expand(like.shape).to(torch.int64).contiguous()
 
 
 def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor],
@@ -97,6 +100,15 @@ def _(ids, weight, pos_weight, positions, prefix, scale):
     return weight.new_empty((ids.shape[0], n_prefix + ids.shape[1], weight.shape[1]))
 
 
+@lru_cache(maxsize=256)
+def _workspace(n_tokens: int, V: int, n_pos: int, d: int) -> int:
+    if V == 0 and n_pos == 0:
+        return 0
+    nb = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().tmac_embed_bwd_workspace(n_tokens, V, n_pos, d, ctypes.byref(nb)), "tmac_embed_bwd_workspace")
+    return nb.value
+
+
 def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optional[torch.Tensor], n_prefix: int,
                          V: int, n_pos: int, scale: float, need_w: bool, need_p: bool,
                          need_f: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -104,30 +116,18 @@ def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optio
     not needed."""
     dev = _lib.require_device(*(t for t in (grad, ids, positions) if t is not None), what="token_embedding backward")
     (B, T), d = ids.shape, int(grad.shape[-1])
-    code, L = _lib.dtype_code(grad.dtype), _lib.lib()
     g = _rows(grad)
     dw, dp, df = (grad.new_empty((n if need else 0, d))
                   for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
-
-    def by_sorted(index, out, factor):
-        nb = ctypes.c_size_t(0)
-        _lib.check(L.tmac_embed_grad_workspace(B * T, out.shape[0], d, ctypes.byref(nb)), "tmac_embed_grad_workspace")
-        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev)
-        _lib.check(L.tmac_embed_grad(_lib.ptr(index), _lib.ptr(g), max(g.stride(0), d), _lib.ptr(out), _lib.ptr(ws),
-                                     nb.value, B, T, n_prefix, d, out.shape[0], factor, code,
-                                     _lib.stream_ptr(dev)), "tmac_embed_grad")
-
+    i, q = _index(ids, ids), _index(positions, ids) if need_p else None
+    nb = _workspace(B * T, V if need_w else 0, n_pos if q is not None else 0, d)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     with _lib.device_guard(dev):
-        if need_w:
-            by_sorted(_index(ids, ids), dw, scale)
-        if need_p and positions is not None:
-            by_sorted(_index(positions, ids), dp, 1.0)
-        by_sum = need_p and positions is None
-        if by_sum or need_f:
-            _lib.check(L.tmac_embed_pos_grad(_lib.ptr(g), max(g.stride(0), d), _lib.ptr(df) if need_f else 0,
-                                             _lib.ptr(dp) if by_sum else 0, B, T, n_prefix, d,
-                                             n_pos if by_sum else 0, code, _lib.stream_ptr(dev)),
-                       "tmac_embed_pos_grad")
+        rc = _lib.lib().tmac_embed_bwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(g), max(g.stride(0), d),
+                                       _lib.ptr(dw) if need_w else 0, _lib.ptr(dp) if need_p else 0,
+                                       _lib.ptr(df) if need_f and n_prefix else 0, _lib.ptr(ws), nb, B, T, n_prefix, d,
+                                       V, n_pos, scale, _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "tmac_embed_bwd")
     return dw, dp, df
 
 
