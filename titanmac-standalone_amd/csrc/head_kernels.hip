@@ -174,7 +174,8 @@ __global__ __launch_bounds__(256, 2) void head_kernel(
   Stat* const sh = reinterpret_cast<Stat*>(smem);
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
-    stat_join(stat[mi], stat_shfl(stat[mi], 32));
+    const Stat& a = stat[mi];
+    stat_join(stat[mi], Stat{lane_xor<32>(a.m), lane_xor<32>(a.mu), lane_xor<32>(a.s), lane_xor<32>(a.h)});
     if (wn == 1 && h == 0) sh[32 * MI * wm + 32 * mi + l32] = stat[mi];
   }
   __syncthreads();
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(const Part* __restrict__
     const Part q = parts[static_cast<int64_t>(p) * M + row];
     stat_join(a, Stat{q.m, q.m == -__builtin_inff() ? 0.f : q.m, q.s, q.h});
   }
-  for (int o = 32; o > 0; o >>= 1) stat_join(a, stat_shfl(a, o));
+  stat_wave(a);
   if (lane) return;
   const float log_s = __builtin_amdgcn_logf(a.s) * kLn2;
   const int64_t t = targets[row];

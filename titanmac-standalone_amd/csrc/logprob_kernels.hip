@@ -14,10 +14,14 @@
 // over the vocabulary and a second kernel joins the parts.
 //
 // Alternatives, without a second pass over the row: beside m each thread keeps the group where it first
-// saw it. Order the threads by (m, earlier group): the k best values lie with the first k threads, since
-// any other thread's best, and so all it has, comes after k threads' bests. Their groups, k of 1024th of
-// the row, are read again, and those not below the k-th thread's best are sorted: at most a few dozen
-// for ordinary rows, any number of them in rounds that keep the best 64.
+// saw it, and the best value of its other groups. Order the threads by (m, earlier group), and take any
+// place in that order that k threads reach: the k best values lie with the threads up to it, since all that
+// another one has comes after k threads' bests. The place is the k-th of 64 that the waves publish (an
+// equal share each: for k up to 8 the k-th of all). Of those threads the best group is read again, 16 bytes
+// of a line each, and the others only where their best reaches the bound too (a thread's groups are
+// strewn over the row, so that reading all of them costs k / 512 of the row's groups but an eighth of its
+// lines for k = 8). What reaches the bound is sorted: a few dozen entries for ordinary rows, any number
+// in rounds that keep the best 64.
 //
 // m and s are kept for the backward, p = e^{z − m} / s: through lse the rounding of a sum near 12 would
 // go into every p.
@@ -29,7 +33,7 @@ using namespace tmac;
 namespace {
 
 constexpr int kMaxTop = 64;
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 2;
 
 // (value, index) as one whole number: larger value first, then lower index; 0 is no entry.
 __device__ __forceinline__ uint64_t top_key(float z, int idx) {
@@ -43,37 +47,37 @@ __device__ __forceinline__ float key_value(uint64_t k) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int x) {
-  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), x);
-  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(v >> 32), x);
-  return static_cast<uint64_t>(hi) << 32 | lo;
-}
-// lanes i and i ^ j exchange so that the larger value is at the lower lane (desc) or the higher
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, int j, bool desc) {
-  const uint64_t o = shfl_xor64(v, j);
-  const bool low = (lane & j) == 0;
+// lanes i and i ^ J exchange so that the larger value is at the lower lane (desc) or the higher
+template <int J>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, bool desc) {
+  const uint64_t o = lane_xor<J>(v);
+  const bool low = (lane & J) == 0;
   return (v > o) == (low == desc) ? v : o;
+}
+template <int J>
+__device__ __forceinline__ uint64_t exchanges(uint64_t v, int lane, bool desc) {
+  v = exchange<J>(v, lane, desc);
+  if constexpr (J > 1) v = exchanges<J / 2>(v, lane, desc);
+  return v;
 }
 // bitonic sort of a wave's 64 keys, descending
 __device__ __forceinline__ uint64_t wave_sort(uint64_t v, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) v = exchange(v, lane, j, (lane & k) == 0);
-  return v;
+  v = exchanges<1>(v, lane, (lane & 2) == 0);
+  v = exchanges<2>(v, lane, (lane & 4) == 0);
+  v = exchanges<4>(v, lane, (lane & 8) == 0);
+  v = exchanges<8>(v, lane, (lane & 16) == 0);
+  v = exchanges<16>(v, lane, (lane & 32) == 0);
+  return exchanges<32>(v, lane, true);
 }
 // the 64 largest of two descending lists, descending; b is given reversed
 __device__ __forceinline__ uint64_t wave_merge(uint64_t a, uint64_t b_rev, int lane) {
-  uint64_t v = a > b_rev ? a : b_rev;
-#pragma unroll
-  for (int j = 32; j > 0; j >>= 1) v = exchange(v, lane, j, true);
-  return v;
+  return exchanges<32>(a > b_rev ? a : b_rev, lane, true);
 }
 
-// buf[0 .. n) -> its 64 largest in buf[0 .. 64), descending, 0 where there are fewer; n <= NT, by all of
-// the workgroup's NT threads.
+// The 64 largest of buf[0 .. n), n <= NT, in descending order in the lanes of wave 0 (0 where there are fewer);
+// by all of the workgroup's NT threads, which have written buf before a barrier.
 template <int NT>
-__device__ void block_top(uint64_t* buf, int n) {
+__device__ uint64_t block_top(uint64_t* buf, int n) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   uint64_t v = tid < n ? buf[tid] : 0;
   const int waves = (n + 63) / 64;
@@ -84,9 +88,7 @@ __device__ void block_top(uint64_t* buf, int n) {
     __syncthreads();
     if (wave % (2 * half) == 0 && wave + half < waves) v = wave_merge(v, buf[64 * (wave + half) + 63 - lane], lane);
   }
-  __syncthreads();
-  if (wave == 0) buf[lane] = v;
-  __syncthreads();
+  return v;
 }
 
 // A row of V values seen as groups of N that are 16-byte aligned: group q holds elements q N − o ..
@@ -106,104 +108,123 @@ __device__ __forceinline__ Groups row_groups(const uint8_t* row, int V) {
   return g;
 }
 
-constexpr int kTopBuf = 64;  // entries kept between rounds
+// What a thread saw of its groups: the best value, the first group that has it (−1: no entry), and the best
+// value of its other groups.
+struct Best {
+  float m, second;
+  int group;
+};
+__device__ __forceinline__ void best_add(Best& a, float m, int group) {
+  a.second = __builtin_amdgcn_fmed3f(a.m, a.second, m);  // second <= m of a
+  if (a.group < 0 || m > a.m) a.group = group;
+  a.m = fmaxf(a.m, m);
+}
 
 template <int NT>
 struct TopShared {
-  uint64_t buf[NT + kTopBuf];
-  int count;
+  uint64_t buf[NT];
+  uint64_t bests[64];   // the waves' highest threads' bests, an equal number of each wave's
+  int group[NT];        // every thread's best group
+  uint16_t thread[NT];  // the threads whose best is among what may be the k best
+  uint16_t again[NT];   // those of them whose other groups have to be looked at too
+  int threads, agains, count;
 };
 
-// The workgroup's k best entries of its groups [q0, q1) of a row, into buf[0 .. k), given each thread's best
-// value `m` and the group `arg` of its first one (arg < 0: the thread saw none).
+// First part of the alternatives, before a barrier.
+template <int NT>
+__device__ __forceinline__ void top_publish(TopShared<NT>& sh, const Best& best) {
+  constexpr int kShare = 64 * 64 / NT;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const uint64_t v = wave_sort(best.group >= 0 ? top_key(best.m, best.group) : 0, lane);
+  if (lane < kShare) sh.bests[(tid >> 6) * kShare + lane] = v;
+  sh.group[tid] = best.group;
+  if (tid == 0) sh.threads = sh.agains = sh.count = 0;
+}
+
+// Second part, after it: the k best entries of the workgroup's groups [q0, q1) of a row, in wave 0's lanes.
 template <int DT, int NT>
-__device__ void block_row_top(TopShared<NT>& sh, const uint8_t* row, int V, const Groups& g, int q0, int q1, int k,
-                              float m, int arg) {
+__device__ uint64_t top_entries(TopShared<NT>& sh, const uint8_t* row, int V, const Groups& g, int q0, int q1, int k,
+                                const Best& best) {
   constexpr int N = kRowVec<DT>, E = kRowSize<DT>;
-  const int tid = threadIdx.x;
-  // thread bests by their group's number; unique, since groups are
-  sh.buf[tid] = arg >= 0 ? top_key(m, arg) : 0;
-  __syncthreads();
-  block_top<NT>(sh.buf, NT);
-  // the group of the k-th thread's best, or of the last if there are fewer threads with entries
-  uint64_t kth = sh.buf[k - 1];
-  int n_thr = k;
-  if (!kth) {
-    n_thr = 0;
-    while (sh.buf[n_thr]) ++n_thr;
+  const int tid = threadIdx.x, lane = tid & 63;
+  // the k-th of the published bests is reached by k threads: every other thread's entries come after those
+  const uint64_t sorted = wave_sort(sh.bests[lane], lane);
+  const uint64_t bound = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(sorted >> 32), k - 1)) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(sorted), k - 1));
+  // nor is an entry of the k best below its value, or, at that value, behind its group; with no bound every
+  // entry may be among them
+  const uint32_t last = bound ? static_cast<uint32_t>((key_index(bound) + 1) * N - 1 - g.o) : ~0u;
+  const uint64_t floor_key = bound ? (bound & ~0xffffffffull) | static_cast<uint32_t>(~last) : 1;
+  const float floor_value = bound ? key_value(bound) : -__builtin_inff();
+  if (best.group >= 0 && top_key(best.m, best.group) >= bound) {
+    sh.thread[atomicAdd(&sh.threads, 1)] = static_cast<uint16_t>(tid);
+    if (best.second >= floor_value) sh.again[atomicAdd(&sh.agains, 1)] = static_cast<uint16_t>(tid);
   }
-  // an entry of the k best is not below the k-th best's value, nor, at that value, behind its group
-  const uint64_t floor_key = kth ? (kth & ~0xffffffffull) |
-                                       static_cast<uint32_t>(~((key_index(kth) + 1) * N - 1 - g.o))
-                                 : 1;
-  __shared__ int s_thr[kMaxTop];
-  if (tid < n_thr) s_thr[tid] = (key_index(sh.buf[tid]) - q0) % NT;
+  __syncthreads();
+  // item i: a group that those threads saw, their best one first (−1 and less: none)
+  const int per = (q1 - q0 + NT - 1) / NT, n_thr = sh.threads;  // groups a thread has, at most
+  const int items = n_thr + sh.agains * per;
+  auto group = [&](int i) {
+    if (i < n_thr) return sh.group[sh.thread[i]];
+    i -= n_thr;
+    const int t = i / per, q = q0 + sh.again[t] + (i - t * per) * NT;
+    return q < q1 && q != sh.group[sh.again[t]] ? q : -1;
+  };
+  auto add = [&](float z, int idx) {
+    if (z >= floor_value) {
+      const uint64_t kk = top_key(z, idx);
+      if (kk >= floor_key) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < NT) sh.buf[at] = kk;
+      }
+    }
+  };
+  for (int i = tid; i < items; i += NT) {
+    const int q = group(i);
+    if (q < 0) continue;
+    const int first = q * N - g.o;
+    const uint8_t* const at = row + static_cast<int64_t>(first) * E;
+    if (q >= g.full0 && q < g.full1) {
+      float z[N];
+      row_load<DT, N>(at, z);
+#pragma unroll
+      for (int e = 0; e < N; ++e) add(z[e], first + e);
+    } else {
+      for (int e = max(0, -first); e < N && first + e < V; ++e) {
+        float z[1];
+        row_load<DT, 1>(at + e * E, z);
+        add(z[0], first + e);
+      }
+    }
+  }
+  __syncthreads();
+  const int total = sh.count;
+  if (total <= NT) return block_top<NT>(sh.buf, total);
+  // too many: again, the e-th values of half of the threads at a time beside the best 64 so far
+  __syncthreads();
   if (tid == 0) sh.count = 0;
-  __syncthreads();
-  const int per = (q1 - q0 + NT - 1) / NT;  // groups a thread has, at most
-  int n = 0;                                // entries in buf, the same in every thread
-  for (int64_t i0 = 0; i0 < static_cast<int64_t>(n_thr) * per; i0 += NT) {
-    const int64_t i = i0 + tid;
-    uint64_t key[N];
-    int mine = 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) key[e] = 0;
-    if (i < static_cast<int64_t>(n_thr) * per) {
-      const int64_t q = q0 + s_thr[i / per] + static_cast<int64_t>(i % per) * NT;
-      if (q < q1) {
-        const int first = static_cast<int>(q * N - g.o);
-        for (int e = 0; e < N; ++e) {
-          const int idx = first + e;
-          if (idx < 0 || idx >= V) continue;
-          float z[1];
-          row_load<DT, 1>(row + static_cast<int64_t>(idx) * E, z);
-          const uint64_t kk = top_key(z[0], idx);
-          if (kk >= floor_key) {
-            key[e] = kk;
-            ++mine;
-          }
-        }
+  for (int i0 = 0; i0 < items; i0 += NT) {
+    const int q = i0 + tid < items ? group(i0 + tid) : -1;
+#pragma unroll 1
+    for (int round = 0; round < 2 * N; ++round) {
+      const int idx = q * N - g.o + (round >> 1);
+      __syncthreads();
+      if (q >= 0 && (tid & 1) == (round & 1) && idx >= 0 && idx < V) {
+        float z[1];
+        row_load<DT, 1>(row + static_cast<int64_t>(idx) * E, z);
+        add(z[0], idx);
       }
-    }
-    if (mine) atomicAdd(&sh.count, mine);
-    __syncthreads();
-    const int total = sh.count;
-    __syncthreads();
-    if (n + total <= NT) {
-      if (tid == 0) sh.count = n;
       __syncthreads();
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (key[e]) sh.buf[atomicAdd(&sh.count, 1)] = key[e];
-      n += total;
+      const int n = sh.count;
+      if (n <= 64) continue;
+      const uint64_t v = block_top<NT>(sh.buf, n);
       __syncthreads();
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      continue;
+      if (tid < 64) sh.buf[tid] = v;
+      if (tid == 0) sh.count = 64;
     }
-    // too many at once: half of the threads' e-th values at a time beside the best 64 so far
-    for (int e = 0; e < N; ++e) {
-      for (int half = 0; half < 2; ++half) {
-        if (n > 64) {
-          block_top<NT>(sh.buf, n);
-          n = 64;
-        }
-        if (tid == 0) sh.count = n;
-        __syncthreads();
-        uint64_t kk = 0;
-#pragma unroll
-        for (int u = 0; u < N; ++u)
-          if (u == e) kk = key[u];
-        if (kk && (tid & 1) == half) sh.buf[atomicAdd(&sh.count, 1)] = kk;
-        __syncthreads();
-        n = sh.count;
-        __syncthreads();
-      }
-    }
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
   }
-  block_top<NT>(sh.buf, n);
+  __syncthreads();
+  return block_top<NT>(sh.buf, sh.count);
 }
 
 struct Row2 {
@@ -258,7 +279,7 @@ __device__ __forceinline__ void logprob_part(const uint8_t* __restrict__ z, cons
                                              uint64_t* __restrict__ ws_top, int block) {
   constexpr int N = kRowVec<DT>, E = kRowSize<DT>, U = kUnroll;
   const int row = block / parts, part = block - row * parts;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x;
   const int64_t target = targets[row];
   const uint8_t* const zp = z + row_offset(zr, row) * E;
   if (!ENT && !TOP && target == ignore) {  // nothing of this row is asked
@@ -273,20 +294,19 @@ __device__ __forceinline__ void logprob_part(const uint8_t* __restrict__ z, cons
   const int per = (g.n + parts - 1) / parts;
   const int q0 = min(part * per, g.n), q1 = min(q0 + per, g.n);
   Stat a = stat_none();
-  int arg = -1;
+  Best best{-__builtin_inff(), -__builtin_inff(), -1};
 
   auto take = [&](int q) {  // a group that is not whole, value by value
     const int first = q * N - g.o;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int idx = first + e;
-      if (idx < 0 || idx >= V) continue;
+    float m = -__builtin_inff();
+    for (int e = max(0, -first); e < N && first + e < V; ++e) {
       float x[1];
-      row_load<DT, 1>(zp + static_cast<int64_t>(idx) * E, x);
-      if (TOP && (arg < 0 || x[0] > a.m)) arg = q;
+      row_load<DT, 1>(zp + static_cast<int64_t>(first + e) * E, x);
+      m = fmaxf(m, x[0]);
       stat_raise(a, x[0]);
       stat_add<ENT>(a, x[0]);
     }
+    if (TOP) best_add(best, m, q);
   };
   int q = q0 + tid;
   if (q < q1 && q < g.full0) {
@@ -309,12 +329,9 @@ __device__ __forceinline__ void logprob_part(const uint8_t* __restrict__ z, cons
     float m = gm[0];
 #pragma unroll
     for (int u = 1; u < U; ++u) m = fmaxf(m, gm[u]);
-    if (TOP && (arg < 0 || m > a.m)) {
-      int first = 0;
+    if (TOP) {
 #pragma unroll
-      for (int u = U - 1; u >= 0; --u)
-        if (gm[u] == m) first = u;
-      arg = q + first * NT;
+      for (int u = 0; u < U; ++u) best_add(best, gm[u], q + u * NT);
     }
     stat_raise(a, m);
 #pragma unroll
@@ -328,7 +345,7 @@ __device__ __forceinline__ void logprob_part(const uint8_t* __restrict__ z, cons
     float m = v[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) m = fmaxf(m, v[e]);
-    if (TOP && (arg < 0 || m > a.m)) arg = q;
+    if (TOP) best_add(best, m, q);
     stat_raise(a, m);
 #pragma unroll
     for (int e = 0; e < N; ++e) stat_add<ENT>(a, v[e]);
@@ -336,40 +353,32 @@ __device__ __forceinline__ void logprob_part(const uint8_t* __restrict__ z, cons
   if (q < q1) take(q);
 
   __shared__ Stat s_stat[NT / 64];
-  const float best = a.m;
-  for (int o = 32; o > 0; o >>= 1) stat_join(a, stat_shfl(a, o));
-  if (lane == 0) s_stat[wave] = a;
-  __syncthreads();
-  a = s_stat[0];
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) stat_join(a, s_stat[w]);
-
-  if (parts == 1) {
-    if (tid == 0) write_row<DT>(out, row, a, zp, target, ignore, V);
-  } else if (tid == 0) {
-    ws_stat[block] = a;
-  }
   if constexpr (TOP) {
     __shared__ TopShared<NT> sh;
-    const bool ok = a.s > 0.f && a.s < __builtin_inff();
+    top_publish<NT>(sh, best);
+    stat_block<NT / 64>(a, s_stat);
     // a part may hold nothing but −inf of a row that has a distribution (s = 0)
-    if (parts > 1 ? a.s < __builtin_inff() : ok) {
-      block_row_top<DT, NT>(sh, zp, V, g, q0, q1, k, best, arg);
-    } else {
-      sh.buf[tid] = 0;
-      __syncthreads();
-    }
+    uint64_t v = 0;
+    if (a.s < __builtin_inff() && (parts > 1 || a.s > 0.f)) v = top_entries<DT, NT>(sh, zp, V, g, q0, q1, k, best);
     if (tid < k) {
       if (parts == 1)
-        write_top(out, row, tid, k, a, sh.buf[tid]);
+        write_top(out, row, tid, k, a, v);
       else
-        ws_top[static_cast<int64_t>(block) * k + tid] = sh.buf[tid];
+        ws_top[static_cast<int64_t>(block) * k + tid] = v;
     }
+  } else {
+    stat_block<NT / 64>(a, s_stat);
+  }
+  if (tid == 0) {
+    if (parts == 1)
+      write_row<DT>(out, row, a, zp, target, ignore, V);
+    else
+      ws_stat[block] = a;
   }
 }
 
 template <int DT, bool ENT, bool TOP, int NT>
-__global__ __launch_bounds__(NT) void logprob_kernel(const uint8_t* __restrict__ z, Row2 zr,
+__global__ __launch_bounds__(NT, 8) void logprob_kernel(const uint8_t* __restrict__ z, Row2 zr,
                                                      const int64_t* __restrict__ targets, int64_t ignore, int V,
                                                      int k, int parts, Out out, Stat* __restrict__ ws_stat,
                                                      uint64_t* __restrict__ ws_top, int blocks) {
@@ -399,28 +408,24 @@ __global__ __launch_bounds__(NT) void logprob_join_kernel(const uint8_t* __restr
   __shared__ Stat s_stat[NT / 64];
   Stat a = stat_none();
   for (int p = tid; p < parts; p += NT) stat_join(a, ws_stat[static_cast<int64_t>(row) * parts + p]);
-  for (int o = 32; o > 0; o >>= 1) stat_join(a, stat_shfl(a, o));
-  if (lane == 0) s_stat[wave] = a;
-  __syncthreads();
-  a = s_stat[0];
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) stat_join(a, s_stat[w]);
+  stat_block<NT / 64>(a, s_stat);
   if (tid == 0)
     write_row<DT>(out, row, a, z + row_offset(zr, row) * kRowSize<DT>, target, ignore, V);
   if (k) {
+    // each wave merges its parts' descending lists, then the waves' lists
     __shared__ uint64_t buf[NT];
-    // 64 kept, NT - 64 new ones a round
-    const int total = parts * k;
-    const uint64_t* const from = ws_top + static_cast<int64_t>(row) * total;
-    buf[tid] = 0;
-    __syncthreads();
-    for (int i0 = 0; i0 < total; i0 += NT - 64) {
-      const int i = i0 + tid - 64;
-      if (tid >= 64) buf[tid] = i < total ? from[i] : 0;
-      __syncthreads();
-      block_top<NT>(buf, NT);
+    uint64_t v = 0;
+    for (int p = wave; p < parts; p += NT / 64) {
+      const uint64_t* const from = ws_top + (static_cast<int64_t>(row) * parts + p) * k;
+      v = wave_merge(v, 63 - lane < k ? from[63 - lane] : 0, lane);
     }
-    if (tid < k) write_top(out, row, tid, k, a, buf[tid]);
+    for (int half = 1; half < NT / 64; half *= 2) {
+      buf[tid] = v;
+      __syncthreads();
+      if (wave % (2 * half) == 0) v = wave_merge(v, buf[64 * (wave + half) + 63 - lane], lane);
+      __syncthreads();
+    }
+    if (tid < k) write_top(out, row, tid, k, a, v);
   }
 }
 
@@ -546,7 +551,10 @@ __global__ __launch_bounds__(1024) void logprob_mean_kernel(const float* __restr
 
 constexpr int64_t kMaxRows = 1 << 30, kMaxV = 1 << 28;
 constexpr int kMaxGrid = 1 << 21;    // workgroups of a launch; they take turns beyond that
-constexpr int kShortRow = 32 << 10;  // bytes of a row below which 256 threads take it
+// Threads of a row: 128 below 32 KB (us, 128 / 256 / 512 threads: 20000 rows of 1000 bf16 18 / 28 / 50, 8000 of
+// 8000 24 / 24 / 31), then 512 (8192 of 128000: 382 / 351 / 344), with alternatives 256 (4096 of 128000: five of
+// them 201 / 197 / 214, twenty 209 / 200 / 218, 64 568 / 243 / 230).
+constexpr int kShortRow = 32 << 10;
 
 int check(int B, int T, int64_t V, int64_t st, int64_t sb, int dtype) {
   if (dtype != TMAC_F32 && dtype != TMAC_BF16 && dtype != TMAC_F16) return TMAC_ERR_DTYPE;
@@ -560,11 +568,12 @@ int launch_status() {
   return err == hipSuccess ? TMAC_OK : static_cast<int>(err);
 }
 
-// Workgroups per row: enough of them for the chip, of at least 2048 groups (32 KB) of the row each.
+// Workgroups per row: about 1024 in all, of at least 1024 groups (16 KB) of the row each. One row of 128000 fp32
+// with 64 alternatives: 13.4 us, with 512 or 256 groups 15.2 and 18.6 (more lists to join).
 int row_parts(int rows, int64_t V, int dtype) {
   const int64_t groups = (V + (dtype == TMAC_F32 ? 3 : 7)) / (dtype == TMAC_F32 ? 4 : 8);
-  int64_t parts = 512 / (rows > 0 ? rows : 1);
-  const int64_t most = groups / 512;
+  int64_t parts = 1024 / (rows > 0 ? rows : 1);
+  const int64_t most = groups / 1024;
   if (parts > most) parts = most;
   return static_cast<int>(parts < 1 ? 1 : parts);
 }
@@ -630,16 +639,19 @@ extern "C" int tmac_logprob_fwd(const void* d_z, int64_t stride_b, int64_t strid
       by_flag(top_k > 0, [&](auto t) {
         constexpr bool ENT = decltype(e)::value, TOP = decltype(t)::value;
         const int blocks = rows * parts, grid = blocks < kMaxGrid ? blocks : kMaxGrid;
-        if (parts > 1 || V * E < kShortRow)
-          logprob_kernel<DT, ENT, TOP, 256><<<grid, 256, 0, s>>>(z, zr, d_targets, ignore_index, v, top_k, parts, out,
-                                                                 ws_stat, ws_top, blocks);
+        auto launch = [&](auto nt) {
+          constexpr int NT = decltype(nt)::value;
+          logprob_kernel<DT, ENT, TOP, NT><<<grid, NT, 0, s>>>(z, zr, d_targets, ignore_index, v, top_k, parts, out,
+                                                               ws_stat, ws_top, blocks);
+        };
+        if (parts == 1 && V * E < kShortRow)
+          launch(std::integral_constant<int, 128>{});
         else
-          logprob_kernel<DT, ENT, TOP, 1024><<<grid, 1024, 0, s>>>(z, zr, d_targets, ignore_index, v, top_k, 1, out,
-                                                                   ws_stat, ws_top, blocks);
+          launch(std::integral_constant<int, TOP ? 256 : 512>{});
       });
     });
     if (parts > 1)
-      logprob_join_kernel<DT, 256><<<rows, 256, 0, s>>>(z, zr, d_targets, ignore_index, v, top_k, parts,
+      logprob_join_kernel<DT, 512><<<rows, 512, 0, s>>>(z, zr, d_targets, ignore_index, v, top_k, parts,
                                                         !d_entropy && !top_k, out, ws_stat, ws_top);
   });
   return launch_status();

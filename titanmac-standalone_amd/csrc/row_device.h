@@ -78,6 +78,75 @@ __device__ __forceinline__ void stat_add(Stat& a, float z) {
   a.s += e;
   if (ENT) a.h = fmaf(e, fmaxf(d, kFar), a.h);
 }
+// The value of lane (lane ^ J), on the vector ALU: quad permutes and mirrors of 8 and 16 lanes, whose
+// compositions are the exchanges by 4 and 8, and the swaps of rows and halves, which return a lane's
+// own value and the other's in an order that depends on the lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_dpp(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0u, x, CTRL, 0xf, 0xf, true);
+}
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  constexpr int kMirror = 0x140, kHalfMirror = 0x141, kReverse4 = 0x1b;
+  if constexpr (J == 1) {
+    return lane_dpp<0xb1>(x);  // 1, 0, 3, 2
+  } else if constexpr (J == 2) {
+    return lane_dpp<0x4e>(x);  // 2, 3, 0, 1
+  } else if constexpr (J == 4) {
+    return lane_dpp<kReverse4>(lane_dpp<kHalfMirror>(x));
+  } else if constexpr (J == 8) {
+    return lane_dpp<kHalfMirror>(lane_dpp<kMirror>(x));
+  } else if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return r[0] ^ r[1] ^ x;
+  } else {
+    static_assert(J == 32, "a power of two below 64");
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return r[0] ^ r[1] ^ x;
+  }
+}
+template <int J>
+__device__ __forceinline__ float lane_xor(float x) {
+  return __uint_as_float(lane_xor<J>(__float_as_uint(x)));
+}
+template <int J>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t x) {
+  return static_cast<uint64_t>(lane_xor<J>(static_cast<uint32_t>(x >> 32))) << 32 |
+         lane_xor<J>(static_cast<uint32_t>(x));
+}
+__device__ __forceinline__ float lanes_max(float x) {
+  x = fmaxf(x, lane_xor<1>(x));
+  x = fmaxf(x, lane_xor<2>(x));
+  x = fmaxf(x, lane_xor<4>(x));
+  x = fmaxf(x, lane_xor<8>(x));
+  x = fmaxf(x, lane_xor<16>(x));
+  return fmaxf(x, lane_xor<32>(x));
+}
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+  x = max(x, lane_xor<1>(x));
+  x = max(x, lane_xor<2>(x));
+  x = max(x, lane_xor<4>(x));
+  x = max(x, lane_xor<8>(x));
+  x = max(x, lane_xor<16>(x));
+  return max(x, lane_xor<32>(x));
+}
+__device__ __forceinline__ float lanes_sum(float x) {
+  x += lane_xor<1>(x);
+  x += lane_xor<2>(x);
+  x += lane_xor<4>(x);
+  x += lane_xor<8>(x);
+  x += lane_xor<16>(x);
+  return x + lane_xor<32>(x);
+}
+
+// a's sums moved to the maximum m >= a.m; where a has no term above −inf they are 0 (or NaN)
+__device__ __forceinline__ void stat_rescale(Stat& a, float m) {
+  const float d = a.m == -__builtin_inff() ? 0.f : fmaxf(a.m - m, kFar), f = exp_d(d);
+  a.h = f * fmaf(a.s, d, a.h);
+  a.s *= f;
+  a.m = m;
+  a.mu = m == -__builtin_inff() ? 0.f : m;
+}
 __device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
   stat_raise(a, b.m);
   // b's terms at a's maximum; where b has none above −inf it has s = h = 0 (or NaN)
@@ -85,8 +154,29 @@ __device__ __forceinline__ void stat_join(Stat& a, const Stat& b) {
   a.h = fmaf(f, fmaf(b.s, d, b.h), a.h);
   a.s = fmaf(f, b.s, a.s);
 }
-__device__ __forceinline__ Stat stat_shfl(const Stat& a, int x) {
-  return Stat{__shfl_xor(a.m, x), __shfl_xor(a.mu, x), __shfl_xor(a.s, x), __shfl_xor(a.h, x)};
+// the statistics of all 64 lanes, in every lane
+__device__ __forceinline__ void stat_wave(Stat& a) {
+  stat_rescale(a, lanes_max(a.m));
+  a.s = lanes_sum(a.s);
+  a.h = lanes_sum(a.h);
+}
+// and of the workgroup's waves, in every thread; sh: one entry per wave, read when this returns
+template <int WAVES>
+__device__ __forceinline__ void stat_block(Stat& a, Stat* sh) {
+  stat_wave(a);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+  __syncthreads();
+  float m = sh[0].m;
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) m = fmaxf(m, sh[w].m);
+  a = Stat{m, m == -__builtin_inff() ? 0.f : m, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    Stat b = sh[w];
+    stat_rescale(b, m);
+    a.s += b.s;
+    a.h += b.h;
+  }
 }
 
 inline bool row_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
