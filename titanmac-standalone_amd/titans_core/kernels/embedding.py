@@ -23,15 +23,15 @@ from .norm import _rows
 _INDEX = (torch.int64, torch.int32)
 
 
-def _table(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """A table whose rows the kernels can read (copied only if they cannot be)."""
-    if t is None or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
-        return t
-    return t.contiguous()
-
-
-def _pitch(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else max(t.stride(0), t.shape[1])
+def _table(t: Optional[torch.Tensor]):
+    """(a table whose rows the kernels can read, copied only if they cannot be; its row pitch)."""
+    if t is None:
+        return t, 0
+    n, d = t.shape
+    pitch, step = t.stride()
+    if (step != 1 and d > 1) or (pitch < d and n > 1):
+        return t.contiguous(), d
+    return t, max(pitch, d)
 
 
 def _check(ids, weight, pos_weight, positions, prefix) -> None:
@@ -82,11 +82,12 @@ def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Option
     out = torch.empty((B, n_prefix + T, d), dtype=weight.dtype, device=dev)
     if out.numel() == 0:
         return out
-    i, q, w, p, f = _index(ids, ids), _index(positions, ids), _table(weight), _table(pos_weight), _table(prefix)
+    i, q = _index(ids, ids), _index(positions, ids)
+    (w, ldw), (p, ldp), (f, ldf) = _table(weight), _table(pos_weight), _table(prefix)
     with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_embed_fwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(w), _pitch(w), _lib.ptr(p), _pitch(p),
-                                       _lib.ptr(f), _pitch(f), _lib.ptr(out), B, T, n_prefix, d, V,
-                                       0 if p is None else p.shape[0], scale, code, _lib.stream_ptr(dev))
+        rc = _lib.lib().tmac_embed_fwd(i.data_ptr(), _lib.ptr(q), w.data_ptr(), ldw, _lib.ptr(p), ldp, _lib.ptr(f), ldf,
+                                       out.data_ptr(), B, T, n_prefix, d, V, 0 if p is None else p.shape[0], scale,
+                                       code, _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_embed_fwd")
     return out
 
@@ -116,17 +117,18 @@ def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optio
     not needed."""
     dev = _lib.require_device(*(t for t in (grad, ids, positions) if t is not None), what="token_embedding backward")
     (B, T), d = ids.shape, int(grad.shape[-1])
-    g = _rows(grad)
-    dw, dp, df = (grad.new_empty((n if need else 0, d))
+    g = grad if grad.is_contiguous() else _rows(grad)
+    ldg = d if g is grad else max(g.stride(0), d)
+    dw, dp, df = (torch.empty((n if need else 0, d), dtype=grad.dtype, device=dev)
                   for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
     i, q = _index(ids, ids), _index(positions, ids) if need_p else None
     nb = _workspace(B * T, V if need_w else 0, n_pos if q is not None else 0, d)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_embed_bwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(g), max(g.stride(0), d),
-                                       _lib.ptr(dw) if need_w else 0, _lib.ptr(dp) if need_p else 0,
-                                       _lib.ptr(df) if need_f and n_prefix else 0, _lib.ptr(ws), nb, B, T, n_prefix, d,
-                                       V, n_pos, scale, _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
+        rc = _lib.lib().tmac_embed_bwd(i.data_ptr(), _lib.ptr(q), g.data_ptr(), ldg, dw.data_ptr() if need_w else 0,
+                                       dp.data_ptr() if need_p else 0, df.data_ptr() if need_f and n_prefix else 0,
+                                       ws.data_ptr(), nb, B, T, n_prefix, d, V, n_pos, scale,
+                                       _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_embed_bwd")
     return dw, dp, df
 

@@ -13,6 +13,7 @@ All sums and results are fp32; gradients have their input's dtype.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -44,51 +45,66 @@ def _check(logits: torch.Tensor, targets: torch.Tensor, what: str) -> None:
 
 
 def _rows3(z: torch.Tensor):
-    """(z as [B, T, V] whose rows the kernels can read, B, T, V): a view, copied only if its rows' values are not
-    neighbours or more than two strides lead to them."""
+    """(z whose rows the kernels can read, stride of B, stride of T, B, T, V), rows seen as [B, T, V]: in place,
+    copied only if their values are not neighbours or more than two strides lead to them."""
     V = z.shape[-1]
-    z = z.reshape(1, 1, V) if z.dim() == 1 else z.unsqueeze(0) if z.dim() == 2 else z
+    if z.is_contiguous():
+        return z, 0, V, 1, z.numel() // V, V
+    z = z.unsqueeze(0).unsqueeze(0) if z.dim() == 1 else z.unsqueeze(0) if z.dim() == 2 else z
     if z.dim() > 3:
-        z = z.reshape(1, -1, V) if z.numel() else z.reshape(0, 0, V)
+        z = z.reshape(1, -1, V)
     if V > 1 and z.stride(2) != 1:
         z = z.contiguous()
-    return z, int(z.shape[0]), int(z.shape[1]), int(V)
+    return z, z.stride(0), z.stride(1), z.shape[0], z.shape[1], V
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
-    return t.to(torch.int64).contiguous()
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
+
+
+@lru_cache(maxsize=256)
+def _workspace(B: int, T: int, V: int, top_k: int, code: int) -> int:
+    nb = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().tmac_logprob_workspace(B, T, V, top_k, code, ctypes.byref(nb)), "tmac_logprob_workspace")
+    return nb.value
 
 
 def _fwd(logits, targets, entropy, top_k, ignore_index, dev):
-    z, B, T, V = _rows3(logits)
-    lead, n = targets.shape, B * T
-    new = lambda shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=dev)  # noqa: E731
-    lp, stats = new(lead), new((n, 2))
-    ent = new(lead if entropy else (0,))
-    ids, top = new((*lead, top_k) if top_k else (0,), torch.int64), new((*lead, top_k) if top_k else (0,))
+    """(logprobs, entropy, top_ids, top_logprobs, stats), None for what is not asked."""
+    code = _lib.dtype_code(logits.dtype)
+    z, sb, st, B, T, V = _rows3(logits)
+    lead, n, f32 = targets.shape, B * T, torch.float32
+    lp, stats = torch.empty(lead, dtype=f32, device=dev), torch.empty((n, 2), dtype=f32, device=dev)
+    ent = torch.empty(lead, dtype=f32, device=dev) if entropy else None
+    ids = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
+    top = torch.empty((*lead, top_k), dtype=f32, device=dev) if top_k else None
     if n:
-        L, nb = _lib.lib(), ctypes.c_size_t(0)
-        code, tg = _lib.dtype_code(z.dtype), _flat(targets)
-        _lib.check(L.tmac_logprob_workspace(B, T, V, top_k, code, ctypes.byref(nb)), "tmac_logprob_workspace")
-        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev) if nb.value else None
+        nb, tg = _workspace(B, T, V, top_k, code), _flat(targets)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         with _lib.device_guard(dev):
-            rc = L.tmac_logprob_fwd(_lib.ptr(z), z.stride(0), z.stride(1), _lib.ptr(tg), ignore_index, _lib.ptr(lp),
-                                    _lib.ptr(ent) if entropy else 0, top_k, _lib.ptr(ids) if top_k else 0,
-                                    _lib.ptr(top) if top_k else 0, _lib.ptr(stats), _lib.ptr(ws), nb.value, B, T, V,
-                                    code, _lib.stream_ptr(dev))
+            rc = _lib.lib().tmac_logprob_fwd(z.data_ptr(), sb, st, tg.data_ptr(), ignore_index, lp.data_ptr(),
+                                             _lib.ptr(ent), top_k, _lib.ptr(ids), _lib.ptr(top), stats.data_ptr(),
+                                             _lib.ptr(ws), nb, B, T, V, code, _lib.stream_ptr(dev))
         _lib.check(rc, "tmac_logprob_fwd")
     return lp, ent, ids, top, stats
+
+
+def _check_call(logits, targets, top_k):
+    _check(logits, targets, "token_logprobs")
+    _lib.dtype_code(logits.dtype)
+    if not 0 <= top_k <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top_k must be in [0, {min(MAX_TOP, logits.shape[-1])}], got {top_k}")
+    return _lib.require_device(logits, targets, what="token_logprobs")
 
 
 def _logprob_fwd(logits: torch.Tensor, targets: torch.Tensor, entropy: bool, top_k: int, ignore_index: int
                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(logprobs, entropy, top_ids, top_logprobs, stats fp32 [rows, 2]); empty tensors for what is not asked."""
-    _check(logits, targets, "token_logprobs")
-    _lib.dtype_code(logits.dtype)
-    if not 0 <= top_k <= min(MAX_TOP, logits.shape[-1]):
-        raise ValueError(f"token_logprobs: top_k must be in [0, {min(MAX_TOP, logits.shape[-1])}], got {top_k}")
-    dev = _lib.require_device(logits, targets, what="token_logprobs")
-    return _fwd(logits, targets, entropy, top_k, ignore_index, dev)
+    dev = _check_call(logits, targets, top_k)
+    out = _fwd(logits, targets, entropy, top_k, ignore_index, dev)
+    # an operator's results are tensors
+    return tuple(torch.empty((0,), dtype=torch.int64 if i == 2 else torch.float32, device=dev) if t is None else t
+                 for i, t in enumerate(out))
 
 
 logprob_fwd = torch.library.custom_op("titanmac::token_logprobs", mutates_args=())(_logprob_fwd)
@@ -120,14 +136,14 @@ def _logprob_bwd(g_lp: Optional[torch.Tensor], g_ent: Optional[torch.Tensor], lo
     """The gradient of the logits; g_lp, g_ent: per row, or one value for all."""
     dev = _lib.require_device(*(t for t in (logits, targets, stats, entropy, g_lp, g_ent) if t is not None),
                               what="token_logprobs backward")
-    z, B, T, V = _rows3(logits)
+    z, sb, st, B, T, V = _rows3(logits)
     dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     if dz.numel() == 0:
         return dz
     (gl, sl), (ge, se) = _row_grad(g_lp), _row_grad(g_ent)
     tg = _flat(targets)
     with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_logprob_bwd(_lib.ptr(z), z.stride(0), z.stride(1), _lib.ptr(tg), ignore_index,
+        rc = _lib.lib().tmac_logprob_bwd(z.data_ptr(), sb, st, tg.data_ptr(), ignore_index,
                                          _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(gl), sl, _lib.ptr(ge), se,
                                          _lib.ptr(dz), B, T, V, _lib.dtype_code(z.dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_logprob_bwd")
@@ -182,7 +198,13 @@ def _backward(ctx, g_lp, g_ent, _g_ids, _g_top, _g_stats):
 
 
 logprob_fwd.register_autograd(_backward, setup_context=_setup)
-_native = _lib.native_function(_logprob_fwd, _setup, _backward, all_outputs=True)
+
+
+def _native_fwd(logits, targets, entropy, top_k, ignore_index):
+    return _fwd(logits, targets, entropy, top_k, ignore_index, _check_call(logits, targets, top_k))
+
+
+_native = _lib.native_function(_native_fwd, _setup, _backward, all_outputs=True)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool = False, top_k: int = 0,
@@ -202,8 +224,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool
     NaN and its top_ids -1. logprobs and entropy are differentiable (a second time too), top_logprobs is not."""
     args = (logits, targets, bool(entropy), int(top_k), int(ignore_index))
     if _lib.direct_call(logits, targets):
-        lp, ent, ids, top, _ = _logprob_fwd(*args)
-    elif _lib.eager_native(logits, targets):
+        return TokenLogprobs(*_fwd(*args, _check_call(logits, targets, args[3]))[:4])
+    if _lib.eager_native(logits, targets):
         lp, ent, ids, top, _ = _native(*args)
     else:
         lp, ent, ids, top, _ = logprob_fwd(*args)
@@ -272,6 +294,13 @@ def token_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_i
 
 # ------------------------------------------------------------------ scores from the hidden states
 
+@lru_cache(maxsize=256)
+def _head_workspace(M: int, V: int, K: int) -> int:
+    nb = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().tmac_head_logprob_workspace(M, V, K, ctypes.byref(nb)), "tmac_head_logprob_workspace")
+    return nb.value
+
+
 def _head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, entropy: bool,
                    ignore_index: int) -> tuple[torch.Tensor, torch.Tensor]:
     """(logprobs, entropy or an empty tensor) of 16-bit hidden [..., K] and weight [V, K], K a multiple of 64."""
@@ -279,16 +308,14 @@ def _head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     dev = _lib.require_device(hidden, weight, targets, what="head_logprobs")
     (V, K), lead, M = weight.shape, targets.shape, targets.numel()
     lp = torch.empty(lead, dtype=torch.float32, device=dev)
-    ent = torch.empty(lead if entropy else (0,), dtype=torch.float32, device=dev)
+    ent = lp.new_empty(lead if entropy else (0,))
     if M:
-        L, nb = _lib.lib(), ctypes.c_size_t(0)
-        x, w, tg = _rows(hidden), _rows(weight), _flat(targets)
-        _lib.check(L.tmac_head_logprob_workspace(M, V, K, ctypes.byref(nb)), "tmac_head_logprob_workspace")
-        ws = torch.empty(nb.value, dtype=torch.uint8, device=dev)
+        x, w, tg, nb = _rows(hidden), _rows(weight), _flat(targets), _head_workspace(M, V, K)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         with _lib.device_guard(dev):
-            rc = L.tmac_head_logprob(_lib.ptr(x), x.stride(0), _lib.ptr(w), w.stride(0), _lib.ptr(tg), ignore_index,
-                                     _lib.ptr(lp), _lib.ptr(ent) if entropy else 0, M, V, K, _lib.ptr(ws), nb.value,
-                                     _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+            rc = _lib.lib().tmac_head_logprob(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), tg.data_ptr(),
+                                              ignore_index, lp.data_ptr(), ent.data_ptr() if entropy else 0, M, V, K,
+                                              ws.data_ptr(), nb, _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
         _lib.check(rc, "tmac_head_logprob")
     return lp, ent
 
