@@ -121,3 +121,16 @@ def test_dispatched_op_stream_and_graph(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, tc.head_logprobs(x, w, t, entropy=True)[:2]))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("K", [256, 384, 512, 640])
+@pytest.mark.parametrize("M,V", [(256, 100003), (240, 104200), (6250, 4001), (500, 50001), (12500, 2017)])
+def test_values_by_resident_rows(dev, M, V, K, dtype):
+    """Widths and row counts whose rows stay in registers: partial row tiles, entry tiles and last strips."""
+    x, w, t = inputs(dev, M, V, K, dtype, seed=M + V + K)
+    t[:2] = torch.tensor([0, V - 1], device=dev)
+    r = tc.head_logprobs(x, w, t, entropy=True)
+    check(x, w, t, r)
+    q = tc.head_logprobs(x, w, t)
+    assert torch.equal(q.logprobs, r.logprobs)
