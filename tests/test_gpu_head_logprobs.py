@@ -124,7 +124,7 @@ def test_dispatched_op_stream_and_graph(dev):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("K", [256, 384, 512, 640])
+@pytest.mark.parametrize("K", [256, 384, 512, 640, 768, 1024])
 @pytest.mark.parametrize("M,V", [(256, 100003), (240, 104200), (6250, 4001), (500, 50001), (12500, 2017)])
 def test_values_by_resident_rows(dev, M, V, K, dtype):
     """Widths and row counts whose rows stay in registers: partial row tiles, entry tiles and last strips."""

@@ -10,8 +10,8 @@
 //
 // head_kernel takes any K and any rows: 192 x 128 tiles (64 x 128 for up to 64 rows) of both operands through
 // two LDS stages of 64-wide steps, two workgroups per CU. Few rows are bound by reading W: 16 rows of 640 x 128000
-// 25 us (6.5 TB/s). Many are bound by the copies into LDS, 53 bytes per clock and CU of about 54: 0.93 PFLOP/s at
-// K = 1024. head_rows_kernel, for K up to 640, keeps the rows in registers instead.
+// 25 us (6.5 TB/s). Many are bound by the copies into LDS, 53 bytes per clock and CU of about 54: 0.99 PFLOP/s at
+// 1503 x 1024 x 50001. head_rows_kernel keeps the rows in registers instead.
 
 #include "row_device.h"
 
@@ -194,25 +194,27 @@ __global__ __launch_bounds__(256, 2) void head_kernel(
   }
 }
 
-// The same for K = 64 KS of up to 640 and rows enough to fill tiles of 256: a wave keeps its 64 rows of X in
-// registers as MFMA operands for the whole strip (32 KS of them), so only the weight passes through LDS: 32
+// The same for K = 64 KS UNITS of up to 640 and rows enough to fill tiles of 256: a wave keeps its 64 rows of X in
+// registers as MFMA operands for the whole strip (2 K / 4 of them), so only the weight passes through LDS: 32
 // entries at a time, each 1 KB operand read feeding two MFMAs. Per CU that is 64 bytes per clock of LDS reads
 // and 16 of copies at the full MFMA rate, where the kernel above needs 107 of 128 and 53 of 54. One wave per
 // SIMD, so the statistics of one tile (a third of its MFMAs' time on the vector ALU) run beside the MFMAs of
 // the next, a few instructions after each, and so do the copies. Four LDS stages; copies are two tiles ahead;
 // the barrier that hands a stage over stands in the middle of the tile before, away from the first use.
+// MI = 1, for K of 768 and 1024: 32 rows a wave, and a tile in two units of half the K.
 // 8192 x 640 x 128000 bf16: 1047 us (1.28 PFLOP/s; the library's product of large squares 1.37), 1434 with the
 // kernel above; with all copies at once after the barrier 1076; with the statistics left to the compiler's
 // schedule, which puts them behind the MFMAs, 1119.
 constexpr int kTile = 32, kStages = 4;
 constexpr int kAhead = 2;  // k-steps that a weight operand is read ahead of its MFMAs (of 4 registers' turns)
 
-template <int DT, bool ENT, int KS>
+template <int DT, bool ENT, int KS, int UNITS, int MI>
 __global__ __launch_bounds__(256, 1) void head_rows_kernel(
     const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W, int64_t ldw,
     const int64_t* __restrict__ targets, int M, int V, int n_mt, int n_nt, int n_strips, int per_strip,
     Part* __restrict__ parts, float* __restrict__ zt, int per_xcd) {
-  constexpr int kK = 4 * KS, kSlab = kTile * 64, kStage = KS * kSlab;  // k-steps of 16; elements
+  // k-steps of 16 of a unit and of a tile; elements of a 64-wide slab and of a unit
+  constexpr int kK = 4 * KS, kAll = UNITS * kK, kSlab = kTile * 64, kStage = KS * kSlab;
   __shared__ __attribute__((aligned(16))) uint16_t smem[kStages * kStage];
 
   const int logical = xcd_logical_id(per_xcd);
@@ -223,32 +225,32 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int l32 = lane & 31, h = lane >> 5;
-  const int m0 = (logical - strip * n_mt) * 256 + 64 * wave;
+  const int m0 = (logical - strip * n_mt) * (128 * MI) + 32 * MI * wave;
 
-  // Each wave copies entries 8 wave .. 8 wave + 7 of every 64-wide slab of a tile (xswz in each slab; entries
-  // past V read the last one).
+  // Each wave copies entries 8 wave .. 8 wave + 7 of every slab of a unit (xswz in each slab; entries past V
+  // read the last one).
   const int crow = 8 * wave + (lane >> 3);
   const uint32_t cchunk = 16u * static_cast<uint32_t>((lane & 7) ^ ((crow >> 1) & 7));
   const uint32_t lds0 = lds_offset(smem) + static_cast<uint32_t>(wave * 1024);
-  auto issue = [&](int i, int s) {  // slab s of tile i of the strip (past its end: the last) into stage i % kStages
+  auto issue = [&](int i, int part, int stage, int s) {  // slab s of a unit of tile i (past the strip: its last)
     const int e0 = (t0 + min(i, n_tiles - 1)) * kTile;
     const uint32_t off = static_cast<uint32_t>(min(crow, V - 1 - e0)) * static_cast<uint32_t>(2 * ldw) + cchunk;
-    dma_lds16(W + static_cast<int64_t>(e0) * ldw + 64 * s, off,
-              lds0 + static_cast<uint32_t>(((i % kStages) * kStage + s * kSlab) * 2));
+    dma_lds16(W + static_cast<int64_t>(e0) * ldw + 64 * (KS * part + s), off,
+              lds0 + static_cast<uint32_t>((stage * kStage + s * kSlab) * 2));
   };
 
-  u32x4 x[2][kK];
-  int target[2];  // −1: no entry of this row is asked for
+  u32x4 x[MI][kAll];
+  int target[MI];  // −1: no entry of this row is asked for
 #pragma unroll
-  for (int mi = 0; mi < 2; ++mi) {
+  for (int mi = 0; mi < MI; ++mi) {
     const int row = min(m0 + 32 * mi + l32, M - 1);
     const uint16_t* const p = X + static_cast<int64_t>(row) * ldx + 8 * h;
 #pragma unroll
-    for (int kk = 0; kk < kK; ++kk) {
+    for (int kk = 0; kk < kAll; ++kk) {
       x[mi][kk] = ldg16(p + 16 * kk);
       // the first 28 operands in vector registers, the others in accumulation registers, which MFMAs read as
       // well: left to itself the compiler copies four registers per MFMA (1183 us for 1119)
-      if (mi * kK + kk >= 28) asm volatile("" : "+a"(x[mi][kk]));
+      if (mi * kAll + kk >= 28) asm volatile("" : "+a"(x[mi][kk]));
     }
     const int64_t t = targets[row];
     target[mi] = m0 + 32 * mi + l32 < M && t >= 0 && t < V ? static_cast<int>(t) : -1;
@@ -257,23 +259,25 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
   int lane_off[4];
 #pragma unroll
   for (int k4 = 0; k4 < 4; ++k4) lane_off[k4] = xswz(l32, 2 * k4 + h);
-  auto read = [&](int i, int kk) {
-    return lds16(smem + (i % kStages) * kStage + (kk >> 2) * kSlab + lane_off[kk & 3]);
+  auto read = [&](int stage, int kk) {  // k-step kk of the unit in that stage
+    return lds16(smem + stage * kStage + (kk >> 2) * kSlab + lane_off[kk & 3]);
   };
 
-  Stat stat[2] = {stat_none(), stat_none()};
+  Stat stat[MI];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) stat[mi] = stat_none();
   // value j of acc[mi] is entry 32 tile + 8 (j / 4) + 4 h + j % 4: what is rare, in branches ahead of the MFMAs
-  auto rare = [&](f32x16(&acc)[2], int i) {
+  auto rare = [&](f32x16(&acc)[MI], int i) {
     const int e0 = (t0 + i) * kTile;
     if (e0 + kTile > V) {
 #pragma unroll
-      for (int mi = 0; mi < 2; ++mi)
+      for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (e0 + 8 * (j >> 2) + 4 * h + (j & 3) >= V) acc[mi][j] = -__builtin_inff();
     }
 #pragma unroll
-    for (int mi = 0; mi < 2; ++mi) {
+    for (int mi = 0; mi < MI; ++mi) {
       if (__ballot(target[mi] >= e0 && target[mi] < e0 + kTile)) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -281,9 +285,9 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
       }
     }
   };
-  auto add = [&](const f32x16(&acc)[2]) {
+  auto add = [&](const f32x16(&acc)[MI]) {
 #pragma unroll
-    for (int mi = 0; mi < 2; ++mi) {
+    for (int mi = 0; mi < MI; ++mi) {
       float m = stat[mi].m;
 #pragma unroll
       for (int j = 0; j < 16; ++j) m = fmaxf(m, acc[mi][j]);
@@ -293,49 +297,57 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
     }
   };
 
-  f32x16 acc[2][2];
+  f32x16 acc[2][MI];
 #pragma unroll
-  for (int mi = 0; mi < 2; ++mi)
+  for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[1][mi][j] = -__builtin_inff();  // no tile before the first
   u32x4 w[4];
   // Tile i: its MFMAs into acc[i % 2], the statistics of tile i − 1 beside them: its maximum in the first four
   // k-steps, the sums moved to it in the fifth, its 32 values over the others. The scheduling barriers keep
   // that order.
-  auto body = [&](int i, f32x16(&cur)[2], f32x16(&old)[2]) {
+  auto body = [&](int i, f32x16(&cur)[MI], f32x16(&old)[MI]) {
     if (i > 0) rare(old, i - 1);
-    float m[2] = {stat[0].m, stat[1].m};
+    constexpr int kMax = 4, kVals = 16 * MI;
+    float m[MI];
 #pragma unroll
-    for (int kk = 0; kk < kK; ++kk) {
-      if (kk == kK / 2) {
-        // the next tile has landed (the one after it may be on its way), and every wave is done with the tile
+    for (int mi = 0; mi < MI; ++mi) m[mi] = stat[mi].m;
+#pragma unroll
+    for (int kk = 0; kk < kAll; ++kk) {
+      const int part = kk / kK, ku = kk % kK, unit = i * UNITS + part;
+      if (ku == kK / 2) {
+        // the next unit has landed (the one after it may be on its way), and every wave is done with the unit
         // before this one (its reads have returned), whose stage the next copies overwrite
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KS) : "memory");
         ring_barrier();
       }
-      w[(kk + kAhead) & 3] = kk + kAhead < kK ? read(i, kk + kAhead) : read(i + 1, kk + kAhead - kK);
+      w[(kk + kAhead) & 3] = ku + kAhead < kK ? read(unit % kStages, ku + kAhead)
+                                              : read((unit + 1) % kStages, ku + kAhead - kK);
 #pragma unroll
-      for (int mi = 0; mi < 2; ++mi)
+      for (int mi = 0; mi < MI; ++mi)
         cur[mi] = Mfma<DT>::run(w[kk & 3], x[mi][kk], kk ? cur[mi] : f32x16{});
-      if (kk >= kK / 2 && kk < kK / 2 + KS) issue(i + 3, kk - kK / 2);
-      if (kk < 4) {
+      if (ku >= kK / 2 && ku < kK / 2 + KS)
+        issue(i + (part + 3) / UNITS, (part + 3) % UNITS, (unit + 3) % kStages, ku - kK / 2);
+      if (kk < kMax) {
 #pragma unroll
-        for (int v = 8 * kk; v < 8 * kk + 8; ++v) m[v >> 4] = fmaxf(m[v >> 4], old[v >> 4][v & 15]);
-      } else if (kk == 4) {
-        stat_rescale(stat[0], m[0]);
-        stat_rescale(stat[1], m[1]);
+        for (int v = kVals / kMax * kk; v < kVals / kMax * (kk + 1); ++v)
+          m[v >> 4] = fmaxf(m[v >> 4], old[v >> 4][v & 15]);
+      } else if (kk == kMax) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) stat_rescale(stat[mi], m[mi]);
       } else {
+        constexpr int kRest = kAll - kMax - 1;
 #pragma unroll
-        for (int v = 32 * (kk - 5) / (kK - 5); v < 32 * (kk - 4) / (kK - 5); ++v)
+        for (int v = kVals * (kk - kMax - 1) / kRest; v < kVals * (kk - kMax) / kRest; ++v)
           stat_add<ENT>(stat[v >> 4], old[v >> 4][v & 15]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 #pragma unroll
-  for (int t = 0; t < 3; ++t)
+  for (int u = 0; u < 3; ++u)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) issue(t, s);
+    for (int s = 0; s < KS; ++s) issue(u / UNITS, u % UNITS, u, s);
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KS) : "memory");
   ring_barrier();
 #pragma unroll
@@ -354,7 +366,7 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup
   // the lane halves hold parts of the same rows
 #pragma unroll
-  for (int mi = 0; mi < 2; ++mi) {
+  for (int mi = 0; mi < MI; ++mi) {
     const Stat& a = stat[mi];
     stat_join(stat[mi], Stat{lane_xor<32>(a.m), lane_xor<32>(a.mu), lane_xor<32>(a.s), lane_xor<32>(a.h)});
     const int row = m0 + 32 * mi + l32;
@@ -390,12 +402,16 @@ __global__ __launch_bounds__(256) void head_join_kernel(const Part* __restrict__
 // ------------------------------------------------------------------ host
 
 // Whether head_rows_kernel takes the call: enough work for its start (its rows are loaded before anything else),
-// and row tiles of 256 that are not emptier than those of 192. us, with it / without, bf16: 256 rows of 640 x
-// 128000 55 / 64, 300 rows 79 / 65, 600 rows 110 / 117, 5000 rows 647 / 851; 512 x 32000: 768 rows 36 / 31, 1000
-// rows 41.5 / 42.8, 5000 rows 150 / 175; 256 x 50000: 1000 rows 36 / 41; 640 x 5000: 3000 rows 36 / 33.
+// and row tiles of 256 (128 where K > 640) that are not emptier than those of 192. us, with it / without, bf16:
+// 256 rows of 640 x 128000 55 / 64, 300 rows 79 / 65, 600 rows 110 / 117, 5000 rows 647 / 851; 512 x 32000: 768 rows
+// 36 / 31, 1000 rows 41.5 / 42.8, 5000 rows 150 / 175; 256 x 50000: 1000 rows 36 / 41; 640 x 5000: 3000 rows 36 / 33;
+// 1024 x 50001: 192 rows 38 / 32, 256 rows 39 / 50, 1503 rows 144 / 155; 768 x 8000: 1503 rows 28 / 26.
 bool rows_applies(int M, int V, int K) {
-  const int64_t own = (M + 255) / 256 * 256ll, other = (M + 191) / 192 * 192ll;
-  return K % 128 == 0 && K >= 256 && K <= 640 && static_cast<int64_t>(M) * V >= 25000000 && 100 * own <= 107 * other;
+  const bool wide = K == 768 || K == 1024;
+  if (!wide && (K % 128 || K < 256 || K > 640)) return false;
+  const int tile = wide ? 128 : 256;
+  const int64_t own = (M + tile - 1) / tile * static_cast<int64_t>(tile), other = (M + 191) / 192 * 192ll;
+  return static_cast<int64_t>(M) * V >= (wide ? 12000000 : 25000000) && 100 * own <= 107 * other;
 }
 
 struct Plan {
@@ -430,7 +446,7 @@ Plan plan(int M, int V, int K) {
   Plan p{};
   if (rows_applies(M, V, K)) {
     p.ks = K / 64;
-    p.n_mt = (M + 255) / 256;
+    p.n_mt = K > 640 ? (M + 127) / 128 : (M + 255) / 256;
     p.n_nt = (V + kTile - 1) / kTile;
     // strips of more than 256 tiles run at the pace of the slowest CU: 8192 x 128000 in one round 1090 us, two 1047
     plan_strips(p, 256, 8, 256);
@@ -490,20 +506,28 @@ extern "C" int tmac_head_logprob(const void* d_X, int64_t ldx, const void* d_W, 
         static_cast<const uint16_t*>(d_X), ldx, static_cast<const uint16_t*>(d_W), ldw, d_targets, M, v, K / 64,
         p.n_mt, p.n_nt, p.n_strips, p.per_strip, parts, zt, per_xcd);
   };
-  auto launch_rows = [&](auto dt, auto e, auto ks) {
-    head_rows_kernel<decltype(dt)::value, decltype(e)::value, decltype(ks)::value><<<8 * per_xcd, 256, 0, s>>>(
+  auto launch_rows = [&](auto dt, auto e, auto ks, auto units) {
+    constexpr int UNITS = decltype(units)::value;
+    head_rows_kernel<decltype(dt)::value, decltype(e)::value, decltype(ks)::value, UNITS, UNITS == 1 ? 2 : 1>
+        <<<8 * per_xcd, 256, 0, s>>>(
         static_cast<const uint16_t*>(d_X), ldx, static_cast<const uint16_t*>(d_W), ldw, d_targets, M, v, p.n_mt,
         p.n_nt, p.n_strips, p.per_strip, parts, zt, per_xcd);
   };
   auto by_rows = [&](auto dt, auto e) {
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, 2> two{};
     if (p.ks == 4)
-      launch_rows(dt, e, std::integral_constant<int, 4>{});
+      launch_rows(dt, e, std::integral_constant<int, 4>{}, one);
     else if (p.ks == 6)
-      launch_rows(dt, e, std::integral_constant<int, 6>{});
+      launch_rows(dt, e, std::integral_constant<int, 6>{}, one);
     else if (p.ks == 8)
-      launch_rows(dt, e, std::integral_constant<int, 8>{});
+      launch_rows(dt, e, std::integral_constant<int, 8>{}, one);
     else if (p.ks == 10)
-      launch_rows(dt, e, std::integral_constant<int, 10>{});
+      launch_rows(dt, e, std::integral_constant<int, 10>{}, one);
+    else if (p.ks == 12)
+      launch_rows(dt, e, std::integral_constant<int, 6>{}, two);
+    else if (p.ks == 16)
+      launch_rows(dt, e, std::integral_constant<int, 8>{}, two);
     else if (p.mi == 1)
       launch(dt, e, std::integral_constant<int, 1>{});
     else
