@@ -687,22 +687,25 @@ int tmac_linear_wgrad(const void* d_dY, int64_t lddy, const void* d_X, int64_t l
  * in fp32, rounded once. ids, pos: int64 [B, T], contiguous. W [V, d], P [n_pos, d] (nullable: no term) and
  * prefix [n_prefix, d] have row pitches ldw, ldp, ldpre. An id (position) outside its table reads
  * nothing and gives a row of NaN. Any d; 16-byte accesses where d, pitches and pointers allow.
- * B·(n_prefix + T), V, n_pos <= 2^30; d <= 2^20. */
+ * d_lists (nullable; tmac_embed_lists_bytes(B·T, V) bytes, 16-byte aligned): receives the tokens of each row of
+ * W, in order, for tmac_embed_bwd, in the same launch. B·(n_prefix + T), V, n_pos <= 2^30; d <= 2^20. */
+int tmac_embed_lists_bytes(int64_t n_tokens, int64_t V, size_t* bytes);
 int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_W, int64_t ldw, const void* d_P,
-                   int64_t ldp, const void* d_prefix, int64_t ldpre, void* d_out, int B, int T, int n_prefix, int d,
-                   int64_t V, int64_t n_pos, float scale, int dtype, void* stream);
+                   int64_t ldp, const void* d_prefix, int64_t ldpre, void* d_out, void* d_lists, size_t lists_bytes,
+                   int B, int T, int n_prefix, int d, int64_t V, int64_t n_pos, float scale, int dtype, void* stream);
 
 /* Its gradients, each nullable, dense, contiguous and in dtype, of g [B, n_prefix + T, d] given as rows of pitch ldg:
  *   dW[v] = scale · Σ_{ids[b, t] = v} g[b, n_prefix + t]    [V, d]
  *   dP[q] = Σ_{pos(b, t) = q} g[b, n_prefix + t]            [n_pos, d]
  *   dprefix[p] = Σ_b g[b, p]                                [n_prefix, d]
  * Rows without a token are zeros, indices outside a table count nowhere. fp32 sums in ascending order of
- * (b, t) (deterministic), rounded once. d_ws: 16-byte aligned, tmac_embed_bwd_workspace(B·T, V, n_pos, d) bytes with
- * V = 0 without d_dW and n_pos = 0 without d_dP or d_pos; none where both are. */
+ * (b, t) (deterministic), rounded once. d_lists: the forward's, for the same ids, B, T, n_prefix and V, or NULL (they
+ * are made of d_ids). d_ws: 16-byte aligned, tmac_embed_bwd_workspace(B·T, V, n_pos, d) bytes with V = 0 without
+ * d_dW or with d_lists, and n_pos = 0 without d_dP or d_pos; none without d_dW where the second is 0 too. */
 int tmac_embed_bwd_workspace(int64_t n_tokens, int64_t V, int64_t n_pos, int d, size_t* ws_bytes);
-int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_g, int64_t ldg, void* d_dW, void* d_dP,
-                   void* d_dprefix, void* d_ws, size_t ws_bytes, int B, int T, int n_prefix, int d, int64_t V,
-                   int64_t n_pos, float scale, int dtype, void* stream);
+int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_lists, const void* d_g, int64_t ldg,
+                   void* d_dW, void* d_dP, void* d_dprefix, void* d_ws, size_t ws_bytes, int B, int T, int n_prefix,
+                   int d, int64_t V, int64_t n_pos, float scale, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Log probabilities of given tokens (F.cross_entropy of models/titanmac.py:666-680 by row, and what a

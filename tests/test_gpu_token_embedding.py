@@ -176,11 +176,13 @@ def test_second_derivative(dev):
 def test_dispatched_op_agrees(dev):
     s = make(2, 77, 30, 40, 3, torch.bfloat16, dev, given=True)
     args = (s["ids"], s["w"].requires_grad_(), s["p"].requires_grad_(), s["pos"], s["f"].requires_grad_(), 3.0)
-    y = ke.token_embedding_fwd(*args)
-    g = torch.autograd.grad(y, (s["w"], s["p"], s["f"]), s["gy"])
-    z = tc.token_embedding(s["ids"], s["w"], s["p"], positions=s["pos"], prefix=s["f"], scale=3.0)
-    h = torch.autograd.grad(z, (s["w"], s["p"], s["f"]), s["gy"])
-    assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(g, h))
+    for lists in (False, True):  # the backward makes the lists of tokens where the forward has not
+        y, made = ke.token_embedding_fwd(*args, lists)
+        assert made.numel() == (ke._lists_bytes(2 * 77, 30) if lists else 0)
+        g = torch.autograd.grad(y, (s["w"], s["p"], s["f"]), s["gy"])
+        z = tc.token_embedding(s["ids"], s["w"], s["p"], positions=s["pos"], prefix=s["f"], scale=3.0)
+        h = torch.autograd.grad(z, (s["w"], s["p"], s["f"]), s["gy"])
+        assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(g, h))
 
 
 def test_other_stream_and_graph(dev):

@@ -63,9 +63,11 @@ def test_fake_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
         ids, w = torch.zeros(2, 3, dtype=torch.long), torch.zeros(5, 8, dtype=torch.bfloat16)
-        y = ke.token_embedding_fwd(ids, w, None, None, w[:4], 1.0)
+        y, lists = ke.token_embedding_fwd(ids, w, None, None, w[:4], 1.0, True)
+        assert lists.shape == (32 + 2 * 32,) and lists.dtype == torch.uint8
+        assert ke.token_embedding_fwd(ids, w, None, None, w[:4], 1.0, False)[1].shape == (0,)
         assert y.shape == (2, 7, 8) and y.dtype == torch.bfloat16
-        dw, dp, df = ke.token_embedding_bwd(y, ids, None, 4, 5, 0, 1.0, True, False, True)
+        dw, dp, df = ke.token_embedding_bwd(y, ids, None, lists, 4, 5, 0, 1.0, True, False, True)
         assert (dw.shape, dp.shape, df.shape) == ((5, 8), (0, 8), (4, 8))
         z = torch.zeros(2, 3, 100, dtype=torch.float16)
         lp, ent, top_ids, top, stats = kl.logprob_fwd(z, ids, False, 6, -100)
@@ -78,16 +80,22 @@ def test_fake_shapes():
 
 
 def test_embedding_argument_errors(lib):
-    # ids, pos, W, ldw, P, ldp, prefix, ldpre, out, B, T, n_prefix, d, V, n_pos, scale, dtype, stream
-    ok = [FAKE, None, FAKE, 64, FAKE, 64, FAKE, 64, FAKE, 2, 3, 4, 64, 100, 50, 1.0, 1, None]
+    n = ctypes.c_size_t(0)
+    for tokens, V in ((0, 1), (1, 3), (6, 100), (32768, 128000), (7, 4)):
+        assert lib.tmac_embed_lists_bytes(tokens, V, ctypes.byref(n)) == 0 and n.value == ke._lists_bytes(tokens, V)
+    assert lib.tmac_embed_lists_bytes(6, 0, ctypes.byref(n)) == -2 and lib.tmac_embed_lists_bytes(6, 1, None) == -1
+    lib.tmac_embed_lists_bytes(6, 100, ctypes.byref(n))
+    # ids, pos, W, ldw, P, ldp, prefix, ldpre, out, lists, bytes, B, T, n_prefix, d, V, n_pos, scale, dtype, stream
+    ok = [FAKE, None, FAKE, 64, FAKE, 64, FAKE, 64, FAKE, FAKE, n.value, 2, 3, 4, 64, 100, 50, 1.0, 1, None]
     for at, value, want in ((0, None, -1), (2, None, -1), (8, None, -1), (6, None, -1), (3, 63, -2), (5, 63, -2),
-                            (7, 63, -2), (9, -1, -2), (12, 0, -2), (12, (1 << 20) + 1, -2), (13, 0, -2),
-                            (13, (1 << 30) + 1, -2), (14, 2, -2), (16, 3, -4), (10, 1 << 30, -2)):
+                            (7, 63, -2), (11, -1, -2), (14, 0, -2), (14, (1 << 20) + 1, -2), (15, 0, -2),
+                            (15, (1 << 30) + 1, -2), (16, 2, -2), (18, 3, -4), (12, 1 << 30, -2),
+                            (10, n.value - 1, -6), (9, FAKE + 8, -5)):
         bad = list(ok)
         bad[at] = value
         assert lib.tmac_embed_fwd(*bad) == want, (at, value)
     empty = list(ok)
-    empty[9] = 0
+    empty[9], empty[11] = None, 0
     assert lib.tmac_embed_fwd(*empty) == 0
     n = ctypes.c_size_t(0)
     assert lib.tmac_embed_bwd_workspace(1000, 50, 0, 64, ctypes.byref(n)) == 0 and n.value >= 4 * (51 + 2000) + 2 * 16 * 64 * 4
@@ -95,15 +103,16 @@ def test_embedding_argument_errors(lib):
     assert lib.tmac_embed_bwd_workspace(1000, 50, (1 << 30) + 1, 64, ctypes.byref(n)) == -2
     assert lib.tmac_embed_bwd_workspace(1000, 50, 0, 64, None) == -1
     lib.tmac_embed_bwd_workspace(6, 100, 50, 64, ctypes.byref(n))
-    # ids, pos, g, ldg, dW, dP, dprefix, ws, ws_bytes, B, T, n_prefix, d, V, n_pos, scale, dtype, stream
-    ok = [FAKE, FAKE, FAKE, 64, FAKE, FAKE, FAKE, FAKE, n.value, 2, 3, 4, 64, 100, 50, 1.0, 1, None]
-    for at, value, want in ((0, None, -1), (2, None, -1), (7, None, -6), (8, n.value - 1, -6), (7, FAKE + 4, -5),
-                            (3, 63, -2), (13, 0, -2), (14, 0, -2), (16, 9, -4), (12, 0, -2), (11, 0, -2), (9, -1, -2)):
+    # ids, pos, lists, g, ldg, dW, dP, dprefix, ws, ws_bytes, B, T, n_prefix, d, V, n_pos, scale, dtype, stream
+    ok = [FAKE, FAKE, None, FAKE, 64, FAKE, FAKE, FAKE, FAKE, n.value, 2, 3, 4, 64, 100, 50, 1.0, 1, None]
+    for at, value, want in ((0, None, -1), (3, None, -1), (8, None, -6), (9, n.value - 1, -6), (8, FAKE + 4, -5),
+                            (4, 63, -2), (14, 0, -2), (15, 0, -2), (17, 9, -4), (13, 0, -2), (12, 0, -2), (10, -1, -2),
+                            (2, FAKE + 8, -5)):
         bad = list(ok)
         bad[at] = value
         assert lib.tmac_embed_bwd(*bad) == want, (at, value)
     bad = list(ok)
-    bad[1], bad[14] = None, 2  # fewer position rows than positions
+    bad[1], bad[15] = None, 2  # fewer position rows than positions
     assert lib.tmac_embed_bwd(*bad) == -2
 
 
@@ -153,7 +162,7 @@ def test_differentiable_gradients_match_autograd():
     assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
     ids = torch.tensor([[0, 2, 2], [4, 7, -1]])
     g = torch.randn(2, 5, 6)
-    dw, dp, df = ke._composed(g, ids, None, 2, 5, 4, 0.5, True, True, True)
+    dw, dp, df = ke._composed(g, ids, None, None, 2, 5, 4, 0.5, True, True, True)
     body = g[:, 2:]
     assert torch.allclose(dw[2], 0.5 * (body[0, 1] + body[0, 2])) and torch.allclose(dw[4], 0.5 * body[1, 0])
     assert torch.all(dw[[1, 3]] == 0) and torch.allclose(dw[0], 0.5 * body[0, 0])

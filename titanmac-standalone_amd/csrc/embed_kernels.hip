@@ -29,44 +29,56 @@ constexpr int kMaxGrid = 1 << 22;  // workgroups of a launch; they take turns be
 int rows_per_block(int cpr, int per) { return kThreads * per > cpr ? kThreads * per / cpr : 1; }
 int grid(int64_t blocks) { return static_cast<int>(blocks < kMaxGrid ? blocks : kMaxGrid); }
 
+struct Lookup {
+  const int64_t *ids, *pos;
+  const uint8_t *W, *P, *prefix;
+  int64_t ldw, ldp, ldpre;
+  uint8_t* out;
+  int rows, T, Np, d;
+  int64_t V, n_pos;
+  float scale;
+  int cpr, rpb;
+};
+
 // One piece per thread and turn: two or four in flight measured 10 and 25 % slower (9.9 us against 10.9 and 12.8
 // for 4 x 4112 rows of 640 bf16: the registers cost more waves than the loads gain).
-template <int DT, int N>
-__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
-    const int64_t* __restrict__ ids, const int64_t* __restrict__ pos, const uint8_t* __restrict__ W,
-    int64_t ldw, const uint8_t* __restrict__ P, int64_t ldp, const uint8_t* __restrict__ prefix, int64_t ldpre,
-    uint8_t* __restrict__ out, int rows, int T, int Np, int d, int64_t V, int64_t n_pos, float scale, int cpr,
-    int rpb) {
+template <int DT, int N, int NT>
+__device__ __forceinline__ void lookup_rows(const Lookup& a, int64_t first, int64_t step) {
   constexpr int E = kRowSize<DT>;
-  const int S = Np + T;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rpb; row0 < rows; row0 += static_cast<int64_t>(gridDim.x) * rpb) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(rpb), rows - row0)) * cpr;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int r = i / cpr, c = (i - r * cpr) * N;
+  const int S = a.Np + a.T;
+  for (int64_t row0 = first * a.rpb; row0 < a.rows; row0 += step * a.rpb) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(a.rpb), a.rows - row0)) * a.cpr;
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const int r = i / a.cpr, c = (i - r * a.cpr) * N;
       const int row = static_cast<int>(row0) + r;
       const int b = row / S, s = row - b * S;
       float v[N];
-      if (s < Np) {
-        row_load<DT, N>(prefix + (s * ldpre + c) * E, v);
+      if (s < a.Np) {
+        row_load<DT, N>(a.prefix + (s * a.ldpre + c) * E, v);
       } else {
-        const int64_t tok = static_cast<int64_t>(b) * T + (s - Np);
-        const int64_t id = ids[tok];
-        const int64_t p = pos ? pos[tok] : s - Np;
+        const int64_t tok = static_cast<int64_t>(b) * a.T + (s - a.Np);
+        const int64_t id = a.ids[tok];
+        const int64_t p = a.pos ? a.pos[tok] : s - a.Np;
         // an index outside its table reads nothing and gives a row of NaN
-        if (id >= 0 && id < V && (!P || (p >= 0 && p < n_pos))) {
+        if (id >= 0 && id < a.V && (!a.P || (p >= 0 && p < a.n_pos))) {
           float q[N];
-          row_load<DT, N>(W + (id * ldw + c) * E, v);
-          if (P) row_load<DT, N>(P + (p * ldp + c) * E, q);
+          row_load<DT, N>(a.W + (id * a.ldw + c) * E, v);
+          if (a.P) row_load<DT, N>(a.P + (p * a.ldp + c) * E, q);
 #pragma unroll
-          for (int e = 0; e < N; ++e) v[e] = P ? fmaf(scale, v[e], q[e]) : scale * v[e];
+          for (int e = 0; e < N; ++e) v[e] = a.P ? fmaf(a.scale, v[e], q[e]) : a.scale * v[e];
         } else {
 #pragma unroll
           for (int e = 0; e < N; ++e) v[e] = __builtin_nanf("");
         }
       }
-      row_store<DT, N>(out + (static_cast<int64_t>(row) * d + c) * E, v);
+      row_store<DT, N>(a.out + (static_cast<int64_t>(row) * a.d + c) * E, v);
     }
   }
+}
+
+template <int DT, int N>
+__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(Lookup a) {
+  lookup_rows<DT, N, kThreads>(a, blockIdx.x, gridDim.x);
 }
 
 // ------------------------------------------------------------------ the sort
@@ -109,15 +121,28 @@ int n_ranges(int64_t V) {
 // row_start[v]: where id v's tokens begin (row_start[V] their number); perm: the row of g of each, in
 // ascending order; key: its id. An id outside [0, V) is in no list.
 // HELD: batches of 64 ids that a wave keeps in registers between the two readings (all it has), or 0.
+struct Lists {
+  int32_t *row_start, *perm, *key;
+};
+struct Tokens {
+  const int64_t* ids;
+  int n;
+  int T;
+  uint32_t T_inv;  // 2^32 / T
+  int Np, V;
+};
+
 template <int HELD>
-__global__ __launch_bounds__(64 * kSortWaves, 8) void embed_sort_kernel(
-    const int64_t* __restrict__ ids, int n_tok, int T, uint32_t T_inv, int Np, int V, int32_t* __restrict__ row_start,
-    int32_t* __restrict__ perm, int32_t* __restrict__ key) {
+__device__ __forceinline__ void sort_range(const Tokens& a, const Lists& to, int block) {
+  const int64_t* const __restrict__ ids = a.ids;
+  const int n_tok = a.n, T = a.T, Np = a.Np, V = a.V;
+  const uint32_t T_inv = a.T_inv;
+  int32_t *const row_start = to.row_start, *const perm = to.perm, *const key = to.key;
   __shared__ int hist[kSortWaves * kMaxRange];
   __shared__ int s_tot[kSortWaves], s_below[kSortWaves];
   constexpr int kAhead = HELD ? HELD : 8, kLoads = kAhead < 8 ? kAhead : 8;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const IdRange range = id_range(blockIdx.x);
+  const IdRange range = id_range(block);
   const int lo = range.lo, R = min(range.n, V - lo);  // lo < V
   const int per = (n_tok + 64 * kSortWaves - 1) / (64 * kSortWaves) * 64;
   const int begin = wave * per, end = min(begin + per, n_tok);
@@ -203,6 +228,23 @@ __global__ __launch_bounds__(64 * kSortWaves, 8) void embed_sort_kernel(
       }
     }
   }
+}
+
+template <int HELD>
+__global__ __launch_bounds__(64 * kSortWaves, 8) void embed_sort_kernel(Tokens t, Lists to) {
+  sort_range<HELD>(t, to, blockIdx.x);
+}
+
+// The lookup of a training step and its tokens' lists in one launch: the sort waits for LDS and L2 most of its
+// time, the lookup for memory.
+template <int DT, int N, int HELD>
+__global__ __launch_bounds__(64 * kSortWaves, 8) void embed_fwd_lists_kernel(Lookup a, Tokens t, Lists to,
+                                                                            int sort_blocks) {
+  const int b = blockIdx.x;
+  if (b < sort_blocks)
+    sort_range<HELD>(t, to, b);
+  else
+    lookup_rows<DT, N, 64 * kSortWaves>(a, b - sort_blocks, gridDim.x - sort_blocks);
 }
 
 // ------------------------------------------------------------------ the sums
@@ -430,43 +472,78 @@ bool wide_rows(const void* p, int64_t ld, int dtype) {
 
 size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
-struct GradWs {
-  size_t perm, key, part, total;
+struct ListsAt {
+  size_t perm, key, total;
 };
-GradWs grad_ws(int64_t n_tok, int64_t V, int d) {
-  GradWs w;
+ListsAt lists_at(int64_t n_tok, int64_t V) {
+  ListsAt w;
   w.perm = up16(4 * static_cast<size_t>(V + 1));
   w.key = w.perm + up16(4 * static_cast<size_t>(n_tok));
-  w.part = w.key + up16(4 * static_cast<size_t>(n_tok));
-  const size_t chunks = n_tok > kList ? static_cast<size_t>((n_tok + kList - 1) / kList) : 0;
-  w.total = w.part + 8 * chunks * static_cast<size_t>(d);
+  w.total = w.key + up16(4 * static_cast<size_t>(n_tok));
   return w;
 }
+Lists lists(void* at, int64_t n_tok, int64_t V) {
+  const ListsAt w = lists_at(n_tok, V);
+  uint8_t* const p = static_cast<uint8_t*>(at);
+  return Lists{reinterpret_cast<int32_t*>(p), reinterpret_cast<int32_t*>(p + w.perm),
+               reinterpret_cast<int32_t*>(p + w.key)};
+}
+size_t part_bytes(int64_t n_tok, int d) {
+  return n_tok > kList ? 8 * static_cast<size_t>((n_tok + kList - 1) / kList) * static_cast<size_t>(d) : 0;
+}
+Tokens tokens(const int64_t* ids, int n_tok, int T, int n_prefix, int64_t V) {
+  return Tokens{ids, n_tok, T, T > 1 ? static_cast<uint32_t>((1ull << 32) / static_cast<uint32_t>(T)) : 0, n_prefix,
+                static_cast<int>(V)};
+}
+constexpr int kHeld = 4;  // batches that the sort of few tokens keeps in registers
+bool held(int n_tok) { return n_tok <= kHeld * 64 * kSortWaves; }
 
 }  // namespace
 
+extern "C" int tmac_embed_lists_bytes(int64_t n_tokens, int64_t V, size_t* bytes) {
+  if (!bytes) return TMAC_ERR_NULL;
+  if (n_tokens < 0 || n_tokens > kMaxRows || V <= 0 || V > kMaxRows) return TMAC_ERR_SHAPE;
+  *bytes = lists_at(n_tokens, V).total;
+  return TMAC_OK;
+}
+
 extern "C" int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_W, int64_t ldw,
                               const void* d_P, int64_t ldp, const void* d_prefix, int64_t ldpre, void* d_out,
-                              int B, int T, int n_prefix, int d, int64_t V, int64_t n_pos, float scale, int dtype,
-                              void* stream) {
+                              void* d_lists, size_t lists_bytes, int B, int T, int n_prefix, int d, int64_t V,
+                              int64_t n_pos, float scale, int dtype, void* stream) {
   const int st = check_sizes(B, T, n_prefix, d, dtype);
   if (st != TMAC_OK) return st;
   if (V <= 0 || V > kMaxRows || ldw < d) return TMAC_ERR_SHAPE;
   if (d_P && (n_pos <= 0 || n_pos > kMaxRows || ldp < d || (!d_pos && n_pos < T))) return TMAC_ERR_SHAPE;
   if (n_prefix && ldpre < d) return TMAC_ERR_SHAPE;
-  const int rows = B * (n_prefix + T);
-  if (rows == 0) return TMAC_OK;
-  if (!d_W || !d_out || (T > 0 && !d_ids) || (n_prefix && !d_prefix)) return TMAC_ERR_NULL;
+  const int rows = B * (n_prefix + T), n_tok = B * T;
+  if (d_lists && lists_bytes < lists_at(n_tok, V).total) return TMAC_ERR_WORKSPACE;
+  if (d_lists && !row_aligned16(d_lists)) return TMAC_ERR_ALIGN;
+  if (rows == 0 && !d_lists) return TMAC_OK;
+  if ((rows && (!d_W || !d_out)) || (n_tok > 0 && !d_ids) || (B > 0 && n_prefix && !d_prefix)) return TMAC_ERR_NULL;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool wide = d % (dtype == TMAC_F32 ? 4 : 8) == 0 && row_aligned16(d_out) && wide_rows(d_W, ldw, dtype) &&
                     wide_rows(d_P, ldp, dtype) && (!n_prefix || wide_rows(d_prefix, ldpre, dtype));
   dispatch(dtype, wide, [&](auto dt, auto n) {
     constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
-    const int cpr = d / N;
-    const int rpb = rows_per_block(cpr, 1);
-    embed_fwd_kernel<DT, N><<<grid((rows + rpb - 1) / rpb), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-        d_ids, d_pos, static_cast<const uint8_t*>(d_W), ldw, static_cast<const uint8_t*>(d_P), ldp,
-        static_cast<const uint8_t*>(d_prefix), ldpre, static_cast<uint8_t*>(d_out), rows, T, n_prefix, d, V, n_pos,
-        scale, cpr, rpb);
+    Lookup a{d_ids, d_pos, static_cast<const uint8_t*>(d_W), static_cast<const uint8_t*>(d_P),
+             static_cast<const uint8_t*>(d_prefix), ldw, ldp, ldpre, static_cast<uint8_t*>(d_out), rows, T, n_prefix, d,
+             V, n_pos, scale, d / N, 1};
+    if (!d_lists) {
+      a.rpb = rows_per_block(a.cpr, 1);
+      embed_fwd_kernel<DT, N><<<grid((rows + a.rpb - 1) / a.rpb), kThreads, 0, s>>>(a);
+      return;
+    }
+    a.rpb = rows_per_block(a.cpr, 64 * kSortWaves / kThreads);
+    const Tokens t = tokens(d_ids, n_tok, T, n_prefix, V);
+    const Lists to = lists(d_lists, n_tok, V);
+    const int sort_blocks = n_ranges(V);
+    const int64_t look = (rows + a.rpb - 1) / a.rpb;
+    const int blocks = sort_blocks + static_cast<int>(look < (1 << 21) ? look : 1 << 21);
+    if (held(n_tok))
+      embed_fwd_lists_kernel<DT, N, kHeld><<<blocks, 64 * kSortWaves, 0, s>>>(a, t, to, sort_blocks);
+    else
+      embed_fwd_lists_kernel<DT, N, 0><<<blocks, 64 * kSortWaves, 0, s>>>(a, t, to, sort_blocks);
   });
   return launch_status();
 }
@@ -476,13 +553,15 @@ extern "C" int tmac_embed_bwd_workspace(int64_t n_tokens, int64_t V, int64_t n_p
   if (n_tokens < 0 || n_tokens > kMaxRows || V < 0 || V > kMaxRows || n_pos < 0 || n_pos > kMaxRows || d <= 0 ||
       d > kMaxD)
     return TMAC_ERR_SHAPE;
-  *ws_bytes = grad_ws(n_tokens, V > n_pos ? V : n_pos, d).total;  // the two sorts take turns
+  // one list at a time: the two sorts take turns
+  *ws_bytes = lists_at(n_tokens, V > n_pos ? V : n_pos).total + part_bytes(n_tokens, d);
   return TMAC_OK;
 }
 
-extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_g, int64_t ldg, void* d_dW,
-                              void* d_dP, void* d_dprefix, void* d_ws, size_t ws_bytes, int B, int T, int n_prefix,
-                              int d, int64_t V, int64_t n_pos, float scale, int dtype, void* stream) {
+extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_lists, const void* d_g,
+                              int64_t ldg, void* d_dW, void* d_dP, void* d_dprefix, void* d_ws, size_t ws_bytes, int B,
+                              int T, int n_prefix, int d, int64_t V, int64_t n_pos, float scale, int dtype,
+                              void* stream) {
   const int st = check_sizes(B, T, n_prefix, d, dtype);
   if (st != TMAC_OK) return st;
   const bool sums = d_dP && !d_pos;  // positions 0 .. T - 1: plain sums, no sort
@@ -491,17 +570,20 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
     return TMAC_ERR_SHAPE;
   const int n_tok = B * T;
   if ((n_tok > 0 || (B > 0 && d_dprefix)) && !d_g) return TMAC_ERR_NULL;
-  if (d_dW && n_tok > 0 && !d_ids) return TMAC_ERR_NULL;
+  if (d_dW && n_tok > 0 && !d_ids && !d_lists) return TMAC_ERR_NULL;
+  if (d_lists && !row_aligned16(d_lists)) return TMAC_ERR_ALIGN;
+  const int64_t v_sort = d_dW && !d_lists ? V : 0, p_sort = d_dP && d_pos ? n_pos : 0;
   size_t need = 0;
-  if (d_dW || (d_dP && d_pos)) tmac_embed_bwd_workspace(n_tok, d_dW ? V : 0, d_dP && d_pos ? n_pos : 0, d, &need);
+  if (d_dW || p_sort) tmac_embed_bwd_workspace(n_tok, v_sort, p_sort, d, &need);
   if (need && (!d_ws || ws_bytes < need)) return TMAC_ERR_WORKSPACE;
   if (need && !row_aligned16(d_ws)) return TMAC_ERR_ALIGN;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool wide = d % (dtype == TMAC_F32 ? 4 : 8) == 0 && row_aligned16(d_dW) && row_aligned16(d_dP) &&
                     row_aligned16(d_dprefix) && wide_rows(d_g, ldg, dtype);
+  const size_t part_at = lists_at(n_tok, v_sort > p_sort ? v_sort : p_sort).total;
 
-  // three launches by sorted tokens (`out`), one for the sums alone
-  auto part = [&](const int64_t* index, void* out, int64_t n_rows, float factor, bool with_sums) {
+  // the gradient `out` of a table by sorted tokens (its lists given, or made of `index`), the sums beside it
+  auto part = [&](const int64_t* index, const void* given, void* out, int64_t n_rows, float factor, bool with_sums) {
     Grad a{};
     a.g = static_cast<const uint8_t*>(d_g);
     a.ldg = ldg;
@@ -516,28 +598,22 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
       a.last = n_prefix + (sums ? static_cast<int>(n_pos) : 0);
     }
     if (out) {
-      uint8_t* const ws = static_cast<uint8_t*>(d_ws);
-      const GradWs w = grad_ws(n_tok, n_rows, d);
-      int32_t* const row_start = reinterpret_cast<int32_t*>(ws);
-      int32_t* const perm = reinterpret_cast<int32_t*>(ws + w.perm);
-      int32_t* const key = reinterpret_cast<int32_t*>(ws + w.key);
-      a.row_start = row_start;
-      a.perm = perm;
-      a.key = key;
-      a.part = reinterpret_cast<float*>(ws + w.part);
+      const Lists to = lists(given ? const_cast<void*>(given) : d_ws, n_tok, n_rows);
+      a.row_start = to.row_start;
+      a.perm = to.perm;
+      a.key = to.key;
+      a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + part_at);
       a.dW = static_cast<uint8_t*>(out);
       a.V = static_cast<int>(n_rows);
       a.scale = factor;
       a.chunks = n_tok > kList ? (n_tok + kList - 1) / kList : 0;
-      const uint32_t T_inv = T > 1 ? static_cast<uint32_t>((1ull << 32) / static_cast<uint32_t>(T)) : 0;
-      auto sort = [&](auto held) {
-        embed_sort_kernel<decltype(held)::value><<<n_ranges(a.V), 64 * kSortWaves, 0, s>>>(
-            index, n_tok, T, T_inv, n_prefix, a.V, row_start, perm, key);
-      };
-      if (n_tok <= 4 * 64 * kSortWaves)
-        sort(std::integral_constant<int, 4>{});
-      else
-        sort(std::integral_constant<int, 0>{});
+      if (!given) {
+        const Tokens t = tokens(index, n_tok, T, n_prefix, n_rows);
+        if (held(n_tok))
+          embed_sort_kernel<kHeld><<<n_ranges(n_rows), 64 * kSortWaves, 0, s>>>(t, to);
+        else
+          embed_sort_kernel<0><<<n_ranges(n_rows), 64 * kSortWaves, 0, s>>>(t, to);
+      }
     }
     dispatch(dtype, wide, [&](auto dt, auto n) {
       constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
@@ -555,9 +631,9 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
   };
   const bool any_sums = sums || d_dprefix;
   if (d_dW)
-    part(d_ids, d_dW, V, scale, any_sums);
+    part(d_ids, d_lists, d_dW, V, scale, any_sums);
   else if (any_sums)
-    part(nullptr, nullptr, 0, 1.f, true);
-  if (d_dP && d_pos) part(d_pos, d_dP, n_pos, 1.f, false);
+    part(nullptr, nullptr, nullptr, 0, 1.f, true);
+  if (p_sort) part(d_pos, nullptr, d_dP, n_pos, 1.f, false);
   return launch_status();
 }

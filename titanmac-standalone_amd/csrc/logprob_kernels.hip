@@ -550,11 +550,12 @@ __global__ __launch_bounds__(1024) void logprob_mean_kernel(const float* __restr
 // ------------------------------------------------------------------ host
 
 constexpr int64_t kMaxRows = 1 << 30, kMaxV = 1 << 28;
-constexpr int kMaxGrid = 1 << 21;    // workgroups of a launch; they take turns beyond that
+constexpr int kMaxGrid = 1 << 21;  // workgroups of a launch; they take turns beyond that
 // Threads of a row: 128 below 32 KB (us, 128 / 256 / 512 threads: 20000 rows of 1000 bf16 18 / 28 / 50, 8000 of
 // 8000 24 / 24 / 31), then 512 (8192 of 128000: 382 / 351 / 344), with alternatives 256 (4096 of 128000: five of
 // them 201 / 197 / 214, twenty 209 / 200 / 218, 64 568 / 243 / 230).
 constexpr int kShortRow = 32 << 10;
+constexpr int kFewRows = 1024;  // whole rows with alternatives up to which 512 threads take one (16 rows: 12.4 us, 256: 14.7)
 
 int check(int B, int T, int64_t V, int64_t st, int64_t sb, int dtype) {
   if (dtype != TMAC_F32 && dtype != TMAC_BF16 && dtype != TMAC_F16) return TMAC_ERR_DTYPE;
@@ -568,10 +569,13 @@ int launch_status() {
   return err == hipSuccess ? TMAC_OK : static_cast<int>(err);
 }
 
-// Workgroups per row: about 1024 in all, of at least 1024 groups (16 KB) of the row each. One row of 128000 fp32
-// with 64 alternatives: 13.4 us, with 512 or 256 groups 15.2 and 18.6 (more lists to join).
+// Workgroups per row: one below 8192 groups (128 KB), whose second launch costs more than it gains (16 rows of 50000
+// bf16 with twenty alternatives: 12.4 us, in six parts 13.5; 200 rows 11.9 against 17.4), else about 1024 in all,
+// of at least 1024 groups each (16 rows of 128000 bf16: 13.5 us, of 4096 groups 15.7, whole rows 18.6; one row of
+// 128000 fp32 with 64 alternatives 13.4, of 256 groups 18.6: more lists to join).
 int row_parts(int rows, int64_t V, int dtype) {
   const int64_t groups = (V + (dtype == TMAC_F32 ? 3 : 7)) / (dtype == TMAC_F32 ? 4 : 8);
+  if (groups < 8192) return 1;
   int64_t parts = 1024 / (rows > 0 ? rows : 1);
   const int64_t most = groups / 1024;
   if (parts > most) parts = most;
@@ -646,8 +650,10 @@ extern "C" int tmac_logprob_fwd(const void* d_z, int64_t stride_b, int64_t strid
         };
         if (parts == 1 && V * E < kShortRow)
           launch(std::integral_constant<int, 128>{});
+        else if (TOP && (parts > 1 || rows > kFewRows))
+          launch(std::integral_constant<int, 256>{});
         else
-          launch(std::integral_constant<int, TOP ? 256 : 512>{});
+          launch(std::integral_constant<int, 512>{});
       });
     });
     if (parts > 1)

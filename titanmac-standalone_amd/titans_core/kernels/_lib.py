@@ -100,11 +100,12 @@ SIGNATURES = {
                         ctypes.c_float, _i, _vp, _vp, _sz, _i, _vp],
     "tmac_silu_bwd": [_vp, _vp, _vp, _i64, _i, _vp],
     "tmac_mse_grad": [_vp, _vp, _vp, _i64, ctypes.c_float, _i, _vp],
-    "tmac_embed_fwd": [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _i64, _i64,
+    "tmac_embed_lists_bytes": [_i64, _i64, ctypes.POINTER(_sz)],
+    "tmac_embed_fwd": [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _i, _i, _i, _i, _i64, _i64,
                        ctypes.c_float, _i, _vp],
     "tmac_embed_bwd_workspace": [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)],
-    "tmac_embed_bwd": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i64, _i64, ctypes.c_float, _i,
-                       _vp],
+    "tmac_embed_bwd": [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i64, _i64, ctypes.c_float,
+                       _i, _vp],
     "tmac_logprob_workspace": [_i, _i, _i64, _i, _i, ctypes.POINTER(_sz)],
     "tmac_logprob_fwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _i, _i, _i64, _i, _vp],
     "tmac_logprob_bwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i, _vp],

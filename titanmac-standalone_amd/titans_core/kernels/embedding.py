@@ -7,7 +7,8 @@ The model looks its tokens up, adds the rows of their positions and puts the per
     out[b, Np + t] = scale * weight[ids[b, t]] + pos_weight[position(b, t)]
 
 ``token_embedding`` does that in one launch. Its gradients are dense, as ``nn.Embedding``'s: the tokens are
-sorted by id and each row's sum is formed in order (deterministic, fp32) and written once.
+sorted by id (where the table needs a gradient, in the lookup's launch) and each row's sum is formed in order
+(deterministic, fp32) and written once.
 """
 from __future__ import annotations
 
@@ -69,10 +70,16 @@ def _index(t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tens
     return t.expand(like.shape).to(torch.int64).contiguous()
 
 
+def _lists_bytes(n_tokens: int, V: int) -> int:
+    """tmac_embed_lists_bytes (in Python, for sizes that are symbols)."""
+    return (4 * V + 19) // 16 * 16 + 2 * ((4 * n_tokens + 15) // 16 * 16)
+
+
 def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor],
-                     positions: Optional[torch.Tensor], prefix: Optional[torch.Tensor],
-                     scale: float) -> torch.Tensor:
-    """[B, Np + T, d] in weight's dtype."""
+                     positions: Optional[torch.Tensor], prefix: Optional[torch.Tensor], scale: float,
+                     make_lists: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """([B, Np + T, d] in weight's dtype, the tokens of each row of weight as the backward reads them, or an empty
+    tensor)."""
     _check(ids, weight, pos_weight, positions, prefix)
     code = _lib.dtype_code(weight.dtype)
     dev = _lib.require_device(*(t for t in (weight, ids, pos_weight, positions, prefix) if t is not None),
@@ -80,39 +87,42 @@ def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Option
     (B, T), (V, d) = ids.shape, weight.shape
     n_prefix = 0 if prefix is None else prefix.shape[0]
     out = torch.empty((B, n_prefix + T, d), dtype=weight.dtype, device=dev)
-    if out.numel() == 0:
-        return out
+    nb = _lists_bytes(B * T, V) if make_lists else 0
+    lists = torch.empty(nb, dtype=torch.uint8, device=dev) if make_lists else out.new_empty(0, dtype=torch.uint8)
+    if out.numel() == 0 and not make_lists:
+        return out, lists
     i, q = _index(ids, ids), _index(positions, ids)
     (w, ldw), (p, ldp), (f, ldf) = _table(weight), _table(pos_weight), _table(prefix)
     with _lib.device_guard(dev):
         rc = _lib.lib().tmac_embed_fwd(i.data_ptr(), _lib.ptr(q), w.data_ptr(), ldw, _lib.ptr(p), ldp, _lib.ptr(f), ldf,
-                                       out.data_ptr(), B, T, n_prefix, d, V, 0 if p is None else p.shape[0], scale,
-                                       code, _lib.stream_ptr(dev))
+                                       out.data_ptr(), lists.data_ptr() if make_lists else 0, nb, B, T, n_prefix, d, V,
+                                       0 if p is None else p.shape[0], scale, code, _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_embed_fwd")
-    return out
+    return out, lists
 
 
 token_embedding_fwd = torch.library.custom_op("titanmac::token_embedding", mutates_args=())(_token_embedding)
 
 
 @token_embedding_fwd.register_fake
-def _(ids, weight, pos_weight, positions, prefix, scale):
-    n_prefix = 0 if prefix is None else prefix.shape[0]
-    return weight.new_empty((ids.shape[0], n_prefix + ids.shape[1], weight.shape[1]))
+def _(ids, weight, pos_weight, positions, prefix, scale, make_lists):
+    n_prefix, (B, T) = 0 if prefix is None else prefix.shape[0], ids.shape
+    nb = _lists_bytes(B * T, weight.shape[0]) if make_lists else 0
+    return weight.new_empty((B, n_prefix + T, weight.shape[1])), weight.new_empty((nb,), dtype=torch.uint8)
 
 
 @lru_cache(maxsize=256)
-def _workspace(n_tokens: int, V: int, n_pos: int, d: int) -> int:
-    if V == 0 and n_pos == 0:
+def _workspace(n_tokens: int, V: int, n_pos: int, d: int, need_w: bool) -> int:
+    if not need_w and n_pos == 0:
         return 0
     nb = ctypes.c_size_t(0)
     _lib.check(_lib.lib().tmac_embed_bwd_workspace(n_tokens, V, n_pos, d, ctypes.byref(nb)), "tmac_embed_bwd_workspace")
     return nb.value
 
 
-def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optional[torch.Tensor], n_prefix: int,
-                         V: int, n_pos: int, scale: float, need_w: bool, need_p: bool,
-                         need_f: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optional[torch.Tensor],
+                         lists: Optional[torch.Tensor], n_prefix: int, V: int, n_pos: int, scale: float,
+                         need_w: bool, need_p: bool, need_f: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of weight [V, d], pos_weight [n_pos, d] and prefix [n_prefix, d] in grad's dtype; empty where
     not needed."""
     dev = _lib.require_device(*(t for t in (grad, ids, positions) if t is not None), what="token_embedding backward")
@@ -121,13 +131,13 @@ def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optio
     ldg = d if g is grad else max(g.stride(0), d)
     dw, dp, df = (torch.empty((n if need else 0, d), dtype=grad.dtype, device=dev)
                   for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
-    i, q = _index(ids, ids), _index(positions, ids) if need_p else None
-    nb = _workspace(B * T, V if need_w else 0, n_pos if q is not None else 0, d)
+    i, q = _index(ids, ids) if lists is None else None, _index(positions, ids) if need_p else None
+    nb = _workspace(B * T, V if need_w and lists is None else 0, n_pos if q is not None else 0, d, need_w)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_embed_bwd(i.data_ptr(), _lib.ptr(q), g.data_ptr(), ldg, dw.data_ptr() if need_w else 0,
-                                       dp.data_ptr() if need_p else 0, df.data_ptr() if need_f and n_prefix else 0,
-                                       ws.data_ptr(), nb, B, T, n_prefix, d, V, n_pos, scale,
+        rc = _lib.lib().tmac_embed_bwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(lists), g.data_ptr(), ldg,
+                                       dw.data_ptr() if need_w else 0, dp.data_ptr() if need_p else 0,
+                                       df.data_ptr() if need_f and n_prefix else 0, ws.data_ptr(), nb, B, T, n_prefix, d, V, n_pos, scale,
                                        _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_embed_bwd")
     return dw, dp, df
@@ -138,20 +148,20 @@ token_embedding_bwd = torch.library.custom_op("titanmac::token_embedding_bwd",
 
 
 @token_embedding_bwd.register_fake
-def _(grad, ids, positions, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
+def _(grad, ids, positions, lists, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
     d = grad.shape[-1]
     return tuple(grad.new_empty((n if need else 0, d))
                  for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
 
 
 def _setup(ctx, inputs, output):
-    ids, weight, pos_weight, positions, prefix, scale = inputs
-    ctx.save_for_backward(ids, positions)
+    ids, weight, pos_weight, positions, prefix, scale, make_lists = inputs
+    ctx.save_for_backward(ids, positions, output[1] if make_lists else None)
     ctx.sizes = (0 if prefix is None else prefix.shape[0], weight.shape[0],
                  0 if pos_weight is None else pos_weight.shape[0], scale)
 
 
-def _composed(grad, ids, positions, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
+def _composed(grad, ids, positions, lists, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
     """The gradients in torch's operations, for a backward that is itself differentiated."""
     g = grad[:, n_prefix:].float()
 
@@ -168,16 +178,16 @@ def _composed(grad, ids, positions, n_prefix, V, n_pos, scale, need_w, need_p, n
             grad[:, :n_prefix].float().sum(0).to(grad.dtype) if need_f else None)
 
 
-def _backward(ctx, grad):
-    ids, positions = ctx.saved_tensors
+def _backward(ctx, grad, *_):
+    ids, positions, lists = ctx.saved_tensors
     need = [ctx.needs_input_grad[i] for i in (1, 2, 4)]
-    args = (grad, ids, positions, *ctx.sizes, *need)
+    args = (grad, ids, positions, lists, *ctx.sizes, *need)
     if torch.is_grad_enabled() and grad.requires_grad:
         dw, dp, df = _composed(*args)
     else:
         op = _token_embedding_bwd if _lib.direct_backward(grad, ids) else token_embedding_bwd
         dw, dp, df = op(*args)
-    return (None, dw if need[0] else None, dp if need[1] else None, None, df if need[2] else None, None)
+    return (None, dw if need[0] else None, dp if need[1] else None, None, df if need[2] else None, None, None)
 
 
 token_embedding_fwd.register_autograd(_backward, setup_context=_setup)
@@ -195,10 +205,11 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optiona
     position outside its table, gives a row of NaN and adds to no gradient.
 
     Differentiable in the three tables (a second time too)."""
-    args = (ids, weight, pos_weight, positions, prefix, float(scale))
     tables = (ids, weight, pos_weight, positions, prefix)
+    # a training step's lists of tokens are made beside the lookup
+    args = (*tables, float(scale), torch.is_grad_enabled() and weight.requires_grad)
     if _lib.direct_call(*tables):
-        return _token_embedding(*args)
+        return _token_embedding(*args)[0]
     if _lib.eager_native(*tables):
         return _native(*args)
-    return token_embedding_fwd(*args)
+    return token_embedding_fwd(*args)[0]
