@@ -59,6 +59,27 @@ def test_logprob_refusals():
         tc.token_logprobs(torch.zeros(2, 100), t, top_k=65)
 
 
+def test_sizes_past_the_kernels_integers_are_refused():
+    """More rows than the kernels count in 32 bits: refused by shape, before anything is read."""
+    one = torch.zeros(1, dtype=torch.bfloat16)
+    for n in ((1 << 30) + 1, (1 << 32) + 5):
+        ids, z = torch.zeros(1, dtype=torch.long).expand(n), one.expand(n, 1)
+        for f in (tc.token_logprobs, tc.token_cross_entropy):
+            with pytest.raises(ValueError, match="rows"):
+                f(z, ids)
+        with pytest.raises(ValueError, match="rows"):
+            tc.head_logprobs(one.expand(n, 64), one.expand(10, 64), ids)
+        w = one.expand(5, 8)
+        for args, kw in (((ids.view(n, 1), w), {}), ((ids.view(1, n), w), {}), ((ids[:0].expand(n, 0), w), {}),
+                         ((ids[:0].expand(n, 0), w), {"prefix": w[:1]}), ((ids[:1].view(1, 1), one.expand(n, 8)), {}),
+                         ((ids[:1].view(1, 1), w, one.expand(n, 8)), {}), ((ids[:1].view(1, 1), one.expand(5, n)), {})):
+            with pytest.raises(ValueError, match="rows"):
+                tc.token_embedding(*args, **kw)
+    for f in (tc.token_logprobs, tc.token_cross_entropy):
+        with pytest.raises(ValueError, match="vocabulary"):
+            f(one.expand(2, (1 << 28) + 1), torch.zeros(2, dtype=torch.long))
+
+
 def test_fake_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():

@@ -22,6 +22,7 @@ from . import _lib
 from .norm import _rows
 
 _INDEX = (torch.int64, torch.int32)
+_MAX_ROWS, _MAX_D = 1 << 30, 1 << 20  # of the result and of a table; of a row
 
 
 def _table(t: Optional[torch.Tensor]):
@@ -62,6 +63,10 @@ def _check(ids, weight, pos_weight, positions, prefix) -> None:
         if positions is None and ids.shape[1] > pos_weight.shape[0]:
             raise ValueError(f"token_embedding: {ids.shape[1]} positions, but pos_weight has "
                              f"{pos_weight.shape[0]} rows")
+    rows = ids.shape[0] * (ids.shape[1] + (0 if prefix is None else prefix.shape[0]))
+    if (max(rows, weight.shape[0], 0 if pos_weight is None else pos_weight.shape[0]) > _MAX_ROWS
+            or max(ids.shape) > _MAX_ROWS or weight.shape[1] > _MAX_D):
+        raise ValueError(f"token_embedding: up to {_MAX_ROWS} rows of up to {_MAX_D} values")
 
 
 def _index(t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -137,8 +142,8 @@ def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optio
     with _lib.device_guard(dev):
         rc = _lib.lib().tmac_embed_bwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(lists), g.data_ptr(), ldg,
                                        dw.data_ptr() if need_w else 0, dp.data_ptr() if need_p else 0,
-                                       df.data_ptr() if need_f and n_prefix else 0, ws.data_ptr(), nb, B, T, n_prefix, d, V, n_pos, scale,
-                                       _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
+                                       df.data_ptr() if need_f and n_prefix else 0, ws.data_ptr(), nb, B, T,
+                                       n_prefix, d, V, n_pos, scale, _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_embed_bwd")
     return dw, dp, df
 
@@ -200,7 +205,7 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optiona
     """scale * weight[ids] + pos_weight[positions], behind the rows of prefix: [B, Np + T, d].
 
     ids: int64 or int32 [B, T]; weight [V, d], pos_weight [n_pos, d] and prefix [Np, d] of one dtype
-    (float32, bfloat16, float16), any d. positions: [B, T] or [T], by default 0 .. T - 1. The sum is formed in
+    (float32, bfloat16, float16), d up to 2^20, up to 2^30 rows. positions: [B, T] or [T], by default 0 .. T - 1. The sum is formed in
     fp32 and rounded once. Nothing is copied to the host to look at the ids: one outside [0, V), or a
     position outside its table, gives a row of NaN and adds to no gradient.
 

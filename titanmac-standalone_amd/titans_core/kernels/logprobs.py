@@ -23,6 +23,7 @@ from . import _lib
 from .linear import _HALF, _MAX_PITCH, _rows
 
 MAX_TOP = 64
+_MAX_ROWS, _MAX_V = 1 << 30, 1 << 28
 _INDEX = (torch.int64, torch.int32)
 
 
@@ -42,6 +43,13 @@ def _check(logits: torch.Tensor, targets: torch.Tensor, what: str) -> None:
                          f"{tuple(targets.shape)}")
     if targets.dtype not in _INDEX:
         raise TypeError(f"{what}: targets must be int64 or int32, got {targets.dtype}")
+    _check_sizes(targets, logits.shape[-1], what)
+
+
+def _check_sizes(targets: torch.Tensor, V: int, what: str) -> None:
+    if targets.numel() > _MAX_ROWS or max(targets.shape, default=0) > _MAX_ROWS or V > _MAX_V:
+        raise ValueError(f"{what}: up to {_MAX_ROWS} rows of a vocabulary of up to {_MAX_V}, got {tuple(targets.shape)} "
+                         f"of {V}")
 
 
 def _rows3(z: torch.Tensor):
@@ -212,7 +220,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool
     """Log probabilities of `targets` under softmax(logits), with what else is asked of each row.
 
     logits [..., V] (float32, bfloat16, float16; any strides, read in place where a row's values are
-    neighbours), targets int64 or int32 [...]. Results, fp32:
+    neighbours), V up to 2^28 and up to 2^30 rows, targets int64 or int32 [...]. Results, fp32:
 
     - logprobs [...]: log softmax(logits)[target]; 0 where target == ignore_index, and NaN for any other
       target outside [0, V) (nothing is copied to the host to look at them);
@@ -340,6 +348,7 @@ def _check_head(hidden, weight, targets) -> None:
                          f"{tuple(hidden.shape)}, got {tuple(targets.shape)}")
     if targets.dtype not in _INDEX:
         raise TypeError(f"head_logprobs: targets must be int64 or int32, got {targets.dtype}")
+    _check_sizes(targets, weight.shape[0], "head_logprobs")
 
 
 def head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, entropy: bool = False,
