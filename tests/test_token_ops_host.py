@@ -191,6 +191,23 @@ def test_differentiable_gradients_match_autograd():
     assert torch.allclose(df, g[:, :2].sum(0))
 
 
+def test_differentiable_gradient_of_ignored_and_refused_rows():
+    """Ignored rows are zeros and not read, a target outside the vocabulary makes its row NaN: in the differentiable
+    form as in the kernel, the loss without any target (a gradient of NaN) among them."""
+    z, t = torch.randn(3, 5), torch.tensor([1, -100, 7])
+    z[1, 2] = float("nan")
+    z.requires_grad_()
+    gl = torch.tensor([1.0, float("nan"), 1.0])
+    first = kl._composed(gl, None, z, t, -100)
+    assert torch.all(first[1] == 0) and torch.isfinite(first[0]).all() and torch.isnan(first[2]).all()
+    second, = torch.autograd.grad((first[:2] * torch.randn(2, 5)).sum(), z)
+    assert torch.all(second[1] == 0) and torch.isfinite(second[0]).all()
+    assert torch.all(kl._composed(torch.full((3,), float("nan")), None, z, torch.full((3,), -100), -100) == 0)
+    # the entropy's gradient does not look at the target
+    only = kl._composed(None, torch.ones(3), z, t, -100)
+    assert torch.isfinite(only[[0, 2]]).all() and torch.isnan(only[1]).all()
+
+
 def test_exported_from_the_package():
     assert _lib.SIGNATURES["tmac_embed_fwd"] and set(tc.__all__) >= {
         "token_embedding", "token_logprobs", "token_cross_entropy", "TokenLogprobs"}

@@ -168,12 +168,15 @@ def _(g_lp, g_ent, logits, targets, stats, entropy, ignore_index):
 
 def _composed(g_lp, g_ent, logits, targets, ignore_index):
     """The gradient in torch's operations, for a backward that is itself differentiated."""
+    given = targets != ignore_index
+    if g_ent is None:  # ignored rows are not read
+        logits = torch.where(given.unsqueeze(-1), logits, 0.0)
     logp = torch.log_softmax(logits.float(), dim=-1)
     p = logp.exp()
     dz = torch.zeros_like(p)
     if g_lp is not None:
-        given = targets != ignore_index
-        g = (g_lp.float() * given).unsqueeze(-1)
+        outside = given & ((targets < 0) | (targets >= p.shape[-1]))  # lp is NaN
+        g = torch.where(given, g_lp.float(), 0.0).masked_fill(outside, float("nan")).unsqueeze(-1)
         at = torch.arange(p.shape[-1], device=p.device) == targets.unsqueeze(-1)
         dz = dz + g * (at.to(p.dtype) - p)
     if g_ent is not None:
