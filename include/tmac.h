@@ -729,7 +729,8 @@ int tmac_logprob_fwd(const void* d_z, int64_t stride_b, int64_t stride_t, const 
 
 /* dz[b, t, j] = g_lp (δ_{j,target} − p_j) − g_H p_j (ln p_j + H), contiguous [B, T, V] in dtype, from the
  * forward's stats and entropy. g_lp, g_entropy (nullable): fp32, one per row at the given stride (0: one
- * value for all). Rows of which nothing was asked are zeros, and not read. */
+ * value for all). Rows of which nothing was asked are zeros, and not read; with g_lp, a target outside [0, V) makes
+ * its row NaN. */
 int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t stride_t, const int64_t* d_targets,
                      int64_t ignore_index, const float* d_stats, const float* d_entropy, const float* d_g_lp,
                      int64_t g_lp_stride, const float* d_g_entropy, int64_t g_entropy_stride, void* d_dz, int B, int T,

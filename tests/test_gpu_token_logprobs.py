@@ -326,6 +326,17 @@ def test_dispatched_op_agrees(dev):
     assert torch.equal(torch.autograd.grad(loss, z)[0], torch.autograd.grad(own, z)[0])
 
 
+def test_entropy_gradient_without_a_target(dev):
+    """The entropy's gradient alone does not look at the targets: any of them, the same bits."""
+    z = logits(dev, (4, 300), torch.float32).requires_grad_()
+    g = torch.tensor([1.0, -2.0, 0.5, 3.0], device=dev)
+    grads = []
+    for t in ([-100] * 4, [5, 300, -1, 1 << 40]):
+        ent = tc.token_logprobs(z, torch.tensor(t, device=dev), entropy=True).entropy
+        grads.append(torch.autograd.grad(ent, z, g)[0])
+    assert torch.isfinite(grads[0]).all() and torch.equal(*grads)
+
+
 @pytest.mark.parametrize("M,V", [(4, 30000), (600, 2000)])
 def test_other_stream_and_graph(dev, M, V):
     z, t = logits(dev, (M, V), torch.bfloat16).requires_grad_(), targets(dev, (M,), V)

@@ -441,8 +441,8 @@ __device__ __forceinline__ void logprob_grad_chunk(
   const int row = static_cast<int>(block / chunks);
   const int chunk = static_cast<int>(block - static_cast<int64_t>(row) * chunks);
   const int64_t target = targets[row];
-  const bool given = target != ignore;
-  const float gl = given && g_lp ? g_lp[row * g_lp_st] : 0.f;
+  const bool given = g_lp && target != ignore;
+  const float gl = given ? g_lp[row * g_lp_st] : 0.f;
   const float ge = ENT ? g_ent[row * g_ent_st] : 0.f;
   const float mu = stats[2 * static_cast<int64_t>(row)], s = stats[2 * static_cast<int64_t>(row) + 1];
   const float inv = 1.f / s, log_s = __builtin_amdgcn_logf(s) * kLn2;
