@@ -134,3 +134,29 @@ def test_values_by_resident_rows(dev, M, V, K, dtype):
     check(x, w, t, r)
     q = tc.head_logprobs(x, w, t)
     assert torch.equal(q.logprobs, r.logprobs)
+
+
+@pytest.mark.parametrize("K", [512, 768, 1024])
+def test_resident_rows_without_a_distribution(dev, K):
+    """NaN and infinite hidden states, targets outside the vocabulary, an entry of -inf in either half of K, and one
+    that is the last of a partial tile."""
+    x, w, t = inputs(dev, 700, 40003, K, torch.bfloat16)
+    t[:7] = torch.tensor([-1, 40003, 2 ** 40, 3, 4, 5, 40002], device=dev)
+    x[3, K - 1] = float("nan")
+    x[4, 0] = float("inf")
+    r = tc.head_logprobs(x, w, t, entropy=True)
+    assert torch.isnan(r.logprobs[:5]).all() and torch.isnan(r.entropy[3:5]).all()
+    ok = torch.ones(700, dtype=torch.bool, device=dev)
+    ok[:5] = False
+    check(x[ok], w, t[ok], tc.TokenLogprobs(r.logprobs[ok], r.entropy[ok]))
+    x, w, t = inputs(dev, 700, 40003, K, torch.bfloat16)
+    x[:, 0], x[:, K - 1] = x[:, 0].abs() + 0.1, x[:, K - 1].abs() + 0.1
+    w[17, 0] = w[40002, K - 1] = float("-inf")
+    t = t.masked_fill((t == 17) | (t == 40002), 3)
+    t[0], t[1] = 17, 40002
+    r = tc.head_logprobs(x, w, t, entropy=True)
+    assert torch.isneginf(r.logprobs[:2]).all()
+    keep = torch.ones(40003, dtype=torch.bool, device=dev)
+    keep[17] = keep[40002] = False
+    rest = (t - (t > 17).long()).masked_fill(t == -100, -100)[2:]
+    check(x[2:], w[keep], rest, tc.TokenLogprobs(r.logprobs[2:], r.entropy[2:]))

@@ -194,28 +194,33 @@ __global__ __launch_bounds__(256, 2) void head_kernel(
   }
 }
 
-// The same for K = 64 KS UNITS of up to 640 and rows enough to fill tiles of 256: a wave keeps its 64 rows of X in
-// registers as MFMA operands for the whole strip (2 K / 4 of them), so only the weight passes through LDS: 32
-// entries at a time, each 1 KB operand read feeding two MFMAs. Per CU that is 64 bytes per clock of LDS reads
-// and 16 of copies at the full MFMA rate, where the kernel above needs 107 of 128 and 53 of 54. One wave per
-// SIMD, so the statistics of one tile (a third of its MFMAs' time on the vector ALU) run beside the MFMAs of
-// the next, a few instructions after each, and so do the copies. Four LDS stages; copies are two tiles ahead;
-// the barrier that hands a stage over stands in the middle of the tile before, away from the first use.
-// MI = 1, for K of 768 and 1024: 32 rows a wave, and a tile in two units of half the K.
+// The same for rows enough to fill its tiles and K = 64 KS of up to 640: a wave keeps its 64 rows of X in registers
+// as MFMA operands for the whole strip (2 K / 4 of them), so only the weight passes through LDS: 32 entries at a
+// time, each 1 KB operand read feeding two MFMAs. Per CU that is 64 bytes per clock of LDS reads and 16 of copies
+// at the full MFMA rate, where the kernel above needs 107 of 128 and 53 of 54. One wave per SIMD, so the statistics
+// of one tile (a third of its MFMAs' time on the vector ALU) run beside the MFMAs of the next, a few instructions
+// after each, and so do the copies. Four LDS stages; copies are two tiles ahead; the barrier that hands a stage
+// over stands in the middle of the tile before, away from the first use.
+// SPLIT = 2, for K = 128 KS of 768 and 1024: two waves share 64 rows, each with half of K in its registers, and
+// exchange products through LDS so that each finishes 32 of the rows; a tile comes in two units, of half of both
+// halves. 1503 x 1024 x 50001 fp16 with entropy 154 us, 159 with 32 rows of all of K a wave (an operand read for
+// each MFMA: 128 bytes per clock of LDS); 8192 x 1024 x 32000 454 and 468.
 // 8192 x 640 x 128000 bf16: 1047 us (1.28 PFLOP/s; the library's product of large squares 1.37), 1434 with the
 // kernel above; with all copies at once after the barrier 1076; with the statistics left to the compiler's
 // schedule, which puts them behind the MFMAs, 1119.
 constexpr int kTile = 32, kStages = 4;
 constexpr int kAhead = 2;  // k-steps that a weight operand is read ahead of its MFMAs (of 4 registers' turns)
 
-template <int DT, bool ENT, int KS, int UNITS, int MI>
+template <int DT, bool ENT, int KS, int SPLIT>
 __global__ __launch_bounds__(256, 1) void head_rows_kernel(
     const uint16_t* __restrict__ X, int64_t ldx, const uint16_t* __restrict__ W, int64_t ldw,
     const int64_t* __restrict__ targets, int M, int V, int n_mt, int n_nt, int n_strips, int per_strip,
     Part* __restrict__ parts, float* __restrict__ zt, int per_xcd) {
-  // k-steps of 16 of a unit and of a tile; elements of a 64-wide slab and of a unit
-  constexpr int kK = 4 * KS, kAll = UNITS * kK, kSlab = kTile * 64, kStage = KS * kSlab;
-  __shared__ __attribute__((aligned(16))) uint16_t smem[kStages * kStage];
+  // a wave's k-steps of 16 of a unit and of a tile; elements of a 64-wide slab and of a unit
+  constexpr int kK = 4 * KS / SPLIT, kAll = 4 * KS, kSlab = kTile * 64, kStage = KS * kSlab;
+  constexpr int kOwn = 2 / SPLIT;  // of the wave's two blocks of 32 rows, those whose statistics it keeps
+  constexpr int kGive = SPLIT == 2 ? 4 * 1024 : 0;  // values of the halves' exchange
+  __shared__ __attribute__((aligned(16))) uint16_t smem[kStages * kStage + 2 * kGive];
 
   const int logical = xcd_logical_id(per_xcd);
   if (logical >= n_mt * n_strips) return;
@@ -225,7 +230,9 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int l32 = lane & 31, h = lane >> 5;
-  const int m0 = (logical - strip * n_mt) * (128 * MI) + 32 * MI * wave;
+  const int half = SPLIT == 2 ? wave & 1 : 0;  // of K
+  const int m0 = (logical - strip * n_mt) * (256 / SPLIT) + 64 * (wave / SPLIT);
+  const int row0[2] = {m0 + 32 * half, m0 + 32 * (1 - half)};  // the wave's own block of rows first
 
   // Each wave copies entries 8 wave .. 8 wave + 7 of every slab of a unit (xswz in each slab; entries past V
   // read the last one).
@@ -233,18 +240,20 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
   const uint32_t cchunk = 16u * static_cast<uint32_t>((lane & 7) ^ ((crow >> 1) & 7));
   const uint32_t lds0 = lds_offset(smem) + static_cast<uint32_t>(wave * 1024);
   auto issue = [&](int i, int part, int stage, int s) {  // slab s of a unit of tile i (past the strip: its last)
+    constexpr int kOf = KS / SPLIT;  // slabs of a unit that lie in one half of K
+    const int slab = s / kOf * KS + part * kOf + s % kOf;
     const int e0 = (t0 + min(i, n_tiles - 1)) * kTile;
     const uint32_t off = static_cast<uint32_t>(min(crow, V - 1 - e0)) * static_cast<uint32_t>(2 * ldw) + cchunk;
-    dma_lds16(W + static_cast<int64_t>(e0) * ldw + 64 * (KS * part + s), off,
+    dma_lds16(W + static_cast<int64_t>(e0) * ldw + 64 * slab, off,
               lds0 + static_cast<uint32_t>((stage * kStage + s * kSlab) * 2));
   };
 
-  u32x4 x[MI][kAll];
-  int target[MI];  // −1: no entry of this row is asked for
+  u32x4 x[2][kAll];
+  int target[kOwn];  // −1: no entry of this row is asked for
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
-    const int row = min(m0 + 32 * mi + l32, M - 1);
-    const uint16_t* const p = X + static_cast<int64_t>(row) * ldx + 8 * h;
+  for (int mi = 0; mi < 2; ++mi) {
+    const int row = min(row0[mi] + l32, M - 1);
+    const uint16_t* const p = X + static_cast<int64_t>(row) * ldx + 64 * KS * half + 8 * h;
 #pragma unroll
     for (int kk = 0; kk < kAll; ++kk) {
       x[mi][kk] = ldg16(p + 16 * kk);
@@ -252,42 +261,54 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
       // well: left to itself the compiler copies four registers per MFMA (1183 us for 1119)
       if (mi * kAll + kk >= 28) asm volatile("" : "+a"(x[mi][kk]));
     }
-    const int64_t t = targets[row];
-    target[mi] = m0 + 32 * mi + l32 < M && t >= 0 && t < V ? static_cast<int>(t) : -1;
+    if (mi < kOwn) {
+      const int64_t t = targets[row];
+      target[mi] = row0[mi] + l32 < M && t >= 0 && t < V ? static_cast<int>(t) : -1;
+    }
   }
-  // this lane's operand of k-step kk lies at chunk 2 (kk % 4) + h of its row in slab kk / 4
+  // this lane's operand of k-step kk lies at chunk 2 (kk % 4) + h of its row in slab kk / 4 (of its half)
   int lane_off[4];
 #pragma unroll
-  for (int k4 = 0; k4 < 4; ++k4) lane_off[k4] = xswz(l32, 2 * k4 + h);
+  for (int k4 = 0; k4 < 4; ++k4) lane_off[k4] = half * (KS / 2) * kSlab + xswz(l32, 2 * k4 + h);
   auto read = [&](int stage, int kk) {  // k-step kk of the unit in that stage
     return lds16(smem + stage * kStage + (kk >> 2) * kSlab + lane_off[kk & 3]);
   };
 
-  Stat stat[MI];
+  Stat stat[kOwn];
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) stat[mi] = stat_none();
-  // value j of acc[mi] is entry 32 tile + 8 (j / 4) + 4 h + j % 4: what is rare, in branches ahead of the MFMAs
-  auto rare = [&](f32x16(&acc)[MI], int i) {
+  for (int mi = 0; mi < kOwn; ++mi) stat[mi] = stat_none();
+  // value j of acc[mi] is entry 32 tile + 8 (j / 4) + 4 h + j % 4: what is rare, in branches
+  auto mask = [&](f32x16(&acc)[2], int i) {
     const int e0 = (t0 + i) * kTile;
     if (e0 + kTile > V) {
 #pragma unroll
-      for (int mi = 0; mi < MI; ++mi)
+      for (int mi = 0; mi < kOwn; ++mi)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (e0 + 8 * (j >> 2) + 4 * h + (j & 3) >= V) acc[mi][j] = -__builtin_inff();
     }
+  };
+  auto pick = [&](const f32x16(&acc)[2], int i) {
+    const int e0 = (t0 + i) * kTile;
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
+    for (int mi = 0; mi < kOwn; ++mi) {
       if (__ballot(target[mi] >= e0 && target[mi] < e0 + kTile)) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (e0 + 8 * (j >> 2) + 4 * h + (j & 3) == target[mi]) zt[m0 + 32 * mi + l32] = acc[mi][j];
+          if (e0 + 8 * (j >> 2) + 4 * h + (j & 3) == target[mi]) zt[row0[mi] + l32] = acc[mi][j];
       }
     }
   };
-  auto add = [&](const f32x16(&acc)[MI]) {
+  // quarter q of the other half's products: given to that wave, and taken from it behind a barrier
+  float* const xch = reinterpret_cast<float*>(smem + kStages * kStage) + 4 * lane;
+  auto give = [&](const f32x16(&acc)[2], int q) {
+    *reinterpret_cast<f32x4*>(xch + 1024 * wave + 256 * q) =
+        f32x4{acc[1][4 * q], acc[1][4 * q + 1], acc[1][4 * q + 2], acc[1][4 * q + 3]};
+  };
+  auto taken = [&](int q) { return *reinterpret_cast<const f32x4*>(xch + 1024 * (wave ^ 1) + 256 * q); };
+  auto add = [&](const f32x16(&acc)[2]) {
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
+    for (int mi = 0; mi < kOwn; ++mi) {
       float m = stat[mi].m;
 #pragma unroll
       for (int j = 0; j < 16; ++j) m = fmaxf(m, acc[mi][j]);
@@ -297,24 +318,29 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
     }
   };
 
-  f32x16 acc[2][MI];
+  f32x16 acc[2][2];
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi)
+  for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[1][mi][j] = -__builtin_inff();  // no tile before the first
   u32x4 w[4];
-  // Tile i: its MFMAs into acc[i % 2], the statistics of tile i − 1 beside them: its maximum in the first four
-  // k-steps, the sums moved to it in the fifth, its 32 values over the others. The scheduling barriers keep
-  // that order.
-  auto body = [&](int i, f32x16(&cur)[MI], f32x16(&old)[MI]) {
-    if (i > 0) rare(old, i - 1);
-    constexpr int kMax = 4, kVals = 16 * MI;
-    float m[MI];
+  // Tile i: its MFMAs into acc[i % 2], the statistics of tile i − 1 beside them: from k-step kSum on its maximum in
+  // four, then the sums moved to it, its values over the others. With K in halves the products are exchanged before:
+  // given in the first four k-steps, taken behind the first unit's barrier. The scheduling barriers keep that order.
+  constexpr int kSum = SPLIT == 2 ? kK / 2 + 2 : 0, kScale = kSum + 4;
+  auto body = [&](int i, f32x16(&cur)[2], f32x16(&old)[2]) {
+    if (i > 0) {
+      mask(old, i - 1);
+      if (SPLIT == 1) pick(old, i - 1);
+    }
+    constexpr int kVals = 16 * kOwn;
+    f32x4 other[4];
+    float m[kOwn];
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) m[mi] = stat[mi].m;
+    for (int mi = 0; mi < kOwn; ++mi) m[mi] = stat[mi].m;
 #pragma unroll
     for (int kk = 0; kk < kAll; ++kk) {
-      const int part = kk / kK, ku = kk % kK, unit = i * UNITS + part;
+      const int part = kk / kK, ku = kk % kK, unit = i * SPLIT + part;
       if (ku == kK / 2) {
         // the next unit has landed (the one after it may be on its way), and every wave is done with the unit
         // before this one (its reads have returned), whose stage the next copies overwrite
@@ -324,21 +350,29 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
       w[(kk + kAhead) & 3] = ku + kAhead < kK ? read(unit % kStages, ku + kAhead)
                                               : read((unit + 1) % kStages, ku + kAhead - kK);
 #pragma unroll
-      for (int mi = 0; mi < MI; ++mi)
+      for (int mi = 0; mi < 2; ++mi)
         cur[mi] = Mfma<DT>::run(w[kk & 3], x[mi][kk], kk ? cur[mi] : f32x16{});
       if (ku >= kK / 2 && ku < kK / 2 + KS)
-        issue(i + (part + 3) / UNITS, (part + 3) % UNITS, (unit + 3) % kStages, ku - kK / 2);
-      if (kk < kMax) {
+        issue(i + (part + 3) / SPLIT, (part + 3) % SPLIT, (unit + 3) % kStages, ku - kK / 2);
+      if (SPLIT == 2 && kk < 4) give(old, kk);
+      if (SPLIT == 2 && kk == kK / 2) {
 #pragma unroll
-        for (int v = kVals / kMax * kk; v < kVals / kMax * (kk + 1); ++v)
+        for (int q = 0; q < 4; ++q) other[q] = taken(q);
+      }
+      if (kk >= kSum && kk < kScale) {
+#pragma unroll
+        for (int v = kVals / 4 * (kk - kSum); v < kVals / 4 * (kk - kSum + 1); ++v) {
+          if (SPLIT == 2) old[0][v] += other[v >> 2][v & 3];
           m[v >> 4] = fmaxf(m[v >> 4], old[v >> 4][v & 15]);
-      } else if (kk == kMax) {
+        }
+      } else if (kk == kScale) {
+        if (SPLIT == 2 && i > 0) pick(old, i - 1);
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) stat_rescale(stat[mi], m[mi]);
-      } else {
-        constexpr int kRest = kAll - kMax - 1;
+        for (int mi = 0; mi < kOwn; ++mi) stat_rescale(stat[mi], m[mi]);
+      } else if (kk > kScale) {
+        constexpr int kRest = kAll - kScale - 1;
 #pragma unroll
-        for (int v = kVals * (kk - kMax - 1) / kRest; v < kVals * (kk - kMax) / kRest; ++v)
+        for (int v = kVals * (kk - kScale - 1) / kRest; v < kVals * (kk - kScale) / kRest; ++v)
           stat_add<ENT>(stat[v >> 4], old[v >> 4][v & 15]);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -347,7 +381,7 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
 #pragma unroll
   for (int u = 0; u < 3; ++u)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) issue(u / UNITS, u % UNITS, u, s);
+    for (int s = 0; s < KS; ++s) issue(u / SPLIT, u % SPLIT, u, s);
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * KS) : "memory");
   ring_barrier();
 #pragma unroll
@@ -356,20 +390,29 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
     body(i, acc[0], acc[1]);
     if (i + 1 < n_tiles) body(i + 1, acc[1], acc[0]);
   }
-  if (n_tiles & 1) {
-    rare(acc[0], n_tiles - 1);
-    add(acc[0]);
-  } else {
-    rare(acc[1], n_tiles - 1);
-    add(acc[1]);
-  }
+  auto last = [&](f32x16(&acc)[2]) {
+    if constexpr (SPLIT == 2) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) give(acc, q);
+      ring_barrier();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[0][j] += taken(j >> 2)[j & 3];
+    }
+    mask(acc, n_tiles - 1);
+    pick(acc, n_tiles - 1);
+    add(acc);
+  };
+  if (n_tiles & 1)
+    last(acc[0]);
+  else
+    last(acc[1]);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup
   // the lane halves hold parts of the same rows
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
+  for (int mi = 0; mi < kOwn; ++mi) {
     const Stat& a = stat[mi];
     stat_join(stat[mi], Stat{lane_xor<32>(a.m), lane_xor<32>(a.mu), lane_xor<32>(a.s), lane_xor<32>(a.h)});
-    const int row = m0 + 32 * mi + l32;
+    const int row = row0[mi] + l32;
     if (h == 0 && row < M) parts[static_cast<int64_t>(strip) * M + row] = Part{a.m, a.s, a.h};
   }
 }
@@ -405,13 +448,14 @@ __global__ __launch_bounds__(256) void head_join_kernel(const Part* __restrict__
 // and row tiles of 256 (128 where K > 640) that are not emptier than those of 192. us, with it / without, bf16:
 // 256 rows of 640 x 128000 55 / 64, 300 rows 79 / 65, 600 rows 110 / 117, 5000 rows 647 / 851; 512 x 32000: 768 rows
 // 36 / 31, 1000 rows 41.5 / 42.8, 5000 rows 150 / 175; 256 x 50000: 1000 rows 36 / 41; 640 x 5000: 3000 rows 36 / 33;
-// 1024 x 50001: 192 rows 38 / 32, 256 rows 39 / 50, 1503 rows 144 / 155; 768 x 8000: 1503 rows 28 / 26.
+// 1024 x 50001: 192 rows 40 / 33, 256 rows 40 / 50, 1503 rows 152 / 165; 1024 x 8000: 1503 rows 37 / 33, x 11000
+// 45 / 48; 768: 384 rows x 32000 30 / 27, x 45000 37 / 39, 1000 rows x 16000 35 / 38.
 bool rows_applies(int M, int V, int K) {
   const bool wide = K == 768 || K == 1024;
   if (!wide && (K % 128 || K < 256 || K > 640)) return false;
   const int tile = wide ? 128 : 256;
   const int64_t own = (M + tile - 1) / tile * static_cast<int64_t>(tile), other = (M + 191) / 192 * 192ll;
-  return static_cast<int64_t>(M) * V >= (wide ? 12000000 : 25000000) && 100 * own <= 107 * other;
+  return static_cast<int64_t>(M) * V >= (wide ? 12500000 : 25000000) && 100 * own <= 107 * other;
 }
 
 struct Plan {
@@ -506,9 +550,8 @@ extern "C" int tmac_head_logprob(const void* d_X, int64_t ldx, const void* d_W, 
         static_cast<const uint16_t*>(d_X), ldx, static_cast<const uint16_t*>(d_W), ldw, d_targets, M, v, K / 64,
         p.n_mt, p.n_nt, p.n_strips, p.per_strip, parts, zt, per_xcd);
   };
-  auto launch_rows = [&](auto dt, auto e, auto ks, auto units) {
-    constexpr int UNITS = decltype(units)::value;
-    head_rows_kernel<decltype(dt)::value, decltype(e)::value, decltype(ks)::value, UNITS, UNITS == 1 ? 2 : 1>
+  auto launch_rows = [&](auto dt, auto e, auto ks, auto split) {
+    head_rows_kernel<decltype(dt)::value, decltype(e)::value, decltype(ks)::value, decltype(split)::value>
         <<<8 * per_xcd, 256, 0, s>>>(
         static_cast<const uint16_t*>(d_X), ldx, static_cast<const uint16_t*>(d_W), ldw, d_targets, M, v, p.n_mt,
         p.n_nt, p.n_strips, p.per_strip, parts, zt, per_xcd);
