@@ -555,7 +555,8 @@ constexpr int kMaxGrid = 1 << 21;  // workgroups of a launch; they take turns be
 // 8000 24 / 24 / 31), then 512 (8192 of 128000: 382 / 351 / 344), with alternatives 256 (4096 of 128000: five of
 // them 201 / 197 / 214, twenty 209 / 200 / 218, 64 568 / 243 / 230).
 constexpr int kShortRow = 32 << 10;
-constexpr int kFewRows = 1024;  // whole rows with alternatives up to which 512 threads take one (16 rows: 12.4 us, 256: 14.7)
+// Whole rows with alternatives up to which 512 threads take one (16 rows: 12.4 us, with 256 threads 14.7).
+constexpr int kFewRows = 1024;
 
 int check(int B, int T, int64_t V, int64_t st, int64_t sb, int dtype) {
   if (dtype != TMAC_F32 && dtype != TMAC_BF16 && dtype != TMAC_F16) return TMAC_ERR_DTYPE;
@@ -681,7 +682,8 @@ extern "C" int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t strid
   by_type(dtype, [&](auto dt) {
     by_flag(d_g_entropy != nullptr, [&](auto e) {
       logprob_grad_kernel<decltype(dt)::value, decltype(e)::value>
-          <<<static_cast<unsigned>(blocks < (1 << 23) ? blocks : 1 << 23), kGradThreads, 0, static_cast<hipStream_t>(stream)>>>(
+          <<<static_cast<unsigned>(blocks < (1 << 23) ? blocks : 1 << 23), kGradThreads, 0,
+             static_cast<hipStream_t>(stream)>>>(
               static_cast<const uint8_t*>(d_z), Row2{stride_b, stride_t, T}, d_targets, ignore_index, d_stats,
               d_entropy, d_g_lp, g_lp_stride, d_g_entropy, g_entropy_stride, static_cast<uint8_t*>(d_dz),
               static_cast<int>(V), static_cast<int>(chunks), blocks);

@@ -57,8 +57,8 @@ constexpr float kFar = -1e4f;  // differences are cut here in products with an e
 
 __device__ __forceinline__ float exp_d(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
-// Running softmax statistics: m the maximum, s = Σ e^{z − m}, h = Σ e^{z − m} (z − m). mu is m, or 0 while nothing above −inf was seen (so that −inf − mu is
-// −inf and not NaN); a NaN, or +inf (whose z − mu is NaN), makes s NaN.
+// Running softmax statistics: m the maximum, s = Σ e^{z − m}, h = Σ e^{z − m} (z − m). mu is m, or 0 while nothing
+// above −inf was seen (so that −inf − mu is −inf and not NaN); a NaN, or +inf (whose z − mu is NaN), makes s NaN.
 struct Stat {
   float m, mu, s, h;
 };

@@ -80,11 +80,8 @@ def _lists_bytes(n_tokens: int, V: int) -> int:
     return (4 * V + 19) // 16 * 16 + 2 * ((4 * n_tokens + 15) // 16 * 16)
 
 
-def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor],
-                     positions: Optional[torch.Tensor], prefix: Optional[torch.Tensor], scale: float,
-                     make_lists: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """([B, Np + T, d] in weight's dtype, the tokens of each row of weight as the backward reads them, or an empty
-    tensor)."""
+def _native_fwd(ids, weight, pos_weight, positions, prefix, scale, make_lists):
+    """([B, Np + T, d] in weight's dtype, the tokens of each row of weight as the backward reads them or None)."""
     _check(ids, weight, pos_weight, positions, prefix)
     code = _lib.dtype_code(weight.dtype)
     dev = _lib.require_device(*(t for t in (weight, ids, pos_weight, positions, prefix) if t is not None),
@@ -93,17 +90,25 @@ def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Option
     n_prefix = 0 if prefix is None else prefix.shape[0]
     out = torch.empty((B, n_prefix + T, d), dtype=weight.dtype, device=dev)
     nb = _lists_bytes(B * T, V) if make_lists else 0
-    lists = torch.empty(nb, dtype=torch.uint8, device=dev) if make_lists else out.new_empty(0, dtype=torch.uint8)
+    lists = torch.empty(nb, dtype=torch.uint8, device=dev) if make_lists else None
     if out.numel() == 0 and not make_lists:
         return out, lists
     i, q = _index(ids, ids), _index(positions, ids)
     (w, ldw), (p, ldp), (f, ldf) = _table(weight), _table(pos_weight), _table(prefix)
     with _lib.device_guard(dev):
         rc = _lib.lib().tmac_embed_fwd(i.data_ptr(), _lib.ptr(q), w.data_ptr(), ldw, _lib.ptr(p), ldp, _lib.ptr(f), ldf,
-                                       out.data_ptr(), lists.data_ptr() if make_lists else 0, nb, B, T, n_prefix, d, V,
+                                       out.data_ptr(), _lib.ptr(lists), nb, B, T, n_prefix, d, V,
                                        0 if p is None else p.shape[0], scale, code, _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_embed_fwd")
     return out, lists
+
+
+def _token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor],
+                     positions: Optional[torch.Tensor], prefix: Optional[torch.Tensor], scale: float,
+                     make_lists: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """_native_fwd; an operator's results are tensors: empty lists for None."""
+    out, lists = _native_fwd(ids, weight, pos_weight, positions, prefix, scale, make_lists)
+    return out, out.new_empty(0, dtype=torch.uint8) if lists is None else lists
 
 
 token_embedding_fwd = torch.library.custom_op("titanmac::token_embedding", mutates_args=())(_token_embedding)
@@ -196,7 +201,7 @@ def _backward(ctx, grad, *_):
 
 
 token_embedding_fwd.register_autograd(_backward, setup_context=_setup)
-_native = _lib.native_function(_token_embedding, _setup, _backward)
+_native = _lib.native_function(_native_fwd, _setup, _backward)
 
 
 def token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor] = None, *,
@@ -205,16 +210,16 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optiona
     """scale * weight[ids] + pos_weight[positions], behind the rows of prefix: [B, Np + T, d].
 
     ids: int64 or int32 [B, T]; weight [V, d], pos_weight [n_pos, d] and prefix [Np, d] of one dtype
-    (float32, bfloat16, float16), d up to 2^20, up to 2^30 rows. positions: [B, T] or [T], by default 0 .. T - 1. The sum is formed in
-    fp32 and rounded once. Nothing is copied to the host to look at the ids: one outside [0, V), or a
-    position outside its table, gives a row of NaN and adds to no gradient.
+    (float32, bfloat16, float16), d up to 2^20, up to 2^30 rows. positions: [B, T] or [T], by default
+    0 .. T - 1. The sum is formed in fp32 and rounded once. Nothing is copied to the host to look at the ids:
+    one outside [0, V), or a position outside its table, gives a row of NaN and adds to no gradient.
 
     Differentiable in the three tables (a second time too)."""
     tables = (ids, weight, pos_weight, positions, prefix)
     # a training step's lists of tokens are made beside the lookup
     args = (*tables, float(scale), torch.is_grad_enabled() and weight.requires_grad)
     if _lib.direct_call(*tables):
-        return _token_embedding(*args)[0]
+        return _native_fwd(*args)[0]
     if _lib.eager_native(*tables):
         return _native(*args)
     return token_embedding_fwd(*args)[0]
