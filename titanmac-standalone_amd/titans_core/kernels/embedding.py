@@ -130,27 +130,39 @@ def _workspace(n_tokens: int, V: int, n_pos: int, d: int, need_w: bool) -> int:
     return nb.value
 
 
+def _native_bwd(grad, ids, positions, lists, n_prefix, V, n_pos, scale, need_w, need_p, need_f):
+    """Gradients of weight [V, d], pos_weight [n_pos, d] and prefix [n_prefix, d] in grad's dtype, None where not
+    needed. Autograd runs it in its own thread, whose waking costs most of a small pass: of 128 us with 16 tokens (in
+    the host's slower state) 76 remain with a backward of nothing, 34 are spent in here, a third of them launching."""
+    (B, T), d, dtype, dev = ids.shape, grad.shape[-1], grad.dtype, grad.device
+    if grad.is_contiguous():
+        g, ldg = grad, d
+    else:
+        g = _rows(grad)
+        ldg = max(g.stride(0), d)
+    dw = torch.empty((V, d), dtype=dtype, device=dev) if need_w else None
+    dp = torch.empty((n_pos, d), dtype=dtype, device=dev) if need_p else None
+    df = torch.empty((n_prefix, d), dtype=dtype, device=dev) if need_f else None
+    i = _index(ids, ids) if need_w and lists is None else None
+    q = _index(positions, ids) if need_p else None
+    nb = _workspace(B * T, V if i is not None else 0, n_pos if q is not None else 0, d, need_w)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    ptr = _lib.ptr
+    with _lib.device_guard(dev):
+        rc = _lib.lib().tmac_embed_bwd(ptr(i), ptr(q), ptr(lists), g.data_ptr(), ldg, ptr(dw), ptr(dp),
+                                       ptr(df) if n_prefix else 0, ptr(ws), nb, B, T, n_prefix, d, V, n_pos, scale,
+                                       _lib.dtype_code(dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "tmac_embed_bwd")
+    return dw, dp, df
+
+
 def _token_embedding_bwd(grad: torch.Tensor, ids: torch.Tensor, positions: Optional[torch.Tensor],
                          lists: Optional[torch.Tensor], n_prefix: int, V: int, n_pos: int, scale: float,
                          need_w: bool, need_p: bool, need_f: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Gradients of weight [V, d], pos_weight [n_pos, d] and prefix [n_prefix, d] in grad's dtype; empty where
-    not needed."""
-    dev = _lib.require_device(*(t for t in (grad, ids, positions) if t is not None), what="token_embedding backward")
-    (B, T), d = ids.shape, int(grad.shape[-1])
-    g = grad if grad.is_contiguous() else _rows(grad)
-    ldg = d if g is grad else max(g.stride(0), d)
-    dw, dp, df = (torch.empty((n if need else 0, d), dtype=grad.dtype, device=dev)
-                  for n, need in ((V, need_w), (n_pos, need_p), (n_prefix, need_f)))
-    i, q = _index(ids, ids) if lists is None else None, _index(positions, ids) if need_p else None
-    nb = _workspace(B * T, V if need_w and lists is None else 0, n_pos if q is not None else 0, d, need_w)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_embed_bwd(_lib.ptr(i), _lib.ptr(q), _lib.ptr(lists), g.data_ptr(), ldg,
-                                       dw.data_ptr() if need_w else 0, dp.data_ptr() if need_p else 0,
-                                       df.data_ptr() if need_f and n_prefix else 0, ws.data_ptr(), nb, B, T,
-                                       n_prefix, d, V, n_pos, scale, _lib.dtype_code(grad.dtype), _lib.stream_ptr(dev))
-    _lib.check(rc, "tmac_embed_bwd")
-    return dw, dp, df
+    """_native_bwd; an operator's results are tensors: empty ones for None."""
+    _lib.require_device(*(t for t in (grad, ids, positions, lists) if t is not None), what="token_embedding backward")
+    out = _native_bwd(grad, ids, positions, lists, n_prefix, V, n_pos, scale, need_w, need_p, need_f)
+    return tuple(grad.new_empty((0, grad.shape[-1])) if t is None else t for t in out)
 
 
 token_embedding_bwd = torch.library.custom_op("titanmac::token_embedding_bwd",
@@ -190,14 +202,15 @@ def _composed(grad, ids, positions, lists, n_prefix, V, n_pos, scale, need_w, ne
 
 def _backward(ctx, grad, *_):
     ids, positions, lists = ctx.saved_tensors
-    need = [ctx.needs_input_grad[i] for i in (1, 2, 4)]
-    args = (grad, ids, positions, lists, *ctx.sizes, *need)
+    _, need_w, need_p, _, need_f, _, _ = ctx.needs_input_grad
     if torch.is_grad_enabled() and grad.requires_grad:
-        dw, dp, df = _composed(*args)
+        run = _composed
+    elif _lib.direct_backward(grad, ids):
+        run = _native_bwd
     else:
-        op = _token_embedding_bwd if _lib.direct_backward(grad, ids) else token_embedding_bwd
-        dw, dp, df = op(*args)
-    return (None, dw if need[0] else None, dp if need[1] else None, None, df if need[2] else None, None, None)
+        run = token_embedding_bwd
+    dw, dp, df = run(grad, ids, positions, lists, *ctx.sizes, need_w, need_p, need_f)
+    return None, dw if need_w else None, dp if need_p else None, None, df if need_f else None, None, None
 
 
 token_embedding_fwd.register_autograd(_backward, setup_context=_setup)

@@ -133,29 +133,37 @@ def _row_grad(g: Optional[torch.Tensor]):
     """(fp32 values of a per-row gradient, stride): stride 0 for one value for all rows."""
     if g is None:
         return None, 0
-    g = g.to(torch.float32)
+    if g.dtype != torch.float32:
+        g = g.to(torch.float32)
+    if g.is_contiguous():
+        return g, 1
     if all(s == 0 for s, n in zip(g.stride(), g.shape) if n > 1):
         return g, 0
     return g.contiguous(), 1
 
 
-def _logprob_bwd(g_lp: Optional[torch.Tensor], g_ent: Optional[torch.Tensor], logits: torch.Tensor,
-                 targets: torch.Tensor, stats: torch.Tensor, entropy: torch.Tensor, ignore_index: int) -> torch.Tensor:
+def _native_bwd(g_lp, g_ent, logits, targets, stats, entropy, ignore_index):
     """The gradient of the logits; g_lp, g_ent: per row, or one value for all."""
-    dev = _lib.require_device(*(t for t in (logits, targets, stats, entropy, g_lp, g_ent) if t is not None),
-                              what="token_logprobs backward")
     z, sb, st, B, T, V = _rows3(logits)
-    dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    if dz.numel() == 0:
+    dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if B * T == 0:
         return dz
     (gl, sl), (ge, se) = _row_grad(g_lp), _row_grad(g_ent)
-    tg = _flat(targets)
+    tg, ptr, dev = _flat(targets), _lib.ptr, logits.device
     with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_logprob_bwd(z.data_ptr(), sb, st, tg.data_ptr(), ignore_index,
-                                         _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(gl), sl, _lib.ptr(ge), se,
-                                         _lib.ptr(dz), B, T, V, _lib.dtype_code(z.dtype), _lib.stream_ptr(dev))
+        rc = _lib.lib().tmac_logprob_bwd(z.data_ptr(), sb, st, tg.data_ptr(), ignore_index, stats.data_ptr(),
+                                         ptr(entropy), ptr(gl), sl, ptr(ge), se, dz.data_ptr(), B, T, V,
+                                         _lib.dtype_code(z.dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "tmac_logprob_bwd")
     return dz
+
+
+def _logprob_bwd(g_lp: Optional[torch.Tensor], g_ent: Optional[torch.Tensor], logits: torch.Tensor,
+                 targets: torch.Tensor, stats: torch.Tensor, entropy: Optional[torch.Tensor], ignore_index: int
+                 ) -> torch.Tensor:
+    _lib.require_device(*(t for t in (logits, targets, stats, entropy, g_lp, g_ent) if t is not None),
+                        what="token_logprobs backward")
+    return _native_bwd(g_lp, g_ent, logits, targets, stats, entropy, ignore_index)
 
 
 logprob_bwd = torch.library.custom_op("titanmac::token_logprobs_bwd", mutates_args=())(_logprob_bwd)
@@ -192,8 +200,8 @@ def _gradient(g_lp, g_ent, logits, targets, stats, entropy, ignore_index):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (g_lp, g_ent, logits)):
         return _composed(g_lp, g_ent, logits, targets, ignore_index)
     direct = all(_lib.direct_backward(g, logits) for g in (g_lp, g_ent) if g is not None)
-    op = _logprob_bwd if direct else logprob_bwd
-    return op(g_lp, g_ent, logits, targets, stats, entropy, ignore_index)
+    run = _native_bwd if direct else logprob_bwd
+    return run(g_lp, g_ent, logits, targets, stats, entropy, ignore_index)
 
 
 def _setup(ctx, inputs, output):
