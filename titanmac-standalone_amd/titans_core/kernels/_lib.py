@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch  # the HIP runtime torch loads (libamdhip64.so.7) also serves libtmac.so
+from torch.autograd import forward_ad
 
 ABI_VERSION = 9
 
@@ -190,15 +191,36 @@ def device_guard(device: torch.device):
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+# asked in every call: bound once
+_compiling, _tracing_state = torch.compiler.is_compiling, torch._C._get_tracing_state
+_functorch_stack, _dispatch_modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
+
+
+def _intercepted() -> bool:
+    """Whether something rewrites, traces or batches torch's calls here: torch.jit.trace, functorch transforms,
+    dispatch modes (fake tensors, make_fx)."""
+    return _tracing_state() is not None or _functorch_stack() is not None or _dispatch_modes() > 0
+
+
+def _no_tangents(*tensors: torch.Tensor | None) -> None:
+    """Refuses forward-mode AD: no op here has a formula for it, and one that was run all the same (directly or
+    through the dispatcher, unless reverse mode is recorded too) would drop the tangents silently."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode AD (jvp) of the TitanMAC kernels is not implemented")
 
 
 def direct_call(*tensors: torch.Tensor | None) -> bool:
     """Whether an op may run its implementation directly instead of through the
-    torch.library dispatcher: eager mode (no torch.compile tracing), plain
+    torch.library dispatcher: eager mode (nothing that traces, batches or transforms calls, whose
+    tensors have no address or whose record would miss the kernel), plain
     tensors (no fake or wrapper subclasses) and no autograd graph to record.
     The dispatcher adds several µs of host time per call, more than many of
-    these kernels take on the GPU."""
-    if torch.compiler.is_compiling():
+    these kernels take on the GPU. Raises for tensors that carry forward-mode tangents."""
+    if _compiling():
+        return False
+    if forward_ad._current_level >= 0:
+        _no_tangents(*tensors)
+    if _intercepted():
         return False
     grad = torch.is_grad_enabled()
     for t in tensors:
@@ -210,20 +232,16 @@ def direct_call(*tensors: torch.Tensor | None) -> bool:
 
 
 def direct_backward(grad: torch.Tensor, *tensors: torch.Tensor | None) -> bool:
-    """direct_call in a backward of the incoming gradient `grad`: with is_grads_batched or under functorch
-    that is a batched tensor, whose Python type is torch.Tensor's own and which has no address."""
-    return (direct_call(grad, *tensors) and torch._C._functorch.peek_interpreter_stack() is None
-            and not torch._C._functorch.is_legacy_batchedtensor(grad))
+    """direct_call in a backward of the incoming gradient `grad`: with is_grads_batched that is a batched
+    tensor, whose Python type is torch.Tensor's own and which has no address."""
+    return direct_call(grad, *tensors) and not torch._C._functorch.is_legacy_batchedtensor(grad)
 
 
 def eager_native(*tensors: torch.Tensor | None) -> bool:
     """Whether an op may record its autograd node with a plain autograd.Function and run its kernels
     directly: eager mode, plain tensors, and nothing that rewrites, traces or intercepts torch calls
-    (torch.compile, torch.jit.trace, functorch transforms, forward-mode AD, function or dispatch modes)."""
-    if (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
-            or torch._C._functorch.peek_interpreter_stack() is not None
-            or torch.autograd.forward_ad._current_level >= 0
-            or torch._C._len_torch_function_stack() or torch._C._len_torch_dispatch_stack()):
+    (torch.compile, _intercepted, forward-mode AD, function modes)."""
+    if (_compiling() or _intercepted() or forward_ad._current_level >= 0 or torch._C._len_torch_function_stack()):
         return False
     return all(t is None or type(t) in _PLAIN for t in tensors)
 
