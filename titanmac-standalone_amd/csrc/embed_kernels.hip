@@ -23,11 +23,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRowsPerBlock = 4 * kThreads;
-constexpr int kMaxGrid = 1 << 22;  // workgroups of a launch; they take turns beyond that
+constexpr int64_t kMaxItems = 1 << 30;  // threads of a launch (one takes less than 2^32); workgroups take turns beyond
 
 // Rows per workgroup and turn: about `per` (at most 4) pieces, cpr of them a row, for each thread.
 int rows_per_block(int cpr, int per) { return kThreads * per > cpr ? kThreads * per / cpr : 1; }
-int grid(int64_t blocks) { return static_cast<int>(blocks < kMaxGrid ? blocks : kMaxGrid); }
+int grid(int64_t blocks, int threads) {
+  return static_cast<int>(blocks < kMaxItems / threads ? blocks : kMaxItems / threads);
+}
 
 struct Lookup {
   const int64_t *ids, *pos;
@@ -283,7 +285,9 @@ struct Grad {
   int V, rpb, chunks, row_blocks;
   float scale;
   uint8_t *dprefix, *dP;  // rows [first, last) of [prefix | positions] by sums over the sequences
-  int B, T, Np, first, last, pos_blocks, pos_rpb;
+  int B, T, Np;
+  int64_t first, last;
+  int pos_blocks, pos_rpb;
   int d, cpr;
 };
 
@@ -337,10 +341,11 @@ template <int DT, int N>
 __device__ __forceinline__ void grad_positions(const Grad& a, int block) {
   constexpr int E = kRowSize<DT>;
   const int S = a.Np + a.T;
-  const int row0 = a.first + block * a.pos_rpb, n = min(a.pos_rpb, a.last - row0) * a.cpr;
+  const int64_t row0 = a.first + static_cast<int64_t>(block) * a.pos_rpb;
+  const int n = static_cast<int>(min(static_cast<int64_t>(a.pos_rpb), a.last - row0)) * a.cpr;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int r = i / a.cpr, c = (i - r * a.cpr) * N;
-    const int s = row0 + r;
+    const int64_t s = row0 + r;
     float v[N] = {};
     if (s < S) {
 #pragma unroll 4
@@ -351,23 +356,21 @@ __device__ __forceinline__ void grad_positions(const Grad& a, int block) {
         for (int e = 0; e < N; ++e) v[e] += x[e];
       }
     }
-    row_store<DT, N>(s < a.Np ? a.dprefix + (static_cast<int64_t>(s) * a.d + c) * E
-                              : a.dP + (static_cast<int64_t>(s - a.Np) * a.d + c) * E,
-                     v);
+    row_store<DT, N>(s < a.Np ? a.dprefix + (s * a.d + c) * E : a.dP + ((s - a.Np) * a.d + c) * E, v);
   }
 }
 
 // The chunks of long lists first, whose sums the next launch waits for.
 template <int DT, int N>
 __global__ __launch_bounds__(kThreads) void embed_grad_kernel(Grad a) {
-  const int blocks = a.chunks + a.pos_blocks + a.row_blocks;
-  for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
+  const int64_t sums = static_cast<int64_t>(a.chunks) + a.pos_blocks, blocks = sums + a.row_blocks;
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     if (b < a.chunks)
-      grad_chunk<DT, N>(a, b);
-    else if (b < a.chunks + a.pos_blocks)
-      grad_positions<DT, N>(a, b - a.chunks);
+      grad_chunk<DT, N>(a, static_cast<int>(b));
+    else if (b < sums)
+      grad_positions<DT, N>(a, static_cast<int>(b - a.chunks));
     else
-      grad_rows<DT, N>(a, b - a.chunks - a.pos_blocks);
+      grad_rows<DT, N>(a, static_cast<int>(b - sums));
   }
 }
 
@@ -437,7 +440,7 @@ constexpr int kMaxD = 1 << 20;
 
 int check_sizes(int B, int T, int Np, int d, int dtype) {
   if (dtype != TMAC_F32 && dtype != TMAC_BF16 && dtype != TMAC_F16) return TMAC_ERR_DTYPE;
-  if (B < 0 || T < 0 || Np < 0 || d <= 0 || d > kMaxD) return TMAC_ERR_SHAPE;
+  if (B < 0 || T < 0 || Np < 0 || Np > kMaxRows || d <= 0 || d > kMaxD) return TMAC_ERR_SHAPE;
   if (static_cast<int64_t>(B) * (static_cast<int64_t>(Np) + T) > kMaxRows) return TMAC_ERR_SHAPE;
   return TMAC_OK;
 }
@@ -531,15 +534,14 @@ extern "C" int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const 
              V, n_pos, scale, d / N, 1};
     if (!d_lists) {
       a.rpb = rows_per_block(a.cpr, 1);
-      embed_fwd_kernel<DT, N><<<grid((rows + a.rpb - 1) / a.rpb), kThreads, 0, s>>>(a);
+      embed_fwd_kernel<DT, N><<<grid((rows + a.rpb - 1) / a.rpb, kThreads), kThreads, 0, s>>>(a);
       return;
     }
     a.rpb = rows_per_block(a.cpr, 64 * kSortWaves / kThreads);
     const Tokens t = tokens(d_ids, n_tok, T, n_prefix, V);
     const Lists to = lists(d_lists, n_tok, V);
-    const int sort_blocks = n_ranges(V);
-    const int64_t look = (rows + a.rpb - 1) / a.rpb;
-    const int blocks = sort_blocks + static_cast<int>(look < (1 << 21) ? look : 1 << 21);
+    const int sort_blocks = n_ranges(V);  // up to 2^21: with the others' 2^20, 3 · 2^30 threads
+    const int blocks = sort_blocks + grid((rows + a.rpb - 1) / a.rpb, 64 * kSortWaves);
     if (held(n_tok))
       embed_fwd_lists_kernel<DT, N, kHeld><<<blocks, 64 * kSortWaves, 0, s>>>(a, t, to, sort_blocks);
     else
@@ -595,7 +597,7 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
       a.dprefix = static_cast<uint8_t*>(d_dprefix);
       a.dP = sums ? static_cast<uint8_t*>(d_dP) : nullptr;
       a.first = d_dprefix ? 0 : n_prefix;
-      a.last = n_prefix + (sums ? static_cast<int>(n_pos) : 0);
+      a.last = n_prefix + (sums ? n_pos : 0);
     }
     if (out) {
       const Lists to = lists(given ? const_cast<void*>(given) : d_ws, n_tok, n_rows);
@@ -621,12 +623,12 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
       a.rpb = rows_per_block(a.cpr, 4);
       a.pos_rpb = rows_per_block(a.cpr, 1);
       a.row_blocks = (a.V + a.rpb - 1) / a.rpb;
-      a.pos_blocks = a.last > a.first ? (a.last - a.first + a.pos_rpb - 1) / a.pos_rpb : 0;
+      a.pos_blocks = static_cast<int>((a.last - a.first + a.pos_rpb - 1) / a.pos_rpb);
       const int64_t blocks = static_cast<int64_t>(a.chunks) + a.pos_blocks + a.row_blocks;
       if (!blocks) return;
-      embed_grad_kernel<DT, N><<<grid(blocks), kThreads, 0, s>>>(a);
+      embed_grad_kernel<DT, N><<<grid(blocks, kThreads), kThreads, 0, s>>>(a);
       if (a.chunks)
-        embed_grad_long_kernel<DT, N><<<grid((a.chunks + kLongChunks - 1) / kLongChunks), 1024, 0, s>>>(a);
+        embed_grad_long_kernel<DT, N><<<grid((a.chunks + kLongChunks - 1) / kLongChunks, 1024), 1024, 0, s>>>(a);
     });
   };
   const bool any_sums = sums || d_dprefix;

@@ -417,29 +417,30 @@ __global__ __launch_bounds__(256, 1) void head_rows_kernel(
   }
 }
 
-// One wave per row: its strips' statistics joined, and the row's results.
+// One wave per row and turn: its strips' statistics joined, and the row's results.
 __global__ __launch_bounds__(256) void head_join_kernel(const Part* __restrict__ parts, const float* __restrict__ zt,
                                                         const int64_t* __restrict__ targets, int64_t ignore,
                                                         float* __restrict__ lp, float* __restrict__ ent, int M, int V,
                                                         int n_strips) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= M) return;
-  Stat a = stat_none();
-  for (int p = lane; p < n_strips; p += 64) {
-    const Part q = parts[static_cast<int64_t>(p) * M + row];
-    stat_join(a, Stat{q.m, q.m == -__builtin_inff() ? 0.f : q.m, q.s, q.h});
+  const int lane = threadIdx.x & 63;
+  for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < M; row += gridDim.x * 4) {
+    Stat a = stat_none();
+    for (int p = lane; p < n_strips; p += 64) {
+      const Part q = parts[static_cast<int64_t>(p) * M + row];
+      stat_join(a, Stat{q.m, q.m == -__builtin_inff() ? 0.f : q.m, q.s, q.h});
+    }
+    stat_wave(a);
+    if (lane) continue;
+    const float log_s = __builtin_amdgcn_logf(a.s) * kLn2;
+    const int64_t t = targets[row];
+    float r = __builtin_nanf("");
+    if (t == ignore)
+      r = 0.f;
+    else if (t >= 0 && t < V)
+      r = (zt[row] - a.mu) - log_s;
+    lp[row] = r;
+    if (ent) ent[row] = log_s - a.h / a.s;
   }
-  stat_wave(a);
-  if (lane) return;
-  const float log_s = __builtin_amdgcn_logf(a.s) * kLn2;
-  const int64_t t = targets[row];
-  float r = __builtin_nanf("");
-  if (t == ignore)
-    r = 0.f;
-  else if (t >= 0 && t < V)
-    r = (zt[row] - a.mu) - log_s;
-  lp[row] = r;
-  if (ent) ent[row] = log_s - a.h / a.s;
 }
 
 // ------------------------------------------------------------------ host
@@ -505,6 +506,7 @@ Plan plan(int M, int V, int K) {
 }
 
 constexpr int64_t kMaxRows = 1 << 30, kMaxV = 1 << 28, kMaxPitch = 1 << 22;
+constexpr int kMaxJoin = 1 << 20;  // workgroups of the join (a launch has less than 2^32 threads)
 
 int check(int M, int64_t V, int K, int dtype) {
   if (dtype != TMAC_BF16 && dtype != TMAC_F16) return TMAC_ERR_DTYPE;
@@ -586,7 +588,9 @@ extern "C" int tmac_head_logprob(const void* d_X, int64_t ldx, const void* d_W, 
     by_entropy(std::integral_constant<int, TMAC_BF16>{});
   else
     by_entropy(std::integral_constant<int, TMAC_F16>{});
-  head_join_kernel<<<(M + 3) / 4, 256, 0, s>>>(parts, zt, d_targets, ignore_index, d_lp, d_entropy, M, v, p.n_strips);
+  const int join = (M + 3) / 4;
+  head_join_kernel<<<join < kMaxJoin ? join : kMaxJoin, 256, 0, s>>>(parts, zt, d_targets, ignore_index, d_lp, d_entropy,
+                                                                     M, v, p.n_strips);
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? TMAC_OK : static_cast<int>(err);
 }

@@ -63,8 +63,9 @@ def _check(ids, weight, pos_weight, positions, prefix) -> None:
         if positions is None and ids.shape[1] > pos_weight.shape[0]:
             raise ValueError(f"token_embedding: {ids.shape[1]} positions, but pos_weight has "
                              f"{pos_weight.shape[0]} rows")
-    rows = ids.shape[0] * (ids.shape[1] + (0 if prefix is None else prefix.shape[0]))
-    if (max(rows, weight.shape[0], 0 if pos_weight is None else pos_weight.shape[0]) > _MAX_ROWS
+    n_prefix = 0 if prefix is None else prefix.shape[0]
+    rows = ids.shape[0] * (ids.shape[1] + n_prefix)
+    if (max(rows, weight.shape[0], 0 if pos_weight is None else pos_weight.shape[0], n_prefix) > _MAX_ROWS
             or max(ids.shape) > _MAX_ROWS or weight.shape[1] > _MAX_D):
         raise ValueError(f"token_embedding: up to {_MAX_ROWS} rows of up to {_MAX_D} values")
 
