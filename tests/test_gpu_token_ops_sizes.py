@@ -31,3 +31,47 @@ def test_head_rows_past_the_joins_workgroups(dev):
     for a, b in ((one.logprobs, many.logprobs), (one.entropy, many.entropy)):
         assert torch.equal(a.expand(times - 1, n), b[:(times - 1) * n].view(times - 1, n))
         assert torch.equal(a[:M - (times - 1) * n], b[(times - 1) * n:])
+
+
+def sums_over_sequences(g, n_prefix, n_pos):
+    """(dP, dprefix) in 64 bits and the sums of magnitudes."""
+    out = []
+    for x in (g.double(), g.double().abs()):
+        s = x.sum(0)
+        dp = torch.zeros(n_pos, g.shape[-1], dtype=torch.float64, device=g.device)
+        dp[:s.shape[0] - n_prefix] = s[n_prefix:]
+        out.append((dp, s[:n_prefix]))
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,T,Np,d,n_pos", [(5000, 3, 4, 640, 64), (20000, 1, 0, 64, 16), (4096, 16, 16, 640, 40),
+                                            (1003, 2, 3, 641, 2), (16, 5, 1, 64, 9), (17, 1, 2, 8, 1), (70, 300, 0, 96, 301)])
+def test_many_sequences(dev, B, T, Np, d, n_pos, dtype):
+    """Default positions and the prefix: sums over the sequences."""
+    g = torch.Generator().manual_seed(B)
+    ids = torch.randint(0, 50, (B, T), generator=g).to(dev)
+    w, p, f = (torch.randn(n, d, generator=g).to(dev, dtype).requires_grad_() for n in (50, n_pos, max(Np, 1)))
+    up = (torch.randn(B, Np + T, d, generator=g) + 0.5).to(dev, dtype)
+    y = tc.token_embedding(ids, w, p, prefix=f if Np else None)
+    tables = (p, f) if Np else (p,)
+    got = torch.autograd.grad(y, tables, up, retain_graph=True)
+    for upstream in (up, torch.stack([up, up], 2)[:, :, 0]):  # rows one after the other, and in steps of two
+        again = torch.autograd.grad(y, tables, upstream, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    want, size = sums_over_sequences(up, Np, n_pos)
+    u = torch.finfo(dtype).eps / 2
+    for a, b, s in zip(got, want, size):
+        # B additions, each rounded, in whatever order, and the result's rounding
+        assert torch.all((a.double() - b).abs() <= B * 2.0 ** -24 * s + u * b.abs() + 1e-30)
+
+
+def test_sums_of_many_sequences_are_not_one_chain(dev):
+    """fp32 sums of 20000 equal values: one after the other they are off by 1.7e-4 of the sum, all roundings going one
+    way; runs of at most 79 of them joined in pairs by at most (79 + 8) half steps, and the result's."""
+    B, d = 20000, 64
+    w, p = torch.zeros(5, d, device=dev), torch.zeros(1, d, device=dev, requires_grad=True)
+    y = tc.token_embedding(torch.zeros(B, 1, dtype=torch.long, device=dev), w, p)
+    g, = torch.autograd.grad(y, p, torch.full_like(y, 0.1))
+    want = B * torch.tensor(0.1).double().item()
+    assert (g.double() - want).abs().max().item() <= (79 + 8 + 1) * 2.0 ** -24 * want

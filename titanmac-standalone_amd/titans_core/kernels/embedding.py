@@ -7,8 +7,8 @@ The model looks its tokens up, adds the rows of their positions and puts the per
     out[b, Np + t] = scale * weight[ids[b, t]] + pos_weight[position(b, t)]
 
 ``token_embedding`` does that in one launch. Its gradients are dense, as ``nn.Embedding``'s: the tokens are
-sorted by id (where the table needs a gradient, in the lookup's launch) and each row's sum is formed in order
-(deterministic, fp32) and written once.
+sorted by id (where the table needs a gradient, in the lookup's launch) and each row's sum is formed in a fixed
+order (deterministic, fp32) and written once.
 """
 from __future__ import annotations
 
