@@ -75,3 +75,51 @@ def test_sums_of_many_sequences_are_not_one_chain(dev):
     g, = torch.autograd.grad(y, p, torch.full_like(y, 0.1))
     want = B * torch.tensor(0.1).double().item()
     assert (g.double() - want).abs().max().item() <= (79 + 8 + 1) * 2.0 ** -24 * want
+
+
+def rows64(z, t):
+    """(lp, H, p, ln p) in 64 bits, ignored targets as 0."""
+    logp = torch.log_softmax(z.double(), -1)
+    lp = logp.gather(-1, t.clamp(min=0)[:, None])[:, 0].masked_fill(t == -100, 0.0)
+    some = torch.where(logp == -math.inf, 0.0, logp)
+    return lp, -(logp.exp() * some).sum(-1), logp.exp(), some
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V", [((1 << 20) + 3, 33), (8191, 253), (8193, 254), (9001, 505), (1025, 506), (7, 1), (9 * 1024, 2)])
+def test_many_short_rows(dev, rows, V, dtype):
+    """The loss, log probabilities and entropies of rows that one wave takes, and of the first that it does not, behind
+    an odd row (none of them aligned alike), with their gradients."""
+    g = torch.Generator().manual_seed(rows)
+    z0 = (torch.randn(rows + 1, V, generator=g) * 2).to(dev, dtype)
+    t = torch.randint(0, V, (rows,), generator=g).to(dev)
+    t[torch.rand(rows, generator=g).to(dev) < 0.1] = -100
+    t[0] = 0
+    z = z0[1:].requires_grad_()
+    loss = tc.token_cross_entropy(z, t)
+    dz, = torch.autograd.grad(loss, z)
+    r = tc.token_logprobs(z, t, entropy=True)
+    gl, ge = torch.randn(rows, generator=g).to(dev), torch.randn(rows, generator=g).to(dev)
+    dz2, = torch.autograd.grad([r.logprobs, r.entropy], z, [gl, ge])
+    n, u = int((t != -100).sum()), torch.finfo(dtype).eps / 2
+    total = 0.0
+    for a in range(0, rows, 1 << 18):
+        at = slice(a, a + (1 << 18))
+        lp, H, p, logp = rows64(z.detach()[at], t[at])
+        total += lp.sum().item()
+        # exponentials, their sum of V terms and a logarithm, each off by roundings of values up to 2 · 2 · 6
+        tol = (V + 64) * 2.0 ** -24
+        assert torch.allclose(r.logprobs[at].double(), lp, rtol=0, atol=tol)
+        assert torch.allclose(r.entropy[at].double(), H, rtol=0, atol=24 * tol)
+        keep = (t[at] != -100).double()
+        hot = torch.zeros_like(p).scatter_(-1, t[at].clamp(min=0)[:, None], 1.0)
+        want = (-keep / n)[:, None] * (hot - p)
+        # |p| is off by tol of itself, the product rounded to the type
+        assert torch.all((dz[at].double() - want).abs() <= u * want.abs() + 2 * tol / n)
+        gk = (gl[at].double() * keep)[:, None]
+        want = gk * (hot - p) - ge[at].double()[:, None] * p * (logp + H[:, None])
+        size = gk.abs() + 48 * ge[at].double().abs()[:, None]
+        assert torch.all((dz2[at].double() - want).abs() <= u * want.abs() + 2 * tol * size)
+    want = -total / n
+    # a thread adds rows / 1024 values, then 16 waves of 64
+    assert abs(loss.double().item() - want) <= u * want + ((rows / 1024 + 22) * 2.0 ** -24 + 2 * (V + 64) * 2.0 ** -24) * max(want, 1)

@@ -430,9 +430,9 @@ __global__ __launch_bounds__(NT) void logprob_join_kernel(const uint8_t* __restr
 }
 
 // Gradient: workgroup (row, chunk of kChunk groups of the output row).
-constexpr int kGradThreads = 256, kGradGroups = 1024;
+constexpr int kGradGroups = 1024;
 
-template <int DT, bool ENT>
+template <int DT, bool ENT, int NT>
 __device__ __forceinline__ void logprob_grad_chunk(
     const uint8_t* __restrict__ z, Row2 zr, const int64_t* __restrict__ targets, int64_t ignore,
     const float* __restrict__ stats, const float* __restrict__ ent, const float* __restrict__ g_lp, int64_t g_lp_st,
@@ -463,7 +463,7 @@ __device__ __forceinline__ void logprob_grad_chunk(
     return bad ? __builtin_nanf("") : r;
   };
   const int q_end = min((chunk + 1) * kGradGroups, g.n);
-  for (int q = chunk * kGradGroups + threadIdx.x; q < q_end; q += kGradThreads) {
+  for (int q = chunk * kGradGroups + threadIdx.x; q < q_end; q += NT) {
     const int first = q * N - g.o;
     const int64_t at = static_cast<int64_t>(first) * E;
     if (q >= g.full0 && q < g.full1) {
@@ -501,17 +501,18 @@ __device__ __forceinline__ void logprob_grad_chunk(
   }
 }
 
-template <int DT, bool ENT>
-__global__ __launch_bounds__(kGradThreads) void logprob_grad_kernel(
+template <int DT, bool ENT, int NT>
+__global__ __launch_bounds__(NT) void logprob_grad_kernel(
     const uint8_t* __restrict__ z, Row2 zr, const int64_t* __restrict__ targets, int64_t ignore,
     const float* __restrict__ stats, const float* __restrict__ ent, const float* __restrict__ g_lp, int64_t g_lp_st,
     const float* __restrict__ g_ent, int64_t g_ent_st, uint8_t* __restrict__ dz, int V, int chunks, int64_t blocks) {
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x)
-    logprob_grad_chunk<DT, ENT>(z, zr, targets, ignore, stats, ent, g_lp, g_lp_st, g_ent, g_ent_st, dz, V, chunks, b);
+    logprob_grad_chunk<DT, ENT, NT>(z, zr, targets, ignore, stats, ent, g_lp, g_lp_st, g_ent, g_ent_st, dz, V, chunks, b);
 }
 
 // The mean of −lp over the rows that are not ignored (NaN where there are none), and −1 / their number for
-// the backward: one workgroup, sums in a fixed order.
+// the backward: one workgroup, sums in a fixed order. Eight rows in flight a thread: 2^18 rows 41 us, one after the other
+// about 87.
 template <int DT>
 __global__ __launch_bounds__(1024) void logprob_mean_kernel(const float* __restrict__ lp,
                                                             const int64_t* __restrict__ targets, int64_t ignore,
@@ -521,7 +522,23 @@ __global__ __launch_bounds__(1024) void logprob_mean_kernel(const float* __restr
   __shared__ int s_n[16];
   float sum = 0.f;
   int n = 0;
-  for (int i = threadIdx.x; i < rows; i += 1024) {
+  constexpr int U = 8;
+  int i = threadIdx.x;
+  for (; i < rows - (U - 1) * 1024; i += U * 1024) {
+    float x[U];
+    int64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = lp[i + 1024 * u];
+      t[u] = targets[i + 1024 * u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      sum += x[u];
+      n += t[u] != ignore;
+    }
+  }
+  for (; i < rows; i += 1024) {
     sum += lp[i];
     n += targets[i] != ignore;
   }
@@ -551,7 +568,11 @@ __global__ __launch_bounds__(1024) void logprob_mean_kernel(const float* __restr
 
 constexpr int64_t kMaxRows = 1 << 30, kMaxV = 1 << 28;
 constexpr int kMaxGrid = 1 << 21;  // workgroups of a launch; they take turns beyond that
-// Threads of a row: 128 below 32 KB (us, 128 / 256 / 512 threads: 20000 rows of 1000 bf16 18 / 28 / 50, 8000 of
+// Groups of a row up to which one wave takes it, forward (without alternatives) and backward: rows this short cost what
+// starting their waves does. us with one wave, and with the widths below: 2^20 rows of 32 bf16 forward 376 / 690, backward
+// 447 / 1070, 2^18 rows of 256 97 / 175 and 116 / 270.
+constexpr int kWaveGroups = 64;
+// Threads of a row otherwise: 128 below 32 KB (us, 128 / 256 / 512 threads: 20000 rows of 1000 bf16 18 / 28 / 50, 8000 of
 // 8000 24 / 24 / 31), then 512 (8192 of 128000: 382 / 351 / 344), with alternatives 256 (4096 of 128000: five of
 // them 201 / 197 / 214, twenty 209 / 200 / 218, 64 568 / 243 / 230).
 constexpr int kShortRow = 32 << 10;
@@ -568,6 +589,12 @@ int check(int B, int T, int64_t V, int64_t st, int64_t sb, int dtype) {
 int launch_status() {
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? TMAC_OK : static_cast<int>(err);
+}
+
+// 16-byte groups of a row at any alignment
+int64_t max_groups(int64_t V, int dtype) {
+  const int n = dtype == TMAC_F32 ? 4 : 8;
+  return (V + n - 2) / n + 1;
 }
 
 // Workgroups per row: one below 8192 groups (128 KB), whose second launch costs more than it gains (16 rows of 50000
@@ -649,6 +676,12 @@ extern "C" int tmac_logprob_fwd(const void* d_z, int64_t stride_b, int64_t strid
           logprob_kernel<DT, ENT, TOP, NT><<<grid, NT, 0, s>>>(z, zr, d_targets, ignore_index, v, top_k, parts, out,
                                                                ws_stat, ws_top, blocks);
         };
+        if constexpr (!TOP) {
+          if (max_groups(V, dtype) <= kWaveGroups) {
+            launch(std::integral_constant<int, 64>{});
+            return;
+          }
+        }
         if (parts == 1 && V * E < kShortRow)
           launch(std::integral_constant<int, 128>{});
         else if (TOP && (parts > 1 || rows > kFewRows))
@@ -676,17 +709,21 @@ extern "C" int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t strid
   if (!d_z || !d_targets || !d_stats || !d_dz || (d_g_entropy && !d_entropy)) return TMAC_ERR_NULL;
   const int E = dtype == TMAC_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(d_z) % E || reinterpret_cast<uintptr_t>(d_dz) % E) return TMAC_ERR_ALIGN;
-  const int64_t groups = (V + 16 / E - 2) / (16 / E) + 1;  // of a row at any alignment
-  const int64_t chunks = (groups + kGradGroups - 1) / kGradGroups;
-  const int64_t blocks = chunks * rows;
+  const int64_t groups = max_groups(V, dtype), chunks = (groups + kGradGroups - 1) / kGradGroups, blocks = chunks * rows;
   by_type(dtype, [&](auto dt) {
     by_flag(d_g_entropy != nullptr, [&](auto e) {
-      logprob_grad_kernel<decltype(dt)::value, decltype(e)::value>
-          <<<static_cast<unsigned>(blocks < (1 << 23) ? blocks : 1 << 23), kGradThreads, 0,
-             static_cast<hipStream_t>(stream)>>>(
-              static_cast<const uint8_t*>(d_z), Row2{stride_b, stride_t, T}, d_targets, ignore_index, d_stats,
-              d_entropy, d_g_lp, g_lp_stride, d_g_entropy, g_entropy_stride, static_cast<uint8_t*>(d_dz),
-              static_cast<int>(V), static_cast<int>(chunks), blocks);
+      auto launch = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        logprob_grad_kernel<decltype(dt)::value, decltype(e)::value, NT>
+            <<<static_cast<unsigned>(blocks < (1 << 23) ? blocks : 1 << 23), NT, 0, static_cast<hipStream_t>(stream)>>>(
+                static_cast<const uint8_t*>(d_z), Row2{stride_b, stride_t, T}, d_targets, ignore_index, d_stats,
+                d_entropy, d_g_lp, g_lp_stride, d_g_entropy, g_entropy_stride, static_cast<uint8_t*>(d_dz),
+                static_cast<int>(V), static_cast<int>(chunks), blocks);
+      };
+      if (groups <= kWaveGroups)
+        launch(std::integral_constant<int, 64>{});
+      else
+        launch(std::integral_constant<int, 256>{});
     });
   });
   return launch_status();
