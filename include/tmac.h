@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define TMAC_ABI_VERSION 9
+#define TMAC_ABI_VERSION 10
 #define TMAC_BLOCK 64
 
 typedef enum {
@@ -740,6 +740,11 @@ int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t stride_t, const 
  * neg_inv = −1 / n. */
 int tmac_logprob_mean(const float* d_lp, const int64_t* d_targets, int64_t ignore_index, int rows, void* d_loss,
                       int dtype, float* d_neg_inv, void* stream);
+
+/* tmac_logprob_bwd for the loss: of every row g_lp = neg_inv · g_loss (one value of g_dtype). */
+int tmac_logprob_mean_bwd(const void* d_z, int64_t stride_b, int64_t stride_t, const int64_t* d_targets,
+                          int64_t ignore_index, const float* d_stats, const float* d_neg_inv, const void* d_g_loss,
+                          int g_dtype, void* d_dz, int B, int T, int64_t V, int dtype, void* stream);
 
 /* The same lp and H for the logits z = X · Wᵀ of the model's head (models/titanmac.py:126-128), which are
  * not stored: X [M, K] and W [V, K] in 16 bit with pitches ldx, ldw, K a multiple of 64, pointers 16-byte

@@ -1,5 +1,5 @@
-"""Grids at the largest sizes that the entry points accept: a launch takes fewer than 2^32 threads. On the CPU, in a
-process of its own whose launches only write their grid down."""
+"""Grids at the largest sizes that the token operators' entry points accept: a launch takes fewer than 2^32 threads. On the CPU, in a
+process of its own whose launches only write their grid down; and refusals."""
 import json
 import shutil
 import subprocess
@@ -57,6 +57,7 @@ for V in (1, 129, 128000, 1 << 28):
         for B, T in ((1, BIG), (BIG, 1), (1, 1), (2, 100)):
             call("tmac_logprob_fwd", A, L(V), L(V), A, L(-100), A, A, I(top), A, A, A, A, WS, I(B), I(T), L(V), I(1), P(0))
             call("tmac_logprob_bwd", A, L(V), L(V), A, L(-100), A, A, A, L(1), A, L(1), A, I(B), I(T), L(V), I(1), P(0))
+            call("tmac_logprob_mean_bwd", A, L(V), L(V), A, L(-100), A, A, A, I(1), A, I(B), I(T), L(V), I(1), P(0))
     for M in (1, 64, 65, 8192, 1 << 26, (1 << 26) + 1, BIG):
         for K in (64, 640, 1024):
             call("tmac_head_logprob", A, L(K), A, L(K), A, L(-100), A, A, I(M), L(V), I(K), A, WS, I(1), P(0))
@@ -89,3 +90,18 @@ def test_prefix_rows_are_counted_without_sequences():
     w = torch.zeros(5, 8)
     with pytest.raises(ValueError, match="rows"):
         tc.token_embedding(torch.zeros(0, 3, dtype=torch.long), w, prefix=w[:1].expand((1 << 32) + 3, 8))
+
+
+def test_loss_gradient_argument_errors(lib):
+    fake = 1 << 20
+    # z, stride_b, stride_t, targets, ignore, stats, neg_inv, g_loss, g_dtype, dz, B, T, V, dtype, stream
+    ok = [fake, 0, 100, fake, -100, fake, fake, fake, 1, fake, 1, 4, 100, 0, None]
+    for at, value, want in ((0, None, -1), (3, None, -1), (5, None, -1), (6, None, -1), (7, None, -1), (9, None, -1),
+                            (8, 3, -4), (0, fake + 2, -5), (9, fake + 1, -5), (2, -1, -2), (10, -1, -2), (12, 0, -2),
+                            (13, 3, -4)):
+        bad = list(ok)
+        bad[at] = value
+        assert lib.tmac_logprob_mean_bwd(*bad) == want, (at, value)
+    empty = list(ok)
+    empty[10] = 0
+    assert lib.tmac_logprob_mean_bwd(*empty) == 0

@@ -432,17 +432,34 @@ __global__ __launch_bounds__(NT) void logprob_join_kernel(const uint8_t* __restr
 // Gradient: workgroup (row, chunk of kChunk groups of the output row).
 constexpr int kGradGroups = 1024;
 
+struct Factor {  // of g_lp: one value of a type in memory, or 1
+  const void* at;
+  int dtype;
+  __device__ __forceinline__ float load() const {
+    float v[1] = {1.f};
+    if (!at) return v[0];
+    if (dtype == TMAC_F32)
+      row_load<TMAC_F32, 1>(at, v);
+    else if (dtype == TMAC_BF16)
+      row_load<TMAC_BF16, 1>(at, v);
+    else
+      row_load<TMAC_F16, 1>(at, v);
+    return v[0];
+  }
+};
+
 template <int DT, bool ENT, int NT>
 __device__ __forceinline__ void logprob_grad_chunk(
     const uint8_t* __restrict__ z, Row2 zr, const int64_t* __restrict__ targets, int64_t ignore,
     const float* __restrict__ stats, const float* __restrict__ ent, const float* __restrict__ g_lp, int64_t g_lp_st,
-    const float* __restrict__ g_ent, int64_t g_ent_st, uint8_t* __restrict__ dz, int V, int chunks, int64_t block) {
+    float g_factor, const float* __restrict__ g_ent, int64_t g_ent_st, uint8_t* __restrict__ dz, int V, int chunks,
+    int64_t block) {
   constexpr int N = kRowVec<DT>, E = kRowSize<DT>;
   const int row = static_cast<int>(block / chunks);
   const int chunk = static_cast<int>(block - static_cast<int64_t>(row) * chunks);
   const int64_t target = targets[row];
   const bool given = g_lp && target != ignore;
-  const float gl = given ? g_lp[row * g_lp_st] : 0.f;
+  const float gl = given ? g_lp[row * g_lp_st] * g_factor : 0.f;
   const float ge = ENT ? g_ent[row * g_ent_st] : 0.f;
   const float mu = stats[2 * static_cast<int64_t>(row)], s = stats[2 * static_cast<int64_t>(row) + 1];
   const float inv = 1.f / s, log_s = __builtin_amdgcn_logf(s) * kLn2;
@@ -505,9 +522,12 @@ template <int DT, bool ENT, int NT>
 __global__ __launch_bounds__(NT) void logprob_grad_kernel(
     const uint8_t* __restrict__ z, Row2 zr, const int64_t* __restrict__ targets, int64_t ignore,
     const float* __restrict__ stats, const float* __restrict__ ent, const float* __restrict__ g_lp, int64_t g_lp_st,
-    const float* __restrict__ g_ent, int64_t g_ent_st, uint8_t* __restrict__ dz, int V, int chunks, int64_t blocks) {
+    Factor factor, const float* __restrict__ g_ent, int64_t g_ent_st, uint8_t* __restrict__ dz, int V, int chunks,
+    int64_t blocks) {
+  const float g_factor = factor.load();
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x)
-    logprob_grad_chunk<DT, ENT, NT>(z, zr, targets, ignore, stats, ent, g_lp, g_lp_st, g_ent, g_ent_st, dz, V, chunks, b);
+    logprob_grad_chunk<DT, ENT, NT>(z, zr, targets, ignore, stats, ent, g_lp, g_lp_st, g_factor, g_ent, g_ent_st, dz, V,
+                                    chunks, b);
 }
 
 // The mean of −lp over the rows that are not ignored (NaN where there are none), and −1 / their number for
@@ -630,6 +650,37 @@ void by_flag(bool on, F&& f) {
 
 size_t stat_bytes(int rows, int parts) { return parts > 1 ? sizeof(Stat) * static_cast<size_t>(rows) * parts : 0; }
 
+int launch_grad(const void* d_z, int64_t stride_b, int64_t stride_t, const int64_t* d_targets, int64_t ignore_index,
+                const float* d_stats, const float* d_entropy, const float* d_g_lp, int64_t g_lp_stride, Factor factor,
+                const float* d_g_entropy, int64_t g_entropy_stride, void* d_dz, int B, int T, int64_t V, int dtype,
+                void* stream) {
+  const int st = check(B, T, V, stride_t, stride_b, dtype);
+  if (st != TMAC_OK) return st;
+  const int rows = B * T;
+  if (rows == 0) return TMAC_OK;
+  if (!d_z || !d_targets || !d_stats || !d_dz || (d_g_entropy && !d_entropy)) return TMAC_ERR_NULL;
+  const int E = dtype == TMAC_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(d_z) % E || reinterpret_cast<uintptr_t>(d_dz) % E) return TMAC_ERR_ALIGN;
+  const int64_t groups = max_groups(V, dtype), chunks = (groups + kGradGroups - 1) / kGradGroups, blocks = chunks * rows;
+  by_type(dtype, [&](auto dt) {
+    by_flag(d_g_entropy != nullptr, [&](auto e) {
+      auto launch = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        logprob_grad_kernel<decltype(dt)::value, decltype(e)::value, NT>
+            <<<static_cast<unsigned>(blocks < (1 << 23) ? blocks : 1 << 23), NT, 0, static_cast<hipStream_t>(stream)>>>(
+                static_cast<const uint8_t*>(d_z), Row2{stride_b, stride_t, T}, d_targets, ignore_index, d_stats,
+                d_entropy, d_g_lp, g_lp_stride, factor, d_g_entropy, g_entropy_stride, static_cast<uint8_t*>(d_dz),
+                static_cast<int>(V), static_cast<int>(chunks), blocks);
+      };
+      if (groups <= kWaveGroups)
+        launch(std::integral_constant<int, 64>{});
+      else
+        launch(std::integral_constant<int, 256>{});
+    });
+  });
+  return launch_status();
+}
+
 }  // namespace
 
 extern "C" int tmac_logprob_workspace(int B, int T, int64_t V, int top_k, int dtype, size_t* ws_bytes) {
@@ -702,31 +753,18 @@ extern "C" int tmac_logprob_bwd(const void* d_z, int64_t stride_b, int64_t strid
                                 const float* d_g_lp, int64_t g_lp_stride, const float* d_g_entropy,
                                 int64_t g_entropy_stride, void* d_dz, int B, int T, int64_t V, int dtype,
                                 void* stream) {
-  const int st = check(B, T, V, stride_t, stride_b, dtype);
-  if (st != TMAC_OK) return st;
-  const int rows = B * T;
-  if (rows == 0) return TMAC_OK;
-  if (!d_z || !d_targets || !d_stats || !d_dz || (d_g_entropy && !d_entropy)) return TMAC_ERR_NULL;
-  const int E = dtype == TMAC_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(d_z) % E || reinterpret_cast<uintptr_t>(d_dz) % E) return TMAC_ERR_ALIGN;
-  const int64_t groups = max_groups(V, dtype), chunks = (groups + kGradGroups - 1) / kGradGroups, blocks = chunks * rows;
-  by_type(dtype, [&](auto dt) {
-    by_flag(d_g_entropy != nullptr, [&](auto e) {
-      auto launch = [&](auto nt) {
-        constexpr int NT = decltype(nt)::value;
-        logprob_grad_kernel<decltype(dt)::value, decltype(e)::value, NT>
-            <<<static_cast<unsigned>(blocks < (1 << 23) ? blocks : 1 << 23), NT, 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const uint8_t*>(d_z), Row2{stride_b, stride_t, T}, d_targets, ignore_index, d_stats,
-                d_entropy, d_g_lp, g_lp_stride, d_g_entropy, g_entropy_stride, static_cast<uint8_t*>(d_dz),
-                static_cast<int>(V), static_cast<int>(chunks), blocks);
-      };
-      if (groups <= kWaveGroups)
-        launch(std::integral_constant<int, 64>{});
-      else
-        launch(std::integral_constant<int, 256>{});
-    });
-  });
-  return launch_status();
+  return launch_grad(d_z, stride_b, stride_t, d_targets, ignore_index, d_stats, d_entropy, d_g_lp, g_lp_stride,
+                     Factor{nullptr, 0}, d_g_entropy, g_entropy_stride, d_dz, B, T, V, dtype, stream);
+}
+
+extern "C" int tmac_logprob_mean_bwd(const void* d_z, int64_t stride_b, int64_t stride_t, const int64_t* d_targets,
+                                     int64_t ignore_index, const float* d_stats, const float* d_neg_inv,
+                                     const void* d_g_loss, int g_dtype, void* d_dz, int B, int T, int64_t V, int dtype,
+                                     void* stream) {
+  if (g_dtype != TMAC_F32 && g_dtype != TMAC_BF16 && g_dtype != TMAC_F16) return TMAC_ERR_DTYPE;
+  if (!d_neg_inv || !d_g_loss) return TMAC_ERR_NULL;
+  return launch_grad(d_z, stride_b, stride_t, d_targets, ignore_index, d_stats, nullptr, d_neg_inv, 0,
+                     Factor{d_g_loss, g_dtype}, nullptr, 0, d_dz, B, T, V, dtype, stream);
 }
 
 extern "C" int tmac_logprob_mean(const float* d_lp, const int64_t* d_targets, int64_t ignore_index, int rows,

@@ -16,7 +16,7 @@ from pathlib import Path
 import torch  # the HIP runtime torch loads (libamdhip64.so.7) also serves libtmac.so
 from torch.autograd import forward_ad
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 F32, BF16, F16 = 0, 1, 2
 EPI_NONE, EPI_GELU = 0, 1
@@ -111,6 +111,7 @@ SIGNATURES = {
     "tmac_logprob_fwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _i, _i, _i64, _i, _vp],
     "tmac_logprob_bwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i, _vp],
     "tmac_logprob_mean": [_vp, _vp, _i64, _i, _vp, _i, _vp, _vp],
+    "tmac_logprob_mean_bwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _i, _i, _i64, _i, _vp],
     "tmac_head_logprob_workspace": [_i, _i64, _i, ctypes.POINTER(_sz)],
     "tmac_head_logprob": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i64, _i, _vp, _sz, _i, _vp],
 }
