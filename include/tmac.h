@@ -698,10 +698,11 @@ int tmac_embed_fwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_W, 
  *   dW[v] = scale · Σ_{ids[b, t] = v} g[b, n_prefix + t]    [V, d]
  *   dP[q] = Σ_{pos(b, t) = q} g[b, n_prefix + t]            [n_pos, d]
  *   dprefix[p] = Σ_b g[b, p]                                [n_prefix, d]
- * Rows without a token are zeros, indices outside a table count nowhere. fp32 sums in an order that the sizes alone
- * decide (deterministic), rounded once. d_lists: the forward's, for the same ids, B, T, n_prefix and V, or NULL (they
- * are made of d_ids). d_ws: 16-byte aligned, tmac_embed_bwd_workspace(B·T, V, n_pos, d) bytes with V = 0 without
- * d_dW or with d_lists, and n_pos = 0 without d_dP or d_pos; none without d_dW where the second is 0 too. */
+ * Rows without a token are zeros; an index outside its own table adds nothing to that table's gradient. fp32 sums
+ * in an order that the sizes alone decide (deterministic), rounded once. d_lists: the forward's, for the same ids, B,
+ * T, n_prefix and V, or NULL (they are made of d_ids). d_ws: 16-byte aligned,
+ * tmac_embed_bwd_workspace(B·T, V, n_pos, d) bytes with V = 0 without d_dW or with d_lists, and n_pos = 0 without d_dP
+ * or d_pos; none without d_dW where the second is 0 too. */
 int tmac_embed_bwd_workspace(int64_t n_tokens, int64_t V, int64_t n_pos, int d, size_t* ws_bytes);
 int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const void* d_lists, const void* d_g, int64_t ldg,
                    void* d_dW, void* d_dP, void* d_dprefix, void* d_ws, size_t ws_bytes, int B, int T, int n_prefix,

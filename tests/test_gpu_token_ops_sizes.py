@@ -123,3 +123,101 @@ def test_many_short_rows(dev, rows, V, dtype):
     want = -total / n
     # a thread adds rows / 1024 values, then 16 waves of 64
     assert abs(loss.double().item() - want) <= u * want + ((rows / 1024 + 22) * 2.0 ** -24 + 2 * (V + 64) * 2.0 ** -24) * max(want, 1)
+
+
+def embedding64(ids, pos, tables, up, scale):
+    """y and the gradients of the three tables in 64 bits, with the sums of their terms' magnitudes and numbers."""
+    w, p, f = tables
+    Np, d = f.shape
+    y = torch.cat([f.double().expand(len(ids), -1, -1), w.double()[ids] * scale + p.double()[pos]], 1)
+    g, out = up.double()[:, Np:].reshape(-1, d), []
+    for index, n, c in ((ids, len(w), scale), (pos, len(p), 1.0)):
+        zero, index = torch.zeros(n, d, dtype=torch.float64, device=g.device), index.reshape(-1)
+        out.append((zero.index_add(0, index, g * c), zero.index_add(0, index, (g * c).abs()), index.bincount(minlength=n)))
+    h = up.double()[:, :Np]
+    return y, [*out, (h.sum(0), h.abs().sum(0), torch.full((Np,), len(ids), device=g.device))]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,V,d,given", [
+    (5, 3333, 700, 16, False), (5, 3333, 20001, 16, True),   # more tokens than a wave reads in one turn (8192 in all)
+    (9, 8192, 8193, 8, False),                               # nine turns of them
+    (2, 40, 60, 4096, False), (3, 50, 30, 1500, True),       # rows of more pieces than a workgroup has threads
+    (1, 70, 3, 9001, False),
+])
+@pytest.mark.parametrize("hot", [0, 1])
+def test_turns_of_the_embedding(dev, B, T, V, d, given, hot, dtype):
+    """Nine of ten tokens are three neighbouring ids: the first, or (hot) ones in the last, wide range."""
+    g = torch.Generator().manual_seed(T + V)
+    ids = torch.randint(0, V, (B, T), generator=g)
+    ids = torch.where(torch.rand(B, T, generator=g) < 0.9, (V - 3) * hot + ids % 3, ids).to(dev)
+    pos = torch.randint(0, 50, (B, T), generator=g).to(dev) if given else torch.arange(T, device=dev).expand(B, T)
+    n_pos = 64 if given else T + 5
+    tables = [torch.randn(n, d, generator=g).to(dev, dtype).requires_grad_() for n in (V, n_pos, 3)]
+    up = torch.randn(B, 3 + T, d, generator=g).to(dev, dtype)
+    y = tc.token_embedding(ids, *tables[:2], positions=pos if given else None, prefix=tables[2], scale=0.75)
+    grads = torch.autograd.grad(y, tables, up)
+    want, sums = embedding64(ids, pos, [t.detach() for t in tables], up, 0.75)
+    u = torch.finfo(dtype).eps / 2
+    assert torch.all((y.double() - want).abs() <= u * want.abs() + 2.0 ** -22 * (want.abs() + 5))
+    for got, (a, size, n) in zip(grads, sums):
+        # n fp32 additions in some order and the factor, then one rounding
+        assert torch.all((got.double() - a).abs() <= u * 1.01 * a.abs() + (n[:, None] + 2) * 2.0 ** -24 * size)
+        assert torch.all(got[n == 0] == 0)
+
+
+@pytest.mark.parametrize("top", [0, 3])
+def test_more_rows_than_workgroups(dev, top):
+    """2^21 rows and some: the forward's workgroups take turns, their shared memory used again."""
+    rows, V = (1 << 21) + 5003, 9
+    g = torch.Generator().manual_seed(top)
+    z = (torch.randn(rows, V, generator=g) * 2).to(dev, torch.bfloat16)
+    t = torch.randint(0, V, (rows,), generator=g).to(dev)
+    t[::7] = -100
+    r = tc.token_logprobs(z, t, entropy=True, top_k=top)
+    tol = (V + 64) * 2.0 ** -24
+    for a in range(0, rows, 1 << 19):
+        at = slice(a, a + (1 << 19))
+        lp, H, _, logp = rows64(z[at], t[at])
+        assert torch.allclose(r.logprobs[at].double(), lp, rtol=0, atol=tol)
+        assert torch.allclose(r.entropy[at].double(), H, rtol=0, atol=24 * tol)
+        if top:
+            ids = torch.sort(z[at].double(), dim=-1, descending=True, stable=True).indices[:, :top]
+            assert torch.equal(r.top_ids[at], ids)
+            assert torch.allclose(r.top_logprobs[at].double(), logp.gather(-1, ids), rtol=0, atol=tol)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 700])
+def test_the_loss_of_ignored_rows_alone(dev, rows):
+    """No row asked for: a loss of NaN, a gradient of zeros, whatever the rows hold."""
+    z = torch.full((rows, 4001), float("nan"), device=dev, dtype=torch.bfloat16)
+    z[-1] = float("inf")
+    z.requires_grad_()
+    loss = tc.token_cross_entropy(z, torch.full((rows,), -100, device=dev))
+    assert torch.isnan(loss)
+    dz, = torch.autograd.grad(loss, z)
+    assert torch.all(dz == 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("given", [False, True])
+def test_each_table_takes_the_tokens_within_it(dev, given, dtype):
+    """A token whose id (position) is outside its table adds to the other table's gradient: that is decided per table."""
+    g = torch.Generator().manual_seed(1)
+    V, n_pos, B, T, d = 11, 9, 3, 40, 24
+    ids = torch.randint(-2, V + 2, (B, T), generator=g).to(dev)
+    pos = torch.randint(-2, n_pos + 2, (B, T), generator=g).to(dev) if given else None
+    n_pos = n_pos if given else T
+    w, p = (torch.randn(n, d, generator=g).to(dev, dtype).requires_grad_() for n in (V, n_pos))
+    up = torch.randint(-2, 3, (B, T, d), generator=g).to(dev, dtype)  # small whole numbers: exact sums
+    y = tc.token_embedding(ids, w, p, positions=pos)
+    at = torch.arange(T, device=dev).expand(B, T) if pos is None else pos
+    outside = (ids < 0) | (ids >= V) | (at < 0) | (at >= n_pos)
+    assert torch.equal(torch.isnan(y).all(-1), outside) and torch.equal(torch.isnan(y).any(-1), outside)
+    grads = torch.autograd.grad(y, (w, p), up, retain_graph=True)
+    up2 = up.clone().requires_grad_()  # recorded: the gradients in torch's operations
+    recorded = torch.autograd.grad(y, (w, p), up2, create_graph=True)
+    for got, rec, index, n in zip(grads, recorded, (ids, at), (V, n_pos)):
+        ok = (index >= 0) & (index < n)
+        want = torch.zeros(n, d, device=dev).index_add(0, index[ok], up[ok].float())
+        assert torch.equal(got.float(), want) and torch.equal(rec.float(), want)

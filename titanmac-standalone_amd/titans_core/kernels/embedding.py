@@ -226,7 +226,8 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, pos_weight: Optiona
     ids: int64 or int32 [B, T]; weight [V, d], pos_weight [n_pos, d] and prefix [Np, d] of one dtype
     (float32, bfloat16, float16), d up to 2^20, up to 2^30 rows. positions: [B, T] or [T], by default
     0 .. T - 1. The sum is formed in fp32 and rounded once. Nothing is copied to the host to look at the ids:
-    one outside [0, V), or a position outside its table, gives a row of NaN and adds to no gradient.
+    one outside [0, V), or a position outside its table, gives a row of NaN and adds nothing to the gradient of the
+    table that it is outside of (the other table's takes the row's gradient as any).
 
     Differentiable in the three tables (a second time too)."""
     tables = (ids, weight, pos_weight, positions, prefix)
