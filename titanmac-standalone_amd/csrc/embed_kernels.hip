@@ -286,7 +286,7 @@ struct Grad {
   float scale;
   uint8_t *dprefix, *dP;  // rows [first, last) of [prefix | positions] by sums over the sequences
   int B, T, Np;
-  int64_t first, last;
+  uint32_t first, last;  // up to 2^31
   int pos_blocks, pos_rpb;
   int runs, run_first, run_pieces, run_blocks;  // and the pieces of rows [run_first, first) by runs of the sequences
   int d, cpr;
@@ -342,12 +342,11 @@ __device__ __forceinline__ void grad_rows(const Grad& a, int block) {
 template <int DT, int N>
 __device__ __forceinline__ void grad_positions(const Grad& a, int block) {
   constexpr int E = kRowSize<DT>;
-  const int S = a.Np + a.T;
-  const int64_t row0 = a.first + static_cast<int64_t>(block) * a.pos_rpb;
-  const int n = static_cast<int>(min(static_cast<int64_t>(a.pos_rpb), a.last - row0)) * a.cpr;
+  const uint32_t S = a.Np + a.T, row0 = a.first + static_cast<uint32_t>(block) * a.pos_rpb;
+  const int n = static_cast<int>(min(static_cast<uint32_t>(a.pos_rpb), a.last - row0)) * a.cpr;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int r = i / a.cpr, c = (i - r * a.cpr) * N;
-    const int64_t s = row0 + r;
+    const uint32_t s = row0 + r;
     float v[N] = {};
     if (s < S) {
 #pragma unroll 4
@@ -358,7 +357,9 @@ __device__ __forceinline__ void grad_positions(const Grad& a, int block) {
         for (int e = 0; e < N; ++e) v[e] += x[e];
       }
     }
-    row_store<DT, N>(s < a.Np ? a.dprefix + (s * a.d + c) * E : a.dP + ((s - a.Np) * a.d + c) * E, v);
+    row_store<DT, N>(s < static_cast<uint32_t>(a.Np) ? a.dprefix + (static_cast<int64_t>(s) * a.d + c) * E
+                                                     : a.dP + (static_cast<int64_t>(s - a.Np) * a.d + c) * E,
+                     v);
   }
 }
 
@@ -411,17 +412,25 @@ __device__ __forceinline__ void grad_runs(const Grad& a, int block) {
                      v);
 }
 
-// The chunks of long lists first, whose sums the next launch waits for.
-template <int DT, int N>
+// The chunks of long lists first, whose sums the next launch waits for. RUNS: whether a.run_blocks is not 0, which
+// takes registers and LDS that every other launch is better without (8 x 4096 tokens of 640 bf16 36.7 us, 40.6 with).
+template <int DT, int N, bool RUNS>
 __global__ __launch_bounds__(kThreads) void embed_grad_kernel(Grad a) {
-  const int64_t runs = static_cast<int64_t>(a.chunks) + a.run_blocks, sums = runs + a.pos_blocks;
-  const int64_t blocks = sums + a.row_blocks;
-  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    if (b < a.chunks)
+  // up to 2^26, 2^19, 2^31 and 2^30
+  const uint32_t chunks = a.chunks, runs = chunks + (RUNS ? a.run_blocks : 0), sums = runs + a.pos_blocks;
+  const uint32_t blocks = sums + a.row_blocks;
+  for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    if (b < chunks) {
       grad_chunk<DT, N>(a, static_cast<int>(b));
-    else if (b < runs)
-      grad_runs<DT, N>(a, static_cast<int>(b - a.chunks));
-    else if (b < sums)
+      continue;
+    }
+    if constexpr (RUNS) {
+      if (b < runs) {
+        grad_runs<DT, N>(a, static_cast<int>(b - chunks));
+        continue;
+      }
+    }
+    if (b < sums)
       grad_positions<DT, N>(a, static_cast<int>(b - runs));
     else
       grad_rows<DT, N>(a, static_cast<int>(b - sums));
@@ -524,9 +533,13 @@ void dispatch(int dtype, bool wide, F&& f) {
 }
 
 // Runs of B sequences that `pieces` pieces of rows are summed in: a power of two, no more than fill the card (2^19
-// threads) and of at least 8 sequences, one turn of loads; 1: one thread a piece.
+// threads) and of at least 8 sequences, one turn of loads; 1: one thread a piece, whose sums hide beside the other
+// table's up to some sequences. us of the gradients with one thread and with runs: 128 x 128 tokens of 640 bf16 29 / 33,
+// 128 x 16 of 256 16.2 / 16.3, 256 x 64 of 640 41 / 34, 512 x 128 81 / 57, 2000 x 64 270 / 137.
+constexpr int kManySequences = 256;
 int n_runs(int B, int64_t pieces) {
   int n = 1;
+  if (B < kManySequences) return n;
   while (2 * n <= kThreads && 2 * n * pieces <= 1 << 19 && B / (2 * n) >= 8) n *= 2;
   return n;
 }
@@ -659,7 +672,7 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
       a.dprefix = static_cast<uint8_t*>(d_dprefix);
       a.dP = sums ? static_cast<uint8_t*>(d_dP) : nullptr;
       a.first = d_dprefix ? 0 : n_prefix;
-      a.last = n_prefix + (sums ? n_pos : 0);
+      a.last = static_cast<uint32_t>(n_prefix) + static_cast<uint32_t>(sums ? n_pos : 0);
     }
     if (out) {
       const Lists to = lists(given ? const_cast<void*>(given) : d_ws, n_tok, n_rows);
@@ -692,12 +705,15 @@ extern "C" int tmac_embed_bwd(const int64_t* d_ids, const int64_t* d_pos, const 
         a.run_first = static_cast<int>(a.first);
         a.run_pieces = static_cast<int>(summed * a.cpr);
         a.run_blocks = (a.run_pieces + kThreads / a.runs - 1) / (kThreads / a.runs);
-        a.first += summed;
+        a.first += static_cast<uint32_t>(summed);
       }
-      a.pos_blocks = static_cast<int>((a.last - a.first + a.pos_rpb - 1) / a.pos_rpb);
+      a.pos_blocks = static_cast<int>((static_cast<int64_t>(a.last) - a.first + a.pos_rpb - 1) / a.pos_rpb);
       const int64_t blocks = static_cast<int64_t>(a.chunks) + a.run_blocks + a.pos_blocks + a.row_blocks;
       if (!blocks) return;
-      embed_grad_kernel<DT, N><<<grid(blocks, kThreads), kThreads, 0, s>>>(a);
+      if (a.run_blocks)
+        embed_grad_kernel<DT, N, true><<<grid(blocks, kThreads), kThreads, 0, s>>>(a);
+      else
+        embed_grad_kernel<DT, N, false><<<grid(blocks, kThreads), kThreads, 0, s>>>(a);
       if (a.chunks)
         embed_grad_long_kernel<DT, N><<<grid((a.chunks + kLongChunks - 1) / kLongChunks, 1024), 1024, 0, s>>>(a);
     });
