@@ -122,14 +122,6 @@ __device__ __forceinline__ float lanes_max(float x) {
   x = fmaxf(x, lane_xor<16>(x));
   return fmaxf(x, lane_xor<32>(x));
 }
-__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
-  x = max(x, lane_xor<1>(x));
-  x = max(x, lane_xor<2>(x));
-  x = max(x, lane_xor<4>(x));
-  x = max(x, lane_xor<8>(x));
-  x = max(x, lane_xor<16>(x));
-  return max(x, lane_xor<32>(x));
-}
 __device__ __forceinline__ float lanes_sum(float x) {
   x += lane_xor<1>(x);
   x += lane_xor<2>(x);
