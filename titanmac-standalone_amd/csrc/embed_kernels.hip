@@ -10,7 +10,7 @@
 //
 // The gradient sums each row's tokens in ascending order of position (deterministic): a sort gives every
 // row of W its list of tokens; a list of up to 16 is summed where its row is written; longer ones (the
-// frequent tokens: a text's first hundred ids are half of it) are summed 16 tokens a workgroup into fp32
+// frequent tokens: with ids that fall off as 1 / (rank + 1) over 128000, the first hundred are 39 % of a text) are summed 16 tokens a workgroup into fp32
 // partial rows that a third kernel adds in order, so one frequent token does not hold one workgroup. With lists
 // of up to 64 tokens in one thread's chain of loads the sums take 54 us instead of 37 for 32768 tokens of 640
 // bf16, V = 128000.
@@ -98,8 +98,10 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
 }
 
 // The ids of a workgroup of the sort: [0, 8), then eight ranges to an octave up to 8192, then 512 each.
-// Low ids are the frequent ones (token tables are made by frequency), and a narrow range is cheap where
-// every batch has some: the ids' bits are what the placing below counts instructions by.
+// A narrow range is cheap where every batch of ids has some in it: the ids' bits are what the placing below counts
+// instructions by. The narrow ones lie low because tables made by frequency have their frequent ids there; where they
+// lie elsewhere it costs time only (8 x 4096 tokens of 640 bf16, V = 128000, the ids permuted: lookup and lists 42 us
+// for 36, sums 44 for 37).
 struct IdRange {
   int lo, n;
 };

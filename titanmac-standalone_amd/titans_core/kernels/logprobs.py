@@ -320,7 +320,8 @@ _ce_native = _lib.native_function(_cross_entropy_fwd, _ce_setup, _ce_backward)
 def token_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100) -> torch.Tensor:
     """The mean of -log softmax(logits)[target] over the targets other than ignore_index (NaN where there are
     none), as F.cross_entropy of [..., V] logits: in their dtype, or fp32 inside torch.autocast. Ignored
-    rows are not read and get zeros as gradient. Other targets outside [0, V) make it NaN."""
+    rows are not read and get zeros as gradient. Other targets outside [0, V) make it NaN. The gradient reads the
+    logits again: autograd refuses it if they were changed in place since."""
     args = (logits, targets, int(ignore_index), torch.is_autocast_enabled("cuda"))
     if _lib.direct_call(logits, targets):
         return _cross_entropy_fwd(*args)[0]

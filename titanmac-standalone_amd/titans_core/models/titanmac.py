@@ -362,6 +362,11 @@ class TitanMAC(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 attention_mask: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
+        """The variant's forward: ``logits``, with a neural memory ``memory_loss``, with labels ``loss``.
+
+        On the kernels nothing is copied to the host to look at ids and labels: an id outside the vocabulary gives
+        its positions NaN, a label outside it (other than -100) a loss of NaN. The loss keeps the logits for its
+        gradient, so autograd refuses the backward if they were changed in place before it: change a copy."""
         if self.neural_memory is not None and self.config.use_neural_memory:
             variant = self.config.titans_variant
             if variant == "MAC":
