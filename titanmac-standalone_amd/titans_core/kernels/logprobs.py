@@ -253,21 +253,45 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, entropy: bool
 
 # ------------------------------------------------------------------ the loss
 
+def _loss_fwd(logits, targets, ignore_index, wide, memory):
+    """(the mean of -lp over the given targets, in logits' dtype or (wide) fp32; what memory(rows, device) gave). That
+    begins with the addresses of lp [rows], stats [rows, 2] and -1 / the targets' number, fp32, which are written."""
+    _check(logits, targets, "token_cross_entropy")
+    code = _lib.dtype_code(logits.dtype)
+    dev = _lib.require_device(logits, targets, what="token_cross_entropy")
+    z, sb, st, B, T, V = _rows3(logits)
+    n, tg, L = B * T, _flat(targets), _lib.lib()
+    loss = torch.empty((), dtype=torch.float32 if wide else logits.dtype, device=dev)
+    lp, stats, inv, *kept = memory(n, dev)
+    nb = _workspace(B, T, V, 0, code) if n else 0
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    with _lib.device_guard(dev):
+        stream, at = _lib.stream_ptr(dev), tg.data_ptr()
+        if n:
+            rc = L.tmac_logprob_fwd(z.data_ptr(), sb, st, at, ignore_index, lp, 0, 0, 0, 0, stats, _lib.ptr(ws), nb, B, T,
+                                    V, code, stream)
+            _lib.check(rc, "tmac_logprob_fwd")
+        rc = L.tmac_logprob_mean(lp, at, ignore_index, n, loss.data_ptr(), _lib.F32 if wide else code, inv, stream)
+    _lib.check(rc, "tmac_logprob_mean")
+    return loss, kept
+
+
+def _apart(n, dev):
+    lp, stats, inv = (torch.empty(s, dtype=torch.float32, device=dev) for s in (n, (n, 2), ()))
+    return lp.data_ptr(), stats.data_ptr(), inv.data_ptr(), inv, stats, lp
+
+
+def _in_one(n, dev):
+    """stats, lp, inv in one tensor: fewer allocations, and one to keep for the backward."""
+    m = torch.empty(3 * n + 1, dtype=torch.float32, device=dev)
+    at = m.data_ptr()
+    return at + 8 * n, at, at + 12 * n, m
+
+
 def _cross_entropy_fwd(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, wide: bool
                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(the mean of -lp over the given targets, in logits' dtype or (wide) fp32; fp32 -1 / their number; stats)."""
-    _check(logits, targets, "token_cross_entropy")
-    code = _lib.F32 if wide else _lib.dtype_code(logits.dtype)
-    _lib.dtype_code(logits.dtype)
-    dev = _lib.require_device(logits, targets, what="token_cross_entropy")
-    lp, _, _, _, stats = _fwd(logits, targets, False, 0, ignore_index, dev)
-    loss = torch.empty((), dtype=torch.float32 if wide else logits.dtype, device=dev)
-    inv = torch.empty((), dtype=torch.float32, device=dev)
-    tg = _flat(targets)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_logprob_mean(_lib.ptr(lp), _lib.ptr(tg), ignore_index, lp.numel(), _lib.ptr(loss), code,
-                                          _lib.ptr(inv), _lib.stream_ptr(dev))
-    _lib.check(rc, "tmac_logprob_mean")
+    """(the loss, fp32 -1 / the targets' number, stats)."""
+    loss, (inv, stats, _) = _loss_fwd(logits, targets, ignore_index, wide, _apart)
     return loss, inv, stats
 
 
@@ -289,32 +313,47 @@ def _ce_setup(ctx, inputs, output):
     ctx.ignore_index = ignore_index
 
 
-def _ce_native_bwd(g_loss, logits, targets, inv, stats, ignore_index):
-    """The gradient of the logits in one launch: this runs in autograd's thread, where each torch operation before it
-    costs the host as much as the launch (and the product of g_loss in 16 bit and inv in fp32 35 us)."""
-    z, sb, st, B, T, V = _rows3(logits)
-    dev = logits.device
-    dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    if B * T:
-        tg = _flat(targets)
-        with _lib.device_guard(dev):
-            rc = _lib.lib().tmac_logprob_mean_bwd(z.data_ptr(), sb, st, tg.data_ptr(), ignore_index, stats.data_ptr(),
-                                                  inv.data_ptr(), g_loss.data_ptr(), _lib.dtype_code(g_loss.dtype),
-                                                  dz.data_ptr(), B, T, V, _lib.dtype_code(z.dtype), _lib.stream_ptr(dev))
-        _lib.check(rc, "tmac_logprob_mean_bwd")
-    return dz
-
-
 def _ce_backward(ctx, g_loss, *_):
     logits, targets, inv, stats = ctx.saved_tensors
-    if _lib.direct_backward(g_loss, logits):
-        return _ce_native_bwd(g_loss, logits, targets, inv, stats, ctx.ignore_index), None, None, None
     g_lp = (g_loss.to(inv.dtype) * inv).expand(targets.shape)
     return _gradient(g_lp, None, logits, targets, stats, None, ctx.ignore_index), None, None, None
 
 
 cross_entropy_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)
-_ce_native = _lib.native_function(_cross_entropy_fwd, _ce_setup, _ce_backward)
+
+
+def _ce_native_fwd(logits, targets, ignore_index, wide):
+    loss, (kept,) = _loss_fwd(logits, targets, ignore_index, wide, _in_one)
+    return loss, kept
+
+
+def _ce_native_setup(ctx, inputs, output):
+    logits, targets, ctx.ignore_index, _wide = inputs
+    ctx.save_for_backward(logits, targets, output[1])
+
+
+def _ce_native_backward(ctx, g_loss):
+    """One launch for g_loss and all: this runs in autograd's thread, where a torch operation costs the host as much as
+    the launch (and the product of a 16-bit g_loss and the fp32 -1 / n 35 us)."""
+    logits, targets, kept = ctx.saved_tensors
+    n, ignore = targets.numel(), ctx.ignore_index
+    if not _lib.direct_backward(g_loss, logits):
+        g_lp = (g_loss.to(kept.dtype) * kept[3 * n]).expand(targets.shape)
+        return _gradient(g_lp, None, logits, targets, kept[:2 * n].view(n, 2), None, ignore), None, None, None
+    z, sb, st, B, T, V = _rows3(logits)
+    dev, at = logits.device, kept.data_ptr()
+    dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if n:
+        tg = _flat(targets)
+        with _lib.device_guard(dev):
+            rc = _lib.lib().tmac_logprob_mean_bwd(z.data_ptr(), sb, st, tg.data_ptr(), ignore, at, at + 12 * n,
+                                                  g_loss.data_ptr(), _lib.dtype_code(g_loss.dtype), dz.data_ptr(), B, T, V,
+                                                  _lib.dtype_code(z.dtype), _lib.stream_ptr(dev))
+        _lib.check(rc, "tmac_logprob_mean_bwd")
+    return dz, None, None, None
+
+
+_ce_native = _lib.native_function(_ce_native_fwd, _ce_native_setup, _ce_native_backward)
 
 
 def token_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100) -> torch.Tensor:
@@ -324,7 +363,7 @@ def token_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, *, ignore_i
     logits again: autograd refuses it if they were changed in place since."""
     args = (logits, targets, int(ignore_index), torch.is_autocast_enabled("cuda"))
     if _lib.direct_call(logits, targets):
-        return _cross_entropy_fwd(*args)[0]
+        return _loss_fwd(*args, _in_one)[0]
     if _lib.eager_native(logits, targets):
         return _ce_native(*args)
     return cross_entropy_fwd(*args)[0]
