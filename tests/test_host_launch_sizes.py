@@ -105,3 +105,4 @@ def test_loss_gradient_argument_errors(lib):
     empty = list(ok)
     empty[10] = 0
     assert lib.tmac_logprob_mean_bwd(*empty) == 0
+    assert lib.tmac_logprob_mean(fake, fake, -100, (1 << 30) + 1, fake, 1, fake, None) == -2

@@ -779,7 +779,7 @@ extern "C" int tmac_logprob_mean_bwd(const void* d_z, int64_t stride_b, int64_t 
 extern "C" int tmac_logprob_mean(const float* d_lp, const int64_t* d_targets, int64_t ignore_index, int rows,
                                  void* d_loss, int dtype, float* d_neg_inv, void* stream) {
   if (dtype != TMAC_F32 && dtype != TMAC_BF16 && dtype != TMAC_F16) return TMAC_ERR_DTYPE;
-  if (rows < 0) return TMAC_ERR_SHAPE;
+  if (rows < 0 || rows > kMaxRows) return TMAC_ERR_SHAPE;
   if (!d_loss || !d_neg_inv || (rows && (!d_lp || !d_targets))) return TMAC_ERR_NULL;
   by_type(dtype, [&](auto dt) {
     logprob_mean_kernel<decltype(dt)::value><<<1, 1024, 0, static_cast<hipStream_t>(stream)>>>(
