@@ -221,15 +221,13 @@ def direct_call(*tensors: torch.Tensor | None) -> bool:
         return False
     if forward_ad._current_level >= 0:
         _no_tangents(*tensors)
-    if _intercepted():
-        return False
     grad = torch.is_grad_enabled()
     for t in tensors:
         if t is None:
             continue
         if type(t) not in _PLAIN or (grad and t.requires_grad):
             return False
-    return True
+    return not _intercepted()
 
 
 def direct_backward(grad: torch.Tensor, *tensors: torch.Tensor | None) -> bool:
