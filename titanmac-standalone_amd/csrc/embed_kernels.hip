@@ -10,10 +10,10 @@
 //
 // The gradient sums each row's tokens in ascending order of position (deterministic): a sort gives every
 // row of W its list of tokens; a list of up to 16 is summed where its row is written; longer ones (the
-// frequent tokens: with ids that fall off as 1 / (rank + 1) over 128000, the first hundred are 39 % of a text) are summed 16 tokens a workgroup into fp32
-// partial rows that a third kernel adds in order, so one frequent token does not hold one workgroup. With lists
-// of up to 64 tokens in one thread's chain of loads the sums take 54 us instead of 37 for 32768 tokens of 640
-// bf16, V = 128000.
+// frequent tokens: with ids that fall off as 1 / (rank + 1) over 128000, the first hundred are 39 % of a text) are
+// summed 16 tokens a workgroup into fp32 partial rows that a third kernel adds in order, so one frequent token does
+// not hold one workgroup. With lists of up to 64 tokens in one thread's chain of loads the sums take 54 us instead
+// of 37 for 32768 tokens of 640 bf16, V = 128000.
 
 #include "row_device.h"
 
