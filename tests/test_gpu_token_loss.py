@@ -76,3 +76,24 @@ def test_fp16_gradients_are_not_lost_in_the_upstream_type(dev):
     got, = torch.autograd.grad(loss, z, g)
     want = torch.tensor([-0.75, 0.25, 0.25, 0.25], dtype=torch.float64, device=dev) * 1000.0 / n
     assert torch.all((got.double() - want).abs() <= (2.0 ** -11 + 2.0 ** -20) * want.abs())
+
+
+@pytest.mark.parametrize("B", [1, 4])
+def test_kept_tensors_away_and_back(dev, B):
+    """What the loss keeps may be moved to the host in between, and is there for a second backward."""
+    gen = torch.Generator().manual_seed(B)
+    z = (torch.randn(B, 30, 1001, generator=gen) * 2).to(dev, torch.bfloat16)
+    t = torch.randint(0, 1001, (B, 30), generator=gen, dtype=torch.int32).to(dev)
+    a, b = (z[:, 3:].detach().requires_grad_() for _ in range(2))
+    want, = torch.autograd.grad(tc.token_cross_entropy(a, t[:, 3:]), a)
+    with torch.autograd.graph.save_on_cpu():
+        loss = tc.token_cross_entropy(b, t[:, 3:])
+    for _ in range(2):
+        got, = torch.autograd.grad(loss, b, retain_graph=True)
+        assert torch.equal(got, want)
+    # recorded: the same in torch's operations, and differentiable again
+    loss = tc.token_cross_entropy(b, t[:, 3:])
+    first, = torch.autograd.grad(loss, b, create_graph=True)
+    assert (first.double() - want.double()).norm() <= 2.0 ** -7 * want.double().norm()
+    second, = torch.autograd.grad(first.float().square().sum(), b)
+    assert torch.isfinite(second).all() and second.abs().sum() > 0
