@@ -205,7 +205,7 @@ def _plain_quantise(x, fmt):
     """Codes and scales of rows [..., d]; in 64 bits, as a value next to a border goes by its quotient."""
     amax = x.abs().amax(-1, keepdim=True).float()
     if fmt == "int8":
-        scale = (amax / 127).clamp(min=TINY)
+        scale = (amax.double() / 127).float().clamp(min=TINY)
         return (x.double() / scale.double()).round().to(torch.int8), scale[..., 0]
     m, e = torch.frexp(amax)  # amax = m 2^e, 1/2 <= m < 1; 448 = 0.875 2^9
     scale = torch.exp2((e - 9 + (m > 0.875)).clamp(min=-126).float())
