@@ -10,7 +10,9 @@
  *     WindowedAttention;
  *   - the ops around them (convolution, norm, projections, the memory's update);
  *   - the model's two ends: the token embedding, and the log probabilities of
- *     given tokens.
+ *     given tokens;
+ *   - the key/value cache of the windowed attention, and the attention of new
+ *     and drafted tokens over it.
  *
  * The reference (bigwolfeman/TitanMAC-Standalone) is pure Python and has no
  * FFI of its own; each entry point below cites the reference call it stands in
@@ -41,7 +43,7 @@
 extern "C" {
 #endif
 
-#define TMAC_ABI_VERSION 10
+#define TMAC_ABI_VERSION 11
 #define TMAC_BLOCK 64
 
 typedef enum {
@@ -73,6 +75,13 @@ typedef enum {
   TMAC_MASK_BOOL = 0,    /* uint8, nonzero = attend (the reference's bool mask) */
   TMAC_MASK_ADD_F32 = 1  /* fp32 added to the scaled scores (the reference's additive mask; -inf = masked) */
 } tmac_mask_format;
+
+/* How a key/value cache holds its rows. */
+typedef enum {
+  TMAC_CACHE_SAME = 0, /* in the type of the values */
+  TMAC_CACHE_INT8 = 1, /* code · scale, codes −127 .. 127, scale = amax / 127 in fp32 */
+  TMAC_CACHE_E4M3 = 2  /* code · scale, OCP e4m3 codes, scale the least power of two with amax <= 448 · scale */
+} tmac_cache_format;
 
 /* Human-readable text for a return code (negative tmac_status or positive hipError_t). */
 const char* tmac_status_string(int code);
@@ -755,6 +764,65 @@ int tmac_head_logprob_workspace(int M, int64_t V, int K, size_t* ws_bytes);
 int tmac_head_logprob(const void* d_X, int64_t ldx, const void* d_W, int64_t ldw, const int64_t* d_targets,
                       int64_t ignore_index, float* d_lp, float* d_entropy, int M, int64_t V, int K, void* d_ws,
                       size_t ws_bytes, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Key/value cache of the windowed attention, and attention over it: what WindowedAttention.forward
+ * (attn/windowed_attention.py:277-334) computes for new tokens behind those that are held. The reference has
+ * no cache: it runs the whole text for every token.
+ * ------------------------------------------------------------------------ */
+
+#define TMAC_CACHE_MAX_TREE 64
+
+/* A cache and the sequences in it.
+ *   d_k, d_v: pools [n_pages, n_heads, page, pitch], contiguous; page 16, 32, 64, 128 or 256; d_head 1..128, pitch
+ *     d_head rounded up to 16, what is behind d_head zeros; n_pages · n_heads · page < 2^40. format TMAC_CACHE_SAME: values
+ *     of dtype; else 8-bit codes with scales d_k_scale, d_v_scale, fp32 [n_pages, n_heads, page] (NULL with SAME).
+ *   d_table: int32 [B, max_pages] at a pitch of table_stride: the page of positions page·j .. page·j + page − 1.
+ *   d_lengths: int32 [B], the positions that each sequence holds, its new rows included; d_counts: int32 [B]
+ *     (nullable), how many are new: up to T, by default T or, where that is less, the length. New row t is
+ *     position length − count + t.
+ * Pools are 16-byte, the others 4-byte aligned. A sequence whose numbers do not fit (length < 0 or past the table, count
+ * < 0, > T or > length) is not written, and reads as NaN; so does a page outside [0, n_pages). */
+typedef struct {
+  void *d_k, *d_v;
+  float *d_k_scale, *d_v_scale;
+  const int32_t *d_table, *d_lengths, *d_counts;
+  int64_t n_pages, table_stride;
+  int n_heads, page, pitch, d_head, max_pages, format, dtype;
+} tmac_cache;
+
+/* The new rows k, v (elements b, head, t at h_strides[0..2], the d_head values of a row contiguous) into the cache. In 8 bits
+ * a code is the nearest to value / scale, ties to even; a row that is not finite is held as NaN. Rows t >= count
+ * are not read. Two sequences must not name the same page where they write. */
+int tmac_cache_write(const tmac_cache* cache, const void* d_new_k, const int64_t* h_k_strides, const void* d_new_v,
+                     const int64_t* h_v_strides, int B, int T, void* stream);
+
+/* Positions 0 .. T − 1 as k, v [B, n_heads, T, d_head], contiguous, in dtype: zeros behind a sequence's length. */
+int tmac_cache_read(const tmac_cache* cache, void* d_out_k, void* d_out_v, int B, int T, void* stream);
+
+/* Of a draft of T rows: row d_path[b, a] (int32 [B, A], at a pitch of path_stride) moves to place a of the draft, for
+ * all a at once; an entry outside [0, count) leaves its place as it is. A <= T <= TMAC_CACHE_MAX_TREE. */
+int tmac_cache_keep(const tmac_cache* cache, const int32_t* d_path, int64_t path_stride, int A, int B, int T,
+                    void* stream);
+
+/* out [B, T, n_q_heads, d_head], contiguous, = softmax(scale · q·kᵀ) · v of the new rows q (elements b, head, t at
+ * h_q_strides) over the cache; query head h reads key head h / (n_q_heads / n_heads). The new rows' keys and
+ * values are in the cache already. The row at position p sees position j if
+ *   p < n_persistent:   j < n_persistent
+ *   otherwise:          j < n_persistent or p − window <= j <= p
+ * With d_tree (int64 [B, T] at a pitch of tree_stride, 0 for one tree; T <= TMAC_CACHE_MAX_TREE) the new rows are a
+ * draft behind base = length − count positions: row t's bit s says that it sees drafted row s, itself included, and a
+ * drafted row's place in the window is base + (bits set in its entry) − 1. It sees the held
+ * positions j < base as above, and drafted row s if also its place is at least its own minus window (or it is stored
+ * below n_persistent). Rows that see nothing, and rows t >= count, are zeros. What a row does not see does not reach
+ * it, whatever is stored there.
+ * Scores, sums and the accumulation are fp32; in 16 bit the probabilities are rounded to dtype. window >= 0.
+ * d_ws: tmac_cached_attn_workspace bytes (0: none), 16-byte aligned. */
+int tmac_cached_attn_workspace(const tmac_cache* cache, int B, int T, int n_q_heads, int64_t window, int n_persistent,
+                               size_t* ws_bytes);
+int tmac_cached_attn(const tmac_cache* cache, const void* d_q, const int64_t* h_q_strides, const int64_t* d_tree,
+                     int64_t tree_stride, void* d_out, void* d_ws, size_t ws_bytes, int B, int T, int n_q_heads,
+                     int64_t window, int n_persistent, float scale, void* stream);
 
 #ifdef __cplusplus
 }

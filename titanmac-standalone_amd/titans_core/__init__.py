@@ -13,8 +13,9 @@ from .attn import (BlockSparseAttention, WindowConfig, WindowedAttention, build_
                    create_block_sparse_attention)
 from .blocks import MLPBlock, RMSNorm, TitanBlock
 from .config import TITANS_VARIANTS, TitanMACConfig
-from .kernels import (BlockELLLinear, BlockELLPattern, TokenLogprobs, block_ell_mm, causal_dwconv, head_logprobs,
-                      rms_norm, token_cross_entropy, token_embedding, token_logprobs, windowed_attention)
+from .kernels import (BlockELLLinear, BlockELLPattern, KVCache, TokenLogprobs, block_ell_mm, cache_keep, cache_read,
+                      cache_write, cached_attention, causal_dwconv, head_logprobs, rms_norm, token_cross_entropy,
+                      token_embedding, token_logprobs, windowed_attention)
 from .memory import DecayGate, DeepMemoryMLP, ForgetGate, NeuralMemory
 from .models import TitanMAC
 
@@ -26,4 +27,4 @@ __all__ = ["TitanMACConfig", "TITANS_VARIANTS", "WindowedAttention", "WindowConf
            "causal_dwconv", "rms_norm", "windowed_attention", "NeuralMemory", "ForgetGate",
            "DecayGate", "DeepMemoryMLP", "TitanMAC", "token_embedding", "token_logprobs",
            "token_cross_entropy", "head_logprobs",
-           "TokenLogprobs"]
+           "TokenLogprobs", "KVCache", "cache_write", "cache_read", "cache_keep", "cached_attention"]
