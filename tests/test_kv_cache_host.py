@@ -60,15 +60,22 @@ def test_refusals():
     refused(TypeError, "unsupported dtype", args=(c, x.double(), table, lengths), names=("write", "read", "attend"))
     refused(ValueError, "(d_head|heads)", args=(c, x[..., :32], table, lengths), names=("write", "attend"))
     refused(ValueError, "heads", args=(c, x[:, :2], table, lengths), names=("write", "attend"))
-    refused(ValueError, "alike", args=(tc.KVCache(c.k, c.v[:, :, :, :32], D), x, table, lengths))
-    refused(ValueError, "pages of", args=(tc.KVCache(c.k, c.v, 50), x, table, lengths))
-    refused(ValueError, "pages of", args=(tc.KVCache(c.k[:, :, :8], c.v[:, :, :8], D), x, table, lengths))
-    refused(ValueError, "contiguous", args=(tc.KVCache(c.k.transpose(0, 1).contiguous().transpose(0, 1), c.v, D), x,
-                                            table, lengths))
+    across = c.k.transpose(0, 1).contiguous().transpose(0, 1)
+    for error, text, bad in ((ValueError, "alike", (c.k, c.v[:, :, :, :32], D)), (ValueError, "alike", (c.k[0], c.v[0], D)),
+                             (ValueError, "pages of", (c.k, c.v, 50)), (ValueError, "contiguous", (across, c.v, D)),
+                             (ValueError, "pages of", (c.k[:, :, :8], c.v[:, :, :8], D)), (ValueError, "pages of", (c.k, c.v, 0)),
+                             (ValueError, "pages of", (c.k[:0], c.v[:0], D)), (TypeError, "dtype", (c.k.double(), c.v.double(), D)),
+                             (RuntimeError, "devices", (c.k, c.v.to("meta"), D))):
+        with pytest.raises(error, match=text):
+            tc.KVCache(*bad)
     for fmt in ("int8", "e4m3"):
         q = parts(fmt=fmt)[0]
         for bad in (None, q.v_scale.half(), q.v_scale[:, :2], q.v_scale.transpose(0, 1).contiguous().transpose(0, 1)):
-            refused(ValueError, "needs k_scale", args=(tc.KVCache(q.k, q.v, D, q.k_scale, bad), x, table, lengths))
+            with pytest.raises(ValueError, match="need k_scale"):
+                tc.KVCache(q.k, q.v, D, q.k_scale, bad)
+        assert tc.KVCache(q.k, q.v, D, q.k_scale, q.v_scale).v_scale is q.v_scale
+    with pytest.raises(AttributeError):
+        c.k = c.v
     with pytest.raises(ValueError, match="k and v must be"):
         tc.cache_write(x, x.half(), c, table, lengths)
     with pytest.raises(ValueError, match="k and v must be"):
@@ -155,12 +162,16 @@ def test_dispatch(monkeypatch):
     kc._workspace.cache_clear()
 
 
+FIELDS = ("d_k", "d_v", "d_k_scale", "d_v_scale", "d_table", "d_lengths", "d_counts", "n_pages", "table_stride", "n_heads",
+          "page", "pitch", "d_head", "max_pages", "format", "dtype")
+
+
 def c_arg(**kw):
     """A cache whose numbers are in order; nothing is read at its addresses."""
     a = {"d_k": FAKE, "d_v": FAKE, "d_k_scale": FAKE, "d_v_scale": FAKE, "d_table": FAKE, "d_lengths": FAKE,
-         "d_counts": None, "n_pages": 10, "table_stride": 4, "n_heads": 3, "page": 16, "pitch": 48, "d_head": 40,
+         "d_counts": 0, "n_pages": 10, "table_stride": 4, "n_heads": 3, "page": 16, "pitch": 48, "d_head": 40,
          "max_pages": 4, "format": 1, "dtype": 1, **kw}
-    return ctypes.byref(kc.CacheArg(*(a[n] for n, _ in kc.CacheArg._fields_)))
+    return kc._CACHE_ARG(*(a[n] or 0 for n in FIELDS))
 
 
 BAD = [({"d_k": None}, -1), ({"d_v": None}, -1), ({"d_table": None}, -1), ({"d_lengths": None}, -1),

@@ -120,7 +120,7 @@ inline int cache_args(const tmac_cache* c, int B, int T, CacheArgs& a) {
     return TMAC_ERR_DTYPE;
   int shift = 4;
   while (shift < 8 && (1 << shift) != c->page) ++shift;
-  if ((1 << shift) != c->page || c->n_heads <= 0 || c->n_heads > (1 << 16) || c->d_head <= 0 || c->d_head > 128 ||
+  if ((1 << shift) != c->page || c->n_heads <= 0 || c->n_heads > 65535 || c->d_head <= 0 || c->d_head > 128 ||
       c->pitch != (c->d_head + 15) / 16 * 16)
     return TMAC_ERR_SHAPE;
   if (c->n_pages <= 0 || c->n_pages >= (INT64_C(1) << 31) || c->n_pages * c->n_heads >= (INT64_C(1) << 40) / c->page)

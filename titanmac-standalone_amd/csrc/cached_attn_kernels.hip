@@ -118,11 +118,16 @@ struct AttnArgs {
   int64_t tree_stride;
   uint8_t* out;
   float* ws;
-  int B, Hq, G, g_log2, n_rb, splits, np, row_cap;
+  int B, Hq, G, g_shift, n_rb, splits, np, row_cap;  // g_shift: log2 of G, or -1
   int window;  // INT_MAX / 2 and above: none
   float scale2;  // scale · log2 e
   bool q_vec, out_vec;
 };
+
+// A division costs a wave a few dozen instructions, in a kernel that may be done in a few hundred.
+__device__ __forceinline__ int by_group(const AttnArgs& a, int r) {
+  return a.g_shift >= 0 ? r >> a.g_shift : static_cast<int>(static_cast<unsigned>(r) / static_cast<unsigned>(a.G));
+}
 
 // What a row sees: j < np, lo <= j <= hi, and drafted rows by bits.
 struct Row {
@@ -187,23 +192,39 @@ __device__ __forceinline__ void row_finish(const Seq& s, int t, float sum, float
   for (int e = 0; e < N; ++e) o[e] = none ? 0.f : o[e] * f;
 }
 
+// values i0 .. i0 + 3 of the result for row t of head h
+template <int DT>
+__device__ __forceinline__ void row_out(const AttnArgs& a, int b, int t, int h, int i0, const float (&o)[4]) {
+  uint8_t* const to = a.out + (((static_cast<int64_t>(b) * a.c.T + t) * a.Hq + h) * a.c.d + i0) * kRowSize<DT>;
+  if (a.out_vec) {  // d a multiple of 4
+    if (i0 >= a.c.d) return;
+    if constexpr (DT == TMAC_F32)
+      *reinterpret_cast<f32x4*>(to) = f32x4{o[0], o[1], o[2], o[3]};
+    else
+      *reinterpret_cast<u32x2*>(to) = u32x2{Mfma<DT>::pack2(o[0], o[1]), Mfma<DT>::pack2(o[2], o[3])};
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float one[1] = {o[e]};
+    if (i0 + e < a.c.d) row_store<DT, 1>(to + e * kRowSize<DT>, one);
+  }
+}
+
 template <int DT, int FMT, int DP, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) {
   using S = Shape<DT, FMT, DP>;
   constexpr int NJ = S::NJ, kRows = 16 * RT, NB = NJ * S::kElem;
   extern __shared__ float sh[];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_waves = blockDim.x >> 6;
-  int id = blockIdx.x;
-  const int rb = id % a.n_rb;
-  id /= a.n_rb;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int hk = id % a.c.n_heads, b = id / a.c.n_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int n_waves = WAVES;
+  const int b = blockIdx.x, hk = blockIdx.y, rb = a.splits == 1 ? blockIdx.z : blockIdx.z / static_cast<unsigned>(a.splits),
+            split = blockIdx.z - rb * a.splits;
   const Seq s = seq_of(a.c, b);
   const int rows_all = a.c.T * a.G, row0 = rb * kRows;
   const int G = a.G;
-  const int t_lo = row0 / G, t_end = (row0 + kRows - 1) / G;
+  const int t_lo = by_group(a, row0), t_end = by_group(a, row0 + kRows - 1);
   const int t_hi = t_end < s.n - 1 ? t_end : s.n - 1;
   const int base = s.len - s.n, len = s.len;
   const bool tree = a.tree != nullptr;
@@ -232,8 +253,12 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
   if (hi >= lo) n_b = (hi >> 5) - b0 + 1;
   if (n_b < 0) n_b = 0;
   const int n_tiles = work ? n_a + n_b : 0;
-  const int tile0 = static_cast<int>(static_cast<int64_t>(n_tiles) * split / a.splits);
-  const int tile1 = static_cast<int>(static_cast<int64_t>(n_tiles) * (split + 1) / a.splits);
+  int tile0 = 0, tile1 = n_tiles;
+  if (a.splits > 1) {
+    const int per = (n_tiles + a.splits - 1u) / static_cast<unsigned>(a.splits);
+    tile0 = per * split < n_tiles ? per * split : n_tiles;
+    tile1 = tile0 + per < n_tiles ? tile0 + per : n_tiles;
+  }
 
   // this lane's rows, one of each 16
   Row row[RT];
@@ -241,9 +266,9 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
   float q32[RT][S::kF32 ? S::kPieces * S::kRun : 1];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = row0 + 16 * rt + n, t = r / G, gg = r - t * G;
-    const bool real = work && t < s.n;
-    row[rt] = real ? row_of(a, s, b, t) : Row{0, 1, 0, 0};
+    const int r = row0 + 16 * rt + n, t = by_group(a, r), gg = r - t * G;
+    const bool real = r < rows_all;  // read whatever the sequence's numbers are, which arrive later
+    row[rt] = work && t < s.n ? row_of(a, s, b, t) : Row{0, 1, 0, 0};
     const uint8_t* const src = a.q + (b * a.qb + (hk * G + gg) * a.qh + t * a.qt) * kRowSize<DT>;
 #pragma unroll
     for (int c = 0; c < S::kPieces; ++c) {
@@ -305,21 +330,29 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
   float v_ref = 0x1p-126f;
   bool cleaned = false;
 
-  for (int it = tile0 + wave; it < tile1; it += n_waves) {
+  // The next tile's pages are looked up while this one is worked on; its keys are asked for when this one's have been
+  // multiplied, its values when this one's have.
+  Piece<16> kp[2][S::kPieces];
+  Piece<NB> vp[8];
+  float ks[8], vs[8];
+  int page_next[2];
+  auto look_up = [&](int it) {
     const int key0 = (it < n_a ? it : b0 + it - n_a) << 5;
-    Piece<16> kp[2][S::kPieces];
-    Piece<NB> vp[8];
-    float ks[8], vs[8];
-    bool bad[2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int key = key0 + 16 * hf;
-      int page = key < len ? table[key >> a.c.page_shift] : 0;
-      bad[hf] = page < 0 || page >= a.c.n_pages;
-      if (bad[hf]) page = 0;
-      const int64_t r = ((static_cast<int64_t>(page) * a.c.n_heads + hk) << a.c.page_shift) + (key & page_mask);
-      const uint8_t* const kb = a.c.k + r * pitch_b;
-      const uint8_t* const vb = a.c.v + r * pitch_b;
+      page_next[hf] = it < tile1 && key < len ? table[key >> a.c.page_shift] : 0;
+    }
+  };
+  auto group_row = [&](int it, int hf, int page) {  // the pool's row of a group of 16 keys
+    const int key = ((it < n_a ? it : b0 + it - n_a) << 5) + 16 * hf;
+    if (page < 0 || page >= a.c.n_pages) page = 0;
+    return ((static_cast<int64_t>(page) * a.c.n_heads + hk) << a.c.page_shift) + (key & page_mask);
+  };
+  auto load_keys = [&](const int64_t (&r)[2]) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint8_t* const kb = a.c.k + r[hf] * pitch_b;
 #pragma unroll
       for (int c = 0; c < S::kPieces; ++c) {
         if (4 * S::kRun * c + S::kRun * g < a.c.pitch)
@@ -327,6 +360,17 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
         else
           kp[hf][c].clear();
       }
+      if constexpr (FMT != kCacheSame) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.ks + r[hf] + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ks[4 * hf + i] = x[i];
+      }
+    }
+  };
+  auto load_values = [&](const int64_t (&r)[2]) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint8_t* const vb = a.c.v + r[hf] * pitch_b;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (v_in)
@@ -335,12 +379,27 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
           vp[4 * hf + i].clear();
       }
       if constexpr (FMT != kCacheSame) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.ks + r + 4 * g);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(a.c.vs + r + 4 * g);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.vs + r[hf] + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ks[4 * hf + i] = x[i], vs[4 * hf + i] = y[i];
+        for (int i = 0; i < 4; ++i) vs[4 * hf + i] = x[i];
       }
     }
+  };
+  int64_t at[2];
+  if (tile0 + wave < tile1) {
+    look_up(tile0 + wave);
+    at[0] = group_row(tile0 + wave, 0, page_next[0]);
+    at[1] = group_row(tile0 + wave, 1, page_next[1]);
+    load_keys(at);
+    load_values(at);
+  }
+  for (int it = tile0 + wave; it < tile1; it += n_waves) {
+    const int key0 = (it < n_a ? it : b0 + it - n_a) << 5;
+    bool bad[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) bad[hf] = page_next[hf] < 0 || page_next[hf] >= a.c.n_pages;
+    const bool more = it + n_waves < tile1;
+    look_up(it + n_waves);
     // every row sees the whole tile (rows that are none see it too: their results are not used)
     const bool full = !bad[0] && !bad[1] && (key0 + 31 < np_all || (key0 >= lo_all && key0 + 31 <= hi_all));
     bool seen[8];  // by any row
@@ -368,30 +427,43 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
 #pragma unroll
       for (int i = 0; i < 8; ++i) vs[i] *= 1.f / v_ref;
     }
-    float p[RT][8];
+    float p[RT][8], ks_now[8];
+    f32x4 sc[RT][2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sc[rt][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < S::kPieces; ++c)
+#pragma unroll
+        for (int e = 0; e < S::kOps; ++e) {
+          const auto key = key_operand<DT, FMT, DP>(kp[hf][c], e);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            if constexpr (S::kF32)
+              sc[rt][hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key, q32[rt][c * S::kRun + e], sc[rt][hf], 0, 0, 0);
+            else
+              sc[rt][hf] = mfma16<DT>(key, q16[rt][c * S::kOps + e], sc[rt][hf]);
+          }
+        }
+    }
+    if constexpr (FMT != kCacheSame) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ks_now[i] = ks[i];
+    }
+    if (more) {
+      at[0] = group_row(it + n_waves, 0, page_next[0]);
+      at[1] = group_row(it + n_waves, 1, page_next[1]);
+      load_keys(at);
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      f32x4 sc[2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        sc[hf] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < S::kPieces; ++c)
-#pragma unroll
-          for (int e = 0; e < S::kOps; ++e) {
-            if constexpr (S::kF32)
-              sc[hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key_operand<DT, FMT, DP>(kp[hf][c], e),
-                                                            q32[rt][c * S::kRun + e], sc[hf], 0, 0, 0);
-            else
-              sc[hf] = mfma16<DT>(key_operand<DT, FMT, DP>(kp[hf][c], e), q16[rt][c * S::kOps + e], sc[hf]);
-          }
-      }
       float x[8], mx = -kInf;
       uint32_t vis = 0xff;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = sc[i >> 2][i & 3] * a.scale2;
-        if constexpr (FMT != kCacheSame) x[i] *= ks[i];
+        x[i] = sc[rt][i >> 2][i & 3] * a.scale2;
+        if constexpr (FMT != kCacheSame) x[i] *= ks_now[i];
       }
       if (!full) {
         vis = 0;
@@ -466,6 +538,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
         for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16<DT>(v, pw[rt], acc[rt][j]);
       }
     }
+    if (more) load_values(at);
   }
 
   if constexpr (kScaled16) {
@@ -499,73 +572,66 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
     }
   }
 
-  // The waves' results side by side in LDS: per wave row_cap rows of kPitchO floats, then (m, l) of each row.
+  // The waves' results are joined in LDS: first the rows' maxima and sums, by which every wave scales what it has, then
+  // the scaled results, summed in the waves' order. Rows of kPitchO floats: 16 rows begin at different banks.
   constexpr int kPitchO = DP + 4;
   const int cap = a.row_cap;
   float* const so = sh + wave * cap * kPitchO;
-  float* const sm = sh + n_waves * cap * kPitchO + wave * cap * 2;
+  float2* const sm = reinterpret_cast<float2*>(sh + WAVES * cap * kPitchO);  // [WAVES][cap]
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = 16 * rt + n;
     float sum = l[rt] + lane_xor<16>(l[rt]);
     sum += lane_xor<32>(sum);
-    if (r < cap) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; j += 4)
-          *reinterpret_cast<f32x4*>(so + r * kPitchO + (4 * g + i) * NJ + j) =
-              f32x4{acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]};
-      if (g == 0) {
-        sm[2 * r] = m[rt];
-        sm[2 * r + 1] = sum;
-      }
-    }
+    if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], sum};
   }
   __syncthreads();
-  const float* const all_m = sh + n_waves * cap * kPitchO;
-  constexpr int N = kRowVec<DT>;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = 16 * rt + n;
+    if (r >= cap) continue;
+    float top = -kInf;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
+    const float f = m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; j += 4)
+        *reinterpret_cast<f32x4*>(so + r * kPitchO + (4 * g + i) * NJ + j) =
+            f32x4{acc[rt][j][i] * f, acc[rt][j + 1][i] * f, acc[rt][j + 2][i] * f, acc[rt][j + 3][i] * f};
+  }
+  __syncthreads();
   const int live = rows_all - row0 < cap ? rows_all - row0 : cap;
-  for (int u = threadIdx.x; u < live * (DP / N); u += blockDim.x) {
-    const int r = u / (DP / N), i0 = u % (DP / N) * N;
-    if (i0 >= a.c.d) continue;
-    float top = -kInf, sum = 0.f, o[N];
-    for (int w = 0; w < n_waves; ++w) top = fmaxf(top, all_m[(w * cap + r) * 2]);
+  for (int u = threadIdx.x; u < live * (DP / 4); u += 64 * WAVES) {
+    const int r = u / (DP / 4), i0 = u % (DP / 4) * 4;
+    float top = -kInf, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = 0.f;
-    for (int w = 0; w < n_waves; ++w) {
-      const float mw = all_m[(w * cap + r) * 2], lw = all_m[(w * cap + r) * 2 + 1];
-      if (mw == -kInf && lw == 0.f) continue;  // nothing seen
-      const float f = mw == top ? 1.f : __builtin_amdgcn_exp2f(mw - top);
-      sum += lw * f;
-      const float* const x = sh + (w * cap + r) * kPitchO + i0;
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] += x[e] * f;
+    for (int w = 0; w < WAVES; ++w) {
+      const float2 x = sm[w * cap + r];
+      sum += x.y * (x.x == top ? 1.f : __builtin_amdgcn_exp2f(x.x - top));
+    }
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(sh + (w * cap + r) * kPitchO + i0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += x[e];
     }
     if (a.splits > 1) {
       const int64_t at = ((static_cast<int64_t>(b) * a.c.n_heads + hk) * a.splits + split) * rows_all + row0 + r;
       float* const po = a.ws + at * (DP + 4);
-#pragma unroll
-      for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(po + i0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+      *reinterpret_cast<f32x4*>(po + i0) = f32x4{o[0], o[1], o[2], o[3]};
       if (i0 == 0) {
         po[DP] = top;
         po[DP + 1] = sum;
       }
       continue;
     }
-    const int t = (row0 + r) / G, gg = row0 + r - t * G;
+    const int t = by_group(a, row0 + r), gg = row0 + r - t * G;
     row_finish(s, t, sum, o);
-    uint8_t* const to =
-        a.out + (((static_cast<int64_t>(b) * a.c.T + t) * a.Hq + hk * G + gg) * a.c.d + i0) * kRowSize<DT>;
-    if (a.out_vec) {
-      row_store<DT, N>(to, o);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float one[1] = {o[e]};
-        if (i0 + e < a.c.d) row_store<DT, 1>(to + e * kRowSize<DT>, one);
-      }
-    }
+    row_out<DT>(a, b, t, hk * G + gg, i0, o);
   }
 }
 
@@ -595,14 +661,9 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
   }
-  const int t = r / a.G, gg = r - t * a.G;
+  const int t = by_group(a, r), gg = r - t * a.G;
   row_finish(seq_of(a.c, b), t, sum, o);
-  uint8_t* const to = a.out + (((static_cast<int64_t>(b) * a.c.T + t) * a.Hq + hk * a.G + gg) * a.c.d + i0) * kRowSize<DT>;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float one[1] = {o[e]};
-    if (i0 + e < a.c.d) row_store<DT, 1>(to + e * kRowSize<DT>, one);
-  }
+  row_out<DT>(a, b, t, hk * a.G + gg, i0, o);
 }
 
 struct Plan {
@@ -622,8 +683,8 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
   int64_t keys = window + c.T + np;
   if (keys > len) keys = len;
   const int64_t tiles = keys / 32 + 2;
-  const int most = p.rt == 1 ? 8 : 4;
-  p.waves = tiles >= most ? most : tiles >= 4 ? 4 : static_cast<int>(tiles);
+  const int most = p.rt > 1 ? 4 : dtype != TMAC_F32 && dp == 64 ? 16 : 8;
+  p.waves = tiles >= 2 * 8 && most == 16 ? 16 : tiles > 4 && most >= 8 ? 8 : 4;
   const int64_t blocks = static_cast<int64_t>(B) * c.n_heads * p.n_rb;
   // enough workgroups for every CU, each wave with 4 tiles at least
   int64_t s = (1024 + blocks - 1) / blocks;
@@ -638,20 +699,28 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
 int check(const tmac_cache* cache, int B, int T, int Hq, int64_t window, int np, CacheArgs& c) {
   const int st = cache_args(cache, B, T, c);
   if (st != TMAC_OK) return st;
-  if (Hq <= 0 || Hq > (1 << 16) || Hq % c.n_heads || static_cast<int64_t>(T) * Hq > (1 << 26)) return TMAC_ERR_SHAPE;
+  if (Hq <= 0 || Hq > 65535 || Hq % c.n_heads || static_cast<int64_t>(T) * Hq > (1 << 26)) return TMAC_ERR_SHAPE;
   if (window < 0 || np < 0) return TMAC_ERR_VALUE;
   return TMAC_OK;
 }
 
+// Most waves of a workgroup with one tile of rows: as many as leave each the registers that it needs.
+template <int DT, int DP>
+constexpr int kMostWaves = DT != TMAC_F32 && DP == 64 ? 16 : 8;
+
 template <int DT, int FMT, int DP>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(a.B) * a.c.n_heads * p.n_rb * p.splits;
+  const dim3 grid(a.B, a.c.n_heads, p.n_rb * p.splits);
   const size_t lds = static_cast<size_t>(p.waves) * p.row_cap * (DP + 4 + 2) * 4;
-  constexpr int kMany = DT == TMAC_F32 ? 2 : 4;
-  if (p.rt == 1)
-    cached_attn_kernel<DT, FMT, DP, 1, 8><<<grid, 64 * p.waves, lds, s>>>(a);
+  constexpr int kMany = DT == TMAC_F32 ? 2 : 4, kMost = kMostWaves<DT, DP>;
+  if (p.rt > 1)
+    cached_attn_kernel<DT, FMT, DP, kMany, 4><<<grid, 64 * 4, lds, s>>>(a);
+  else if (p.waves == 4)
+    cached_attn_kernel<DT, FMT, DP, 1, 4><<<grid, 64 * 4, lds, s>>>(a);
+  else if (p.waves == 8)
+    cached_attn_kernel<DT, FMT, DP, 1, 8><<<grid, 64 * 8, lds, s>>>(a);
   else
-    cached_attn_kernel<DT, FMT, DP, kMany, 4><<<grid, 64 * p.waves, lds, s>>>(a);
+    cached_attn_kernel<DT, FMT, DP, 1, kMost><<<grid, 64 * kMost, lds, s>>>(a);
   if (p.splits > 1) {
     const int64_t threads = static_cast<int64_t>(a.B) * a.c.n_heads * a.c.T * a.G * (DP / 4);
     cached_attn_join_kernel<DT, DP><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(a);
@@ -702,8 +771,7 @@ extern "C" int tmac_cached_attn(const tmac_cache* cache, const void* d_q, const 
   const Plan p = plan(a.c, cache->dtype, B, T * G, window, n_persistent);
   if (p.ws && (!d_ws || ws_bytes < p.ws)) return TMAC_ERR_WORKSPACE;
   if (p.ws && !row_aligned16(d_ws)) return TMAC_ERR_ALIGN;
-  if (static_cast<int64_t>(B) * a.c.n_heads * p.n_rb * p.splits > (1 << 22) ||
-      static_cast<int64_t>(B) * n_q_heads * T > (1 << 26))
+  if (static_cast<int64_t>(p.n_rb) * p.splits > 65535 || static_cast<int64_t>(B) * n_q_heads * T > (1 << 26))
     return TMAC_ERR_SHAPE;
   const int n = cache->dtype == TMAC_F32 ? 4 : 8;
   a.q = static_cast<const uint8_t*>(d_q);
@@ -711,13 +779,13 @@ extern "C" int tmac_cached_attn(const tmac_cache* cache, const void* d_q, const 
   a.tree = d_tree, a.tree_stride = tree_stride;
   a.out = static_cast<uint8_t*>(d_out);
   a.ws = static_cast<float*>(d_ws);
-  a.B = B, a.Hq = n_q_heads, a.G = G, a.n_rb = p.n_rb, a.splits = p.splits, a.row_cap = p.row_cap;
+  a.B = B, a.Hq = n_q_heads, a.G = G, a.g_shift = G & (G - 1) ? -1 : __builtin_ctz(G), a.n_rb = p.n_rb, a.splits = p.splits, a.row_cap = p.row_cap;
   constexpr int kMost = 1 << 30;
   a.np = n_persistent < kMost ? n_persistent : kMost;
   a.window = window < kMost ? static_cast<int>(window) : kMost;
   a.scale2 = scale * kLog2e;
   a.q_vec = row_aligned16(d_q) && a.c.d % n == 0 && a.qb % n == 0 && a.qh % n == 0 && a.qt % n == 0;
-  a.out_vec = row_aligned16(d_out) && a.c.d % n == 0;
+  a.out_vec = row_aligned16(d_out) && a.c.d % 4 == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->dtype == TMAC_F32)
     by_format<TMAC_F32>(cache->format, a, p, s);

@@ -113,11 +113,11 @@ SIGNATURES = {
     "tmac_logprob_mean": [_vp, _vp, _i64, _i, _vp, _i, _vp, _vp],
     "tmac_logprob_mean_bwd": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _i, _i, _i64, _i, _vp],
     "tmac_head_logprob_workspace": [_i, _i64, _i, ctypes.POINTER(_sz)],
-    "tmac_cache_write": [_vp, _vp, _i64p, _vp, _i64p, _i, _i, _vp],
+    "tmac_cache_write": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "tmac_cache_read": [_vp, _vp, _vp, _i, _i, _vp],
     "tmac_cache_keep": [_vp, _vp, _i64, _i, _i, _i, _vp],
     "tmac_cached_attn_workspace": [_vp, _i, _i, _i, _i64, _i, ctypes.POINTER(_sz)],
-    "tmac_cached_attn": [_vp, _vp, _i64p, _vp, _i64, _vp, _vp, _sz, _i, _i, _i, _i64, _i, ctypes.c_float, _vp],
+    "tmac_cached_attn": [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _sz, _i, _i, _i, _i64, _i, ctypes.c_float, _vp],
     "tmac_head_logprob": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i64, _i, _vp, _sz, _i, _vp],
 }
 

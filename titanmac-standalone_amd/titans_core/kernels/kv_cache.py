@@ -20,7 +20,9 @@ page outside the pools.
 from __future__ import annotations
 
 import ctypes
+import struct
 from functools import lru_cache
+from operator import itemgetter
 from typing import Optional, Union
 
 import torch
@@ -34,28 +36,64 @@ PAGES = (16, 32, 64, 128, 256)
 MAX_HEAD, MAX_TREE = 128, 64
 _NO_WINDOW = 1 << 30
 
-
-class CacheArg(ctypes.Structure):
-    """tmac_cache."""
-    _fields_ = [("d_k", ctypes.c_void_p), ("d_v", ctypes.c_void_p), ("d_k_scale", ctypes.c_void_p),
-                ("d_v_scale", ctypes.c_void_p), ("d_table", ctypes.c_void_p), ("d_lengths", ctypes.c_void_p),
-                ("d_counts", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("table_stride", ctypes.c_int64),
-                ("n_heads", ctypes.c_int), ("page", ctypes.c_int), ("pitch", ctypes.c_int), ("d_head", ctypes.c_int),
-                ("max_pages", ctypes.c_int), ("format", ctypes.c_int), ("dtype", ctypes.c_int)]
+# tmac_cache as bytes (a ctypes.Structure takes 2 us more to fill, as much as such a call's launch), and strides
+_CACHE_ARG = struct.Struct("7Q2q7i4x").pack
+_STRIDES = struct.Struct("3q").pack
+_DTYPE = _lib._DTYPE_CODE
+_ptr = _lib.ptr
 
 
-class KVCache:
+class KVCache(tuple):
     """Pools of keys and values: ``k``, ``v`` [n_pages, n_heads, page, pitch], contiguous, rows of d_head values behind
     which are zeros up to the pitch (d_head rounded up to 16); page 16, 32, 64, 128 or 256, d_head up to 128. Their
     type is the model's (float32, bfloat16, float16), or int8 or float8_e4m3fn with a scale for each row in ``k_scale``,
-    ``v_scale`` (float32 [n_pages, n_heads, page]): a value is code · scale. ``KVCache.new`` makes them."""
+    ``v_scale`` (float32 [n_pages, n_heads, page]): a value is code · scale. ``KVCache.new`` makes them.
 
-    __slots__ = ("k", "v", "d_head", "k_scale", "v_scale")
+    Immutable, and checked here once: the tensors' contents change, they themselves are not to be resized or replaced
+    (a change of device makes another KVCache)."""
 
-    def __init__(self, k: torch.Tensor, v: torch.Tensor, d_head: Optional[int] = None,
-                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.d_head = k.shape[-1] if d_head is None else d_head
+    __slots__ = ()
+    k, v, k_scale, v_scale, d_head = (property(itemgetter(i)) for i in range(5))
+
+    def __new__(cls, k: torch.Tensor, v: torch.Tensor, d_head: Optional[int] = None,
+                k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 4 or v.shape != shape or v.dtype != dtype:
+            raise ValueError(f"KVCache: the pools must be [n_pages, n_heads, page, pitch], alike, got {tuple(shape)} {dtype} "
+                             f"and {tuple(v.shape)} {v.dtype}")
+        n, heads, page, pitch = shape
+        d = pitch if d_head is None else int(d_head)
+        if page not in PAGES or not 1 <= d <= MAX_HEAD or pitch != (d + 15) // 16 * 16 or n < 1 or heads < 1:
+            raise ValueError(f"KVCache: pages of {PAGES} rows of d_head (1..{MAX_HEAD}) rounded up to 16 values, got "
+                             f"{tuple(shape)} for d_head {d}")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("KVCache: the pools must be contiguous")
+        device = k.device
+        if v.device != device:
+            raise RuntimeError(f"KVCache: tensors on different devices ({device} and {v.device})")
+        fmt = _FORMATS.get(dtype, SAME)
+        if fmt != SAME:
+            for s in (k_scale, v_scale):
+                if s is None or s.dtype != torch.float32 or s.shape != shape[:3] or not s.is_contiguous():
+                    raise ValueError(f"KVCache: pools of {dtype} need k_scale and v_scale, float32 {tuple(shape[:3])}, "
+                                     "contiguous")
+                if s.device != device:
+                    raise RuntimeError(f"KVCache: tensors on different devices ({device} and {s.device})")
+            changing = (k, v, k_scale, v_scale)
+        else:
+            if dtype not in _DTYPE:
+                raise TypeError(f"KVCache: unsupported dtype {dtype}; expected float32, bfloat16, float16, int8 or "
+                                "float8_e4m3fn")
+            k_scale = v_scale = None
+            changing = (k, v)
+        return tuple.__new__(cls, (k, v, k_scale, v_scale, d, fmt, heads, shape, device, changing))
+
+    def __getnewargs__(self):
+        return self.k, self.v, self.d_head, self.k_scale, self.v_scale
+
+    def __repr__(self):
+        n, heads, page, _ = self.k.shape
+        return (f"KVCache({n} pages of {page}, {heads} heads of {self.d_head}, {self.k.dtype}, {self.k.device})")
 
     @classmethod
     def new(cls, n_pages: int, n_heads: int, d_head: int, *, page: int = 64, dtype: torch.dtype = torch.bfloat16,
@@ -63,7 +101,7 @@ class KVCache:
         """An empty cache (zeros) of values of dtype, held as they are or as fmt "int8" or "e4m3"."""
         if fmt is not None and fmt not in _NAMES:
             raise ValueError(f"KVCache: fmt must be None, 'int8' or 'e4m3', got {fmt!r}")
-        if dtype not in _lib._DTYPE_CODE:
+        if dtype not in _DTYPE:
             raise TypeError(f"KVCache: dtype must be float32, bfloat16 or float16, got {dtype}")
         if page not in PAGES or not 1 <= d_head <= MAX_HEAD or n_pages < 1 or n_heads < 1:
             raise ValueError(f"KVCache: page must be one of {PAGES} and d_head 1..{MAX_HEAD}, got {page}, {d_head} "
@@ -75,38 +113,29 @@ class KVCache:
                    d_head, scale(), scale())
 
 
-def _check_cache(what: str, c: KVCache, table, lengths, counts, dtype: torch.dtype, T: int, B: int) -> None:
-    k, v, ks, vs = c.k, c.v, c.k_scale, c.v_scale
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"{what}: the pools must be [n_pages, n_heads, page, pitch], alike, got {tuple(k.shape)} {k.dtype} "
-                         f"and {tuple(v.shape)} {v.dtype}")
-    if k.shape[2] not in PAGES or not 1 <= c.d_head <= MAX_HEAD or k.shape[3] != -(-c.d_head // 16) * 16:
-        raise ValueError(f"{what}: pages of {PAGES} rows of d_head (1..{MAX_HEAD}) rounded up to 16 values, got "
-                         f"{tuple(k.shape)} for d_head {c.d_head}")
-    if not (k.is_contiguous() and v.is_contiguous()):
-        raise ValueError(f"{what}: the pools must be contiguous")
-    if dtype not in _lib._DTYPE_CODE:
+def _check(what: str, cache: KVCache, table, lengths, counts, dtype: torch.dtype, T: int, B: int) -> None:
+    """The sequences' description, and whether the cache holds values of dtype."""
+    k, _, _, _, _, fmt, heads, shape, _, _ = cache
+    if dtype not in _DTYPE:
         raise TypeError(f"{what}: unsupported dtype {dtype}; expected float32, bfloat16 or float16")
-    if k.dtype in _FORMATS:
-        for s in (ks, vs):
-            if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or not s.is_contiguous():
-                raise ValueError(f"{what}: a cache in {k.dtype} needs k_scale and v_scale, float32 {tuple(k.shape[:3])}, "
-                                 "contiguous")
-    elif k.dtype != dtype:
+    if fmt == SAME and k.dtype != dtype:
         raise TypeError(f"{what}: a cache of {k.dtype} does not hold {dtype}")
-    if table.dtype != torch.int32 or lengths.dtype != torch.int32 or (counts is not None and counts.dtype != torch.int32):
+    i32 = torch.int32
+    if table.dtype != i32 or lengths.dtype != i32 or (counts is not None and counts.dtype != i32):
         raise TypeError(f"{what}: table, lengths and counts must be int32")
-    if table.dim() != 2 or table.shape[0] != B or table.shape[1] == 0:
+    at = table.shape
+    if len(at) != 2 or at[0] != B or at[1] == 0:
         raise ValueError(f"{what}: table must be [{B}, pages], got {tuple(table.shape)}")
-    for name, t in (("lengths", lengths), ("counts", counts)):
-        if t is not None and t.shape != (B,):
-            raise ValueError(f"{what}: {name} must be [{B}], got {tuple(t.shape)}")
-    if B > 1 << 20 or T * k.shape[1] > 1 << 26 or table.shape[1] > (1 << 30) // k.shape[2]:
+    if lengths.dim() != 1 or lengths.shape[0] != B:
+        raise ValueError(f"{what}: lengths must be [{B}], got {tuple(lengths.shape)}")
+    if counts is not None and (counts.dim() != 1 or counts.shape[0] != B):
+        raise ValueError(f"{what}: counts must be [{B}], got {tuple(counts.shape)}")
+    if B > 1 << 20 or T * heads > 1 << 26 or at[1] > (1 << 30) // shape[2]:
         raise ValueError(f"{what}: up to 2^20 sequences, 2^26 rows of one and 2^30 positions")
 
 
-def _no_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_grad(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
@@ -115,53 +144,73 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+def _rows(t: torch.Tensor):
+    """(a table [B, n] that the kernels can read, its pitch; any where there is one row)."""
+    n = t.shape[1]
+    pitch, step = t.stride()
+    if (step != 1 and n != 1) or (pitch < n and t.shape[0] > 1):
+        return t.contiguous(), n
+    return t, pitch if t.shape[0] > 1 else n
+
+
+def _run(what: str, device: torch.device, tensors, name: str, *args) -> None:
+    """The library's function on the current stream of the device of all of the tensors."""
+    if device.type != "cuda":
+        _lib.require_device(*(t for t in tensors if t is not None), what=what)
+        index, now = None, None  # on the CPU the library's calls are replaced
+    else:
+        for t in tensors:
+            if t is not None and t.device != device:
+                raise RuntimeError(f"{what}: tensors on different devices ({device} and {t.device})")
+        index, now = device.index, torch._C._cuda_getDevice()
+    fn = getattr(_lib.lib(), name)
+    if index == now:
+        rc = fn(*args, _lib.stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_ptr(device))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _arg(cache: KVCache, table, pitch: int, lengths, counts, dtype: torch.dtype) -> bytes:
+    """tmac_cache."""
+    k, v, ks, vs, d, fmt, heads, shape, _, _ = cache
+    return _CACHE_ARG(k.data_ptr(), v.data_ptr(), 0 if ks is None else ks.data_ptr(), 0 if vs is None else vs.data_ptr(),
+                      table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(), shape[0], pitch,
+                      heads, shape[2], shape[3], d, table.shape[1], fmt, _DTYPE[dtype])
+
+
+def _flat(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Pitch of a table's rows (any, if there is one row)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _arg(k, v, ks, vs, table, lengths, counts, d, dtype) -> CacheArg:
-    n, h, page, pitch = k.shape
-    p = _lib.ptr
-    return CacheArg(k.data_ptr(), v.data_ptr(), p(ks), p(vs), table.data_ptr(), lengths.data_ptr(), p(counts), n,
-                    _pitch(table), h, page, pitch, d, table.shape[1], _FORMATS.get(k.dtype, SAME),
-                    _lib._DTYPE_CODE[dtype])
-
-
-def _strides(t: torch.Tensor):
-    """(batch, head, row) strides of [B, H, T, d]."""
-    return (ctypes.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
-
-
-def _table(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+def _changed(cache: KVCache) -> None:
+    """What autograd (or a caller's own cache) keeps of the pools is out of date."""
+    tensors = cache[9]
+    if tensors[0].is_inference():
+        tensors = [t for t in tensors if not t.is_inference()]
+    torch.autograd.graph.increment_version(tensors)
 
 
 # ------------------------------------------------------------------ write
 
-def _native_write(new_k, new_v, k, v, ks, vs, table, lengths, counts, d) -> None:
-    dev = _lib.require_device(*(t for t in (k, v, new_k, new_v, ks, vs, table, lengths, counts) if t is not None),
-                              what="cache_write")
-    B, _, T, _ = new_k.shape
-    if new_k.numel() == 0:
+def _native_write(k, v, cache, table, lengths, counts) -> None:
+    B, H, T, d = k.shape
+    if B * T == 0:
         return
-    new_k, new_v, table, lengths, counts = _unit(new_k), _unit(new_v), _table(table), _flat(lengths), _flat(counts)
-    arg = _arg(k, v, ks, vs, table, lengths, counts, d, new_k.dtype)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_cache_write(ctypes.byref(arg), new_k.data_ptr(), _strides(new_k), new_v.data_ptr(),
-                                         _strides(new_v), B, T, _lib.stream_ptr(dev))
-    _lib.check(rc, "tmac_cache_write")
+    k, v, lengths, counts = _unit(k), _unit(v), _flat(lengths), _flat(counts)
+    table, pitch = _rows(table)
+    _run("cache_write", cache[8], (k, v, table, lengths, counts), "tmac_cache_write",
+         _arg(cache, table, pitch, lengths, counts, k.dtype), k.data_ptr(), _STRIDES(*k.stride()[:3]), v.data_ptr(),
+         _STRIDES(*v.stride()[:3]), B, T)
 
 
 @torch.library.custom_op("titanmac::cache_write", mutates_args=("k", "v", "ks", "vs"))
 def cache_write_op(new_k: torch.Tensor, new_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                    ks: Optional[torch.Tensor], vs: Optional[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor,
                    counts: Optional[torch.Tensor], d: int) -> None:
-    _native_write(new_k, new_v, k, v, ks, vs, table, lengths, counts, d)
+    _native_write(new_k, new_v, KVCache(k, v, d, ks, vs), table, lengths, counts)
 
 
 @cache_write_op.register_fake
@@ -176,52 +225,40 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.T
     In 8 bits every row has its own scale: int8 codes are value / scale rounded to nearest (ties to even) with scale =
     max |value| / 127, e4m3 codes likewise with the least power of two that holds the row as scale (both at least
     2^-126). A row that is not finite is held as NaN. Pages that are written must not belong to two sequences."""
-    what = "cache_write"
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"{what}: k and v must be [B, n_heads, T, d_head], alike, got {tuple(k.shape)} {k.dtype} and "
-                         f"{tuple(v.shape)} {v.dtype}")
+        raise ValueError(f"cache_write: k and v must be [B, n_heads, T, d_head], alike, got {tuple(k.shape)} {k.dtype} "
+                         f"and {tuple(v.shape)} {v.dtype}")
     B, H, T, d = k.shape
-    _check_cache(what, cache, table, lengths, counts, k.dtype, T, B)
-    if H != cache.k.shape[1] or d != cache.d_head:
-        raise ValueError(f"{what}: the cache has {cache.k.shape[1]} heads of {cache.d_head}, k is {tuple(k.shape)}")
-    _no_grad(what, k, v, cache.k, cache.v)
-    args = (k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths, counts, cache.d_head)
-    if _lib.direct_call(*args[:-1]):
-        _native_write(*args)
+    _check("cache_write", cache, table, lengths, counts, k.dtype, T, B)
+    if H != cache[6] or d != cache[4]:
+        raise ValueError(f"cache_write: the cache has {cache[6]} heads of {cache[4]}, k is {tuple(k.shape)}")
+    if _lib.direct_call(k, v, table, lengths, counts, *cache[9]):
+        _native_write(k, v, cache, table, lengths, counts)
         _changed(cache)
     else:
-        cache_write_op(*args)
-
-
-def _changed(cache: KVCache) -> None:
-    """What autograd (or a caller's cache) keeps of the pools is out of date."""
-    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
-        if t is not None and not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+        _refuse_grad("cache_write", k, v, cache[0], cache[1])
+        cache_write_op(k, v, *cache[:4], table, lengths, counts, cache[4])
 
 
 # ------------------------------------------------------------------ read
 
-def _native_read(k, v, ks, vs, table, lengths, T, d, dtype):
-    dev = _lib.require_device(*(t for t in (k, v, ks, vs, table, lengths) if t is not None), what="cache_read")
-    B, H = table.shape[0], k.shape[1]
-    out_k = torch.empty((B, H, T, d), dtype=dtype, device=dev)
-    out_v = torch.empty((B, H, T, d), dtype=dtype, device=dev)
-    if out_k.numel() == 0:
-        return out_k, out_v
-    table, lengths = _table(table), _flat(lengths)
-    arg = _arg(k, v, ks, vs, table, lengths, None, d, dtype)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_cache_read(ctypes.byref(arg), out_k.data_ptr(), out_v.data_ptr(), B, T, _lib.stream_ptr(dev))
-    _lib.check(rc, "tmac_cache_read")
-    return out_k, out_v
+def _native_read(cache, table, lengths, T, dtype):
+    B, H, d, device = table.shape[0], cache[6], cache[4], cache[8]
+    k = torch.empty((B, H, T, d), dtype=dtype, device=device)
+    v = torch.empty((B, H, T, d), dtype=dtype, device=device)
+    if B * T:
+        lengths = _flat(lengths)
+        table, pitch = _rows(table)
+        _run("cache_read", device, (table, lengths), "tmac_cache_read", _arg(cache, table, pitch, lengths, None, dtype),
+             k.data_ptr(), v.data_ptr(), B, T)
+    return k, v
 
 
 @torch.library.custom_op("titanmac::cache_read", mutates_args=())
 def cache_read_op(k: torch.Tensor, v: torch.Tensor, ks: Optional[torch.Tensor], vs: Optional[torch.Tensor],
                   table: torch.Tensor, lengths: torch.Tensor, T: int, d: int,
                   dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    return _native_read(k, v, ks, vs, table, lengths, T, d, dtype)
+    return _native_read(KVCache(k, v, d, ks, vs), table, lengths, T, dtype)
 
 
 @cache_read_op.register_fake
@@ -233,39 +270,38 @@ def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, n_pos
                dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Positions 0 .. n_positions − 1 of every sequence as k, v [B, n_heads, n_positions, d_head]: zeros behind a
     sequence's length. dtype: the values' type (default: the cache's, bfloat16 for one in 8 bits)."""
-    what = "cache_read"
     if dtype is None:
-        dtype = torch.bfloat16 if cache.k.dtype in _FORMATS else cache.k.dtype
+        dtype = torch.bfloat16 if cache[5] else cache[0].dtype
     T = int(n_positions)
     if T < 0:
-        raise ValueError(f"{what}: n_positions must not be negative, got {T}")
-    _check_cache(what, cache, table, lengths, None, dtype, T, lengths.shape[0] if lengths.dim() == 1 else -1)
-    _no_grad(what, cache.k, cache.v)
-    args = (cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths)
-    run = _native_read if _lib.direct_call(*args) else cache_read_op
-    return run(*args, T, cache.d_head, dtype)
+        raise ValueError(f"cache_read: n_positions must not be negative, got {T}")
+    _check("cache_read", cache, table, lengths, None, dtype, T, lengths.shape[0] if lengths.dim() == 1 else -1)
+    if _lib.direct_call(table, lengths, *cache[9]):
+        return _native_read(cache, table, lengths, T, dtype)
+    _refuse_grad("cache_read", cache[0], cache[1])
+    return cache_read_op(*cache[:4], table, lengths, T, cache[4], dtype)
 
 
 # ------------------------------------------------------------------ keep
 
-def _native_keep(k, v, ks, vs, table, lengths, counts, path, T, d) -> None:
-    dev = _lib.require_device(*(t for t in (k, v, ks, vs, table, lengths, counts, path) if t is not None),
-                              what="cache_keep")
+def _native_keep(cache, table, lengths, counts, path, T) -> None:
     B, A = path.shape
     if B == 0 or A == 0:
         return
-    table, lengths, counts, path = _table(table), _flat(lengths), _flat(counts), _table(path)
-    arg = _arg(k, v, ks, vs, table, lengths, counts, d, torch.bfloat16 if k.dtype in _FORMATS else k.dtype)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_cache_keep(ctypes.byref(arg), path.data_ptr(), _pitch(path), A, B, T, _lib.stream_ptr(dev))
-    _lib.check(rc, "tmac_cache_keep")
+    lengths, counts = _flat(lengths), _flat(counts)
+    table, pitch = _rows(table)
+    path, path_pitch = _rows(path)
+    # 8-bit rows are moved as they are, whatever the type of the values
+    _run("cache_keep", cache[8], (table, lengths, counts, path), "tmac_cache_keep",
+         _arg(cache, table, pitch, lengths, counts, torch.bfloat16 if cache[5] else cache[0].dtype), path.data_ptr(),
+         path_pitch, A, B, T)
 
 
 @torch.library.custom_op("titanmac::cache_keep", mutates_args=("k", "v", "ks", "vs"))
 def cache_keep_op(k: torch.Tensor, v: torch.Tensor, ks: Optional[torch.Tensor], vs: Optional[torch.Tensor],
                   table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor], path: torch.Tensor, T: int,
                   d: int) -> None:
-    _native_keep(k, v, ks, vs, table, lengths, counts, path, T, d)
+    _native_keep(KVCache(k, v, d, ks, vs), table, lengths, counts, path, T)
 
 
 @cache_keep_op.register_fake
@@ -278,62 +314,58 @@ def cache_keep(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, path:
     """Of each sequence's draft, its last ``counts`` rows (up to 64; one number for all, or int32 [B]): row path[b, a]
     (int32 [B, A]) moves to place a of the draft, for all a at once. An entry outside the draft (−1) leaves its place as
     it is. The caller then shortens ``lengths`` to the rows that were kept."""
-    what = "cache_keep"
-    T = MAX_TREE if isinstance(counts, torch.Tensor) else int(counts)
     n = counts if isinstance(counts, torch.Tensor) else None
+    T = MAX_TREE if n is not None else int(counts)
     if path.dim() != 2 or path.dtype != torch.int32:
-        raise ValueError(f"{what}: path must be int32 [B, rows], got {path.dtype} {tuple(path.shape)}")
+        raise ValueError(f"cache_keep: path must be int32 [B, rows], got {path.dtype} {tuple(path.shape)}")
     if not 0 <= T <= MAX_TREE or path.shape[1] > T:
-        raise ValueError(f"{what}: drafts of up to {MAX_TREE} rows, no more kept than drafted, got {T} and "
+        raise ValueError(f"cache_keep: drafts of up to {MAX_TREE} rows, no more kept than drafted, got {T} and "
                          f"{path.shape[1]}")
-    dtype = torch.bfloat16 if cache.k.dtype in _FORMATS else cache.k.dtype
-    _check_cache(what, cache, table, lengths, n, dtype, T, path.shape[0])
-    _no_grad(what, cache.k, cache.v)
-    args = (cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths, n, path)
-    if _lib.direct_call(*args):
-        _native_keep(*args, T, cache.d_head)
+    if path.shape[0] > 32767:
+        raise ValueError(f"cache_keep: up to 32767 sequences, got {path.shape[0]}")
+    _check("cache_keep", cache, table, lengths, n, torch.bfloat16 if cache[5] else cache[0].dtype, T, path.shape[0])
+    if _lib.direct_call(table, lengths, n, path, *cache[9]):
+        _native_keep(cache, table, lengths, n, path, T)
         _changed(cache)
     else:
-        cache_keep_op(*args, T, cache.d_head)
+        _refuse_grad("cache_keep", cache[0], cache[1])
+        cache_keep_op(*cache[:4], table, lengths, n, path, T, cache[4])
 
 
 # ------------------------------------------------------------------ attention
 
 @lru_cache(maxsize=512)
-def _workspace(shape, max_pages, d, fmt, dtype, B, T, Hq, window, n_persistent) -> int:
-    n, h, page, pitch = shape
-    fake = 256  # sizes only: nothing is read there
-    arg = CacheArg(fake, fake, fake, fake, fake, fake, None, n, max_pages, h, page, pitch, d, max_pages, fmt, dtype)
+def _workspace(heads, page, d, max_pages, fmt, dtype, B, T, Hq, window, n_persistent) -> int:
+    at = 256  # sizes only: nothing is read there
+    arg = _CACHE_ARG(at, at, at, at, at, at, 0, 1, max_pages, heads, page, (d + 15) // 16 * 16, d, max_pages, fmt, dtype)
     nb = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().tmac_cached_attn_workspace(ctypes.byref(arg), B, T, Hq, window, n_persistent, ctypes.byref(nb)),
+    _lib.check(_lib.lib().tmac_cached_attn_workspace(arg, B, T, Hq, window, n_persistent, ctypes.byref(nb)),
                "tmac_cached_attn_workspace")
     return nb.value
 
 
-def _native_attn(q, k, v, ks, vs, table, lengths, counts, tree, window, n_persistent, scale, d):
-    """[B, T, Hq, d]."""
-    dev = _lib.require_device(*(t for t in (q, k, v, ks, vs, table, lengths, counts, tree) if t is not None),
-                              what="cached_attention")
+def _native_attn(q, cache, table, lengths, counts, tree, window, n_persistent, scale):
+    """[B, H, T, d], a view of [B, T, H, d]."""
+    _, _, _, _, d, fmt, heads, shape, device, _ = cache
     B, H, T, _ = q.shape
-    out = torch.empty((B, T, H, d), dtype=q.dtype, device=dev)
-    if out.numel() == 0:
+    dtype = q.dtype
+    out = torch.empty_strided((B, H, T, d), (T * H * d, d, H * d, 1), dtype=dtype, device=device)
+    if B * T == 0:
         return out
-    q, table, lengths, counts = _unit(q), _table(table), _flat(lengths), _flat(counts)
-    arg = _arg(k, v, ks, vs, table, lengths, counts, d, q.dtype)
-    if tree is None:
-        tree_stride = 0
-    else:
-        tree = _unit(tree)
-        tree_stride = 0 if tree.dim() == 1 else _pitch(tree)
-        if tree.dim() == 2 and tree_stride < T and tree_stride != 0:
-            tree, tree_stride = tree.contiguous(), T
-    nb = _workspace(tuple(k.shape), table.shape[1], d, arg.format, arg.dtype, B, T, H, window, n_persistent)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    with _lib.device_guard(dev):
-        rc = _lib.lib().tmac_cached_attn(ctypes.byref(arg), q.data_ptr(), _strides(q), _lib.ptr(tree), tree_stride,
-                                         out.data_ptr(), _lib.ptr(ws), nb, B, T, H, window, n_persistent, scale,
-                                         _lib.stream_ptr(dev))
-    _lib.check(rc, "tmac_cached_attn")
+    q, lengths, counts = _unit(q), _flat(lengths), _flat(counts)
+    table, pitch = _rows(table)
+    tree_stride = 0
+    if tree is not None:
+        if tree.dim() == 1:
+            tree = _unit(tree)
+        else:
+            tree, tree_stride = _rows(tree)
+    nb = _workspace(heads, shape[2], d, table.shape[1], fmt, _DTYPE[dtype], B, T, H, window, n_persistent)
+    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    _run("cached_attention", device, (q, table, lengths, counts, tree), "tmac_cached_attn",
+         _arg(cache, table, pitch, lengths, counts, dtype), q.data_ptr(), _STRIDES(*q.stride()[:3]),
+         0 if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), _ptr(ws), nb, B, T, H, window, n_persistent,
+         scale)
     return out
 
 
@@ -342,13 +374,13 @@ def cached_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ks: O
                         vs: Optional[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor,
                         counts: Optional[torch.Tensor], tree: Optional[torch.Tensor], window: int, n_persistent: int,
                         scale: float, d: int) -> torch.Tensor:
-    return _native_attn(q, k, v, ks, vs, table, lengths, counts, tree, window, n_persistent, scale, d)
+    return _native_attn(q, KVCache(k, v, d, ks, vs), table, lengths, counts, tree, window, n_persistent, scale)
 
 
 @cached_attention_op.register_fake
 def _(q, k, v, ks, vs, table, lengths, counts, tree, window, n_persistent, scale, d):
     B, H, T, _ = q.shape
-    return q.new_empty((B, T, H, d))
+    return q.new_empty((B, T, H, d)).transpose(1, 2)
 
 
 def cached_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths: torch.Tensor,
@@ -369,27 +401,27 @@ def cached_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengt
     What a row does not see never reaches its result, whatever is stored there. Scores, sums and the accumulation are in
     fp32; in 16 bit the probabilities are rounded to q's type before they meet the values. scale defaults to
     1/sqrt(d_head). No gradient."""
-    what = "cached_attention"
     if q.dim() != 4:
-        raise ValueError(f"{what}: q must be [B, H, T, d_head], got {tuple(q.shape)}")
+        raise ValueError(f"cached_attention: q must be [B, H, T, d_head], got {tuple(q.shape)}")
     B, H, T, d = q.shape
-    _check_cache(what, cache, table, lengths, counts, q.dtype, T, B)
-    heads = cache.k.shape[1]
-    if d != cache.d_head or H == 0 or H % heads:
-        raise ValueError(f"{what}: the cache has {heads} heads of {cache.d_head}, q is {tuple(q.shape)}")
+    _check("cached_attention", cache, table, lengths, counts, q.dtype, T, B)
+    if d != cache[4] or H == 0 or H % cache[6]:
+        raise ValueError(f"cached_attention: the cache has {cache[6]} heads of {cache[4]}, q is {tuple(q.shape)}")
     if B * H * T > 1 << 26:
-        raise ValueError(f"{what}: up to 2^26 query rows, got {B * H * T}")
+        raise ValueError(f"cached_attention: up to 2^26 query rows, got {B * H * T}")
     window = _NO_WINDOW if window_size is None else min(int(window_size), _NO_WINDOW)
-    n_persistent = int(n_persistent)
+    n_persistent = min(int(n_persistent), _NO_WINDOW)
     if window < 0 or n_persistent < 0:
-        raise ValueError(f"{what}: window_size and n_persistent must not be negative, got {window_size}, {n_persistent}")
+        raise ValueError(f"cached_attention: window_size and n_persistent must not be negative, got {window_size}, "
+                         f"{n_persistent}")
     if tree is not None:
         if tree.dtype != torch.int64 or tuple(tree.shape) not in ((B, T), (T,)):
-            raise ValueError(f"{what}: tree must be int64 [{B}, {T}] or [{T}], got {tree.dtype} {tuple(tree.shape)}")
+            raise ValueError(f"cached_attention: tree must be int64 [{B}, {T}] or [{T}], got {tree.dtype} "
+                             f"{tuple(tree.shape)}")
         if T > MAX_TREE:
-            raise ValueError(f"{what}: a draft has up to {MAX_TREE} rows, got {T}")
-    _no_grad(what, q, cache.k, cache.v)
-    tensors = (q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths, counts, tree)
-    run = _native_attn if _lib.direct_call(*tensors) else cached_attention_op
-    out = run(*tensors, window, min(n_persistent, _NO_WINDOW), float(d ** -0.5 if scale is None else scale), d)
-    return out.transpose(1, 2)
+            raise ValueError(f"cached_attention: a draft has up to {MAX_TREE} rows, got {T}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if _lib.direct_call(q, table, lengths, counts, tree, *cache[9]):
+        return _native_attn(q, cache, table, lengths, counts, tree, window, n_persistent, scale)
+    _refuse_grad("cached_attention", q, cache[0], cache[1])
+    return cached_attention_op(q, *cache[:4], table, lengths, counts, tree, window, n_persistent, scale, d)
