@@ -118,9 +118,9 @@ struct AttnArgs {
   int64_t tree_stride;
   uint8_t* out;
   float* ws;
-  int B, Hq, G, g_shift, n_rb, splits, np, row_cap;  // g_shift: log2 of G, or -1
+  int B, Hq, G, g_shift, n_rb, splits, np, row_cap, per_xcd, n_blocks;  // g_shift: log2 of G, or -1
   int window;  // INT_MAX / 2 and above: none
-  float scale2;  // scale · log2 e
+  float scale2, q_sign;  // |scale| · log2 e (1 for scale 0); the queries are taken times q_sign, the scale's sign
   bool q_vec, out_vec;
 };
 
@@ -129,49 +129,95 @@ __device__ __forceinline__ int by_group(const AttnArgs& a, int r) {
   return a.g_shift >= 0 ? r >> a.g_shift : static_cast<int>(static_cast<unsigned>(r) / static_cast<unsigned>(a.G));
 }
 
-// What a row sees: j < np, lo <= j <= hi, and drafted rows by bits.
+// What a row sees: j < np, lo <= j <= lo + span, and drafted rows by bits. (kNowhere: past every position.)
+constexpr int kNowhere = 1 << 30;
 struct Row {
-  int np, lo, hi;
+  int np, lo;
+  uint32_t span;
   uint64_t bits;
 };
+__device__ __forceinline__ Row no_row() { return Row{0, kNowhere, 0, 0}; }
 
-__device__ __forceinline__ bool sees(const Row& r, int j, int base, bool tree) {
-  bool v = (j < r.np) | ((j >= r.lo) & (j <= r.hi));
-  if (tree) {
-    const uint32_t s = static_cast<uint32_t>(j - base);
-    v |= s < 64u && ((r.bits >> (s & 63u)) & 1);
-  }
-  return v;
+__device__ __forceinline__ bool in_span(int j, int lo, uint32_t span) { return static_cast<uint32_t>(j - lo) <= span; }
+__device__ __forceinline__ bool sees(const Row& r, int j, int base) {
+  const uint32_t s = static_cast<uint32_t>(j - base);
+  return (j < r.np) | in_span(j, r.lo, r.span) | (s < 64u && (r.bits >> (s & 63u) & 1));
 }
 
 __device__ __forceinline__ int bits_set(int64_t x) { return static_cast<int>(__popcll(static_cast<uint64_t>(x))); }
 
 // Row t of sequence s. Without a tree position p = base + t.
 __device__ __forceinline__ Row row_of(const AttnArgs& a, const Seq& s, int b, int t) {
-  Row r{0, 1, 0, 0};
+  Row r = no_row();
   if (t >= s.n) return r;
   const int base = s.len - s.n, np = a.np < s.len ? a.np : s.len;
   if (!a.tree) {
-    const int p = base + t;
+    const int p = base + t, lo = p - a.window > 0 ? p - a.window : 0;
     r.np = np;
     if (p >= a.np) {
-      r.lo = p - a.window > 0 ? p - a.window : 0;
-      r.hi = p;
+      r.lo = lo;
+      r.span = p - lo;
     }
     return r;
   }
   const int64_t* const tree = a.tree + b * a.tree_stride;
   const uint64_t have = s.n >= 64 ? ~0ull : (1ull << s.n) - 1;
-  const int p = base + bits_set(tree[t]) - 1;
+  const int p = base + bits_set(tree[t]) - 1, lo = p - a.window > 0 ? p - a.window : 0;
   r.np = np < base ? np : base;
-  r.lo = p - a.window > 0 ? p - a.window : 0;
-  r.hi = base - 1;
+  if (lo < base) {
+    r.lo = lo;
+    r.span = base - 1 - lo;
+  }
   r.bits = static_cast<uint64_t>(tree[t]) & have;
   if (a.window < 2 * TMAC_CACHE_MAX_TREE) {  // drafted rows may be behind the window: their places differ by up to 64
     for (int u = 0; u < s.n; ++u)
       if (base + bits_set(tree[u]) - 1 < p - a.window && base + u >= a.np) r.bits &= ~(1ull << u);
   }
   return r;
+}
+
+// The 32 bits of x from bit s on (s may be negative: zeros below bit 0).
+__device__ __forceinline__ uint32_t bits_from(uint64_t x, int s) {
+  if (s >= 64 || s <= -32) return 0;
+  return static_cast<uint32_t>(s >= 0 ? x >> s : x << -s);
+}
+
+// The keys of a block of rows t_lo .. t_hi, as tiles of 32: those with persistent keys, then those of [lo, hi] behind
+// them. Every key that a row sees is below np or in [lo, hi]; every row sees the keys below np_all and in
+// [lo_all, hi_all].
+struct Keys {
+  int np, np_all, lo, hi, lo_all, hi_all, n_a, b0, n_tiles;
+  __device__ __forceinline__ int first(int it) const { return (it < n_a ? it : b0 + it - n_a) << 5; }
+  __device__ __forceinline__ bool all_see(int key0) const {
+    return key0 + 31 < np_all || (key0 >= lo_all && key0 + 31 <= hi_all);
+  }
+};
+
+__device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Seq& s, int t_lo, int t_hi) {
+  Keys k;
+  const int base = s.len - s.n;
+  k.np = a.np < s.len ? a.np : s.len;
+  k.np_all = k.np;
+  if (a.tree) {  // places from base - 1 (a row that sees no drafted row) to base + 63
+    k.lo = base - 1 - a.window;
+    k.lo_all = base + 63 - a.window;
+    k.hi = s.len - 1;
+    k.hi_all = base - 1;
+    if (base < k.np_all) k.np_all = base;
+  } else {
+    k.lo = base + t_lo - a.window;
+    k.lo_all = base + t_hi - a.window;
+    k.hi = base + t_hi;
+    k.hi_all = base + t_lo;
+    if (k.hi < a.np) k.hi = -1;          // persistent rows only
+    if (k.hi_all < a.np) k.hi_all = -1;  // some persistent rows
+  }
+  if (k.lo < k.np) k.lo = k.np;
+  k.n_a = (k.np + 31) >> 5;
+  k.b0 = k.lo >> 5 > k.n_a ? k.lo >> 5 : k.n_a;
+  const int n_b = k.hi >= k.lo ? (k.hi >> 5) - k.b0 + 1 : 0;
+  k.n_tiles = s.ok && t_lo < s.n ? k.n_a + (n_b > 0 ? n_b : 0) : 0;
+  return k;
 }
 
 // w with what is not finite in it (two 16-bit values, or one fp32) replaced by zeros
@@ -211,88 +257,84 @@ __device__ __forceinline__ void row_out(const AttnArgs& a, int b, int t, int h, 
   }
 }
 
-template <int DT, int FMT, int DP, int RT, int WAVES>
+// ROWS: the workgroup's waves hold a block of rows each and walk the same keys, for many rows (their loads meet in the
+// first-level cache); otherwise they hold the same rows and share the keys out.
+template <int DT, int FMT, int DP, int RT, int WAVES, bool ROWS>
 __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) {
   using S = Shape<DT, FMT, DP>;
   constexpr int NJ = S::NJ, kRows = 16 * RT, NB = NJ * S::kElem;
+  constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
   extern __shared__ float sh[];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr int n_waves = WAVES;
-  const int b = blockIdx.x, hk = blockIdx.y, rb = a.splits == 1 ? blockIdx.z : blockIdx.z / static_cast<unsigned>(a.splits),
-            split = blockIdx.z - rb * a.splits;
-  const Seq s = seq_of(a.c, b);
-  const int rows_all = a.c.T * a.G, row0 = rb * kRows;
-  const int G = a.G;
-  const int t_lo = by_group(a, row0), t_end = by_group(a, row0 + kRows - 1);
-  const int t_hi = t_end < s.n - 1 ? t_end : s.n - 1;
-  const int base = s.len - s.n, len = s.len;
-  const bool tree = a.tree != nullptr;
-  const bool work = s.ok && t_lo < s.n;
-
-  // the keys that any row sees: [0, np) and [lo, hi]; lo_all, hi_all: seen by all rows
-  const int np = a.np < len ? a.np : len;
-  int np_all = np, lo, hi, lo_all, hi_all;
-  if (tree) {  // places from base - 1 (a row that sees no drafted row) to base + 63
-    lo = base - 1 - a.window;
-    lo_all = base + 63 - a.window;
-    hi = len - 1;
-    hi_all = base - 1;
-    np_all = np < base ? np : base;
+  int b, hk, rb, split;
+  if constexpr (ROWS) {  // the blocks of a sequence's head, which read the same keys, on one XCD
+    int id = xcd_logical_id(a.per_xcd);
+    if (id >= a.n_blocks) return;
+    rb = id % a.n_rb, id /= a.n_rb;
+    split = id % a.splits, id /= a.splits;
+    hk = id % a.c.n_heads, b = id / a.c.n_heads;
+    rb = rb * WAVES + wave;
   } else {
-    lo = base + t_lo - a.window;
-    lo_all = base + t_hi - a.window;
-    hi = base + t_hi;
-    hi_all = base + t_lo;
-    if (hi < a.np) hi = -1;            // only persistent rows
-    if (hi_all < a.np) hi_all = -1;    // some
+    b = blockIdx.x, hk = blockIdx.y;
+    rb = a.splits == 1 ? blockIdx.z : blockIdx.z / static_cast<unsigned>(a.splits);
+    split = blockIdx.z - rb * a.splits;
   }
-  if (lo < np) lo = np;
-  int n_a = (np + 31) >> 5, b0 = lo >> 5, n_b = 0;
-  if (b0 < n_a) b0 = n_a;
-  if (hi >= lo) n_b = (hi >> 5) - b0 + 1;
-  if (n_b < 0) n_b = 0;
-  const int n_tiles = work ? n_a + n_b : 0;
-  int tile0 = 0, tile1 = n_tiles;
+  const Seq s = seq_of(a.c, b);
+  const int rows_all = a.c.T * a.G, row0 = rb * kRows, G = a.G;
+  const int t_lo = by_group(a, row0), t_end = by_group(a, row0 + kRows - 1);
+  const Keys keys = keys_of(a, s, t_lo, t_end < s.n - 1 ? t_end : s.n - 1);
+  const int base = s.len - s.n, len = s.len;
+  int tile0 = 0, tile1 = keys.n_tiles;
   if (a.splits > 1) {
-    const int per = (n_tiles + a.splits - 1u) / static_cast<unsigned>(a.splits);
-    tile0 = per * split < n_tiles ? per * split : n_tiles;
-    tile1 = tile0 + per < n_tiles ? tile0 + per : n_tiles;
+    const int per = (keys.n_tiles + a.splits - 1u) / static_cast<unsigned>(a.splits);
+    tile0 = per * split < keys.n_tiles ? per * split : keys.n_tiles;
+    tile1 = tile0 + per < keys.n_tiles ? tile0 + per : keys.n_tiles;
   }
+  constexpr int kStep = ROWS ? 1 : WAVES;
+  if (!ROWS) tile0 += wave;
 
-  // this lane's rows, one of each 16
+  // The queries of this lane's rows, one of each 16. They are read whatever the sequence's numbers are, which arrive
+  // later.
   Row row[RT];
   u32x4 q16[RT][S::kF32 ? 1 : S::kPieces * S::kOps];
   float q32[RT][S::kF32 ? S::kPieces * S::kRun : 1];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = row0 + 16 * rt + n, t = by_group(a, r), gg = r - t * G;
-    const bool real = r < rows_all;  // read whatever the sequence's numbers are, which arrive later
-    row[rt] = work && t < s.n ? row_of(a, s, b, t) : Row{0, 1, 0, 0};
+    const bool real = r < rows_all;
+    row[rt] = real && keys.n_tiles ? row_of(a, s, b, t) : no_row();
     const uint8_t* const src = a.q + (b * a.qb + (hk * G + gg) * a.qh + t * a.qt) * kRowSize<DT>;
 #pragma unroll
     for (int c = 0; c < S::kPieces; ++c) {
+      const int i0 = 4 * S::kRun * c + S::kRun * g;
+      if (!S::kF32 && a.q_vec) {
+#pragma unroll
+        for (int e = 0; e < S::kOps; ++e) {
+          u32x4 w{0, 0, 0, 0};
+          if (real && i0 + 8 * e < a.c.d) w = *reinterpret_cast<const u32x4*>(src + (i0 + 8 * e) * 2);
+          q16[rt][S::kF32 ? 0 : c * S::kOps + e] = w;
+        }
+        continue;
+      }
       float x[S::kRun];
 #pragma unroll
       for (int u = 0; u < S::kRun; ++u) x[u] = 0.f;
-      const int i0 = 4 * S::kRun * c + S::kRun * g;
       if (real) {
-        if (a.q_vec) {
-          constexpr int N = kRowVec<DT>;
+        if (S::kF32 && a.q_vec) {
 #pragma unroll
-          for (int u = 0; u < S::kRun; u += N) {
+          for (int u = 0; u < S::kRun; u += 4) {
             if (i0 + u >= a.c.d) continue;
-            float y[N];
-            row_load<DT, N>(src + (i0 + u) * kRowSize<DT>, y);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(src + (i0 + u) * 4);
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[u + e] = y[e];
+            for (int e = 0; e < 4; ++e) x[u + e] = y[e];
           }
         } else {
 #pragma unroll
           for (int u = 0; u < S::kRun; ++u) {
             float y[1] = {0.f};
             if (i0 + u < a.c.d) row_load<DT, 1>(src + (i0 + u) * kRowSize<DT>, y);
-            x[u] = y[0];
+            x[u] = y[0] * a.q_sign;
           }
         }
       }
@@ -311,123 +353,104 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
     }
   }
 
+  // m: the largest score so far (not scaled); mu: it times scale2, what exponents are taken relative to (0 while there
+  // is none); l: this lane's part of the sum
   f32x4 acc[RT][NJ];
-  float m[RT], l[RT];
+  float m[RT], mu[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -kInf;
-    l[rt] = 0.f;
+    mu[rt] = l[rt] = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   const int page_mask = (1 << a.c.page_shift) - 1, pitch_b = a.c.pitch * S::kElem;
-  const int k_off = n * pitch_b + g * 16;                  // of a key's first piece, in a group of 16 keys
-  const int v_off = 4 * g * pitch_b + n * NB;              // of the values' pieces, likewise
-  const bool v_in = n * NJ < a.c.pitch;                    // columns of d: others are not read
+  const bool narrow = a.c.pitch < DP;
+  // Byte offsets of this lane's pieces in a group of 16 keys. Columns past the pitch are read as the row's first: of keys
+  // they are cleared, of values they end in results that are not stored.
+  int k_off[S::kPieces];
+#pragma unroll
+  for (int c = 0; c < S::kPieces; ++c) {
+    const int col = S::kRun * (4 * c + g);
+    k_off[c] = n * pitch_b + (col < a.c.pitch ? col * S::kElem : 0);
+  }
+  const int v_off = 4 * g * pitch_b + (n * NJ < a.c.pitch ? n * NB : 0);
   const int32_t* const table = a.c.table + b * a.c.table_stride;
-  constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
-  float v_ref = 0x1p-126f;
-  bool cleaned = false;
 
   // The next tile's pages are looked up while this one is worked on; its keys are asked for when this one's have been
   // multiplied, its values when this one's have.
   Piece<16> kp[2][S::kPieces];
   Piece<NB> vp[8];
   float ks[8], vs[8];
-  int page_next[2];
+  int page[2];
+  int64_t at[2];  // the pool's rows of the tile's two groups of 16 keys
   auto look_up = [&](int it) {
-    const int key0 = (it < n_a ? it : b0 + it - n_a) << 5;
+    const int key0 = keys.first(it);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int key = key0 + 16 * hf;
-      page_next[hf] = it < tile1 && key < len ? table[key >> a.c.page_shift] : 0;
+      page[hf] = it < tile1 && key < len ? table[key >> a.c.page_shift] : 0;
     }
   };
-  auto group_row = [&](int it, int hf, int page) {  // the pool's row of a group of 16 keys
-    const int key = ((it < n_a ? it : b0 + it - n_a) << 5) + 16 * hf;
-    if (page < 0 || page >= a.c.n_pages) page = 0;
-    return ((static_cast<int64_t>(page) * a.c.n_heads + hk) << a.c.page_shift) + (key & page_mask);
-  };
-  auto load_keys = [&](const int64_t (&r)[2]) {
+  auto place = [&](int it) {
+    const int key0 = keys.first(it);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const uint8_t* const kb = a.c.k + r[hf] * pitch_b;
+      const int p = static_cast<unsigned>(page[hf]) < static_cast<unsigned>(a.c.n_pages) ? page[hf] : 0;
+      at[hf] = ((static_cast<int64_t>(p) * a.c.n_heads + hk) << a.c.page_shift) + ((key0 + 16 * hf) & page_mask);
+    }
+  };
+  auto load_keys = [&]() {
 #pragma unroll
-      for (int c = 0; c < S::kPieces; ++c) {
-        if (4 * S::kRun * c + S::kRun * g < a.c.pitch)
-          kp[hf][c].load(kb + k_off + 64 * c);
-        else
-          kp[hf][c].clear();
-      }
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint8_t* const kb = a.c.k + at[hf] * pitch_b;
+#pragma unroll
+      for (int c = 0; c < S::kPieces; ++c) kp[hf][c].load(kb + k_off[c]);
       if constexpr (FMT != kCacheSame) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.ks + r[hf] + 4 * g);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.ks + at[hf] + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) ks[4 * hf + i] = x[i];
       }
     }
   };
-  auto load_values = [&](const int64_t (&r)[2]) {
+  auto load_values = [&]() {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const uint8_t* const vb = a.c.v + r[hf] * pitch_b;
+      const uint8_t* const vb = a.c.v + at[hf] * pitch_b;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (v_in)
-          vp[4 * hf + i].load(vb + v_off + i * pitch_b);
-        else
-          vp[4 * hf + i].clear();
-      }
+      for (int i = 0; i < 4; ++i) vp[4 * hf + i].load(vb + i * pitch_b + v_off);
       if constexpr (FMT != kCacheSame) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.vs + r[hf] + 4 * g);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.vs + at[hf] + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) vs[4 * hf + i] = x[i];
       }
     }
   };
-  int64_t at[2];
-  if (tile0 + wave < tile1) {
-    look_up(tile0 + wave);
-    at[0] = group_row(tile0 + wave, 0, page_next[0]);
-    at[1] = group_row(tile0 + wave, 1, page_next[1]);
-    load_keys(at);
-    load_values(at);
+  if (tile0 < tile1) {
+    look_up(tile0);
+    place(tile0);
+    load_keys();
+    load_values();
   }
-  for (int it = tile0 + wave; it < tile1; it += n_waves) {
-    const int key0 = (it < n_a ? it : b0 + it - n_a) << 5;
+  float v_ref = 0x1p-126f;
+  bool cleaned = false;
+
+  for (int it = tile0; it < tile1; it += kStep) {
+    const int key0 = keys.first(it);
     bool bad[2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) bad[hf] = page_next[hf] < 0 || page_next[hf] >= a.c.n_pages;
-    const bool more = it + n_waves < tile1;
-    look_up(it + n_waves);
+    for (int hf = 0; hf < 2; ++hf) bad[hf] = static_cast<unsigned>(page[hf]) >= static_cast<unsigned>(a.c.n_pages);
+    const bool more = it + kStep < tile1;
+    look_up(it + kStep);
     // every row sees the whole tile (rows that are none see it too: their results are not used)
-    const bool full = !bad[0] && !bad[1] && (key0 + 31 < np_all || (key0 >= lo_all && key0 + 31 <= hi_all));
-    bool seen[8];  // by any row
+    const bool full = !bad[0] && !bad[1] && keys.all_see(key0);
+
+    if (narrow) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
-      seen[i] = full || (!bad[i >> 2] && (key < np || (key >= lo && key <= hi)));
+      for (int c = 0; c < S::kPieces; ++c)
+        if (S::kRun * (4 * c + g) >= a.c.pitch) kp[0][c].clear(), kp[1][c].clear();
     }
-    // fp16 probabilities times a scale of the values: relative to a power of two above all scales so far
-    if constexpr (kScaled16) {
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, seen[i] ? vs[i] : 0.f);
-      top = fmaxf(top, lane_xor<16>(top));
-      top = fmaxf(top, lane_xor<32>(top));
-      if (top > v_ref) {  // the same in all lanes
-        const float to = __uint_as_float(((__float_as_uint(top) >> 23) + (top < 0x1p126f)) << 23);
-        const float f = v_ref / to;
-        v_ref = to;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vs[i] *= 1.f / v_ref;
-    }
-    float p[RT][8], ks_now[8];
     f32x4 sc[RT][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -447,80 +470,120 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
           }
         }
     }
-    if constexpr (FMT != kCacheSame) {
+    float x[RT][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ks_now[i] = ks[i];
-    }
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[rt][i] = sc[rt][i >> 2][i & 3];
+        if constexpr (FMT != kCacheSame) x[rt][i] *= ks[i];
+      }
     if (more) {
-      at[0] = group_row(it + n_waves, 0, page_next[0]);
-      at[1] = group_row(it + n_waves, 1, page_next[1]);
-      load_keys(at);
+      place(it + kStep);
+      load_keys();
+    }
+
+    uint32_t vis[RT];  // bit i: the row sees key i of this lane's eight
+    if (!full) {
+      const int kb = key0 + 4 * g;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        vis[rt] = 0;
+        if (a.tree) {
+          const uint32_t w = bits_from(row[rt].bits, kb - base), w2 = bits_from(row[rt].bits, kb + 16 - base);
+          vis[rt] = (w & 15u) | (w2 & 15u) << 4;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = kb + 16 * (i >> 2) + (i & 3);
+          const bool v = (key < row[rt].np) | in_span(key, row[rt].lo, row[rt].span);
+          vis[rt] |= v ? 1u << i : 0u;
+          if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
+        }
+        if (bad[0] || bad[1]) {  // a page that is none: NaN for the rows that see it
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (bad[i >> 2] && (vis[rt] >> i & 1)) x[rt][i] = __builtin_nanf("");
+        }
+      }
+      // Values of keys that no row sees may be anything: zeros in their place. So may be those that some rows see
+      // and others do not (0 times infinity): zeros here, added after the loop for the rows that see them.
+      const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
+      const int lo = keys.hi >= keys.lo ? keys.lo : kNowhere;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = kb + 16 * (i >> 2) + (i & 3);
+        const uint32_t on = (((key < keys.np) | in_span(key, lo, span)) & !bad[i >> 2]) ? ~0u : 0u;
+#pragma unroll
+        for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
+        if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
+      }
+      if (FMT == kCacheSame && a.c.T > 1) {
+        uint32_t changed = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int w = 0; w < NB / 4; ++w) {
+            const uint32_t y = finite_only<DT>(vp[i].w[w]);
+            changed |= y ^ vp[i].w[w];
+            vp[i].w[w] = y;
+          }
+        if (__any(changed != 0)) cleaned = true;
+      }
+    }
+    // fp16 probabilities times a scale of the values: relative to a power of two above all scales so far
+    if constexpr (kScaled16) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, vs[i]);
+      if (__any(top > v_ref)) {
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+        const float to = __uint_as_float(((__float_as_uint(top) >> 23) + (top < 0x1p126f)) << 23);
+        const float f = v_ref / to;
+        v_ref = to;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
+      }
+      const float inv = 1.f / v_ref;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vs[i] *= inv;
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float x[8], mx = -kInf;
-      uint32_t vis = 0xff;
+      float mx = x[rt][0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = sc[rt][i >> 2][i & 3] * a.scale2;
-        if constexpr (FMT != kCacheSame) x[i] *= ks_now[i];
-      }
-      if (!full) {
-        vis = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
-          const bool v = sees(row[rt], key, base, tree);
-          if (bad[i >> 2]) x[i] = __builtin_nanf("");
-          if (!v) x[i] = -kInf;
-          vis |= static_cast<uint32_t>(v) << i;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[rt][i]);
       if (__any(mx > m[rt])) {
         mx = fmaxf(mx, lane_xor<16>(mx));
         mx = fmaxf(mx, lane_xor<32>(mx));
-        const float to = fmaxf(m[rt], mx);
-        const float f = to == m[rt] ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
+        const float to = fmaxf(m[rt], mx), mu_to = to == -kInf ? 0.f : to * a.scale2;
+        const float f = to == m[rt] || m[rt] == -kInf ? 1.f : __builtin_amdgcn_exp2f(mu[rt] - mu_to);
         m[rt] = to;
+        mu[rt] = mu_to;
         l[rt] *= f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
       }
-      const float mu = m[rt] == -kInf ? 0.f : m[rt];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float e = __builtin_amdgcn_exp2f(x[i] - mu);
+        const float e = __builtin_amdgcn_exp2f(fmaf(x[rt][i], a.scale2, -mu[rt]));
         l[rt] += e;
-        if constexpr (FMT != kCacheSame) e = vis >> i & 1 ? e * vs[i] : 0.f;
-        p[rt][i] = e;
+        x[rt][i] = FMT != kCacheSame ? e * vs[i] : e;
       }
-    }
-    // Values of keys that no row sees may be anything: zeros in their place. So may be those that some rows see and
-    // others do not (0 times infinity): zeros here, added after the loop for the rows that see them.
-    if (!full) {
-      uint32_t changed = 0;
+      if (FMT != kCacheSame && !full && a.c.T > 1) {  // 0 times a scale of NaN
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (!seen[i]) vp[i].clear();
-        if (FMT == kCacheSame && a.c.T > 1) {
-#pragma unroll
-          for (int w = 0; w < NB / 4; ++w) {
-            const uint32_t x = finite_only<DT>(vp[i].w[w]);
-            changed |= x ^ vp[i].w[w];
-            vp[i].w[w] = x;
-          }
-        }
+        for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
       }
-      if (FMT == kCacheSame && __any(changed != 0)) cleaned = true;
     }
     u32x4 pw[RT];
     if constexpr (!S::kF32) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) pw[rt][w] = Mfma<DT>::pack2(p[rt][2 * w], p[rt][2 * w + 1]);
+        for (int w = 0; w < 4; ++w) pw[rt][w] = Mfma<DT>::pack2(x[rt][2 * w], x[rt][2 * w + 1]);
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -530,7 +593,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
           const float v = value_f32<FMT, NB>(vp[i], j);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
-            acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[rt][i], acc[rt][j], 0, 0, 0);
+            acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
         }
       } else {
         const u32x4 v = value_operand<DT, FMT, NB>(vp, j);
@@ -538,9 +601,8 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
         for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16<DT>(v, pw[rt], acc[rt][j]);
       }
     }
-    if (more) load_values(at);
+    if (more) load_values();
   }
-
   if constexpr (kScaled16) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -549,9 +611,9 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
   }
   if (FMT == kCacheSame && cleaned) {
     // What was taken for zeros and is not finite, to the rows that see it.
-    for (int it = tile0 + wave; it < tile1; it += n_waves) {
-      const int key0 = (it < n_a ? it : b0 + it - n_a) << 5;
-      if (key0 + 31 < np_all || (key0 >= lo_all && key0 + 31 <= hi_all)) continue;
+    for (int it = tile0; it < tile1; it += kStep) {
+      const int key0 = keys.first(it);
+      if (keys.all_see(key0)) continue;
       for (int key = key0; key < key0 + 32 && key < len; ++key) {
         const int64_t r = cache_row(a.c, b, key, hk);
         if (r < 0) continue;
@@ -566,10 +628,50 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
             if (__builtin_isfinite(v[0])) continue;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-              if (sees(row[rt], key, base, tree)) acc[rt][j][i] += v[0];
+              if (sees(row[rt], key, base)) acc[rt][j][i] += v[0];
           }
       }
     }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += lane_xor<16>(l[rt]);
+    l[rt] += lane_xor<32>(l[rt]);
+    // rows that saw nothing but NaN have a sum of NaN and no maximum: 0 stands for it
+    if (m[rt] != -kInf || l[rt] != l[rt]) m[rt] = mu[rt];
+  }
+
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + 16 * rt + n;
+      if (r >= rows_all) continue;
+      const int t = by_group(a, r), gg = r - t * G;
+      if (a.splits > 1) {
+        const int64_t to = ((static_cast<int64_t>(b) * a.c.n_heads + hk) * a.splits + split) * rows_all + r;
+        float* const po = a.ws + to * (DP + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; j += 4)
+            *reinterpret_cast<f32x4*>(po + (4 * g + i) * NJ + j) =
+                f32x4{acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]};
+        if (g == 0) {
+          po[DP] = m[rt];
+          po[DP + 1] = l[rt];
+        }
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; j += 4) {
+          float o[4] = {acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]};
+          row_finish(s, t, l[rt], o);
+          row_out<DT>(a, b, t, hk * G + gg, (4 * g + i) * NJ + j, o);
+        }
+    }
+    return;
   }
 
   // The waves' results are joined in LDS: first the rows' maxima and sums, by which every wave scales what it has, then
@@ -581,9 +683,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = 16 * rt + n;
-    float sum = l[rt] + lane_xor<16>(l[rt]);
-    sum += lane_xor<32>(sum);
-    if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], sum};
+    if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], l[rt]};
   }
   __syncthreads();
 #pragma unroll
@@ -610,18 +710,15 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const float2 x = sm[w * cap + r];
-      sum += x.y * (x.x == top ? 1.f : __builtin_amdgcn_exp2f(x.x - top));
-    }
+      const float2 y = sm[w * cap + r];
+      sum += y.y * (y.x == top ? 1.f : __builtin_amdgcn_exp2f(y.x - top));
+      const f32x4 z = *reinterpret_cast<const f32x4*>(sh + (w * cap + r) * kPitchO + i0);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(sh + (w * cap + r) * kPitchO + i0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += x[e];
+      for (int e = 0; e < 4; ++e) o[e] += z[e];
     }
     if (a.splits > 1) {
-      const int64_t at = ((static_cast<int64_t>(b) * a.c.n_heads + hk) * a.splits + split) * rows_all + row0 + r;
-      float* const po = a.ws + at * (DP + 4);
+      const int64_t to = ((static_cast<int64_t>(b) * a.c.n_heads + hk) * a.splits + split) * rows_all + row0 + r;
+      float* const po = a.ws + to * (DP + 4);
       *reinterpret_cast<f32x4*>(po + i0) = f32x4{o[0], o[1], o[2], o[3]};
       if (i0 == 0) {
         po[DP] = top;
@@ -668,31 +765,42 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(AttnArgs a) {
 
 struct Plan {
   int rt, waves, n_rb, splits, row_cap;
+  bool rows;
   size_t ws;
 };
 
-// rows: query rows per key head; blocks of rows of all sequences and heads; tiles of keys that a block may have to walk
+// Most tiles of 16 rows that a wave holds: the registers of one whose 256 leave two waves to a SIMD.
 Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np) {
   Plan p{};
   const int dp = c.pitch <= 64 ? 64 : 128;
-  p.rt = rows <= 16 ? 1 : dtype == TMAC_F32 ? 2 : 4;
-  const int cap = 16 * p.rt;
-  p.n_rb = (rows + cap - 1) / cap;
-  p.row_cap = rows < cap ? rows : cap;
+  p.rt = rows <= 16 ? 1 : 2;
+  p.rows = rows > 64;
   const int64_t len = static_cast<int64_t>(c.max_pages) << c.page_shift;
   int64_t keys = window + c.T + np;
   if (keys > len) keys = len;
-  const int64_t tiles = keys / 32 + 2;
-  const int most = p.rt > 1 ? 4 : dtype != TMAC_F32 && dp == 64 ? 16 : 8;
-  p.waves = tiles >= 2 * 8 && most == 16 ? 16 : tiles > 4 && most >= 8 ? 8 : 4;
-  const int64_t blocks = static_cast<int64_t>(B) * c.n_heads * p.n_rb;
-  // enough workgroups for every CU, each wave with 4 tiles at least
-  int64_t s = (1024 + blocks - 1) / blocks;
-  const int64_t by_len = tiles / (4 * p.waves);
-  if (s > by_len) s = by_len;
+  const int64_t tiles = keys / 32 + 2, heads = static_cast<int64_t>(B) * c.n_heads;
+  const int cap = 16 * p.rt;
+  int64_t s = 1;
+  if (p.rows) {
+    p.waves = 4;
+    p.n_rb = (rows + 4 * cap - 1) / (4 * cap);
+    // two workgroups for every CU, each with 32 tiles at least
+    const int64_t blocks = heads * p.n_rb;
+    s = blocks < 512 ? 512 / blocks : 1;
+    if (s > tiles / 32) s = tiles / 32;
+  } else {
+    p.n_rb = (rows + cap - 1) / cap;
+    p.row_cap = rows < cap ? rows : cap;
+    const int64_t blocks = heads * p.n_rb;
+    p.waves = dtype == TMAC_F32 && dp == 128 ? 4 : 8;  // 512 registers for wide fp32 rows
+    if (p.rt == 1 && (tiles <= 4 || (blocks >= 512 && tiles <= 24))) p.waves = 4;
+    // enough workgroups for every CU, each wave with 4 tiles at least
+    s = (512 + blocks - 1) / blocks;
+    if (s > tiles / (4 * p.waves)) s = tiles / (4 * p.waves);
+  }
   if (s > 64) s = 64;
   p.splits = s < 1 ? 1 : static_cast<int>(s);
-  p.ws = p.splits > 1 ? static_cast<size_t>(B) * c.n_heads * p.splits * rows * (dp + 4) * 4 : 0;
+  p.ws = p.splits > 1 ? static_cast<size_t>(heads) * p.splits * rows * (dp + 4) * 4 : 0;
   return p;
 }
 
@@ -700,27 +808,25 @@ int check(const tmac_cache* cache, int B, int T, int Hq, int64_t window, int np,
   const int st = cache_args(cache, B, T, c);
   if (st != TMAC_OK) return st;
   if (Hq <= 0 || Hq > 65535 || Hq % c.n_heads || static_cast<int64_t>(T) * Hq > (1 << 26)) return TMAC_ERR_SHAPE;
+  if (static_cast<int64_t>(B) * Hq * T > (1 << 26)) return TMAC_ERR_SHAPE;
   if (window < 0 || np < 0) return TMAC_ERR_VALUE;
   return TMAC_OK;
 }
 
-// Most waves of a workgroup with one tile of rows: as many as leave each the registers that it needs.
-template <int DT, int DP>
-constexpr int kMostWaves = DT != TMAC_F32 && DP == 64 ? 16 : 8;
-
 template <int DT, int FMT, int DP>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
-  const dim3 grid(a.B, a.c.n_heads, p.n_rb * p.splits);
   const size_t lds = static_cast<size_t>(p.waves) * p.row_cap * (DP + 4 + 2) * 4;
-  constexpr int kMany = DT == TMAC_F32 ? 2 : 4, kMost = kMostWaves<DT, DP>;
-  if (p.rt > 1)
-    cached_attn_kernel<DT, FMT, DP, kMany, 4><<<grid, 64 * 4, lds, s>>>(a);
-  else if (p.waves == 4)
-    cached_attn_kernel<DT, FMT, DP, 1, 4><<<grid, 64 * 4, lds, s>>>(a);
-  else if (p.waves == 8)
-    cached_attn_kernel<DT, FMT, DP, 1, 8><<<grid, 64 * 8, lds, s>>>(a);
-  else
-    cached_attn_kernel<DT, FMT, DP, 1, kMost><<<grid, 64 * kMost, lds, s>>>(a);
+  const dim3 grid(a.B, a.c.n_heads, p.n_rb * p.splits);
+  if (p.rows) {
+    cached_attn_kernel<DT, FMT, DP, 2, 4, true><<<8 * a.per_xcd, 256, 0, s>>>(a);
+  } else if (p.rt == 2) {
+    constexpr int kWaves = DT == TMAC_F32 && DP == 128 ? 4 : 8;
+    cached_attn_kernel<DT, FMT, DP, 2, kWaves, false><<<grid, 64 * kWaves, lds, s>>>(a);
+  } else if (p.waves == 4) {
+    cached_attn_kernel<DT, FMT, DP, 1, 4, false><<<grid, 64 * 4, lds, s>>>(a);
+  } else if constexpr (!(DT == TMAC_F32 && DP == 128)) {
+    cached_attn_kernel<DT, FMT, DP, 1, 8, false><<<grid, 64 * 8, lds, s>>>(a);
+  }
   if (p.splits > 1) {
     const int64_t threads = static_cast<int64_t>(a.B) * a.c.n_heads * a.c.T * a.G * (DP / 4);
     cached_attn_join_kernel<DT, DP><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(a);
@@ -771,20 +877,21 @@ extern "C" int tmac_cached_attn(const tmac_cache* cache, const void* d_q, const 
   const Plan p = plan(a.c, cache->dtype, B, T * G, window, n_persistent);
   if (p.ws && (!d_ws || ws_bytes < p.ws)) return TMAC_ERR_WORKSPACE;
   if (p.ws && !row_aligned16(d_ws)) return TMAC_ERR_ALIGN;
-  if (static_cast<int64_t>(p.n_rb) * p.splits > 65535 || static_cast<int64_t>(B) * n_q_heads * T > (1 << 26))
-    return TMAC_ERR_SHAPE;
+  const int64_t blocks = static_cast<int64_t>(B) * a.c.n_heads * p.n_rb * p.splits;  // below 2^27 by check()
   const int n = cache->dtype == TMAC_F32 ? 4 : 8;
   a.q = static_cast<const uint8_t*>(d_q);
   a.qb = h_q_strides[0], a.qh = h_q_strides[1], a.qt = h_q_strides[2];
   a.tree = d_tree, a.tree_stride = tree_stride;
   a.out = static_cast<uint8_t*>(d_out);
   a.ws = static_cast<float*>(d_ws);
-  a.B = B, a.Hq = n_q_heads, a.G = G, a.g_shift = G & (G - 1) ? -1 : __builtin_ctz(G), a.n_rb = p.n_rb, a.splits = p.splits, a.row_cap = p.row_cap;
+  a.B = B, a.Hq = n_q_heads, a.G = G, a.g_shift = G & (G - 1) ? -1 : __builtin_ctz(G), a.n_rb = p.n_rb;
+  a.splits = p.splits, a.row_cap = p.row_cap, a.n_blocks = static_cast<int>(blocks), a.per_xcd = (a.n_blocks + 7) / 8;
   constexpr int kMost = 1 << 30;
   a.np = n_persistent < kMost ? n_persistent : kMost;
   a.window = window < kMost ? static_cast<int>(window) : kMost;
-  a.scale2 = scale * kLog2e;
-  a.q_vec = row_aligned16(d_q) && a.c.d % n == 0 && a.qb % n == 0 && a.qh % n == 0 && a.qt % n == 0;
+  a.scale2 = scale == 0.f ? 1.f : fabsf(scale) * kLog2e;
+  a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : scale;
+  a.q_vec = a.q_sign == 1.f && row_aligned16(d_q) && a.c.d % n == 0 && a.qb % n == 0 && a.qh % n == 0 && a.qt % n == 0;
   a.out_vec = row_aligned16(d_out) && a.c.d % 4 == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (cache->dtype == TMAC_F32)
