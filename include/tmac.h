@@ -775,7 +775,7 @@ int tmac_head_logprob(const void* d_X, int64_t ldx, const void* d_W, int64_t ldw
 
 /* A cache and the sequences in it.
  *   d_k, d_v: pools [n_pages, n_heads, page, pitch], contiguous; page 16, 32, 64, 128 or 256; d_head 1..128, pitch
- *     d_head rounded up to 16, what is behind d_head zeros; n_pages · n_heads · page < 2^40. format TMAC_CACHE_SAME: values
+ *     d_head rounded up to 16, what is behind d_head zeros; n_heads · page · pitch < 2^29, n_pages < 2^31, n_pages · n_heads · page < 2^40. format TMAC_CACHE_SAME: values
  *     of dtype; else 8-bit codes with scales d_k_scale, d_v_scale, fp32 [n_pages, n_heads, page] (NULL with SAME).
  *   d_table: int32 [B, max_pages] at a pitch of table_stride: the page of positions page·j .. page·j + page − 1.
  *   d_lengths: int32 [B], the positions that each sequence holds, its new rows included; d_counts: int32 [B]

@@ -123,6 +123,8 @@ inline int cache_args(const tmac_cache* c, int B, int T, CacheArgs& a) {
   if ((1 << shift) != c->page || c->n_heads <= 0 || c->n_heads > 65535 || c->d_head <= 0 || c->d_head > 128 ||
       c->pitch != (c->d_head + 15) / 16 * 16)
     return TMAC_ERR_SHAPE;
+  // a page's bytes are counted in 32 bits
+  if (static_cast<int64_t>(c->n_heads) * c->page * c->pitch >= (1 << 29)) return TMAC_ERR_SHAPE;
   if (c->n_pages <= 0 || c->n_pages >= (INT64_C(1) << 31) || c->n_pages * c->n_heads >= (INT64_C(1) << 40) / c->page)
     return TMAC_ERR_SHAPE;
   // positions are counted in 32 bits, and so are the threads of a launch (up to 32 a row)

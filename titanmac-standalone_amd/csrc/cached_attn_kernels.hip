@@ -260,7 +260,7 @@ __device__ __forceinline__ void row_out(const AttnArgs& a, int b, int t, int h, 
 // ROWS: the workgroup's waves hold a block of rows each and walk the same keys, for many rows (their loads meet in the
 // first-level cache); otherwise they hold the same rows and share the keys out.
 template <int DT, int FMT, int DP, int RT, int WAVES, bool ROWS>
-__global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) void cached_attn_kernel(AttnArgs a) {
   using S = Shape<DT, FMT, DP>;
   constexpr int NJ = S::NJ, kRows = 16 * RT, NB = NJ * S::kElem;
   constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
@@ -378,37 +378,48 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
   const int v_off = 4 * g * pitch_b + (n * NJ < a.c.pitch ? n * NB : 0);
   const int32_t* const table = a.c.table + b * a.c.table_stride;
 
-  // The next tile's pages are looked up while this one is worked on; its keys are asked for when this one's have been
-  // multiplied, its values when this one's have.
+  // A tile's pages are looked up two tiles ahead; its keys are asked for when those of the tile before have been
+  // multiplied, its values when those have. A tile has two pages where pages are of 16 rows.
   Piece<16> kp[2][S::kPieces];
   Piece<NB> vp[8];
   float ks[8], vs[8];
-  int page[2];
-  int64_t at[2];  // the pool's rows of the tile's two groups of 16 keys
+  const bool halves = a.c.page_shift < 5;
+  int page[2], page_next[2] = {0, 0};  // of the tile whose rows were last asked for, and of the one behind it
+  int key_next = 0;                    // the first key of the latter
+  int64_t at[2];                       // byte offsets of the tile's two groups of 16 keys in the pools
+  int64_t at_scale[2];                 // and their rows
+  const uint32_t page_rows = static_cast<uint32_t>(a.c.n_heads) << a.c.page_shift, page_bytes = page_rows * pitch_b;
+  const uint32_t head_rows = static_cast<uint32_t>(hk) << a.c.page_shift;
   auto look_up = [&](int it) {
-    const int key0 = keys.first(it);
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int key = key0 + 16 * hf;
-      page[hf] = it < tile1 && key < len ? table[key >> a.c.page_shift] : 0;
-    }
+    if (it >= tile1) return;
+    key_next = keys.first(it);
+    page_next[0] = table[key_next >> a.c.page_shift];
+    if (halves) page_next[1] = key_next + 16 < len ? table[(key_next + 16) >> a.c.page_shift] : 0;
   };
-  auto place = [&](int it) {
-    const int key0 = keys.first(it);
+  auto place = [&]() {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int p = static_cast<unsigned>(page[hf]) < static_cast<unsigned>(a.c.n_pages) ? page[hf] : 0;
-      at[hf] = ((static_cast<int64_t>(p) * a.c.n_heads + hk) << a.c.page_shift) + ((key0 + 16 * hf) & page_mask);
+      if (hf && !halves) {
+        page[1] = page[0];
+        at[1] = at[0] + 16 * pitch_b;
+        at_scale[1] = at_scale[0] + 16;
+        continue;
+      }
+      page[hf] = page_next[hf];
+      const uint32_t p = static_cast<uint32_t>(page[hf]) < static_cast<uint32_t>(a.c.n_pages) ? page[hf] : 0;
+      const uint32_t r = head_rows + ((key_next + 16 * hf) & page_mask);
+      at[hf] = static_cast<int64_t>(static_cast<uint64_t>(p) * page_bytes + r * pitch_b);
+      if (FMT != kCacheSame) at_scale[hf] = static_cast<int64_t>(static_cast<uint64_t>(p) * page_rows + r);
     }
   };
   auto load_keys = [&]() {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const uint8_t* const kb = a.c.k + at[hf] * pitch_b;
+      const uint8_t* const kb = a.c.k + at[hf];
 #pragma unroll
       for (int c = 0; c < S::kPieces; ++c) kp[hf][c].load(kb + k_off[c]);
       if constexpr (FMT != kCacheSame) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.ks + at[hf] + 4 * g);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.ks + at_scale[hf] + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) ks[4 * hf + i] = x[i];
       }
@@ -417,32 +428,34 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
   auto load_values = [&]() {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const uint8_t* const vb = a.c.v + at[hf] * pitch_b;
+      const uint8_t* const vb = a.c.v + at[hf];
 #pragma unroll
       for (int i = 0; i < 4; ++i) vp[4 * hf + i].load(vb + i * pitch_b + v_off);
       if constexpr (FMT != kCacheSame) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.vs + at[hf] + 4 * g);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.c.vs + at_scale[hf] + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) vs[4 * hf + i] = x[i];
       }
     }
   };
+  int key_now = 0;
   if (tile0 < tile1) {
     look_up(tile0);
-    place(tile0);
+    key_now = key_next;
+    place();
     load_keys();
     load_values();
+    look_up(tile0 + kStep);
   }
   float v_ref = 0x1p-126f;
   bool cleaned = false;
 
   for (int it = tile0; it < tile1; it += kStep) {
-    const int key0 = keys.first(it);
+    const int key0 = key_now;
     bool bad[2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) bad[hf] = static_cast<unsigned>(page[hf]) >= static_cast<unsigned>(a.c.n_pages);
     const bool more = it + kStep < tile1;
-    look_up(it + kStep);
     // every row sees the whole tile (rows that are none see it too: their results are not used)
     const bool full = !bad[0] && !bad[1] && keys.all_see(key0);
 
@@ -479,8 +492,10 @@ __global__ __launch_bounds__(64 * WAVES, 1) void cached_attn_kernel(AttnArgs a) 
         if constexpr (FMT != kCacheSame) x[rt][i] *= ks[i];
       }
     if (more) {
-      place(it + kStep);
+      key_now = key_next;
+      place();
       load_keys();
+      look_up(it + 2 * kStep);
     }
 
     uint32_t vis[RT];  // bit i: the row sees key i of this lane's eight

@@ -66,6 +66,9 @@ class KVCache(tuple):
         if page not in PAGES or not 1 <= d <= MAX_HEAD or pitch != (d + 15) // 16 * 16 or n < 1 or heads < 1:
             raise ValueError(f"KVCache: pages of {PAGES} rows of d_head (1..{MAX_HEAD}) rounded up to 16 values, got "
                              f"{tuple(shape)} for d_head {d}")
+        if heads * page * pitch >= 1 << 29 or n >= 1 << 31 or n * heads * page >= 1 << 40:
+            raise ValueError(f"KVCache: a page has fewer than 2^29 values, pools fewer than 2^31 pages and 2^40 rows, got "
+                             f"{tuple(shape)}")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("KVCache: the pools must be contiguous")
         device = k.device
