@@ -182,19 +182,24 @@ __device__ __forceinline__ uint32_t bits_from(uint64_t x, int s) {
   return static_cast<uint32_t>(s >= 0 ? x >> s : x << -s);
 }
 
-// The keys of a block of rows t_lo .. t_hi, as tiles of 32: those with persistent keys, then those of [lo, hi] behind
+// The keys of a block of rows t_lo .. t_hi, as tiles of 2^SH: those with persistent keys, then those of [lo, hi] behind
 // them. Every key that a row sees is below np or in [lo, hi]; every row sees the keys below np_all and in
 // [lo_all, hi_all].
+template <int SH>
 struct Keys {
   int np, np_all, lo, hi, lo_all, hi_all, n_a, b0, n_tiles;
-  __device__ __forceinline__ int first(int it) const { return (it < n_a ? it : b0 + it - n_a) << 5; }
-  __device__ __forceinline__ bool all_see(int key0) const {
-    return key0 + 31 < np_all || (key0 >= lo_all && key0 + 31 <= hi_all);
+  __device__ __forceinline__ int first(int it) const { return (it < n_a ? it : b0 + it - n_a) << SH; }
+  __device__ __forceinline__ bool all_see(int key0, int last = (1 << SH) - 1) const {
+    return key0 + last < np_all || (key0 >= lo_all && key0 + last <= hi_all);
+  }
+  __device__ __forceinline__ bool any_sees(int key0, int last) const {
+    return key0 < np || (key0 + last >= lo && key0 <= hi);
   }
 };
 
-__device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Seq& s, int t_lo, int t_hi) {
-  Keys k;
+template <int SH = 5>
+__device__ __forceinline__ Keys<SH> keys_of(const AttnArgs& a, const Seq& s, int t_lo, int t_hi) {
+  Keys<SH> k;
   const int base = s.len - s.n;
   k.np = a.np < s.len ? a.np : s.len;
   k.np_all = k.np;
@@ -213,9 +218,9 @@ __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Seq& s, int t_l
     if (k.hi_all < a.np) k.hi_all = -1;  // some persistent rows
   }
   if (k.lo < k.np) k.lo = k.np;
-  k.n_a = (k.np + 31) >> 5;
-  k.b0 = k.lo >> 5 > k.n_a ? k.lo >> 5 : k.n_a;
-  const int n_b = k.hi >= k.lo ? (k.hi >> 5) - k.b0 + 1 : 0;
+  k.n_a = (k.np + (1 << SH) - 1) >> SH;
+  k.b0 = k.lo >> SH > k.n_a ? k.lo >> SH : k.n_a;
+  const int n_b = k.hi >= k.lo ? (k.hi >> SH) - k.b0 + 1 : 0;
   k.n_tiles = s.ok && t_lo < s.n ? k.n_a + (n_b > 0 ? n_b : 0) : 0;
   return k;
 }
@@ -227,6 +232,78 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
   constexpr uint32_t kExp = DT == TMAC_BF16 ? 0x7f807f80u : 0x7c007c00u, kLow = DT == TMAC_BF16 ? 0x00800080u : 0x04000400u;
   const uint32_t top = ((w & kExp) + kLow) & 0x80008000u;  // the top bit of a half whose exponent is all ones
   return w & ~((top >> 15) * 0xffffu);
+}
+
+// Bit i: the row sees the i-th of this lane's eight keys kb, kb + 1, .. kb + 3, kb + 16, .. kb + 19.
+__device__ __forceinline__ uint32_t row_sees(const Row& r, int kb, int base, bool tree) {
+  uint32_t vis = 0;
+  if (tree) vis = (bits_from(r.bits, kb - base) & 15u) | (bits_from(r.bits, kb + 16 - base) & 15u) << 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int key = kb + 16 * (i >> 2) + (i & 3);
+    vis |= (key < r.np) | in_span(key, r.lo, r.span) ? 1u << i : 0u;
+  }
+  return vis;
+}
+
+// The running softmax of a row, as the lanes that hold it have it. m: the largest score so far (not scaled); mu: it
+// times scale2, what exponents are taken relative to (0 while there is none); l: this lane's part of the sum.
+struct Soft {
+  float m, mu, l;
+};
+
+// Scores x (−inf where masked) become e^{x − m}; what was summed up before moves to the new maximum.
+template <int NJ>
+__device__ __forceinline__ void soften(Soft& s, float (&x)[8], f32x4 (&acc)[NJ], float scale2) {
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+  if (__any(mx > s.m)) {
+    mx = fmaxf(mx, lane_xor<16>(mx));
+    mx = fmaxf(mx, lane_xor<32>(mx));
+    const float to = fmaxf(s.m, mx), mu_to = to == -kInf ? 0.f : to * scale2;
+    const float f = to == s.m || s.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(s.mu - mu_to);
+    s.m = to;
+    s.mu = mu_to;
+    s.l *= f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[j] *= f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale2, -s.mu));
+    s.l += x[i];
+  }
+}
+// The row's statistics from its lanes': m is now in units of scale2.
+__device__ __forceinline__ void soft_join(Soft& s) {
+  s.l += lane_xor<16>(s.l);
+  s.l += lane_xor<32>(s.l);
+  // rows that saw nothing but NaN have a sum of NaN and no maximum: 0 stands for it
+  if (s.m != -kInf || s.l != s.l) s.m = s.mu;
+}
+
+// A power of two above every scale vs so far, for fp16 probabilities times a scale (v_ref); what was summed up before
+// moves to it, and vs becomes relative to it.
+template <int RT, int NJ>
+__device__ __forceinline__ void relate_scales(float& v_ref, float (&vs)[8], f32x4 (&acc)[RT][NJ]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, vs[i]);
+  if (__any(top > v_ref)) {
+    top = fmaxf(top, lane_xor<16>(top));
+    top = fmaxf(top, lane_xor<32>(top));
+    const float to = __uint_as_float(((__float_as_uint(top) >> 23) + (top < 0x1p126f)) << 23);
+    const float f = v_ref / to;
+    v_ref = to;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
+  }
+  const float inv = 1.f / v_ref;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) vs[i] *= inv;
 }
 
 // o / sum; zeros for a row that sees nothing or is none, NaN where the sequence's numbers do not fit
@@ -257,8 +334,8 @@ __device__ __forceinline__ void row_out(const AttnArgs& a, int b, int t, int h, 
   }
 }
 
-// ROWS: the workgroup's waves hold a block of rows each and walk the same keys, for many rows (their loads meet in the
-// first-level cache); otherwise they hold the same rows and share the keys out.
+// ROWS: the workgroup's waves hold a block of rows each and walk the same keys, for many rows in fp32 (whose products
+// take four times as long as their operands' loads); otherwise they hold the same rows and share the keys out.
 template <int DT, int FMT, int DP, int RT, int WAVES, bool ROWS>
 __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) void cached_attn_kernel(AttnArgs a) {
   using S = Shape<DT, FMT, DP>;
@@ -283,8 +360,9 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
   const Seq s = seq_of(a.c, b);
   const int rows_all = a.c.T * a.G, row0 = rb * kRows, G = a.G;
   const int t_lo = by_group(a, row0), t_end = by_group(a, row0 + kRows - 1);
-  const Keys keys = keys_of(a, s, t_lo, t_end < s.n - 1 ? t_end : s.n - 1);
+  const Keys<5> keys = keys_of(a, s, t_lo, t_end < s.n - 1 ? t_end : s.n - 1);
   const int base = s.len - s.n, len = s.len;
+  const bool tree = a.tree != nullptr;
   int tile0 = 0, tile1 = keys.n_tiles;
   if (a.splits > 1) {
     const int per = (keys.n_tiles + a.splits - 1u) / static_cast<unsigned>(a.splits);
@@ -353,14 +431,11 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
     }
   }
 
-  // m: the largest score so far (not scaled); mu: it times scale2, what exponents are taken relative to (0 while there
-  // is none); l: this lane's part of the sum
   f32x4 acc[RT][NJ];
-  float m[RT], mu[RT], l[RT];
+  Soft soft[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -kInf;
-    mu[rt] = l[rt] = 0.f;
+    soft[rt] = Soft{-kInf, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -503,18 +578,10 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
       const int kb = key0 + 4 * g;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        vis[rt] = 0;
-        if (a.tree) {
-          const uint32_t w = bits_from(row[rt].bits, kb - base), w2 = bits_from(row[rt].bits, kb + 16 - base);
-          vis[rt] = (w & 15u) | (w2 & 15u) << 4;
-        }
+        vis[rt] = row_sees(row[rt], kb, base, tree);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = kb + 16 * (i >> 2) + (i & 3);
-          const bool v = (key < row[rt].np) | in_span(key, row[rt].lo, row[rt].span);
-          vis[rt] |= v ? 1u << i : 0u;
+        for (int i = 0; i < 8; ++i)
           if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
-        }
         if (bad[0] || bad[1]) {  // a page that is none: NaN for the rows that see it
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -546,51 +613,17 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
         if (__any(changed != 0)) cleaned = true;
       }
     }
-    // fp16 probabilities times a scale of the values: relative to a power of two above all scales so far
-    if constexpr (kScaled16) {
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, vs[i]);
-      if (__any(top > v_ref)) {
-        top = fmaxf(top, lane_xor<16>(top));
-        top = fmaxf(top, lane_xor<32>(top));
-        const float to = __uint_as_float(((__float_as_uint(top) >> 23) + (top < 0x1p126f)) << 23);
-        const float f = v_ref / to;
-        v_ref = to;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
-      }
-      const float inv = 1.f / v_ref;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vs[i] *= inv;
-    }
+    if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float mx = x[rt][0];
+      soften(soft[rt], x[rt], acc[rt], a.scale2);
+      if constexpr (FMT != kCacheSame) {
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[rt][i]);
-      if (__any(mx > m[rt])) {
-        mx = fmaxf(mx, lane_xor<16>(mx));
-        mx = fmaxf(mx, lane_xor<32>(mx));
-        const float to = fmaxf(m[rt], mx), mu_to = to == -kInf ? 0.f : to * a.scale2;
-        const float f = to == m[rt] || m[rt] == -kInf ? 1.f : __builtin_amdgcn_exp2f(mu[rt] - mu_to);
-        m[rt] = to;
-        mu[rt] = mu_to;
-        l[rt] *= f;
+        for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
+        if (!full && a.c.T > 1) {  // 0 times a scale of NaN
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(x[rt][i], a.scale2, -mu[rt]));
-        l[rt] += e;
-        x[rt][i] = FMT != kCacheSame ? e * vs[i] : e;
-      }
-      if (FMT != kCacheSame && !full && a.c.T > 1) {  // 0 times a scale of NaN
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
+          for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
+        }
       }
     }
     u32x4 pw[RT];
@@ -649,12 +682,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
     }
   }
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += lane_xor<16>(l[rt]);
-    l[rt] += lane_xor<32>(l[rt]);
-    // rows that saw nothing but NaN have a sum of NaN and no maximum: 0 stands for it
-    if (m[rt] != -kInf || l[rt] != l[rt]) m[rt] = mu[rt];
-  }
+  for (int rt = 0; rt < RT; ++rt) soft_join(soft[rt]);
 
   if constexpr (ROWS) {
 #pragma unroll
@@ -672,8 +700,8 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
             *reinterpret_cast<f32x4*>(po + (4 * g + i) * NJ + j) =
                 f32x4{acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]};
         if (g == 0) {
-          po[DP] = m[rt];
-          po[DP + 1] = l[rt];
+          po[DP] = soft[rt].m;
+          po[DP + 1] = soft[rt].l;
         }
         continue;
       }
@@ -682,7 +710,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
 #pragma unroll
         for (int j = 0; j < NJ; j += 4) {
           float o[4] = {acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]};
-          row_finish(s, t, l[rt], o);
+          row_finish(s, t, soft[rt].l, o);
           row_out<DT>(a, b, t, hk * G + gg, (4 * g + i) * NJ + j, o);
         }
     }
@@ -698,7 +726,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = 16 * rt + n;
-    if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], l[rt]};
+    if (r < cap && g == 0) sm[wave * cap + r] = float2{soft[rt].m, soft[rt].l};
   }
   __syncthreads();
 #pragma unroll
@@ -708,7 +736,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
     float top = -kInf;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
-    const float f = m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
+    const float f = soft[rt].m == top ? 1.f : __builtin_amdgcn_exp2f(soft[rt].m - top);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -744,6 +772,336 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
     const int t = by_group(a, row0 + r), gg = row0 + r - t * G;
     row_finish(s, t, sum, o);
     row_out<DT>(a, b, t, hk * G + gg, i0, o);
+  }
+}
+
+// Many rows (16 bit): a workgroup of four waves takes 128 rows, each wave 32 of them, and all walk the same keys, 64 at a time,
+// through LDS. Its threads read whole rows of the cache (a lane's own operand of a key, 16 bytes of each of 16 rows, costs
+// the first-level cache an access per lane: 54 of the 66 us of a chunk of 1024 rows that read its operands so),
+// 8-bit codes become 16-bit values once for all waves, and the values' operand is a transposed read. Two stages: the next
+// one is stored while this one is worked on, and the one behind it is on its way to registers.
+template <int DT, int FMT, int DP>
+__global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
+  constexpr int RT = 2, kWaves = 4, kRows = 16 * RT, NJ = DP / 16, kPieces = DP / 32, kHalves = DP / 64;
+  constexpr int kKeys = 64, kHalfTile = kKeys * 64, kTile = kHalves * kHalfTile;  // of 16-bit values
+  constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
+  // a thread's share of a stage: kLoads pieces of 16 bytes of keys and as many of values
+  constexpr int kElem = FMT == kCacheSame ? 2 : 1, kChunks = DP * kElem / 16, kLoads = kKeys * kChunks / 256;
+  static_assert(kLoads >= 1, "a stage gives every thread a piece");
+  __shared__ __attribute__((aligned(16))) uint16_t sk[2][kTile], sv[2][kTile];
+  __shared__ float s_ks[2][kKeys], s_vs[2][kKeys];
+  __shared__ int s_cleaned;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = xcd_logical_id(a.per_xcd);  // the blocks of a sequence's head, which read the same keys, on one XCD
+  if (id >= a.n_blocks) return;
+  const int rb = id % a.n_rb;
+  id /= a.n_rb;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int hk = id % a.c.n_heads, b = id / a.c.n_heads;
+  const Seq s = seq_of(a.c, b);
+  const int rows_all = a.c.T * a.G, first_row = rb * kWaves * kRows, row0 = first_row + wave * kRows, G = a.G;
+  const int base = s.len - s.n, len = s.len;
+  const bool tree = a.tree != nullptr;
+  auto rows_keys = [&](int r0, int r1, auto sh) {
+    const int t_lo = by_group(a, r0), t_end = by_group(a, r1);
+    return keys_of<decltype(sh)::value>(a, s, t_lo, t_end < s.n - 1 ? t_end : s.n - 1);
+  };
+  // of the workgroup, in stages, and of this wave
+  const Keys<6> keys = rows_keys(first_row, first_row + kWaves * kRows - 1, std::integral_constant<int, 6>{});
+  const Keys<5> mine = rows_keys(row0, row0 + kRows - 1, std::integral_constant<int, 5>{});
+  int tile0 = 0, tile1 = keys.n_tiles;
+  if (a.splits > 1) {
+    const int per = (keys.n_tiles + a.splits - 1u) / static_cast<unsigned>(a.splits);
+    tile0 = per * split < keys.n_tiles ? per * split : keys.n_tiles;
+    tile1 = tile0 + per < keys.n_tiles ? tile0 + per : keys.n_tiles;
+  }
+
+  // This thread's rows of a stage and its piece of them: threads in a row read a row's pieces one after the other.
+  const int piece = threadIdx.x % kChunks, my_row = threadIdx.x / kChunks;
+  constexpr int kRowStep = 256 / kChunks;
+  const int col = piece * (16 / kElem), pitch_b = a.c.pitch * kElem, page_mask = (1 << a.c.page_shift) - 1;
+  const uint32_t page_rows = static_cast<uint32_t>(a.c.n_heads) << a.c.page_shift;
+  const uint32_t head_rows = static_cast<uint32_t>(hk) << a.c.page_shift;
+  const int32_t* const table = a.c.table + b * a.c.table_stride;
+  const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
+  const int span_lo = keys.hi >= keys.lo ? keys.lo : kNowhere;
+  u32x4 rk[kLoads], rv[kLoads];
+  float r_ks = 0.f, r_vs = 0.f;
+  int page[kLoads], scale_page = 0;
+  bool seen[kLoads], bad[kLoads];
+  auto look_up = [&](int it) {
+    const int key0 = keys.first(it);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int key = key0 + my_row + u * kRowStep;
+      page[u] = key < len ? table[key >> a.c.page_shift] : -1;
+    }
+    if (FMT != kCacheSame && threadIdx.x < kKeys) {
+      const int key = key0 + static_cast<int>(threadIdx.x);
+      scale_page = key < len ? table[key >> a.c.page_shift] : -1;
+    }
+  };
+  auto load = [&](int it) {
+    const int key0 = keys.first(it);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int key = key0 + my_row + u * kRowStep;
+      const bool there = static_cast<uint32_t>(page[u]) < static_cast<uint32_t>(a.c.n_pages) && key < len;
+      seen[u] = there && ((key < keys.np) | in_span(key, span_lo, span));
+      bad[u] = !there && key < len;
+      rk[u] = rv[u] = u32x4{0, 0, 0, 0};
+      if (there && col < a.c.pitch) {
+        const int64_t off = (static_cast<int64_t>(page[u]) * page_rows + head_rows + (key & page_mask)) * pitch_b + piece * 16;
+        rk[u] = *reinterpret_cast<const u32x4*>(a.c.k + off);
+        rv[u] = *reinterpret_cast<const u32x4*>(a.c.v + off);
+      }
+    }
+    if (FMT != kCacheSame && threadIdx.x < kKeys) {
+      const int key = key0 + static_cast<int>(threadIdx.x);
+      r_ks = r_vs = 0.f;
+      if (static_cast<uint32_t>(scale_page) < static_cast<uint32_t>(a.c.n_pages) && key < len) {
+        const int64_t r = static_cast<int64_t>(scale_page) * page_rows + head_rows + (key & page_mask);
+        r_ks = a.c.ks[r];
+        if ((key < keys.np) | in_span(key, span_lo, span)) r_vs = a.c.vs[r];
+      } else if (key < len) {
+        r_ks = 1.f;  // NaN in the keys
+      }
+    }
+  };
+  auto store = [&](int it, int st) {
+    const bool part = !keys.all_see(keys.first(it));
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int r = my_row + u * kRowStep;
+      // values that no row sees may be anything: zeros. A page that is none: keys of NaN.
+      if (!seen[u]) rv[u] = u32x4{0, 0, 0, 0};
+      if constexpr (FMT == kCacheSame) {
+        if (part) {  // rows that do not see a value must not meet what is not finite: see below
+          uint32_t changed = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t y = finite_only<DT>(rv[u][w]);
+            changed |= y ^ rv[u][w];
+            rv[u][w] = y;
+          }
+          if (changed) s_cleaned = 1;
+        }
+        if (bad[u]) rk[u] = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+        const int to = (piece >> 3) * kHalfTile + swz64(r, piece & 7);
+        sts16(&sk[st][to], rk[u]);
+        sts16(&sv[st][to], rv[u]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 8 of the piece's 16 values
+          u32x4 x, y;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            x[2 * w] = code2<DT, FMT, false>(rk[u][2 * h + w]);
+            x[2 * w + 1] = code2<DT, FMT, true>(rk[u][2 * h + w]);
+            y[2 * w] = code2<DT, FMT, false>(rv[u][2 * h + w]);
+            y[2 * w + 1] = code2<DT, FMT, true>(rv[u][2 * h + w]);
+          }
+          if (bad[u]) x = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+          const int chunk = 2 * piece + h, to = (chunk >> 3) * kHalfTile + swz64(r, chunk & 7);
+          sts16(&sk[st][to], x);
+          sts16(&sv[st][to], y);
+        }
+      }
+    }
+    if (FMT != kCacheSame && threadIdx.x < kKeys) {
+      s_ks[st][threadIdx.x] = r_ks;
+      s_vs[st][threadIdx.x] = r_vs;
+    }
+  };
+
+  // the queries of this lane's rows, one of each 16: values 32 c + 8 g .. of piece c
+  Row row[RT];
+  u32x4 q[RT][kPieces];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + 16 * rt + n, t = by_group(a, r), gg = r - t * G;
+    const bool real = r < rows_all;
+    row[rt] = real && keys.n_tiles ? row_of(a, s, b, t) : no_row();
+    const uint8_t* const src = a.q + (b * a.qb + (hk * G + gg) * a.qh + t * a.qt) * 2;
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      const int i0 = 32 * c + 8 * g;
+      u32x4 w{0, 0, 0, 0};
+      if (a.q_vec) {
+        if (real && i0 < a.c.d) w = *reinterpret_cast<const u32x4*>(src + i0 * 2);
+      } else if (real) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          float y[1] = {0.f};
+          if (i0 + u < a.c.d) row_load<DT, 1>(src + (i0 + u) * 2, y);
+          x[u] = y[0] * a.q_sign;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = Mfma<DT>::pack2(x[2 * u], x[2 * u + 1]);
+      }
+      q[rt][c] = w;
+    }
+  }
+  f32x4 acc[RT][NJ];
+  Soft soft[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    soft[rt] = Soft{-kInf, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float v_ref = 0x1p-126f;
+
+  if (threadIdx.x == 0) s_cleaned = 0;
+  __syncthreads();
+  if (tile0 < tile1) {
+    look_up(tile0);
+    load(tile0);
+    if (tile0 + 1 < tile1) look_up(tile0 + 1);
+    store(tile0, 0);
+    if (tile0 + 1 < tile1) {
+      load(tile0 + 1);
+      if (tile0 + 2 < tile1) look_up(tile0 + 2);
+    }
+    __syncthreads();
+  }
+  for (int it = tile0; it < tile1; ++it) {
+    const int st = (it - tile0) & 1;
+    if (it + 1 < tile1) {
+      store(it + 1, st ^ 1);
+      if (it + 2 < tile1) {
+        load(it + 2);
+        if (it + 3 < tile1) look_up(it + 3);
+      }
+    }
+    const int stage0 = keys.first(it);
+#pragma unroll 1
+    for (int sub = 0; sub < kKeys; sub += 32) {
+      const int key0 = stage0 + sub;
+      if (!mine.any_sees(key0, 31)) continue;
+      float x[RT][8];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        f32x4 sc[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          const u32x4 key = lds16(&sk[st][(c >> 1) * kHalfTile + swz64(sub + 16 * hf + n, (4 * c + g) & 7)]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = mfma16<DT>(key, q[rt][c], sc[rt]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[rt][4 * hf + i] = sc[rt][i];
+      }
+      float vs[8];
+      if constexpr (FMT != kCacheSame) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&s_ks[st][sub + 16 * hf + 4 * g]);
+          const f32x4 z = *reinterpret_cast<const f32x4*>(&s_vs[st][sub + 16 * hf + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            vs[4 * hf + i] = z[i];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) x[rt][4 * hf + i] *= y[i];
+          }
+        }
+      }
+      const bool full = mine.all_see(key0);
+      uint32_t vis[RT];
+      if (!full) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          vis[rt] = row_sees(row[rt], key0 + 4 * g, base, tree);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
+        }
+      }
+      if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
+      u32x4 pw[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        soften(soft[rt], x[rt], acc[rt], a.scale2);
+        if constexpr (FMT != kCacheSame) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
+          if (!full) {  // 0 times a scale of NaN
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) pw[rt][w] = Mfma<DT>::pack2(x[rt][2 * w], x[rt][2 * w + 1]);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const u32x4 v = lds_read_tr4x2_swz64(&sv[st][(j >> 2) * kHalfTile], sub + 4 * g, sub + 16 + 4 * g, 16 * (j & 3), lane);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16<DT>(v, pw[rt], acc[rt][j]);
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (kScaled16) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[rt][j] *= v_ref;
+  }
+  if (FMT == kCacheSame && s_cleaned) {
+    // What was taken for zeros and is not finite, to the rows that see it.
+    for (int it = tile0; it < tile1; ++it) {
+      const int key0 = keys.first(it);
+      if (keys.all_see(key0)) continue;
+      for (int key = key0; key < key0 + kKeys && key < len; ++key) {
+        if (!((key < keys.np) | in_span(key, span_lo, span))) continue;
+        const int64_t r = cache_row(a.c, b, key, hk);
+        if (r < 0) continue;
+        const uint8_t* const vb = a.c.v + r * pitch_b;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = 16 * j + 4 * g + i;
+            float v[1] = {0.f};
+            if (c < a.c.d) row_load<DT, 1>(vb + c * 2, v);
+            if (__builtin_isfinite(v[0])) continue;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              if (sees(row[rt], key, base)) acc[rt][j][i] += v[0];
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    soft_join(soft[rt]);
+    const int r = row0 + 16 * rt + n;
+    if (r >= rows_all) continue;
+    const int t = by_group(a, r), gg = r - t * G;
+    const int64_t to = ((static_cast<int64_t>(b) * a.c.n_heads + hk) * a.splits + split) * rows_all + r;
+    float* const po = a.ws + to * (DP + 4);
+    if (a.splits > 1 && g == 0) {
+      po[DP] = soft[rt].m;
+      po[DP + 1] = soft[rt].l;
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      float o[4] = {acc[rt][j][0], acc[rt][j][1], acc[rt][j][2], acc[rt][j][3]};
+      if (a.splits > 1) {
+        *reinterpret_cast<f32x4*>(po + 16 * j + 4 * g) = f32x4{o[0], o[1], o[2], o[3]};
+      } else {
+        row_finish(s, t, soft[rt].l, o);
+        row_out<DT>(a, b, t, hk * G + gg, 16 * j + 4 * g, o);
+      }
+    }
   }
 }
 
@@ -833,7 +1191,10 @@ void launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const size_t lds = static_cast<size_t>(p.waves) * p.row_cap * (DP + 4 + 2) * 4;
   const dim3 grid(a.B, a.c.n_heads, p.n_rb * p.splits);
   if (p.rows) {
-    cached_attn_kernel<DT, FMT, DP, 2, 4, true><<<8 * a.per_xcd, 256, 0, s>>>(a);
+    if constexpr (DT == TMAC_F32)
+      cached_attn_kernel<DT, FMT, DP, 2, 4, true><<<8 * a.per_xcd, 256, 0, s>>>(a);
+    else
+      cached_attn_rows_kernel<DT, FMT, DP><<<8 * a.per_xcd, 256, 0, s>>>(a);
   } else if (p.rt == 2) {
     constexpr int kWaves = DT == TMAC_F32 && DP == 128 ? 4 : 8;
     cached_attn_kernel<DT, FMT, DP, 2, kWaves, false><<<grid, 64 * kWaves, lds, s>>>(a);
