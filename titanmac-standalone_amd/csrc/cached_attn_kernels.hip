@@ -1166,7 +1166,10 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     p.row_cap = rows < cap ? rows : cap;
     const int64_t blocks = heads * p.n_rb;
     p.waves = dtype == TMAC_F32 && dp == 128 ? 4 : 8;  // 512 registers for wide fp32 rows
-    if (p.rt == 1 && (tiles <= 4 || (blocks >= 512 && tiles <= 24))) p.waves = 4;
+    // Half as many where the workgroups are many already and the tiles few. Eight waves with 32 rows fill a CU's
+    // registers alone: 320 such blocks of 19 tiles 21.6 us, with four waves 16.7; 20 blocks 10.6 and 11.5. With 16
+    // rows: 640 blocks of 17 tiles 16.6 and 14.3, of 33 tiles 34 and 37.
+    if (tiles <= 4 || (p.rt == 2 ? blocks > 256 : blocks >= 512 && tiles <= 24)) p.waves = 4;
     // enough workgroups for every CU, each wave with 4 tiles at least
     s = (512 + blocks - 1) / blocks;
     if (s > tiles / (4 * p.waves)) s = tiles / (4 * p.waves);
@@ -1196,8 +1199,10 @@ void launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     else
       cached_attn_rows_kernel<DT, FMT, DP><<<8 * a.per_xcd, 256, 0, s>>>(a);
   } else if (p.rt == 2) {
-    constexpr int kWaves = DT == TMAC_F32 && DP == 128 ? 4 : 8;
-    cached_attn_kernel<DT, FMT, DP, 2, kWaves, false><<<grid, 64 * kWaves, lds, s>>>(a);
+    if constexpr (!(DT == TMAC_F32 && DP == 128)) {
+      if (p.waves == 8) cached_attn_kernel<DT, FMT, DP, 2, 8, false><<<grid, 64 * 8, lds, s>>>(a);
+    }
+    if (p.waves == 4) cached_attn_kernel<DT, FMT, DP, 2, 4, false><<<grid, 64 * 4, lds, s>>>(a);
   } else if (p.waves == 4) {
     cached_attn_kernel<DT, FMT, DP, 1, 4, false><<<grid, 64 * 4, lds, s>>>(a);
   } else if constexpr (!(DT == TMAC_F32 && DP == 128)) {
