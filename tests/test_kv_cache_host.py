@@ -229,3 +229,50 @@ def test_argument_errors(lib):
         assert attn(c_arg(**long), t=1, w=1 << 30, **kw) == want
     # the window bounds what a row sees, and with it the workspace
     assert size(c_arg(**long), t=1, w=500) == 0 and n.value == 0
+
+
+def config(**kw):
+    return tc.TitanMACConfig(**{**dict(vocab_size=20, d_model=32, n_heads=2, n_layers=1, d_ff=32, max_seq_len=16,
+                                       n_persistent=0, window_size=4, use_block_sparse=False), **kw})
+
+
+def test_decoding_refusals():
+    for kw, text in (({"use_block_sparse": True}, "use_block_sparse"), ({"causal": False}, "causal"),
+                     ({"use_neural_memory": True}, "neural memory")):
+        with pytest.raises(ValueError, match=text):
+            tc.TitanMAC(config(**kw)).new_decode_state(1)
+    m = tc.TitanMAC(config()).eval()
+    for args in ((0,), (1, 0), (1, 17)):
+        with pytest.raises(ValueError, match="max_tokens"):
+            m.new_decode_state(*args)
+    with pytest.raises(ValueError, match="fmt"):
+        m.new_decode_state(1, fmt="int4")
+    state = m.new_decode_state(2, 10)
+    ids = torch.zeros(2, 11, dtype=torch.long)
+    with pytest.raises(ValueError, match="do not fit"):
+        m.decode(ids, state)
+    assert state.used == 0 and state.lengths.tolist() == [0, 0]
+    with pytest.raises(ValueError, match="2 sequences"):
+        m.decode(ids[:1], state)
+    for bad in (torch.ones(2), torch.ones(3, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="counts"):
+            m.decode(ids[:, :3], state, counts=bad)
+    for bad in (torch.ones(3), torch.ones(2, 2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="tree"):
+            m.decode(ids[:, :3], state, tree=bad)
+    with pytest.raises(RuntimeError, match="no draft"):
+        state.keep(torch.zeros(2, 1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="GPU"):
+        m.decode(ids[:, :3], state)
+    state = m.new_decode_state(2, 10)
+    assert m.decode(ids[:, :0], state).shape == (2, 0, 20)
+    with pytest.raises(ValueError, match="generate"):
+        m.generate(ids[:, :0], 3)
+    c, t, n = state.caches[0], state.table, state.lengths
+    for attention, text in ((tc.WindowedAttention(config(attention_dropout=0.1)).train(), "dropout"),
+                            (tc.WindowedAttention(config(causal=False)), "causal")):
+        with pytest.raises(ValueError, match=text):
+            attention.forward_cached(torch.zeros(2, 1, 32), c, t, n)
+    block = tc.TitanBlock(config(use_block_sparse=True))
+    with pytest.raises(ValueError, match="use_block_sparse"):
+        block.forward_cached(torch.zeros(1, 1, 32), None, None, None)

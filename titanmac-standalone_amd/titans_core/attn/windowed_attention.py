@@ -21,8 +21,9 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
+from ..kernels.kv_cache import KVCache, cache_write, cached_attention
 from ..kernels.linear import Projection
-from ..kernels.window_attn import windowed_attention_qkv
+from ..kernels.window_attn import _split_heads, windowed_attention_qkv
 
 
 @dataclass
@@ -129,3 +130,18 @@ class WindowedAttention(nn.Module):
         out = windowed_attention_qkv(qkv, self.n_heads, self.window_size, self.num_persistent, self.causal,
                                      attn_mask=attn_mask, dropout_p=p)
         return self.dropout(self.out_proj(out))
+
+    def forward_cached(self, x: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, *,
+                       counts: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward of the new rows x [B, T, d_model] behind those that the cache holds, which take theirs in: the rows
+        of forward over the whole text, to rounding (and to the cache's own). table, lengths, counts and tree as in
+        ``cached_attention``. Causal attention without dropout only, no gradient."""
+        if not self.causal:
+            raise ValueError("forward_cached: rows of attention that is not causal change with what follows them")
+        if self.training and self.dropout_p > 0:
+            raise ValueError("forward_cached: no dropout; call eval() first")
+        B, T, D = x.shape
+        q, k, v = _split_heads(self.qkv_proj(x), self.n_heads)
+        cache_write(k, v, cache, table, lengths, counts=counts)
+        out = cached_attention(q, cache, table, lengths, self.window_size, self.num_persistent, counts=counts, tree=tree)
+        return self.out_proj(out.transpose(1, 2).reshape(B, T, D))

@@ -49,3 +49,11 @@ class TitanBlock(nn.Module):
     def forward(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         x = x + self.attention(self.norm_attn(x), attn_mask=attn_mask)
         return x + self.mlp(self.norm_mlp(x))
+
+    def forward_cached(self, x: torch.Tensor, cache, table, lengths, **kw) -> torch.Tensor:
+        """forward of new rows behind those that the cache holds (``WindowedAttention.forward_cached``)."""
+        if not isinstance(self.attention, WindowedAttention):
+            raise ValueError("forward_cached: BlockSparseAttention's persistent rows see every key and change with every "
+                             "token; build the block with use_block_sparse=False")
+        x = x + self.attention.forward_cached(self.norm_attn(x), cache, table, lengths, **kw)
+        return x + self.mlp(self.norm_mlp(x))

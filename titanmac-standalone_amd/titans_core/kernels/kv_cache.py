@@ -40,7 +40,6 @@ _NO_WINDOW = 1 << 30
 _CACHE_ARG = struct.Struct("7Q2q7i4x").pack
 _STRIDES = struct.Struct("3q").pack
 _DTYPE = _lib._DTYPE_CODE
-_ptr = _lib.ptr
 
 
 class KVCache(tuple):
@@ -89,7 +88,8 @@ class KVCache(tuple):
                                 "float8_e4m3fn")
             k_scale = v_scale = None
             changing = (k, v)
-        return tuple.__new__(cls, (k, v, k_scale, v_scale, d, fmt, heads, shape, device, changing))
+        return tuple.__new__(cls, (k, v, k_scale, v_scale, d, fmt, heads, shape, device, changing,
+                                   dtype if fmt == SAME else None, (1 << 30) // page))
 
     def __getnewargs__(self):
         return self.k, self.v, self.d_head, self.k_scale, self.v_scale
@@ -116,35 +116,39 @@ class KVCache(tuple):
                    d_head, scale(), scale())
 
 
-def _check(what: str, cache: KVCache, table, lengths, counts, dtype: torch.dtype, T: int, B: int) -> None:
-    """The sequences' description, and whether the cache holds values of dtype."""
-    k, _, _, _, _, fmt, heads, shape, _, _ = cache
-    if dtype not in _DTYPE:
-        raise TypeError(f"{what}: unsupported dtype {dtype}; expected float32, bfloat16 or float16")
-    if fmt == SAME and k.dtype != dtype:
-        raise TypeError(f"{what}: a cache of {k.dtype} does not hold {dtype}")
-    i32 = torch.int32
-    if table.dtype != i32 or lengths.dtype != i32 or (counts is not None and counts.dtype != i32):
+def _sequences(what: str, cache: KVCache, table, lengths, counts, dtype: torch.dtype, T: int, B: int):
+    """(table, its pitch, lengths, counts) as the kernels read them, of sequences whose description is in order and whose
+    values the cache holds."""
+    held, i32 = cache[10], torch.int32
+    if held is not dtype and (held is not None or dtype not in _DTYPE):
+        if dtype not in _DTYPE:
+            raise TypeError(f"{what}: unsupported dtype {dtype}; expected float32, bfloat16 or float16")
+        raise TypeError(f"{what}: a cache of {held} does not hold {dtype}")
+    if not (table.dtype is i32 and lengths.dtype is i32 and (counts is None or counts.dtype is i32)):
         raise TypeError(f"{what}: table, lengths and counts must be int32")
-    at = table.shape
+    at, n = table.shape, lengths.shape
     if len(at) != 2 or at[0] != B or at[1] == 0:
-        raise ValueError(f"{what}: table must be [{B}, pages], got {tuple(table.shape)}")
-    if lengths.dim() != 1 or lengths.shape[0] != B:
-        raise ValueError(f"{what}: lengths must be [{B}], got {tuple(lengths.shape)}")
-    if counts is not None and (counts.dim() != 1 or counts.shape[0] != B):
-        raise ValueError(f"{what}: counts must be [{B}], got {tuple(counts.shape)}")
-    if B > 1 << 20 or T * heads > 1 << 26 or at[1] > (1 << 30) // shape[2]:
+        raise ValueError(f"{what}: table must be [{B}, pages], got {tuple(at)}")
+    if len(n) != 1 or n[0] != B:
+        raise ValueError(f"{what}: lengths must be [{B}], got {tuple(n)}")
+    if counts is not None:
+        if counts.shape != n:
+            raise ValueError(f"{what}: counts must be [{B}], got {tuple(counts.shape)}")
+        if not counts.is_contiguous():
+            counts = counts.contiguous()
+    if B > 1 << 20 or T * cache[6] > 1 << 26 or at[1] > cache[11]:
         raise ValueError(f"{what}: up to 2^20 sequences, 2^26 rows of one and 2^30 positions")
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    pitch, step = table.stride()
+    if step != 1 or pitch < at[1]:
+        table, pitch = _rows(table)
+    return table, pitch, lengths, counts
 
 
 def _refuse_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad()")
-
-
-def _unit(t: torch.Tensor) -> torch.Tensor:
-    """t with its last dimension contiguous."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _rows(t: torch.Tensor):
@@ -178,14 +182,10 @@ def _run(what: str, device: torch.device, tensors, name: str, *args) -> None:
 
 def _arg(cache: KVCache, table, pitch: int, lengths, counts, dtype: torch.dtype) -> bytes:
     """tmac_cache."""
-    k, v, ks, vs, d, fmt, heads, shape, _, _ = cache
+    k, v, ks, vs, d, fmt, heads, shape = cache[:8]
     return _CACHE_ARG(k.data_ptr(), v.data_ptr(), 0 if ks is None else ks.data_ptr(), 0 if vs is None else vs.data_ptr(),
                       table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(), shape[0], pitch,
                       heads, shape[2], shape[3], d, table.shape[1], fmt, _DTYPE[dtype])
-
-
-def _flat(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _changed(cache: KVCache) -> None:
@@ -198,22 +198,26 @@ def _changed(cache: KVCache) -> None:
 
 # ------------------------------------------------------------------ write
 
-def _native_write(k, v, cache, table, lengths, counts) -> None:
-    B, H, T, d = k.shape
+def _native_write(k, v, cache, table, pitch, lengths, counts) -> None:
+    B, _, T, d = k.shape
     if B * T == 0:
         return
-    k, v, lengths, counts = _unit(k), _unit(v), _flat(lengths), _flat(counts)
-    table, pitch = _rows(table)
+    at_k, at_v = k.stride(), v.stride()
+    if (at_k[3] != 1 or at_v[3] != 1) and d > 1:
+        k, v = k.contiguous(), v.contiguous()
+        at_k, at_v = k.stride(), v.stride()
     _run("cache_write", cache[8], (k, v, table, lengths, counts), "tmac_cache_write",
-         _arg(cache, table, pitch, lengths, counts, k.dtype), k.data_ptr(), _STRIDES(*k.stride()[:3]), v.data_ptr(),
-         _STRIDES(*v.stride()[:3]), B, T)
+         _arg(cache, table, pitch, lengths, counts, k.dtype), k.data_ptr(), _STRIDES(*at_k[:3]), v.data_ptr(),
+         _STRIDES(*at_v[:3]), B, T)
 
 
 @torch.library.custom_op("titanmac::cache_write", mutates_args=("k", "v", "ks", "vs"))
 def cache_write_op(new_k: torch.Tensor, new_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                    ks: Optional[torch.Tensor], vs: Optional[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor,
                    counts: Optional[torch.Tensor], d: int) -> None:
-    _native_write(new_k, new_v, KVCache(k, v, d, ks, vs), table, lengths, counts)
+    cache = KVCache(k, v, d, ks, vs)
+    _native_write(new_k, new_v, cache, *_sequences("cache_write", cache, table, lengths, counts, new_k.dtype,
+                                                   new_k.shape[2], new_k.shape[0]))
 
 
 @cache_write_op.register_fake
@@ -228,15 +232,16 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.T
     In 8 bits every row has its own scale: int8 codes are value / scale rounded to nearest (ties to even) with scale =
     max |value| / 127, e4m3 codes likewise with the least power of two that holds the row as scale (both at least
     2^-126). A row that is not finite is held as NaN. Pages that are written must not belong to two sequences."""
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"cache_write: k and v must be [B, n_heads, T, d_head], alike, got {tuple(k.shape)} {k.dtype} "
-                         f"and {tuple(v.shape)} {v.dtype}")
-    B, H, T, d = k.shape
-    _check("cache_write", cache, table, lengths, counts, k.dtype, T, B)
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.shape != shape or v.dtype is not dtype:
+        raise ValueError(f"cache_write: k and v must be [B, n_heads, T, d_head], alike, got {tuple(shape)} {dtype} and "
+                         f"{tuple(v.shape)} {v.dtype}")
+    B, H, T, d = shape
+    table, pitch, lengths, counts = _sequences("cache_write", cache, table, lengths, counts, dtype, T, B)
     if H != cache[6] or d != cache[4]:
-        raise ValueError(f"cache_write: the cache has {cache[6]} heads of {cache[4]}, k is {tuple(k.shape)}")
+        raise ValueError(f"cache_write: the cache has {cache[6]} heads of {cache[4]}, k is {tuple(shape)}")
     if _lib.direct_call(k, v, table, lengths, counts, *cache[9]):
-        _native_write(k, v, cache, table, lengths, counts)
+        _native_write(k, v, cache, table, pitch, lengths, counts)
         _changed(cache)
     else:
         _refuse_grad("cache_write", k, v, cache[0], cache[1])
@@ -245,13 +250,11 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.T
 
 # ------------------------------------------------------------------ read
 
-def _native_read(cache, table, lengths, T, dtype):
-    B, H, d, device = table.shape[0], cache[6], cache[4], cache[8]
+def _native_read(cache, table, pitch, lengths, T, dtype):
+    B, H, d, device = lengths.shape[0], cache[6], cache[4], cache[8]
     k = torch.empty((B, H, T, d), dtype=dtype, device=device)
     v = torch.empty((B, H, T, d), dtype=dtype, device=device)
     if B * T:
-        lengths = _flat(lengths)
-        table, pitch = _rows(table)
         _run("cache_read", device, (table, lengths), "tmac_cache_read", _arg(cache, table, pitch, lengths, None, dtype),
              k.data_ptr(), v.data_ptr(), B, T)
     return k, v
@@ -261,7 +264,9 @@ def _native_read(cache, table, lengths, T, dtype):
 def cache_read_op(k: torch.Tensor, v: torch.Tensor, ks: Optional[torch.Tensor], vs: Optional[torch.Tensor],
                   table: torch.Tensor, lengths: torch.Tensor, T: int, d: int,
                   dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    return _native_read(KVCache(k, v, d, ks, vs), table, lengths, T, dtype)
+    cache = KVCache(k, v, d, ks, vs)
+    table, pitch, lengths, _ = _sequences("cache_read", cache, table, lengths, None, dtype, T, lengths.shape[0])
+    return _native_read(cache, table, pitch, lengths, T, dtype)
 
 
 @cache_read_op.register_fake
@@ -274,37 +279,39 @@ def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, n_pos
     """Positions 0 .. n_positions − 1 of every sequence as k, v [B, n_heads, n_positions, d_head]: zeros behind a
     sequence's length. dtype: the values' type (default: the cache's, bfloat16 for one in 8 bits)."""
     if dtype is None:
-        dtype = torch.bfloat16 if cache[5] else cache[0].dtype
+        dtype = cache[10] or torch.bfloat16
     T = int(n_positions)
     if T < 0:
         raise ValueError(f"cache_read: n_positions must not be negative, got {T}")
-    _check("cache_read", cache, table, lengths, None, dtype, T, lengths.shape[0] if lengths.dim() == 1 else -1)
+    table, pitch, lengths, _ = _sequences("cache_read", cache, table, lengths, None, dtype, T,
+                                          lengths.shape[0] if lengths.dim() == 1 else -1)
     if _lib.direct_call(table, lengths, *cache[9]):
-        return _native_read(cache, table, lengths, T, dtype)
+        return _native_read(cache, table, pitch, lengths, T, dtype)
     _refuse_grad("cache_read", cache[0], cache[1])
     return cache_read_op(*cache[:4], table, lengths, T, cache[4], dtype)
 
 
 # ------------------------------------------------------------------ keep
 
-def _native_keep(cache, table, lengths, counts, path, T) -> None:
+def _native_keep(cache, table, pitch, lengths, counts, path, T) -> None:
     B, A = path.shape
     if B == 0 or A == 0:
         return
-    lengths, counts = _flat(lengths), _flat(counts)
-    table, pitch = _rows(table)
-    path, path_pitch = _rows(path)
+    path_pitch, step = path.stride()
+    if step != 1 or path_pitch < A:
+        path, path_pitch = _rows(path)
     # 8-bit rows are moved as they are, whatever the type of the values
     _run("cache_keep", cache[8], (table, lengths, counts, path), "tmac_cache_keep",
-         _arg(cache, table, pitch, lengths, counts, torch.bfloat16 if cache[5] else cache[0].dtype), path.data_ptr(),
-         path_pitch, A, B, T)
+         _arg(cache, table, pitch, lengths, counts, cache[10] or torch.bfloat16), path.data_ptr(), path_pitch, A, B, T)
 
 
 @torch.library.custom_op("titanmac::cache_keep", mutates_args=("k", "v", "ks", "vs"))
 def cache_keep_op(k: torch.Tensor, v: torch.Tensor, ks: Optional[torch.Tensor], vs: Optional[torch.Tensor],
                   table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor], path: torch.Tensor, T: int,
                   d: int) -> None:
-    _native_keep(KVCache(k, v, d, ks, vs), table, lengths, counts, path, T)
+    cache = KVCache(k, v, d, ks, vs)
+    _native_keep(cache, *_sequences("cache_keep", cache, table, lengths, counts, cache[10] or torch.bfloat16, T,
+                                    path.shape[0]), path, T)
 
 
 @cache_keep_op.register_fake
@@ -319,16 +326,17 @@ def cache_keep(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, path:
     it is. The caller then shortens ``lengths`` to the rows that were kept."""
     n = counts if isinstance(counts, torch.Tensor) else None
     T = MAX_TREE if n is not None else int(counts)
-    if path.dim() != 2 or path.dtype != torch.int32:
+    at = path.shape
+    if len(at) != 2 or path.dtype is not torch.int32:
         raise ValueError(f"cache_keep: path must be int32 [B, rows], got {path.dtype} {tuple(path.shape)}")
-    if not 0 <= T <= MAX_TREE or path.shape[1] > T:
+    if not 0 <= T <= MAX_TREE or at[1] > T:
         raise ValueError(f"cache_keep: drafts of up to {MAX_TREE} rows, no more kept than drafted, got {T} and "
                          f"{path.shape[1]}")
-    if path.shape[0] > 32767:
-        raise ValueError(f"cache_keep: up to 32767 sequences, got {path.shape[0]}")
-    _check("cache_keep", cache, table, lengths, n, torch.bfloat16 if cache[5] else cache[0].dtype, T, path.shape[0])
+    if at[0] > 32767:
+        raise ValueError(f"cache_keep: up to 32767 sequences, got {at[0]}")
+    table, pitch, lengths, n = _sequences("cache_keep", cache, table, lengths, n, cache[10] or torch.bfloat16, T, at[0])
     if _lib.direct_call(table, lengths, n, path, *cache[9]):
-        _native_keep(cache, table, lengths, n, path, T)
+        _native_keep(cache, table, pitch, lengths, n, path, T)
         _changed(cache)
     else:
         _refuse_grad("cache_keep", cache[0], cache[1])
@@ -347,28 +355,31 @@ def _workspace(heads, page, d, max_pages, fmt, dtype, B, T, Hq, window, n_persis
     return nb.value
 
 
-def _native_attn(q, cache, table, lengths, counts, tree, window, n_persistent, scale):
+def _native_attn(q, cache, table, pitch, lengths, counts, tree, window, n_persistent, scale):
     """[B, H, T, d], a view of [B, T, H, d]."""
-    _, _, _, _, d, fmt, heads, shape, device, _ = cache
-    B, H, T, _ = q.shape
-    dtype = q.dtype
+    B, H, T, d = q.shape
+    dtype, device = q.dtype, cache[8]
     out = torch.empty_strided((B, H, T, d), (T * H * d, d, H * d, 1), dtype=dtype, device=device)
     if B * T == 0:
         return out
-    q, lengths, counts = _unit(q), _flat(lengths), _flat(counts)
-    table, pitch = _rows(table)
-    tree_stride = 0
+    at_q = q.stride()
+    if at_q[3] != 1 and d > 1:
+        q = q.contiguous()
+        at_q = q.stride()
+    tree_stride = tree_ptr = 0
     if tree is not None:
         if tree.dim() == 1:
-            tree = _unit(tree)
+            tree = tree.contiguous()
         else:
-            tree, tree_stride = _rows(tree)
-    nb = _workspace(heads, shape[2], d, table.shape[1], fmt, _DTYPE[dtype], B, T, H, window, n_persistent)
+            tree_stride, step = tree.stride()
+            if step != 1 or tree_stride < T:
+                tree, tree_stride = _rows(tree)
+        tree_ptr = tree.data_ptr()
+    nb = _workspace(cache[6], cache[7][2], d, table.shape[1], cache[5], _DTYPE[dtype], B, T, H, window, n_persistent)
     ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
     _run("cached_attention", device, (q, table, lengths, counts, tree), "tmac_cached_attn",
-         _arg(cache, table, pitch, lengths, counts, dtype), q.data_ptr(), _STRIDES(*q.stride()[:3]),
-         0 if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), _ptr(ws), nb, B, T, H, window, n_persistent,
-         scale)
+         _arg(cache, table, pitch, lengths, counts, dtype), q.data_ptr(), _STRIDES(*at_q[:3]), tree_ptr, tree_stride,
+         out.data_ptr(), 0 if ws is None else ws.data_ptr(), nb, B, T, H, window, n_persistent, scale)
     return out
 
 
@@ -377,7 +388,9 @@ def cached_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ks: O
                         vs: Optional[torch.Tensor], table: torch.Tensor, lengths: torch.Tensor,
                         counts: Optional[torch.Tensor], tree: Optional[torch.Tensor], window: int, n_persistent: int,
                         scale: float, d: int) -> torch.Tensor:
-    return _native_attn(q, KVCache(k, v, d, ks, vs), table, lengths, counts, tree, window, n_persistent, scale)
+    cache = KVCache(k, v, d, ks, vs)
+    return _native_attn(q, cache, *_sequences("cached_attention", cache, table, lengths, counts, q.dtype, q.shape[2],
+                                              q.shape[0]), tree, window, n_persistent, scale)
 
 
 @cached_attention_op.register_fake
@@ -404,10 +417,11 @@ def cached_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengt
     What a row does not see never reaches its result, whatever is stored there. Scores, sums and the accumulation are in
     fp32; in 16 bit the probabilities are rounded to q's type before they meet the values. scale defaults to
     1/sqrt(d_head). No gradient."""
-    if q.dim() != 4:
-        raise ValueError(f"cached_attention: q must be [B, H, T, d_head], got {tuple(q.shape)}")
-    B, H, T, d = q.shape
-    _check("cached_attention", cache, table, lengths, counts, q.dtype, T, B)
+    shape = q.shape
+    if len(shape) != 4:
+        raise ValueError(f"cached_attention: q must be [B, H, T, d_head], got {tuple(shape)}")
+    B, H, T, d = shape
+    table, pitch, lengths, counts = _sequences("cached_attention", cache, table, lengths, counts, q.dtype, T, B)
     if d != cache[4] or H == 0 or H % cache[6]:
         raise ValueError(f"cached_attention: the cache has {cache[6]} heads of {cache[4]}, q is {tuple(q.shape)}")
     if B * H * T > 1 << 26:
@@ -425,6 +439,6 @@ def cached_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengt
             raise ValueError(f"cached_attention: a draft has up to {MAX_TREE} rows, got {T}")
     scale = d ** -0.5 if scale is None else float(scale)
     if _lib.direct_call(q, table, lengths, counts, tree, *cache[9]):
-        return _native_attn(q, cache, table, lengths, counts, tree, window, n_persistent, scale)
+        return _native_attn(q, cache, table, pitch, lengths, counts, tree, window, n_persistent, scale)
     _refuse_grad("cached_attention", q, cache[0], cache[1])
     return cached_attention_op(q, *cache[:4], table, lengths, counts, tree, window, n_persistent, scale, d)

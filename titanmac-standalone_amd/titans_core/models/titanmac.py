@@ -16,7 +16,8 @@ Every block op runs on the HIP kernels (RMSNorm, depthwise conv, tile-sparse att
 Block-ELL MLP when configured), the neural memory's update on its HIP step, the embeddings and the
 loss on theirs (``token_embedding``, ``token_cross_entropy``), and the dense projections and the LM
 head on hipBLASLt. ``score``, which the reference lacks, gives each token's log probability without
-storing the logits.
+storing the logits; ``decode`` and ``generate``, which it lacks too, answer token by token from a cache of
+keys and values (``models/decoding.py``).
 
 One change of schedule, not of result: when the memory is read-only (eval mode without
 ``enable_test_time_memory``), ``forward_mac``'s segments do not depend on each other. The
@@ -40,8 +41,11 @@ from ..blocks.titan_block import TitanBlock
 from ..config import TitanMACConfig
 from ..kernels import _lib
 from ..kernels.embedding import token_embedding
+from ..kernels.kv_cache import MAX_TREE, KVCache
 from ..kernels.logprobs import head_logprobs, token_cross_entropy, token_logprobs
+from ..attn.windowed_attention import WindowedAttention
 from ..memory.neural_memory import NeuralMemory
+from .decoding import DecodeState, draft_depths
 
 
 _IGNORE = -100  # F.cross_entropy's ignore_index
@@ -415,6 +419,99 @@ class TitanMAC(nn.Module):
         out = {n: t for n, t in r._asdict().items() if t is not None}
         if memory_loss is not None:
             out["memory_loss"] = memory_loss
+        return out
+
+    # ------------------------------------------------------------------ decoding
+
+    def new_decode_state(self, batch: int, max_tokens: Optional[int] = None, *, fmt: Optional[str] = None,
+                         page: int = 64) -> DecodeState:
+        """Empty caches for ``batch`` sequences of up to max_tokens (default: max_seq_len) tokens, with the persistent rows
+        already in them. fmt: None holds keys and values in the model's type, "int8" and "e4m3" in 8 bits with a
+        scale per row (``KVCache``). For models of causal WindowedAttention (use_block_sparse=False) without a neural
+        memory."""
+        cfg = self.config
+        if self.neural_memory is not None:
+            raise ValueError("new_decode_state: a neural memory's tokens depend on whole segments; there is no cache of it")
+        for layer in self.layers:
+            if not isinstance(layer.attention, WindowedAttention) or not layer.attention.causal:
+                raise ValueError("new_decode_state: the layers must be causal WindowedAttention (use_block_sparse=False)")
+        room = cfg.max_seq_len if max_tokens is None else int(max_tokens)
+        if batch < 1 or not 1 <= room <= cfg.max_seq_len:
+            raise ValueError(f"new_decode_state: batch must be positive and max_tokens 1..{cfg.max_seq_len}, got {batch}, "
+                             f"{room}")
+        w, Np = self.embed_tokens.weight, self._n_persistent()
+        per = -(-(Np + room) // page)
+        caches = [KVCache.new(batch * per, cfg.n_heads, cfg.d_head, page=page, dtype=w.dtype, fmt=fmt, device=w.device)
+                  for _ in self.layers]
+        table = torch.arange(batch * per, dtype=torch.int32, device=w.device).view(batch, per)
+        state = DecodeState(caches, table, torch.full((batch,), Np, dtype=torch.int32, device=w.device), Np, room)
+        if Np:
+            with torch.no_grad():
+                x = self.persistent_tokens.unsqueeze(0).expand(batch, -1, -1)
+                for layer, cache in zip(self.layers, caches):
+                    x = layer.forward_cached(x, cache, table, state.lengths)
+        return state
+
+    @torch.no_grad()
+    def decode(self, input_ids: torch.Tensor, state: DecodeState, *, counts: Optional[torch.Tensor] = None,
+               tree: Optional[torch.Tensor] = None, last: bool = False) -> torch.Tensor:
+        """Logits [B, T, vocab] of tokens that follow those which ``state`` holds, and which it then holds too: forward's
+        rows for them, to rounding. Any T: a prompt, a part of one, single tokens. last: only of each sequence's last new
+        token, [B, 1, vocab].
+
+        counts (int32 [B]): how many of the T are tokens; the rest is padding, whose logits say nothing. tree (int64
+        [B, T] or [T], T up to 64): the tokens are a draft, as in ``cached_attention``; ``state.keep`` then says
+        which of them stay. Hooks of the blocks and their attention are not run."""
+        B, T = input_ids.shape
+        if B != state.lengths.shape[0]:
+            raise ValueError(f"decode: the state has {state.lengths.shape[0]} sequences, input_ids is "
+                             f"{tuple(input_ids.shape)}")
+        if T == 0:
+            return self.lm_head.weight.new_empty((B, 0, self.config.vocab_size))
+        if counts is not None and (counts.shape != (B,) or counts.dtype != torch.int32):
+            raise ValueError(f"decode: counts must be int32 [{B}], got {counts.dtype} {tuple(counts.shape)}")
+        if tree is not None and (T > MAX_TREE or tree.dtype != torch.int64 or tuple(tree.shape) not in ((B, T), (T,))):
+            raise ValueError(f"decode: tree must be int64 [{B}, {T}] or [{T}], T up to {MAX_TREE}, got {tree.dtype} "
+                             f"{tuple(tree.shape)}")
+        place = torch.arange(T, device=input_ids.device) if tree is None else draft_depths(tree)
+        positions = (state.lengths - state.n_persistent).unsqueeze(1) + place
+        state._advance(T, counts, tree is not None)
+        x = self._embed_at(input_ids, positions)
+        for layer, cache in zip(self.layers, state.caches):
+            x = layer.forward_cached(x, cache, state.table, state.lengths, counts=counts, tree=tree)
+        if last:
+            if counts is None:
+                x = x[:, -1:]
+            else:
+                at = (counts.long() - 1).clamp(min=0)
+                x = x.gather(1, at.view(B, 1, 1).expand(B, 1, x.shape[-1]))
+        return self.lm_head(self.norm(x))
+
+    def _embed_at(self, input_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        """Token plus position rows [B, T, d] at given positions; padding may be past the table's last."""
+        tok, pos = self.embed_tokens, self.embed_positions
+        if (_plain_lookup(tok) and _plain_lookup(pos) and input_ids.dtype in (torch.int64, torch.int32)
+                and tok.weight.is_cuda and _lib.eager_native(input_ids, tok.weight, pos.weight)):
+            return token_embedding(input_ids, tok.weight, pos.weight, positions=positions)
+        return tok(input_ids) + pos(positions.clamp(0, pos.num_embeddings - 1))
+
+    @torch.no_grad()
+    def generate(self, input_ids: torch.Tensor, n_tokens: int, *, counts: Optional[torch.Tensor] = None,
+                 fmt: Optional[str] = None) -> torch.Tensor:
+        """The n_tokens [B, n_tokens] that follow the prompts input_ids [B, T] if each is the likeliest (ties: the lower
+        id). counts (int32 [B]): the prompts' lengths; fmt: how keys and values are held (``new_decode_state``)."""
+        B, T = input_ids.shape
+        if T < 1 or n_tokens < 0:
+            raise ValueError(f"generate: needs prompts and n_tokens >= 0, got {tuple(input_ids.shape)}, {n_tokens}")
+        out = torch.empty((B, n_tokens), dtype=torch.int64, device=input_ids.device)
+        if n_tokens == 0:
+            return out
+        state = self.new_decode_state(B, T + n_tokens - 1, fmt=fmt)
+        logits = self.decode(input_ids, state, counts=counts, last=True)
+        for i in range(n_tokens):
+            out[:, i] = logits[:, 0].argmax(-1)
+            if i + 1 < n_tokens:
+                logits = self.decode(out[:, i:i + 1], state, last=True)
         return out
 
     # ------------------------------------------------------------------ utilities
