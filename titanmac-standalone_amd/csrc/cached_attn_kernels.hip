@@ -1105,7 +1105,9 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
   }
 }
 
-// The parts of a row: one group of DP / N lanes joins them in order.
+// The parts of a row, joined in their order. Up to kFewParts of them: DP / 4 threads a row, four parts' loads in flight.
+constexpr int kFewParts = 8, kMostParts = 64;
+
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void cached_attn_join_kernel(AttnArgs a) {
   constexpr int N = 4, L = DP / N;
@@ -1119,17 +1121,75 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(AttnArgs a) {
   const int b = static_cast<int>(bh / a.c.n_heads), hk = static_cast<int>(bh % a.c.n_heads);
   const float* const p0 = a.ws + (bh * a.splits * rows_all + r) * (DP + 4);
   const int64_t step = static_cast<int64_t>(rows_all) * (DP + 4);
-  float top = -kInf, sum = 0.f;
-  float o[N] = {0.f, 0.f, 0.f, 0.f};
-  for (int w = 0; w < a.splits; ++w) top = fmaxf(top, p0[w * step + DP]);
-  for (int w = 0; w < a.splits; ++w) {
-    const float mw = p0[w * step + DP], lw = p0[w * step + DP + 1];
-    if (mw == -kInf && lw == 0.f) continue;
-    const float f = mw == top ? 1.f : __builtin_amdgcn_exp2f(mw - top);
-    sum += lw * f;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p0 + w * step + i0);
+  float m[kFewParts], l[kFewParts];
+  f32x4 x[kFewParts];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
+  for (int w = 0; w < kFewParts; ++w) {
+    const int64_t at = w < a.splits ? w * step : 0;
+    m[w] = p0[at + DP];
+    l[w] = w < a.splits ? p0[at + DP + 1] : 0.f;
+    x[w] = *reinterpret_cast<const f32x4*>(p0 + at + i0);
+  }
+  float top = m[0], sum = 0.f, o[N] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 1; w < kFewParts; ++w) top = fmaxf(top, m[w]);
+#pragma unroll
+  for (int w = 0; w < kFewParts; ++w) {
+    if (w >= a.splits) break;
+    const float f = m[w] == top ? 1.f : __builtin_amdgcn_exp2f(m[w] - top);
+    sum += l[w] * f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += x[w][e] * f;
+  }
+  const int t = by_group(a, r), gg = r - t * a.G;
+  row_finish(seq_of(a.c, b), t, sum, o);
+  row_out<DT>(a, b, t, hk * a.G + gg, i0, o);
+}
+
+// More parts: a workgroup a row. Lane w of each wave holds part w's statistics; every DP / 4 threads sum up each
+// 1024 / DP-th part, and those sums meet in LDS.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void cached_attn_join_many_kernel(AttnArgs a) {
+  constexpr int L = DP / 4, kGroups = 256 / L, kEach = kMostParts / kGroups;
+  __shared__ __attribute__((aligned(16))) f32x4 part[kGroups][L];
+  __shared__ float factor[kMostParts];
+  const int rows_all = a.c.T * a.G, lane = threadIdx.x & 63;
+  const int64_t bh = static_cast<int64_t>(blockIdx.x) / rows_all;
+  const int r = static_cast<int>(blockIdx.x % rows_all);
+  const int b = static_cast<int>(bh / a.c.n_heads), hk = static_cast<int>(bh % a.c.n_heads);
+  const float* const p0 = a.ws + (bh * a.splits * rows_all + r) * (DP + 4);
+  const int64_t step = static_cast<int64_t>(rows_all) * (DP + 4);
+  const int group = threadIdx.x / L, i0 = threadIdx.x % L * 4;
+  f32x4 x[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int w = group + k * kGroups;
+    x[k] = *reinterpret_cast<const f32x4*>(p0 + (w < a.splits ? w * step : 0) + i0);
+  }
+  const bool have = lane < a.splits;
+  const float m = have ? p0[lane * step + DP] : -kInf, l = have ? p0[lane * step + DP + 1] : 0.f;
+  const float top = lanes_max(m), f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+  const float sum = lanes_sum(l * f);
+  if (threadIdx.x < kMostParts) factor[threadIdx.x] = f;
+  __syncthreads();
+  f32x4 y{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int w = group + k * kGroups;
+    if (w >= a.splits) break;
+    const float g = factor[w];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] += x[k][e] * g;
+  }
+  part[group][threadIdx.x % L] = y;
+  __syncthreads();
+  if (group || i0 >= a.c.d) return;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) {
+    const f32x4 z = part[k][threadIdx.x];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += z[e];
   }
   const int t = by_group(a, r), gg = r - t * a.G;
   row_finish(seq_of(a.c, b), t, sum, o);
@@ -1145,6 +1205,7 @@ struct Plan {
 // Most tiles of 16 rows that a wave holds: the registers of one whose 256 leave two waves to a SIMD.
 Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np) {
   Plan p{};
+  const bool same = !c.ks;
   const int dp = c.pitch <= 64 ? 64 : 128;
   p.rt = rows <= 16 ? 1 : 2;
   p.rows = rows > 64;
@@ -1157,10 +1218,11 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
   if (p.rows) {
     p.waves = 4;
     p.n_rb = (rows + 4 * cap - 1) / (4 * cap);
-    // two workgroups for every CU, each with 32 tiles at least
+    // two workgroups for every CU, each with 8 tiles at least: 160 blocks of 130 tiles 121 us whole, 65 in three parts,
+    // 20 blocks of 66 tiles 60 and 24 in eight
     const int64_t blocks = heads * p.n_rb;
-    s = blocks < 512 ? 512 / blocks : 1;
-    if (s > tiles / 32) s = tiles / 32;
+    s = 512 / blocks;
+    if (s > tiles / 8) s = tiles / 8;
   } else {
     p.n_rb = (rows + cap - 1) / cap;
     p.row_cap = rows < cap ? rows : cap;
@@ -1170,11 +1232,18 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     // registers alone: 320 such blocks of 19 tiles 21.6 us, with four waves 16.7; 20 blocks 10.6 and 11.5. With 16
     // rows: 640 blocks of 17 tiles 16.6 and 14.3, of 33 tiles 34 and 37.
     if (tiles <= 4 || (p.rt == 2 ? blocks > 256 : blocks >= 512 && tiles <= 24)) p.waves = 4;
-    // enough workgroups for every CU, each wave with 4 tiles at least
-    s = (512 + blocks - 1) / blocks;
-    if (s > tiles / (4 * p.waves)) s = tiles / (4 * p.waves);
+    // Few blocks with long axes in parts, until each CU has a workgroup of four waves (two in 8 bits, whose tiles are
+    // half as large). 10 blocks of 512 tiles 88 us whole, 14 in 25 parts; 80 of 130 tiles 25.7 and 19.4 in three; 96 of 130
+    // with d = 128 56 and 41 in two; 160 33 and 35 in three; in 8 bits 40 of 130 23.8 and 11.9 in 12, 160 26.0 and 23.5
+    // in three, 240 30 and 35 in two. Shorter axes gain less than the second launch costs the host (10 blocks of 34 tiles
+    // 9.5 and 7.9).
+    if (tiles > 48) {
+      s = same ? 256 / blocks : 512 / blocks >= 3 ? 512 / blocks : 1;
+      if (s > tiles / 4) s = tiles / 4;
+      if (s > 1) p.waves = 4;
+    }
   }
-  if (s > 64) s = 64;
+  if (s > kMostParts) s = kMostParts;
   p.splits = s < 1 ? 1 : static_cast<int>(s);
   p.ws = p.splits > 1 ? static_cast<size_t>(heads) * p.splits * rows * (dp + 4) * 4 : 0;
   return p;
@@ -1208,10 +1277,11 @@ void launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
   } else if constexpr (!(DT == TMAC_F32 && DP == 128)) {
     cached_attn_kernel<DT, FMT, DP, 1, 8, false><<<grid, 64 * 8, lds, s>>>(a);
   }
-  if (p.splits > 1) {
-    const int64_t threads = static_cast<int64_t>(a.B) * a.c.n_heads * a.c.T * a.G * (DP / 4);
-    cached_attn_join_kernel<DT, DP><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(a);
-  }
+  const int64_t rows = static_cast<int64_t>(a.B) * a.c.n_heads * a.c.T * a.G;
+  if (p.splits > kFewParts)  // at most 512 blocks of up to 128 rows are parted, so these are few
+    cached_attn_join_many_kernel<DT, DP><<<static_cast<unsigned>(rows), 256, 0, s>>>(a);
+  else if (p.splits > 1)
+    cached_attn_join_kernel<DT, DP><<<static_cast<unsigned>((rows * (DP / 4) + 255) / 256), 256, 0, s>>>(a);
 }
 
 template <int DT, int FMT>
