@@ -818,11 +818,15 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
     tile1 = tile0 + per < keys.n_tiles ? tile0 + per : keys.n_tiles;
   }
 
-  // This thread's rows of a stage and its piece of them: threads in a row read a row's pieces one after the other.
+  // This thread's rows of a stage and its piece of them: threads in a row read a row's pieces one after the other. A
+  // wave's rows of each load lie in one group of 16, so in one page: its place is the wave's to work out.
   const int piece = threadIdx.x % kChunks, my_row = threadIdx.x / kChunks;
   constexpr int kRowStep = 256 / kChunks;
+  static_assert(kRowStep % 16 == 0 && 64 / kChunks <= 16, "rows of a wave's load lie in one group of 16");
   const int col = piece * (16 / kElem), pitch_b = a.c.pitch * kElem, page_mask = (1 << a.c.page_shift) - 1;
-  const uint32_t page_rows = static_cast<uint32_t>(a.c.n_heads) << a.c.page_shift;
+  const int my_off = (my_row & 15) * pitch_b + (col < a.c.pitch ? piece * 16 : 0);
+  const bool narrow = a.c.pitch < DP;
+  const uint32_t page_rows = static_cast<uint32_t>(a.c.n_heads) << a.c.page_shift, page_bytes = page_rows * pitch_b;
   const uint32_t head_rows = static_cast<uint32_t>(hk) << a.c.page_shift;
   const int32_t* const table = a.c.table + b * a.c.table_stride;
   const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
@@ -830,36 +834,33 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
   u32x4 rk[kLoads], rv[kLoads];
   float r_ks = 0.f, r_vs = 0.f;
   int page[kLoads], scale_page = 0;
-  bool seen[kLoads], bad[kLoads];
+  bool bad[kLoads];  // of what is in registers: a page that is none
+  auto group_key = [&](int it, int u) {
+    return keys.first(it) + ((wave * (64 / kChunks) + u * kRowStep) & ~15);
+  };
   auto look_up = [&](int it) {
-    const int key0 = keys.first(it);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const int key = key0 + my_row + u * kRowStep;
-      page[u] = key < len ? table[key >> a.c.page_shift] : -1;
+      const int key = group_key(it, u);
+      page[u] = key < len ? table[key >> a.c.page_shift] : 0;
     }
     if (FMT != kCacheSame && threadIdx.x < kKeys) {
-      const int key = key0 + static_cast<int>(threadIdx.x);
+      const int key = keys.first(it) + static_cast<int>(threadIdx.x);
       scale_page = key < len ? table[key >> a.c.page_shift] : -1;
     }
   };
   auto load = [&](int it) {
-    const int key0 = keys.first(it);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const int key = key0 + my_row + u * kRowStep;
-      const bool there = static_cast<uint32_t>(page[u]) < static_cast<uint32_t>(a.c.n_pages) && key < len;
-      seen[u] = there && ((key < keys.np) | in_span(key, span_lo, span));
-      bad[u] = !there && key < len;
-      rk[u] = rv[u] = u32x4{0, 0, 0, 0};
-      if (there && col < a.c.pitch) {
-        const int64_t off = (static_cast<int64_t>(page[u]) * page_rows + head_rows + (key & page_mask)) * pitch_b + piece * 16;
-        rk[u] = *reinterpret_cast<const u32x4*>(a.c.k + off);
-        rv[u] = *reinterpret_cast<const u32x4*>(a.c.v + off);
-      }
+      bad[u] = static_cast<uint32_t>(page[u]) >= static_cast<uint32_t>(a.c.n_pages);
+      const uint32_t p = bad[u] ? 0 : page[u];  // rows past the end are those of some page: no row sees them
+      const int64_t off = static_cast<int64_t>(static_cast<uint64_t>(p) * page_bytes +
+                                               (head_rows + (group_key(it, u) & page_mask)) * pitch_b);
+      rk[u] = *reinterpret_cast<const u32x4*>(a.c.k + off + my_off);
+      rv[u] = *reinterpret_cast<const u32x4*>(a.c.v + off + my_off);
     }
     if (FMT != kCacheSame && threadIdx.x < kKeys) {
-      const int key = key0 + static_cast<int>(threadIdx.x);
+      const int key = keys.first(it) + static_cast<int>(threadIdx.x);
       r_ks = r_vs = 0.f;
       if (static_cast<uint32_t>(scale_page) < static_cast<uint32_t>(a.c.n_pages) && key < len) {
         const int64_t r = static_cast<int64_t>(scale_page) * page_rows + head_rows + (key & page_mask);
@@ -871,14 +872,19 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
     }
   };
   auto store = [&](int it, int st) {
-    const bool part = !keys.all_see(keys.first(it));
+    const int stage0 = keys.first(it);
+    const bool part = !keys.all_see(stage0);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const int r = my_row + u * kRowStep;
-      // values that no row sees may be anything: zeros. A page that is none: keys of NaN.
-      if (!seen[u]) rv[u] = u32x4{0, 0, 0, 0};
-      if constexpr (FMT == kCacheSame) {
-        if (part) {  // rows that do not see a value must not meet what is not finite: see below
+      if (narrow && col >= a.c.pitch) rk[u] = u32x4{0, 0, 0, 0};
+      if (part) {
+        // values that no row sees may be anything: zeros
+        const int key = stage0 + r;
+        const uint32_t on = (key < keys.np) | in_span(key, span_lo, span) ? ~0u : 0u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) rv[u][w] &= on;
+        if constexpr (FMT == kCacheSame) {  // rows that do not see a value must not meet what is not finite: see below
           uint32_t changed = 0;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -888,7 +894,10 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
           }
           if (changed) s_cleaned = 1;
         }
-        if (bad[u]) rk[u] = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+      }
+      constexpr uint32_t kNan2 = 0x7fff7fffu;
+      if constexpr (FMT == kCacheSame) {
+        if (bad[u]) rk[u] = u32x4{kNan2, kNan2, kNan2, kNan2};
         const int to = (piece >> 3) * kHalfTile + swz64(r, piece & 7);
         sts16(&sk[st][to], rk[u]);
         sts16(&sv[st][to], rv[u]);
@@ -903,7 +912,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
             y[2 * w] = code2<DT, FMT, false>(rv[u][2 * h + w]);
             y[2 * w + 1] = code2<DT, FMT, true>(rv[u][2 * h + w]);
           }
-          if (bad[u]) x = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+          if (bad[u]) x = u32x4{kNan2, kNan2, kNan2, kNan2};
           const int chunk = 2 * piece + h, to = (chunk >> 3) * kHalfTile + swz64(r, chunk & 7);
           sts16(&sk[st][to], x);
           sts16(&sv[st][to], y);
