@@ -120,7 +120,7 @@ struct AttnArgs {
   float* ws;
   int B, Hq, G, g_shift, n_rb, splits, np, row_cap, per_xcd, n_blocks;  // g_shift: log2 of G, or -1
   int window;  // INT_MAX / 2 and above: none
-  float scale2, q_sign;  // |scale| · log2 e (1 for scale 0); the queries are taken times q_sign, the scale's sign
+  float scale2, slack, q_sign;  // slack: kSlack / scale2; scale2: |scale| · log2 e (1 for scale 0); the queries are taken times q_sign, the scale's sign
   bool q_vec, out_vec;
 };
 
@@ -246,41 +246,46 @@ __device__ __forceinline__ uint32_t row_sees(const Row& r, int kb, int base, boo
   return vis;
 }
 
-// The running softmax of a row, as the lanes that hold it have it. m: the largest score so far (not scaled); mu: it
-// times scale2, what exponents are taken relative to (0 while there is none); l: this lane's part of the sum.
+// The running softmax of a row, as the lanes that hold it have it. Exponents are taken relative to mu, which is a score
+// times scale2 (0 while there is none) and moves only for one that is more than kSlack above it: up to then
+// exponentials stay below 2^kSlack, where the sums in fp32 and the probabilities in 16 bit are as good. Moving costs as
+// much as a tile's exponentials, and a wave's 16 rows have a new largest score in two of three tiles of 40. lim: that
+// bound, not scaled; l: this lane's part of the sum.
+constexpr float kSlack = 8.f;
 struct Soft {
-  float m, mu, l;
+  float lim, mu, l;
 };
 
-// Scores x (−inf where masked) become e^{x − m}; what was summed up before moves to the new maximum.
+// Scores x (−inf where masked) become exponentials; what was summed up before moves with mu.
 template <int NJ>
-__device__ __forceinline__ void soften(Soft& s, float (&x)[8], f32x4 (&acc)[NJ], float scale2) {
+__device__ __forceinline__ void soften(Soft& s, float (&x)[8], f32x4 (&acc)[NJ], const AttnArgs& a) {
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-  if (__any(mx > s.m)) {
+  if (__any(mx > s.lim)) {
     mx = fmaxf(mx, lane_xor<16>(mx));
     mx = fmaxf(mx, lane_xor<32>(mx));
-    const float to = fmaxf(s.m, mx), mu_to = to == -kInf ? 0.f : to * scale2;
-    const float f = to == s.m || s.m == -kInf ? 1.f : __builtin_amdgcn_exp2f(s.mu - mu_to);
-    s.m = to;
-    s.mu = mu_to;
-    s.l *= f;
+    if (mx > s.lim) {  // the same in the row's four lanes
+      const float to = mx * a.scale2, f = s.lim == -kInf ? 1.f : __builtin_amdgcn_exp2f(s.mu - to);
+      s.lim = mx + a.slack;
+      s.mu = to;
+      s.l *= f;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[j] *= f;
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
+    }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale2, -s.mu));
+    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], a.scale2, -s.mu));
     s.l += x[i];
   }
 }
-// The row's statistics from its lanes': m is now in units of scale2.
-__device__ __forceinline__ void soft_join(Soft& s) {
+// The row's sum from its lanes', and what it is relative to: mu, or −inf for a row that saw nothing (one that saw
+// nothing but NaN has a sum of NaN).
+__device__ __forceinline__ float soft_join(Soft& s) {
   s.l += lane_xor<16>(s.l);
   s.l += lane_xor<32>(s.l);
-  // rows that saw nothing but NaN have a sum of NaN and no maximum: 0 stands for it
-  if (s.m != -kInf || s.l != s.l) s.m = s.mu;
+  return s.lim == -kInf && s.l == s.l ? -kInf : s.mu;
 }
 
 // A power of two above every scale vs so far, for fp16 probabilities times a scale (v_ref); what was summed up before
@@ -616,7 +621,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
     if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      soften(soft[rt], x[rt], acc[rt], a.scale2);
+      soften(soft[rt], x[rt], acc[rt], a);
       if constexpr (FMT != kCacheSame) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
@@ -681,8 +686,9 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
       }
     }
   }
+  float m[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) soft_join(soft[rt]);
+  for (int rt = 0; rt < RT; ++rt) m[rt] = soft_join(soft[rt]);
 
   if constexpr (ROWS) {
 #pragma unroll
@@ -700,7 +706,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
             *reinterpret_cast<f32x4*>(po + (4 * g + i) * NJ + j) =
                 f32x4{acc[rt][j][i], acc[rt][j + 1][i], acc[rt][j + 2][i], acc[rt][j + 3][i]};
         if (g == 0) {
-          po[DP] = soft[rt].m;
+          po[DP] = m[rt];
           po[DP + 1] = soft[rt].l;
         }
         continue;
@@ -726,7 +732,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = 16 * rt + n;
-    if (r < cap && g == 0) sm[wave * cap + r] = float2{soft[rt].m, soft[rt].l};
+    if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], soft[rt].l};
   }
   __syncthreads();
 #pragma unroll
@@ -736,7 +742,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
     float top = -kInf;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
-    const float f = soft[rt].m == top ? 1.f : __builtin_amdgcn_exp2f(soft[rt].m - top);
+    const float f = m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1037,7 +1043,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
       u32x4 pw[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        soften(soft[rt], x[rt], acc[rt], a.scale2);
+        soften(soft[rt], x[rt], acc[rt], a);
         if constexpr (FMT != kCacheSame) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
@@ -1091,14 +1097,14 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    soft_join(soft[rt]);
+    const float m = soft_join(soft[rt]);
     const int r = row0 + 16 * rt + n;
     if (r >= rows_all) continue;
     const int t = by_group(a, r), gg = r - t * G;
     const int64_t to = ((static_cast<int64_t>(b) * a.c.n_heads + hk) * a.splits + split) * rows_all + r;
     float* const po = a.ws + to * (DP + 4);
     if (a.splits > 1 && g == 0) {
-      po[DP] = soft[rt].m;
+      po[DP] = m;
       po[DP + 1] = soft[rt].l;
     }
 #pragma unroll
@@ -1350,6 +1356,7 @@ extern "C" int tmac_cached_attn(const tmac_cache* cache, const void* d_q, const 
   a.np = n_persistent < kMost ? n_persistent : kMost;
   a.window = window < kMost ? static_cast<int>(window) : kMost;
   a.scale2 = scale == 0.f ? 1.f : fabsf(scale) * kLog2e;
+  a.slack = kSlack / a.scale2;
   a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : scale;
   a.q_vec = a.q_sign == 1.f && row_aligned16(d_q) && a.c.d % n == 0 && a.qb % n == 0 && a.qh % n == 0 && a.qt % n == 0;
   a.out_vec = row_aligned16(d_out) && a.c.d % 4 == 0;
