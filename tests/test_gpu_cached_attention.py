@@ -169,6 +169,98 @@ def test_what_a_row_does_not_see(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,d", [(None, 64), (90, 64), (None, 128), (70, 40)])
+def test_what_rows_of_a_chunk_do_not_see(dev, dtype, window, d):
+    """The same in a chunk of many rows: every row is as if what it does not see were not there, and what it sees reaches
+    it, wherever that lies (before the chunk, in it, where all rows of some see it and not all of others)."""
+    B, H, T, lens = 2, 2, 200, [330, 200]
+    c, table, lengths = filled(dev, B, H, d, 32, lens, dtype, None, fill=NAN)
+    q = queries(dev, B, H, T, d, dtype)
+    want = tc.cached_attention(q, c, table, lengths, window, 4)
+    masks = seen_by(B, T, lens, [T, T], window, 4)
+    spots = ((-60, "v", math.inf), (0, "k", NAN), (63, "v", -math.inf), (64, "v", NAN), (127, "v", math.inf), (199, "v", NAN))
+    for b in range(B):
+        for t, kv, bad in spots:
+            pos = lens[b] - T + t
+            if pos >= 0:
+                getattr(c, kv)[table[b, pos // 32].long(), :, pos % 32, 3] = bad
+    got = tc.cached_attention(q, c, table, lengths, window, 4)
+    for b in range(B):
+        here = [(lens[b] - T + t, kv, bad) for t, kv, bad in spots if lens[b] - T + t >= 0]
+        hit = masks[b].to(dev)[:, [p for p, _, _ in here]]
+        key = torch.tensor([kv == "k" for _, kv, _ in here], device=dev)
+        vals = torch.tensor([bad for _, _, bad in here], device=dev)
+        assert torch.equal(got[b][:, ~hit.any(-1)], want[b][:, ~hit.any(-1)])
+        nan_row = (hit & key).any(-1)
+        assert torch.isnan(got[b][:, nan_row]).all()
+        plus, minus, nan = ((hit & ~key & m).any(-1) & ~nan_row for m in (vals == math.inf, vals == -math.inf, vals.isnan()))
+        col = got[b][:, :, 3]
+        assert torch.isnan(col[:, nan | (plus & minus)]).all()
+        assert torch.all(col[:, plus & ~minus & ~nan] == math.inf) and torch.all(col[:, minus & ~plus & ~nan] == -math.inf)
+        assert torch.equal(got[b][:, ~nan_row, 4:], want[b][:, ~nan_row, 4:])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_pages_that_are_none(dev, T, dtype, fmt):
+    """A page outside the pool is NaN for the rows that see it and nothing to the others; so are numbers that do not
+    fit for a whole sequence."""
+    lens = [T + 100, T + 100, T + 20, T]
+    c, table, lengths = filled(dev, 4, 2, 64, 16, lens, dtype, fmt, fill=NAN)
+    q = queries(dev, 4, 2, T, 64, dtype)
+    window, n_persistent = 50, 4
+    want = tc.cached_attention(q, c, table, lengths, window, n_persistent)
+    masks = seen_by(4, T, lens, [T] * 4, window, n_persistent)
+    table[0, 1], table[0, 2] = -1, 2 ** 31 - 1          # in front of the window: not looked at, or not seen
+    table[1, (lens[1] - 1) // 16] = c.k.shape[0]        # the last page
+    bad = lengths.clone()
+    bad[3] = table.shape[1] * 16 + 1
+    got = tc.cached_attention(q, c, table, bad, window, n_persistent)
+    assert torch.isnan(got[3]).all() and torch.equal(got[2], want[2])
+    for b, pages in ((0, (1, 2)), (1, ((lens[1] - 1) // 16,))):
+        m = masks[b].to(dev)
+        hit = torch.stack([m[:, 16 * j:16 * j + 16].any(-1) for j in pages]).any(0)
+        assert torch.isnan(got[b][:, hit]).all() and torch.equal(got[b][:, ~hit], want[b][:, ~hit])
+
+
+def test_a_row_of_nan_in_8_bits(dev):
+    """A row that was not finite when it was written: NaN for the rows that see its key or value, nothing to the others."""
+    for fmt, dtype, T in (("int8", torch.bfloat16, 150), ("e4m3", torch.float16, 150), ("int8", torch.float16, 9),
+                          ("e4m3", torch.float32, 70)):
+        B, H, d, lens = 1, 2, 64, [T + 30]
+        c, table, lengths = filled(dev, B, H, d, 16, lens, dtype, fmt, fill=NAN)
+        q = queries(dev, B, H, T, d, dtype)
+        want = tc.cached_attention(q, c, table, lengths, 40)
+        k = torch.randn(B, H, 1, d, device=dev).to(dtype)
+        pos = lens[0] - 5
+        at = torch.tensor([pos + 1], dtype=torch.int32, device=dev)
+        old = (c.k[table[0, pos // 16].long(), :, pos % 16].clone(), c.k_scale[table[0, pos // 16].long(), :, pos % 16].clone())
+        v = k.clone()
+        v[..., 7] = math.inf
+        tc.cache_write(k, v, c, table, at)
+        c.k[table[0, pos // 16].long(), :, pos % 16], c.k_scale[table[0, pos // 16].long(), :, pos % 16] = old
+        got = tc.cached_attention(q, c, table, lengths, 40)
+        m = seen_by(B, T, lens, [T], 40, 0)[0].to(dev)[:, pos]
+        assert torch.isnan(got[0][:, m]).all() and torch.equal(got[0][:, ~m], want[0][:, ~m]) and m.any() and (~m).any()
+
+
+def test_compiled(dev):
+    c, table, lengths = filled(dev, 2, 2, 64, 32, [70, 40], torch.bfloat16, "int8")
+    q = queries(dev, 2, 4, 3, 64, torch.bfloat16)
+
+    def step(q, k, v):
+        tc.cache_write(k, v, c, table, lengths)
+        return tc.cached_attention(q * 2, c, table, lengths, 30, 2) + 1
+
+    k, v = (torch.randn(2, 2, 3, 64, device=dev).bfloat16() for _ in range(2))
+    want = step(q, k, v)
+    with torch.no_grad():
+        got = torch.compile(step, backend="aot_eager")(q, k, v)
+    assert torch.equal(want, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("H,d,S,window,n_persistent", [(10, 64, 300, 128, 16), (3, 40, 77, 20, 0), (2, 128, 130, 500, 4)])
 def test_as_windowed_attention(dev, H, d, S, window, n_persistent, dtype):
     """A text that arrives in chunks of any size gets what windowed_attention gives for all of it."""

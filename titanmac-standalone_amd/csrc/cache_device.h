@@ -83,31 +83,41 @@ __device__ __forceinline__ float code_scale(uint32_t amax) {
   }
 }
 
-// rne(x / s) for |x| <= 127 s (within a rounding): from an approximate quotient, decided by the remainder x − q s. That
-// is exact in an fma: for |x| >= s it is a multiple of s's last bit below 0.6 s, for q = 0 it is x, and for q = ±1
-// and |x| >= s/2 the operands are within a factor of two of each other; for q = ±1 and |x| < s/2 it may be
-// rounded, to s/2 at the least, and a tie goes to 0 as |x| < s/2 does.
-__device__ __forceinline__ int int8_code(float x, float s, float inv) {
-  const float q = rintf(x * inv), r = fmaf(-q, s, x), h = 0.5f * s;
-  const int i = static_cast<int>(q);
-  const bool odd = i & 1;
-  if (r > h || (r == h && odd)) return i + 1;
-  if (r < -h || (r == -h && odd)) return i - 1;
-  return i;
-}
-
 // Four values as codes of scale s, one byte each.
+//
+// int8: rne(x / s) for |x| <= 127 s (within a rounding), from an approximate quotient q, decided by the remainder x − q s.
+// That is exact in an fma: for |x| >= s it is a multiple of s's last bit below 0.6 s, for q = 0 it is x, and for
+// q = ±1 and |x| >= s/2 the operands are within a factor of two of each other; for q = ±1 and |x| < s/2 it may be
+// rounded, to s/2 at the least, and a tie goes to 0 as |x| < s/2 does. q is one off, or the remainder a tie, for few
+// rows: the others take one comparison for their four values.
 template <int FMT>
 __device__ __forceinline__ uint32_t to_code4(float a, float b, float c, float d, float s) {
+  if (s != s) return 0;
   if constexpr (FMT == kCacheInt8) {
-    if (s != s) return 0;
-    const float inv = __builtin_amdgcn_rcpf(s);
-    return (int8_code(a, s, inv) & 255) | (int8_code(b, s, inv) & 255) << 8 | (int8_code(c, s, inv) & 255) << 16 |
-           static_cast<uint32_t>(int8_code(d, s, inv) & 255) << 24;
+    const float x[4] = {a, b, c, d}, inv = __builtin_amdgcn_rcpf(s), h = 0.5f * s;
+    float q[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i] = rintf(x[i] * inv);
+      r[i] = fmaf(-q[i], s, x[i]);
+    }
+    int code[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) code[i] = static_cast<int>(q[i]);
+    if (fmaxf(fmaxf(fabsf(r[0]), fabsf(r[1])), fmaxf(fabsf(r[2]), fabsf(r[3]))) >= h) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool odd = code[i] & 1;
+        if (r[i] > h || (r[i] == h && odd))
+          code[i] += 1;
+        else if (r[i] < -h || (r[i] == -h && odd))
+          code[i] -= 1;
+      }
+    }
+    return (code[0] & 255) | (code[1] & 255) << 8 | (code[2] & 255) << 16 | static_cast<uint32_t>(code[3] & 255) << 24;
   } else {
-    if (s != s) return 0;
     const float inv = __uint_as_float(0x7f000000u - __float_as_uint(s));  // 1 / s, a power of two: exact products
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true));
   }
 }

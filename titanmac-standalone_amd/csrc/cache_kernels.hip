@@ -34,56 +34,63 @@ struct Strides {
   int64_t b, h, t;
 };
 
-// lanes_log2: log2 of the lanes of a row. grid.x: rows (t, h) of one sequence's keys or values, grid.y: 2 B of those.
+// a chunk of a row into a pool, from chunk i on; all 64 lanes take part
+template <int DT, int FMT, int N>
+__device__ __forceinline__ void put_chunk(uint8_t* pool, float* scales, int64_t row, int pitch, int i, int lanes_log2,
+                                          const float (&x)[N]) {
+  const bool mine = row >= 0 && i < pitch;
+  if constexpr (FMT == kCacheSame) {
+    if (mine) row_store<DT, N>(pool + (row * pitch + i) * kRowSize<DT>, x);
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const uint32_t w = __float_as_uint(x[u]) & 0x7fffffffu;
+      m = w > m ? w : m;
+    }
+    for (int o = 1; o < 1 << lanes_log2; o <<= 1) {
+      const uint32_t w = __shfl_xor(m, o);
+      m = w > m ? w : m;
+    }
+    const float scale = code_scale<FMT>(m);
+    if (!mine) return;
+    uint8_t* const to = pool + row * pitch + i;
+    if constexpr (N == 4) {
+      *reinterpret_cast<uint32_t*>(to) = to_code4<FMT>(x[0], x[1], x[2], x[3], scale);
+    } else {
+      *reinterpret_cast<u32x2*>(to) = u32x2{to_code4<FMT>(x[0], x[1], x[2], x[3], scale),
+                                            to_code4<FMT>(x[4], x[5], x[6], x[7], scale)};
+    }
+    if (i == 0) scales[row] = scale;
+  }
+}
+
+// lanes_log2: log2 of the lanes of a row. grid.x: rows (t, h) of a sequence, grid.y: sequences. A row's key and value by
+// the same lanes: one look at the table, two loads in flight (8 prompts of 2047 rows of 10 heads
+// of 64 bf16 18.2 us, 4.6 TB/s; with a row's key and value apart 21.4). The order of the rows makes no difference.
 template <int DT, int FMT, bool VEC>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a, const uint8_t* __restrict__ k, Strides ks,
                                                           const uint8_t* __restrict__ v, Strides vs, int B,
                                                           int lanes_log2) {
   constexpr int N = kRowVec<DT>;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t r = at >> lanes_log2;
+  const uint32_t r = static_cast<uint32_t>(at >> lanes_log2);
   const int i = static_cast<int>(at & ((1 << lanes_log2) - 1)) * N;
   // heads fastest: the heads of a token lie together in a projection's output
-  const int t = static_cast<int>(r / a.n_heads), h = static_cast<int>(r % a.n_heads);
-  for (int y = blockIdx.y; y < 2 * B; y += gridDim.y) {
-    const int b = y >> 1;
-    const bool is_v = y & 1;
+  const int t = static_cast<int>(r / static_cast<uint32_t>(a.n_heads)), h = static_cast<int>(r - t * a.n_heads);
+  for (int b = blockIdx.y; b < B; b += gridDim.y) {
     const Seq s = seq_of(a, b);
     int64_t row = -1;
-    if (s.ok && t < s.n) row = cache_row(a, b, s.len - s.n + t, h);
-    const Strides st = is_v ? vs : ks;
-    float x[N];
-    if (row >= 0) {
-      load_chunk<DT, VEC, N>((is_v ? v : k) + (b * st.b + h * st.h + t * st.t) * kRowSize<DT>, i, a.d, x);
-    } else {
+    float x[N], y[N];
 #pragma unroll
-      for (int u = 0; u < N; ++u) x[u] = 0.f;
+    for (int u = 0; u < N; ++u) x[u] = y[u] = 0.f;
+    if (s.ok && t < s.n) {
+      load_chunk<DT, VEC, N>(k + (b * ks.b + h * ks.h + t * ks.t) * kRowSize<DT>, i, a.d, x);
+      load_chunk<DT, VEC, N>(v + (b * vs.b + h * vs.h + t * vs.t) * kRowSize<DT>, i, a.d, y);
+      row = cache_row(a, b, s.len - s.n + t, h);
     }
-    if constexpr (FMT == kCacheSame) {
-      if (row >= 0 && i < a.pitch) row_store<DT, N>((is_v ? a.v : a.k) + (row * a.pitch + i) * kRowSize<DT>, x);
-    } else {
-      uint32_t m = 0;
-#pragma unroll
-      for (int u = 0; u < N; ++u) {
-        const uint32_t w = __float_as_uint(x[u]) & 0x7fffffffu;
-        m = w > m ? w : m;
-      }
-      for (int o = 1; o < 1 << lanes_log2; o <<= 1) {  // all 64 lanes take part
-        const uint32_t w = __shfl_xor(m, o);
-        m = w > m ? w : m;
-      }
-      const float scale = code_scale<FMT>(m);
-      if (row >= 0 && i < a.pitch) {
-        uint8_t* const to = (is_v ? a.v : a.k) + row * a.pitch + i;
-        if constexpr (N == 4) {
-          *reinterpret_cast<uint32_t*>(to) = to_code4<FMT>(x[0], x[1], x[2], x[3], scale);
-        } else {
-          *reinterpret_cast<u32x2*>(to) = u32x2{to_code4<FMT>(x[0], x[1], x[2], x[3], scale),
-                                                to_code4<FMT>(x[4], x[5], x[6], x[7], scale)};
-        }
-        if (i == 0) (is_v ? a.vs : a.ks)[row] = scale;
-      }
-    }
+    put_chunk<DT, FMT, N>(a.k, a.ks, row, a.pitch, i, lanes_log2, x);
+    put_chunk<DT, FMT, N>(a.v, a.vs, row, a.pitch, i, lanes_log2, y);
   }
 }
 
@@ -104,38 +111,40 @@ __device__ __forceinline__ void pool_load(const uint8_t* pool, const float* scal
   }
 }
 
-// Rows (h, t), t fastest: those of a page are together on both sides.
+// Rows (h, t), t fastest: those of a page are together on both sides. Key and value by the same lanes.
 template <int DT, int FMT, bool VEC>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a, uint8_t* __restrict__ k, uint8_t* __restrict__ v,
                                                          int B, int T, int lanes_log2) {
   constexpr int N = kRowVec<DT>;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t r = at >> lanes_log2;
+  const uint32_t r = static_cast<uint32_t>(at >> lanes_log2);
   const int i = static_cast<int>(at & ((1 << lanes_log2) - 1)) * N;
-  const int h = static_cast<int>(r / T), t = static_cast<int>(r % T);
+  const int h = static_cast<int>(r / static_cast<uint32_t>(T)), t = static_cast<int>(r - h * static_cast<uint32_t>(T));
   if (h >= a.n_heads || i >= a.d) return;
-  for (int y = blockIdx.y; y < 2 * B; y += gridDim.y) {
-    const int b = y >> 1;
-    const bool is_v = y & 1;
+  for (int b = blockIdx.y; b < B; b += gridDim.y) {
     const int len = a.lengths[b];
     const bool ok = len >= 0 && len <= (static_cast<int64_t>(a.max_pages) << a.page_shift);
-    float x[N];
+    float x[N], y[N];
     const int64_t row = ok && t < len ? cache_row(a, b, t, h) : -1;
     if (row >= 0) {
-      pool_load<DT, FMT, N>(is_v ? a.v : a.k, is_v ? a.vs : a.ks, row, a.pitch, i, x);
+      pool_load<DT, FMT, N>(a.k, a.ks, row, a.pitch, i, x);
+      pool_load<DT, FMT, N>(a.v, a.vs, row, a.pitch, i, y);
     } else {
       const float fill = ok && t >= len ? 0.f : __builtin_nanf("");
 #pragma unroll
-      for (int u = 0; u < N; ++u) x[u] = fill;
+      for (int u = 0; u < N; ++u) x[u] = y[u] = fill;
     }
-    uint8_t* const to = (is_v ? v : k) + (((static_cast<int64_t>(b) * a.n_heads + h) * T + t) * a.d + i) * kRowSize<DT>;
+    const int64_t to = (((static_cast<int64_t>(b) * a.n_heads + h) * T + t) * a.d + i) * kRowSize<DT>;
     if (VEC) {
-      row_store<DT, N>(to, x);
+      row_store<DT, N>(k + to, x);
+      row_store<DT, N>(v + to, y);
     } else {
 #pragma unroll
       for (int u = 0; u < N; ++u) {
-        const float one[1] = {x[u]};
-        if (i + u < a.d) row_store<DT, 1>(to + u * kRowSize<DT>, one);
+        if (i + u >= a.d) continue;
+        const float one[1] = {x[u]}, two[1] = {y[u]};
+        row_store<DT, 1>(k + to + u * kRowSize<DT>, one);
+        row_store<DT, 1>(v + to + u * kRowSize<DT>, two);
       }
     }
   }
@@ -220,7 +229,7 @@ void by_types(int dtype, int format, bool vec, F f) {
 }
 
 constexpr int kMaxGridY = 65535;
-int grid_y(int B) { return 2 * static_cast<int64_t>(B) < kMaxGridY ? 2 * B : kMaxGridY - 1; }
+int grid_y(int B) { return B < kMaxGridY ? B : kMaxGridY; }
 
 }  // namespace
 

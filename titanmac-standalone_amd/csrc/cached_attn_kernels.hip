@@ -294,7 +294,7 @@ template <int RT, int NJ>
 __device__ __forceinline__ void relate_scales(float& v_ref, float (&vs)[8], f32x4 (&acc)[RT][NJ]) {
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, vs[i]);
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(vs[i]));
   if (__any(top > v_ref)) {
     top = fmaxf(top, lane_xor<16>(top));
     top = fmaxf(top, lane_xor<32>(top));

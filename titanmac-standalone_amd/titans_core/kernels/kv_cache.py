@@ -231,7 +231,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.T
 
     In 8 bits every row has its own scale: int8 codes are value / scale rounded to nearest (ties to even) with scale =
     max |value| / 127, e4m3 codes likewise with the least power of two that holds the row as scale (both at least
-    2^-126). A row that is not finite is held as NaN. Pages that are written must not belong to two sequences."""
+    2^-126). A row that is not finite is held as NaN. Pages that are written must not belong to two sequences, and k and v
+    must not share memory with the pools."""
     shape, dtype = k.shape, k.dtype
     if len(shape) != 4 or v.shape != shape or v.dtype is not dtype:
         raise ValueError(f"cache_write: k and v must be [B, n_heads, T, d_head], alike, got {tuple(shape)} {dtype} and "
