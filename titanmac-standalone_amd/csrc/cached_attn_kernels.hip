@@ -57,30 +57,48 @@ struct Piece {
 
 // What a kernel's types and head width mean for its loads. DT: the values' type; FMT: how the cache holds them; DP: 64
 // or 128, at least the pitch.
+//
+// fp32 on codes of 8 bits runs on the 16-bit matrix cores all the same: a code is exact in bfloat16, and an fp32 value is
+// the sum of three bfloat16 numbers (8 bits each of its 24), so three products give what an fp32 one gives, in a fifth
+// of its time.
 template <int DT, int FMT, int DP>
 struct Shape {
+  static constexpr bool kF32 = DT == TMAC_F32 && FMT == kCacheSame;  // fp32 products
+  static constexpr int kType = DT == TMAC_F32 ? TMAC_BF16 : DT;      // of the others
+  static constexpr int kParts = DT == TMAC_F32 && FMT != kCacheSame ? 3 : 1;
   static constexpr int kElem = FMT != kCacheSame ? 1 : DT == TMAC_F32 ? 4 : 2;  // bytes of a stored value
   static constexpr int kRun = 16 / kElem;           // values in 16 bytes: a lane's piece of a key
   static constexpr int kPieces = DP / (4 * kRun);   // of each key, per lane; piece c of group g: 4 kRun c + kRun g ..
-  static constexpr int kOps = DT == TMAC_F32 ? kRun : kRun / 8;  // products per piece
+  static constexpr int kOps = kF32 ? kRun : kRun / 8;  // products per piece
   static constexpr int NJ = DP / 16;                // columns of the values per lane, products per 32 keys
-  static constexpr bool kF32 = DT == TMAC_F32;
 };
+
+// Whether a wave needs more than half of a SIMD's registers: four waves a workgroup then.
+constexpr bool wide(int dtype, bool same, int dp, int rt) { return dtype == TMAC_F32 && dp == 128 && (same || rt > 1); }
+
+// x, y as the sum of P bfloat16 pairs (P = 1: rounded to TYPE)
+template <int TYPE, int P>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&w)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    w[i] = Mfma<TYPE>::pack2(x, y);
+    x -= Mfma<TYPE>::to_f32(static_cast<uint16_t>(w[i]));
+    y -= Mfma<TYPE>::to_f32(static_cast<uint16_t>(w[i] >> 16));
+  }
+}
 
 // operand e of a key's piece
 template <int DT, int FMT, int DP>
 __device__ __forceinline__ auto key_operand(const Piece<16>& p, int e) {
-  if constexpr (DT == TMAC_F32) {
-    if constexpr (FMT == kCacheSame)
-      return __uint_as_float(p.w[e]);
-    else
-      return code4<FMT>(p.w[e >> 2])[e & 3];
+  if constexpr (DT == TMAC_F32 && FMT == kCacheSame) {
+    return __uint_as_float(p.w[e]);
   } else if constexpr (FMT == kCacheSame) {
     return u32x4{p.w[0], p.w[1], p.w[2], p.w[3]};
   } else {
+    constexpr int kType = Shape<DT, FMT, DP>::kType;
     const uint32_t lo = p.w[2 * e], hi = p.w[2 * e + 1];
-    return u32x4{code2<DT, FMT, false>(lo), code2<DT, FMT, true>(lo), code2<DT, FMT, false>(hi),
-                 code2<DT, FMT, true>(hi)};
+    return u32x4{code2<kType, FMT, false>(lo), code2<kType, FMT, true>(lo), code2<kType, FMT, false>(hi),
+                 code2<kType, FMT, true>(hi)};
   }
 }
 
@@ -101,15 +119,6 @@ __device__ __forceinline__ u32x4 value_operand(const Piece<NB> (&v)[8], int j) {
   }
   return r;
 }
-// one value in fp32
-template <int FMT, int NB>
-__device__ __forceinline__ float value_f32(const Piece<NB>& v, int j) {
-  if constexpr (FMT == kCacheSame)
-    return __uint_as_float(v.w[j]);
-  else
-    return code4<FMT>(v.w[j >> 2])[j & 3];
-}
-
 struct AttnArgs {
   CacheArgs c;
   const uint8_t* q;
@@ -241,7 +250,7 @@ __device__ __forceinline__ uint32_t row_sees(const Row& r, int kb, int base, boo
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int key = kb + 16 * (i >> 2) + (i & 3);
-    vis |= (key < r.np) | in_span(key, r.lo, r.span) ? 1u << i : 0u;
+    vis |= ((key < r.np) | in_span(key, r.lo, r.span)) ? 1u << i : 0u;
   }
   return vis;
 }
@@ -342,7 +351,7 @@ __device__ __forceinline__ void row_out(const AttnArgs& a, int b, int t, int h, 
 // ROWS: the workgroup's waves hold a block of rows each and walk the same keys, for many rows in fp32 (whose products
 // take four times as long as their operands' loads); otherwise they hold the same rows and share the keys out.
 template <int DT, int FMT, int DP, int RT, int WAVES, bool ROWS>
-__global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) void cached_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 1 : 2)) void cached_attn_kernel(AttnArgs a) {
   using S = Shape<DT, FMT, DP>;
   constexpr int NJ = S::NJ, kRows = 16 * RT, NB = NJ * S::kElem;
   constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
@@ -380,7 +389,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
   // The queries of this lane's rows, one of each 16. They are read whatever the sequence's numbers are, which arrive
   // later.
   Row row[RT];
-  u32x4 q16[RT][S::kF32 ? 1 : S::kPieces * S::kOps];
+  u32x4 q16[RT][S::kParts][S::kF32 ? 1 : S::kPieces * S::kOps];
   float q32[RT][S::kF32 ? S::kPieces * S::kRun : 1];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -391,12 +400,12 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
 #pragma unroll
     for (int c = 0; c < S::kPieces; ++c) {
       const int i0 = 4 * S::kRun * c + S::kRun * g;
-      if (!S::kF32 && a.q_vec) {
+      if (DT != TMAC_F32 && a.q_vec) {
 #pragma unroll
         for (int e = 0; e < S::kOps; ++e) {
           u32x4 w{0, 0, 0, 0};
           if (real && i0 + 8 * e < a.c.d) w = *reinterpret_cast<const u32x4*>(src + (i0 + 8 * e) * 2);
-          q16[rt][S::kF32 ? 0 : c * S::kOps + e] = w;
+          q16[rt][0][S::kF32 ? 0 : c * S::kOps + e] = w;
         }
         continue;
       }
@@ -404,7 +413,7 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
 #pragma unroll
       for (int u = 0; u < S::kRun; ++u) x[u] = 0.f;
       if (real) {
-        if (S::kF32 && a.q_vec) {
+        if (DT == TMAC_F32 && a.q_vec) {
 #pragma unroll
           for (int u = 0; u < S::kRun; u += 4) {
             if (i0 + u >= a.c.d) continue;
@@ -427,10 +436,13 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
       } else {
 #pragma unroll
         for (int e = 0; e < S::kOps; ++e) {
-          u32x4 w;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) w[u] = Mfma<DT>::pack2(x[8 * e + 2 * u], x[8 * e + 2 * u + 1]);
-          q16[rt][c * S::kOps + e] = w;
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[S::kParts];
+            split2<S::kType, S::kParts>(x[8 * e + 2 * u], x[8 * e + 2 * u + 1], w);
+#pragma unroll
+            for (int i = 0; i < S::kParts; ++i) q16[rt][i][c * S::kOps + e][u] = w[i];
+          }
         }
       }
     }
@@ -556,10 +568,13 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
           const auto key = key_operand<DT, FMT, DP>(kp[hf][c], e);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            if constexpr (S::kF32)
+            if constexpr (S::kF32) {
               sc[rt][hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key, q32[rt][c * S::kRun + e], sc[rt][hf], 0, 0, 0);
-            else
-              sc[rt][hf] = mfma16<DT>(key, q16[rt][c * S::kOps + e], sc[rt][hf]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < S::kParts; ++i)
+                sc[rt][hf] = mfma16<S::kType>(key, q16[rt][i][c * S::kOps + e], sc[rt][hf]);
+            }
           }
         }
     }
@@ -631,27 +646,34 @@ __global__ __launch_bounds__(64 * WAVES, DT == TMAC_F32 && DP == 128 ? 1 : 2) vo
         }
       }
     }
-    u32x4 pw[RT];
+    u32x4 pw[RT][S::kParts];
     if constexpr (!S::kF32) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) pw[rt][w] = Mfma<DT>::pack2(x[rt][2 * w], x[rt][2 * w + 1]);
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w[S::kParts];
+          split2<S::kType, S::kParts>(x[rt][2 * u], x[rt][2 * u + 1], w);
+#pragma unroll
+          for (int i = 0; i < S::kParts; ++i) pw[rt][i][u] = w[i];
+        }
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       if constexpr (S::kF32) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = value_f32<FMT, NB>(vp[i], j);
+          const float v = __uint_as_float(vp[i].w[j]);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
             acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
         }
       } else {
-        const u32x4 v = value_operand<DT, FMT, NB>(vp, j);
+        const u32x4 v = value_operand<S::kType, FMT, NB>(vp, j);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16<DT>(v, pw[rt], acc[rt][j]);
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < S::kParts; ++i) acc[rt][j] = mfma16<S::kType>(v, pw[rt][i], acc[rt][j]);
       }
     }
     if (more) load_values();
@@ -887,7 +909,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
       if (part) {
         // values that no row sees may be anything: zeros
         const int key = stage0 + r;
-        const uint32_t on = (key < keys.np) | in_span(key, span_lo, span) ? ~0u : 0u;
+        const uint32_t on = ((key < keys.np) | in_span(key, span_lo, span)) ? ~0u : 0u;
 #pragma unroll
         for (int w = 0; w < 4; ++w) rv[u][w] &= on;
         if constexpr (FMT == kCacheSame) {  // rows that do not see a value must not meet what is not finite: see below
@@ -1242,7 +1264,7 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     p.n_rb = (rows + cap - 1) / cap;
     p.row_cap = rows < cap ? rows : cap;
     const int64_t blocks = heads * p.n_rb;
-    p.waves = dtype == TMAC_F32 && dp == 128 ? 4 : 8;  // 512 registers for wide fp32 rows
+    p.waves = wide(dtype, same, dp, p.rt) ? 4 : 8;
     // Half as many where the workgroups are many already and the tiles few. Eight waves with 32 rows fill a CU's
     // registers alone: 320 such blocks of 19 tiles 21.6 us, with four waves 16.7; 20 blocks 10.6 and 11.5. With 16
     // rows: 640 blocks of 17 tiles 16.6 and 14.3, of 33 tiles 34 and 37.
@@ -1283,13 +1305,13 @@ void launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     else
       cached_attn_rows_kernel<DT, FMT, DP><<<8 * a.per_xcd, 256, 0, s>>>(a);
   } else if (p.rt == 2) {
-    if constexpr (!(DT == TMAC_F32 && DP == 128)) {
+    if constexpr (!wide(DT, FMT == kCacheSame, DP, 2)) {
       if (p.waves == 8) cached_attn_kernel<DT, FMT, DP, 2, 8, false><<<grid, 64 * 8, lds, s>>>(a);
     }
     if (p.waves == 4) cached_attn_kernel<DT, FMT, DP, 2, 4, false><<<grid, 64 * 4, lds, s>>>(a);
   } else if (p.waves == 4) {
     cached_attn_kernel<DT, FMT, DP, 1, 4, false><<<grid, 64 * 4, lds, s>>>(a);
-  } else if constexpr (!(DT == TMAC_F32 && DP == 128)) {
+  } else if constexpr (!wide(DT, FMT == kCacheSame, DP, 1)) {
     cached_attn_kernel<DT, FMT, DP, 1, 8, false><<<grid, 64 * 8, lds, s>>>(a);
   }
   const int64_t rows = static_cast<int64_t>(a.B) * a.c.n_heads * a.c.T * a.G;
