@@ -44,7 +44,8 @@ def test_single_tokens(dev, H, heads, d, dtype, fmt):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("H,heads,d,T", [(2, 2, 64, 2), (4, 2, 64, 9), (3, 3, 128, 17), (5, 1, 40, 64), (2, 1, 64, 100),
-                                         (1, 1, 33, 130)])
+                                         (1, 1, 33, 130), (64, 8, 64, 130), (64, 8, 128, 70), (40, 8, 40, 100),
+                                         (32, 32, 96, 90)])
 def test_chunks(dev, H, heads, d, T, dtype, fmt):
     """Chunks that begin at every place: in the persistent rows, behind them, far behind; fewer rows than T."""
     lens = [T, T + 1, T + 40, 200, 131, T]
@@ -74,7 +75,8 @@ def trees(dev, B, T, seed, shape):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", ["tree", "any"])
-@pytest.mark.parametrize("H,heads,d,T", [(2, 2, 64, 1), (4, 2, 64, 13), (3, 1, 128, 64), (2, 2, 40, 61)])
+@pytest.mark.parametrize("H,heads,d,T", [(2, 2, 64, 1), (4, 2, 64, 13), (3, 1, 128, 64), (2, 2, 40, 61),
+                                         (96, 8, 64, 40), (64, 8, 128, 64)])
 def test_trees(dev, H, heads, d, T, shape, dtype, fmt):
     lens = [T, T + 1, T + 100, 200, 77 + T // 2]
     news = [T, T, T, T, T // 2]
@@ -102,7 +104,7 @@ def test_chain_is_a_chunk(dev, dtype, fmt):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("H,heads,d,T", [(2, 2, 64, 1), (8, 1, 128, 1), (2, 1, 64, 30)])
+@pytest.mark.parametrize("H,heads,d,T", [(2, 2, 64, 1), (8, 1, 128, 1), (2, 1, 64, 30), (32, 16, 64, 1), (24, 24, 96, 2)])
 def test_long_axis_in_parts(dev, H, heads, d, T, dtype, fmt):
     """Few rows over many keys: several workgroups share them, some without a key that is seen."""
     lens, news = [5000, 37, 3111], [T, T, max(1, T // 3)]
@@ -110,6 +112,14 @@ def test_long_axis_in_parts(dev, H, heads, d, T, dtype, fmt):
         first = run(dev, 3, H, heads, d, 64, lens, news, T, window, n_persistent, dtype, fmt, spread=2.0)
         o, q, c, table, lengths, counts = first
         assert torch.equal(o, tc.cached_attention(q, c, table, lengths, window, n_persistent, counts=counts))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_chunks_in_parts(dev, d, dtype, fmt):
+    """Many rows over many keys, of which parts see none."""
+    run(dev, 3, 64, 8, d, 32, [1500, 130, 700], [130, 130, 60], 130, 900, 16, dtype, fmt, spread=2.0)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -170,11 +180,12 @@ def test_what_a_row_does_not_see(dev, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("window,d", [(None, 64), (90, 64), (None, 128), (70, 40)])
-def test_what_rows_of_a_chunk_do_not_see(dev, dtype, window, d):
+@pytest.mark.parametrize("H,heads", [(2, 2), (48, 24)])
+def test_what_rows_of_a_chunk_do_not_see(dev, H, heads, window, d, dtype):
     """The same in a chunk of many rows: every row is as if what it does not see were not there, and what it sees reaches
     it, wherever that lies (before the chunk, in it, where all rows of some see it and not all of others)."""
-    B, H, T, lens = 2, 2, 200, [330, 200]
-    c, table, lengths = filled(dev, B, H, d, 32, lens, dtype, None, fill=NAN)
+    B, T, lens = 2, 200, [330, 200]
+    c, table, lengths = filled(dev, B, heads, d, 32, lens, dtype, None, fill=NAN)
     q = queries(dev, B, H, T, d, dtype)
     want = tc.cached_attention(q, c, table, lengths, window, 4)
     masks = seen_by(B, T, lens, [T, T], window, 4)
@@ -202,13 +213,13 @@ def test_what_rows_of_a_chunk_do_not_see(dev, dtype, window, d):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T", [3, 40, 200])
-def test_pages_that_are_none(dev, T, dtype, fmt):
+@pytest.mark.parametrize("T,H,heads", [(3, 2, 2), (40, 2, 2), (200, 2, 2), (200, 32, 8)])
+def test_pages_that_are_none(dev, T, H, heads, dtype, fmt):
     """A page outside the pool is NaN for the rows that see it and nothing to the others; so are numbers that do not
     fit for a whole sequence."""
     lens = [T + 100, T + 100, T + 20, T]
-    c, table, lengths = filled(dev, 4, 2, 64, 16, lens, dtype, fmt, fill=NAN)
-    q = queries(dev, 4, 2, T, 64, dtype)
+    c, table, lengths = filled(dev, 4, heads, 64, 16, lens, dtype, fmt, fill=NAN)
+    q = queries(dev, 4, H, T, 64, dtype)
     window, n_persistent = 50, 4
     want = tc.cached_attention(q, c, table, lengths, window, n_persistent)
     masks = seen_by(4, T, lens, [T] * 4, window, n_persistent)
@@ -226,13 +237,15 @@ def test_pages_that_are_none(dev, T, dtype, fmt):
 
 def test_a_row_of_nan_in_8_bits(dev):
     """A row that was not finite when it was written: NaN for the rows that see its key or value, nothing to the others."""
-    for fmt, dtype, T in (("int8", torch.bfloat16, 150), ("e4m3", torch.float16, 150), ("int8", torch.float16, 9),
-                          ("e4m3", torch.float32, 70)):
-        B, H, d, lens = 1, 2, 64, [T + 30]
-        c, table, lengths = filled(dev, B, H, d, 16, lens, dtype, fmt, fill=NAN)
+    for fmt, dtype, T, H, heads in (("int8", torch.bfloat16, 150, 2, 2), ("e4m3", torch.float16, 150, 2, 2),
+                                    ("int8", torch.float16, 9, 2, 2), ("e4m3", torch.float32, 70, 2, 2),
+                                    ("int8", torch.bfloat16, 150, 128, 32), ("e4m3", torch.float16, 150, 128, 32),
+                                    ("int8", torch.float32, 150, 128, 32)):
+        B, d, lens = 1, 64, [T + 30]
+        c, table, lengths = filled(dev, B, heads, d, 16, lens, dtype, fmt, fill=NAN)
         q = queries(dev, B, H, T, d, dtype)
         want = tc.cached_attention(q, c, table, lengths, 40)
-        k = torch.randn(B, H, 1, d, device=dev).to(dtype)
+        k = torch.randn(B, heads, 1, d, device=dev).to(dtype)
         pos = lens[0] - 5
         at = torch.tensor([pos + 1], dtype=torch.int32, device=dev)
         old = (c.k[table[0, pos // 16].long(), :, pos % 16].clone(), c.k_scale[table[0, pos // 16].long(), :, pos % 16].clone())

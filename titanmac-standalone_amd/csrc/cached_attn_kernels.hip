@@ -1239,24 +1239,29 @@ struct Plan {
   size_t ws;
 };
 
-// Most tiles of 16 rows that a wave holds: the registers of one whose 256 leave two waves to a SIMD.
+// How the rows (G·T of each key head and sequence) and the keys are shared out. Times in us, 16-bit unless said.
 Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np) {
   Plan p{};
   const bool same = !c.ks;
   const int dp = c.pitch <= 64 ? 64 : 128;
-  p.rt = rows <= 16 ? 1 : 2;
-  p.rows = rows > 64;
   const int64_t len = static_cast<int64_t>(c.max_pages) << c.page_shift;
   int64_t keys = window + c.T + np;
   if (keys > len) keys = len;
-  const int64_t tiles = keys / 32 + 2, heads = static_cast<int64_t>(B) * c.n_heads;
+  const int64_t tiles = keys / 32 + 2, heads = static_cast<int64_t>(B) * c.n_heads, n16 = heads * ((rows + 15) / 16);
+  // Waves with rows of their own, where there are many: 1280 tiles of 16 rows on 130 of keys 56, with the keys shared
+  // out 75; 15680 on 9 43 and 71; 1024 on 130 67 and 92; 780 on 36 23.7 and 15.0; 160 on 66 17.2 and 15.4.
+  p.rows = rows > 64 && n16 >= 1000;
+  // 32 rows a workgroup, 16 where those are few and the keys as well: 640 tiles of rows on 19 of keys 13.5 with 16, 15.6
+  // with 32; 320 on 7 7.4 and 8.5; 108 on 29 10.2 and 13.3; 1280 on 19 22.4 and 20.6; 2560 60 and 40; 128 on 130 28.8 and
+  // 24. Wide fp32 rows: 690 on 48 188 and 150.
+  p.rt = rows <= 16 || (tiles <= 48 && n16 <= (wide(dtype, same, dp, 1) ? 256 : 704)) ? 1 : 2;
   const int cap = 16 * p.rt;
   int64_t s = 1;
   if (p.rows) {
+    p.rt = 2;
     p.waves = 4;
-    p.n_rb = (rows + 4 * cap - 1) / (4 * cap);
-    // two workgroups for every CU, each with 8 tiles at least: 160 blocks of 130 tiles 121 us whole, 65 in three parts,
-    // 20 blocks of 66 tiles 60 and 24 in eight
+    p.n_rb = (rows + 127) / 128;
+    // two workgroups for every CU, each with 8 tiles at least: 160 blocks of 130 tiles 121 whole, 65 in three parts
     const int64_t blocks = heads * p.n_rb;
     s = 512 / blocks;
     if (s > tiles / 8) s = tiles / 8;
@@ -1264,13 +1269,12 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     p.n_rb = (rows + cap - 1) / cap;
     p.row_cap = rows < cap ? rows : cap;
     const int64_t blocks = heads * p.n_rb;
-    p.waves = wide(dtype, same, dp, p.rt) ? 4 : 8;
-    // Half as many where the workgroups are many already and the tiles few. Eight waves with 32 rows fill a CU's
-    // registers alone: 320 such blocks of 19 tiles 21.6 us, with four waves 16.7; 20 blocks 10.6 and 11.5. With 16
-    // rows: 640 blocks of 17 tiles 16.6 and 14.3, of 33 tiles 34 and 37.
-    if (tiles <= 4 || (p.rt == 2 ? blocks > 256 : blocks >= 512 && tiles <= 24)) p.waves = 4;
+    // Four waves a workgroup instead of eight where the tiles are few, or the workgroups many: eight waves with 32 rows
+    // fill a CU's registers alone (320 blocks of 19 tiles 21.6, with four waves 16.7; 20 blocks 10.6 and 11.5); with 16
+    // rows 640 blocks of 17 tiles 16.6 and 14.3, 504 17.2 and 12.0, 160 8.9 and 9.4, 640 of 33 34 and 37.
+    p.waves = tiles <= 8 || wide(dtype, same, dp, p.rt) || (blocks > 256 && (p.rt == 2 || tiles <= 24)) ? 4 : 8;
     // Few blocks with long axes in parts, until each CU has a workgroup of four waves (two in 8 bits, whose tiles are
-    // half as large). 10 blocks of 512 tiles 88 us whole, 14 in 25 parts; 80 of 130 tiles 25.7 and 19.4 in three; 96 of 130
+    // half as large). 10 blocks of 512 tiles 88 whole, 14 in 25 parts; 80 of 130 tiles 25.7 and 19.4 in three; 96 of 130
     // with d = 128 56 and 41 in two; 160 33 and 35 in three; in 8 bits 40 of 130 23.8 and 11.9 in 12, 160 26.0 and 23.5
     // in three, 240 30 and 35 in two. Shorter axes gain less than the second launch costs the host (10 blocks of 34 tiles
     // 9.5 and 7.9).
