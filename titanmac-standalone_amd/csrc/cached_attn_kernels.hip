@@ -76,7 +76,7 @@ struct Shape {
 // Whether a wave needs more than half of a SIMD's registers: four waves a workgroup then.
 constexpr bool wide(int dtype, bool same, int dp, int rt) { return dtype == TMAC_F32 && dp == 128 && (same || rt > 1); }
 
-// x, y as the sum of P bfloat16 pairs (P = 1: rounded to TYPE)
+// x, y as the sum of P pairs of TYPE, each the nearest to what the ones before leave
 template <int TYPE, int P>
 __device__ __forceinline__ void split2(float x, float y, uint32_t (&w)[P]) {
 #pragma unroll
@@ -450,12 +450,6 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
 
   f32x4 acc[RT][NJ];
   Soft soft[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    soft[rt] = Soft{-kInf, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
 
   const int page_mask = (1 << a.c.page_shift) - 1, pitch_b = a.c.pitch * S::kElem;
   const bool narrow = a.c.pitch < DP;
@@ -530,153 +524,217 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
       }
     }
   };
-  int key_now = 0;
-  if (tile0 < tile1) {
-    look_up(tile0);
-    key_now = key_next;
-    place();
-    load_keys();
-    load_values();
-    look_up(tile0 + kStep);
-  }
-  float v_ref = 0x1p-126f;
-  bool cleaned = false;
-
-  for (int it = tile0; it < tile1; it += kStep) {
-    const int key0 = key_now;
-    bool bad[2];
+  // With 16 rows a wave, whose time goes into the cache's reading, 16-bit probabilities are two numbers (16 bits and more
+  // of them), which leaves the result's own rounding as the only one of its size; with more rows they are rounded once.
+  // The second number may be 0 or below it, which times an infinite value is NaN where the probability's product is
+  // infinite: a wave that finds its sums not finite starts again with two equal halves, and takes those sums' results.
+  constexpr int kProbs = S::kParts > 1 ? S::kParts : RT == 1 ? 2 : 1;
+  constexpr bool kAgain = kProbs == 2 && FMT == kCacheSame;
+  bool halves_only = false, cleaned;
+  float v_ref;
+  // This wave's place in LDS: row_cap rows of kPitchO floats, so that 16 rows begin at different banks.
+  constexpr int kPitchO = DP + 4;
+  const int cap = a.row_cap;
+  float* const so = sh + wave * cap * kPitchO;
+  auto put_sums = [&](auto factor) {
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) bad[hf] = static_cast<unsigned>(page[hf]) >= static_cast<unsigned>(a.c.n_pages);
-    const bool more = it + kStep < tile1;
-    // every row sees the whole tile (rows that are none see it too: their results are not used)
-    const bool full = !bad[0] && !bad[1] && keys.all_see(key0);
-
-    if (narrow) {
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = 16 * rt + n;
+      if (r >= cap) continue;
+      float f;
+      if constexpr (std::is_same_v<decltype(factor), float>)
+        f = factor;
+      else
+        f = factor(rt);
 #pragma unroll
-      for (int c = 0; c < S::kPieces; ++c)
-        if (S::kRun * (4 * c + g) >= a.c.pitch) kp[0][c].clear(), kp[1][c].clear();
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; j += 4)
+          *reinterpret_cast<f32x4*>(so + r * kPitchO + (4 * g + i) * NJ + j) =
+              f32x4{acc[rt][j][i] * f, acc[rt][j + 1][i] * f, acc[rt][j + 2][i] * f, acc[rt][j + 3][i] * f};
     }
-    f32x4 sc[RT][2];
+  };
+  for (;;) {
+    cleaned = false;
+    v_ref = 0x1p-126f;
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int rt = 0; rt < RT; ++rt) {
+      soft[rt] = Soft{-kInf, 0.f, 0.f};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sc[rt][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < S::kPieces; ++c)
-#pragma unroll
-        for (int e = 0; e < S::kOps; ++e) {
-          const auto key = key_operand<DT, FMT, DP>(kp[hf][c], e);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            if constexpr (S::kF32) {
-              sc[rt][hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key, q32[rt][c * S::kRun + e], sc[rt][hf], 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int i = 0; i < S::kParts; ++i)
-                sc[rt][hf] = mfma16<S::kType>(key, q16[rt][i][c * S::kOps + e], sc[rt][hf]);
-            }
-          }
-        }
+      for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    float x[RT][8];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[rt][i] = sc[rt][i >> 2][i & 3];
-        if constexpr (FMT != kCacheSame) x[rt][i] *= ks[i];
-      }
-    if (more) {
+    int key_now = 0;
+    if (tile0 < tile1) {
+      look_up(tile0);
       key_now = key_next;
       place();
       load_keys();
-      look_up(it + 2 * kStep);
+      load_values();
+      look_up(tile0 + kStep);
     }
+    for (int it = tile0; it < tile1; it += kStep) {
+      const int key0 = key_now;
+      bool bad[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) bad[hf] = static_cast<unsigned>(page[hf]) >= static_cast<unsigned>(a.c.n_pages);
+      const bool more = it + kStep < tile1;
+      // every row sees the whole tile (rows that are none see it too: their results are not used)
+      const bool full = !bad[0] && !bad[1] && keys.all_see(key0);
 
-    uint32_t vis[RT];  // bit i: the row sees key i of this lane's eight
-    if (!full) {
-      const int kb = key0 + 4 * g;
+      if (narrow) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        vis[rt] = row_sees(row[rt], kb, base, tree);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
-        if (bad[0] || bad[1]) {  // a page that is none: NaN for the rows that see it
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (bad[i >> 2] && (vis[rt] >> i & 1)) x[rt][i] = __builtin_nanf("");
-        }
+        for (int c = 0; c < S::kPieces; ++c)
+          if (S::kRun * (4 * c + g) >= a.c.pitch) kp[0][c].clear(), kp[1][c].clear();
       }
-      // Values of keys that no row sees may be anything: zeros in their place. So may be those that some rows see
-      // and others do not (0 times infinity): zeros here, added after the loop for the rows that see them.
-      const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
-      const int lo = keys.hi >= keys.lo ? keys.lo : kNowhere;
+      f32x4 sc[RT][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = kb + 16 * (i >> 2) + (i & 3);
-        const uint32_t on = (((key < keys.np) | in_span(key, lo, span)) & !bad[i >> 2]) ? ~0u : 0u;
+      for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
-        for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
-        if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
-      }
-      if (FMT == kCacheSame && a.c.T > 1) {
-        uint32_t changed = 0;
+        for (int rt = 0; rt < RT; ++rt) sc[rt][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int c = 0; c < S::kPieces; ++c)
 #pragma unroll
-          for (int w = 0; w < NB / 4; ++w) {
-            const uint32_t y = finite_only<DT>(vp[i].w[w]);
-            changed |= y ^ vp[i].w[w];
-            vp[i].w[w] = y;
+          for (int e = 0; e < S::kOps; ++e) {
+            const auto key = key_operand<DT, FMT, DP>(kp[hf][c], e);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              if constexpr (S::kF32) {
+                sc[rt][hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key, q32[rt][c * S::kRun + e], sc[rt][hf], 0, 0, 0);
+              } else {
+#pragma unroll
+                for (int i = 0; i < S::kParts; ++i)
+                  sc[rt][hf] = mfma16<S::kType>(key, q16[rt][i][c * S::kOps + e], sc[rt][hf]);
+              }
+            }
           }
-        if (__any(changed != 0)) cleaned = true;
       }
-    }
-    if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      soften(soft[rt], x[rt], acc[rt], a);
-      if constexpr (FMT != kCacheSame) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
-        if (!full && a.c.T > 1) {  // 0 times a scale of NaN
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
-        }
-      }
-    }
-    u32x4 pw[RT][S::kParts];
-    if constexpr (!S::kF32) {
+      float x[RT][8];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t w[S::kParts];
-          split2<S::kType, S::kParts>(x[rt][2 * u], x[rt][2 * u + 1], w);
-#pragma unroll
-          for (int i = 0; i < S::kParts; ++i) pw[rt][i][u] = w[i];
+        for (int i = 0; i < 8; ++i) {
+          x[rt][i] = sc[rt][i >> 2][i & 3];
+          if constexpr (FMT != kCacheSame) x[rt][i] *= ks[i];
         }
-    }
+      if (more) {
+        key_now = key_next;
+        place();
+        load_keys();
+        look_up(it + 2 * kStep);
+      }
+
+      uint32_t vis[RT];  // bit i: the row sees key i of this lane's eight
+      if (!full) {
+        const int kb = key0 + 4 * g;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      if constexpr (S::kF32) {
+        for (int rt = 0; rt < RT; ++rt) {
+          vis[rt] = row_sees(row[rt], kb, base, tree);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
+          if (bad[0] || bad[1]) {  // a page that is none: NaN for the rows that see it
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (bad[i >> 2] && (vis[rt] >> i & 1)) x[rt][i] = __builtin_nanf("");
+          }
+        }
+        // Values of keys that no row sees may be anything: zeros in their place. So may be those that some rows see
+        // and others do not (0 times infinity): zeros here, added after the loop for the rows that see them.
+        const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
+        const int lo = keys.hi >= keys.lo ? keys.lo : kNowhere;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = __uint_as_float(vp[i].w[j]);
+          const int key = kb + 16 * (i >> 2) + (i & 3);
+          const uint32_t on = (((key < keys.np) | in_span(key, lo, span)) & !bad[i >> 2]) ? ~0u : 0u;
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
+          for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
+          if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
         }
-      } else {
-        const u32x4 v = value_operand<S::kType, FMT, NB>(vp, j);
+        if (FMT == kCacheSame && a.c.T > 1) {
+          uint32_t changed = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int w = 0; w < NB / 4; ++w) {
+              const uint32_t y = finite_only<DT>(vp[i].w[w]);
+              changed |= y ^ vp[i].w[w];
+              vp[i].w[w] = y;
+            }
+          if (__any(changed != 0)) cleaned = true;
+        }
+      }
+      if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        soften(soft[rt], x[rt], acc[rt], a);
+        if constexpr (FMT != kCacheSame) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
+          if (!full && a.c.T > 1) {  // 0 times a scale of NaN
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
+          }
+        }
+      }
+      u32x4 pw[RT][kProbs];
+      if constexpr (!S::kF32) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int i = 0; i < S::kParts; ++i) acc[rt][j] = mfma16<S::kType>(v, pw[rt][i], acc[rt][j]);
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[kProbs];
+            if (kAgain && halves_only)
+              w[0] = w[kProbs - 1] = Mfma<S::kType>::pack2(0.5f * x[rt][2 * u], 0.5f * x[rt][2 * u + 1]);
+            else
+              split2<S::kType, kProbs>(x[rt][2 * u], x[rt][2 * u + 1], w);
+#pragma unroll
+            for (int i = 0; i < kProbs; ++i) pw[rt][i][u] = w[i];
+          }
       }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if constexpr (S::kF32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float v = __uint_as_float(vp[i].w[j]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
+          }
+        } else {
+          const u32x4 v = value_operand<S::kType, FMT, NB>(vp, j);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<S::kType>(v, pw[rt][i], acc[rt][j]);
+        }
+      }
+      if (more) load_values();
     }
-    if (more) load_values();
+    if (!kAgain || halves_only) break;
+    float t = 0.f;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t = fmaf(acc[rt][j][i], 0.f, t);
+    if (!__any(t != t)) break;
+    halves_only = true;
+    put_sums(1.f);
+  }
+  if (kAgain && halves_only) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (16 * rt + n >= a.row_cap) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const float first = so[(16 * rt + n) * kPitchO + (4 * g + i) * NJ + j];
+          if (__builtin_isfinite(first)) acc[rt][j][i] = first;
+        }
+    }
   }
   if constexpr (kScaled16) {
 #pragma unroll
@@ -745,11 +803,8 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
     return;
   }
 
-  // The waves' results are joined in LDS: first the rows' maxima and sums, by which every wave scales what it has, then
-  // the scaled results, summed in the waves' order. Rows of kPitchO floats: 16 rows begin at different banks.
-  constexpr int kPitchO = DP + 4;
-  const int cap = a.row_cap;
-  float* const so = sh + wave * cap * kPitchO;
+  // The waves' results are joined in LDS: first the rows' references and sums, by which every wave scales what it has, then
+  // the scaled results, summed in the waves' order.
   float2* const sm = reinterpret_cast<float2*>(sh + WAVES * cap * kPitchO);  // [WAVES][cap]
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -757,21 +812,12 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
     if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], soft[rt].l};
   }
   __syncthreads();
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = 16 * rt + n;
-    if (r >= cap) continue;
+  put_sums([&](int rt) {
     float top = -kInf;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
-    const float f = m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; j += 4)
-        *reinterpret_cast<f32x4*>(so + r * kPitchO + (4 * g + i) * NJ + j) =
-            f32x4{acc[rt][j][i] * f, acc[rt][j + 1][i] * f, acc[rt][j + 2][i] * f, acc[rt][j + 3][i] * f};
-  }
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + 16 * rt + n].x);
+    return m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
+  });
   __syncthreads();
   const int live = rows_all - row0 < cap ? rows_all - row0 : cap;
   for (int u = threadIdx.x; u < live * (DP / 4); u += 64 * WAVES) {
