@@ -554,6 +554,17 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
               f32x4{acc[rt][j][i] * f, acc[rt][j + 1][i] * f, acc[rt][j + 2][i] * f, acc[rt][j + 3][i] * f};
     }
   };
+  int key_now = 0;
+  auto first_tile = [&]() {
+    if (tile0 >= tile1) return;
+    look_up(tile0);
+    key_now = key_next;
+    place();
+    load_keys();
+    load_values();
+    look_up(tile0 + kStep);
+  };
+  first_tile();
   for (;;) {
     cleaned = false;
     v_ref = 0x1p-126f;
@@ -562,15 +573,6 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
       soft[rt] = Soft{-kInf, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    int key_now = 0;
-    if (tile0 < tile1) {
-      look_up(tile0);
-      key_now = key_next;
-      place();
-      load_keys();
-      load_values();
-      look_up(tile0 + kStep);
     }
     for (int it = tile0; it < tile1; it += kStep) {
       const int key0 = key_now;
@@ -722,6 +724,7 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
     if (!__any(t != t)) break;
     halves_only = true;
     put_sums(1.f);
+    first_tile();
   }
   if (kAgain && halves_only) {
 #pragma unroll
