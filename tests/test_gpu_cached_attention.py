@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import titans_core as tc
-from cache_cases import FORMATS, E, check_attention, empty_cache, filled, gen, make_table, seen_by
+from cache_cases import FORMATS, E, check_attention, empty_cache, filled, gen, make_table, pool_rows, seen_by
 
 pytestmark = pytest.mark.gpu
 
@@ -401,3 +401,48 @@ def test_serving_step_by_step(dev):
         check_attention(got, q[:, :, :46], fresh, table, [46] * B, [46] * B, masks)
         for x, y in zip(tc.cache_read(c, table, at(46), 46), tc.cache_read(fresh, table, at(46), 46)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H,heads", [(2, 2, 2), (40, 2, 2), (200, 2, 2), (200, 128, 32)])
+def test_a_large_value_beside_small_ones(dev, T, H, heads, dtype, fmt):
+    """A value of the type's size beside values of 0.01: nothing to the rows that do not see it, nor to a row that gives it
+    a probability of e^-40."""
+    lens = [T + 60]
+    c, table, lengths = filled(dev, 1, heads, 64, 32, lens, dtype, fmt)
+    q = queries(dev, 1, H, T, 64, dtype)
+    k = torch.randn(1, heads, lens[0], 64, device=dev).to(dtype)
+    v = (torch.randn(1, heads, lens[0], 64, device=dev) * 0.01).to(dtype)
+    tc.cache_write(k, v, c, table, lengths)
+    want = tc.cached_attention(q, c, table, lengths, 50)
+    v[:, :, -1] = 60000 * torch.rand(1, heads, 64, device=dev)
+    tc.cache_write(k, v, c, table, lengths)
+    got = tc.cached_attention(q, c, table, lengths, 50)
+    assert torch.equal(got[:, :, :-1], want[:, :, :-1]) and not torch.equal(got[:, :, -1], want[:, :, -1])
+
+    ones = torch.ones(1, H, 1, 64, dtype=dtype, device=dev)
+    k[:, :, :-1], k[:, :, -1] = 1, -4   # scores of 8 and -32
+    tc.cache_write(k, v, c, table, lengths)
+    got = tc.cached_attention(ones, c, table, lengths, 50).double()
+    w = pool_rows(c, table, 0, lens[0], "v")[:, -51:-1].mean(1).repeat_interleave(H // heads, 0)[None, :, None]
+    # e^-40 60000 < 3e-13; the sum over 50 keys, two numbers of the probability (2^-16 of it) and the result's rounding
+    half = {torch.float32: 2 * E, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    assert torch.all((got - w).abs() <= half * w.abs() + 0.05 * (2.0 ** -16 + 500 * E) + 2.0 ** -25 * (dtype == torch.float16)
+                     + 3e-13)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_draft_of_one(dev, dtype, fmt):
+    """A drafted row that does not see itself, and one whose window ends at a row that is not finite."""
+    window, base = 20, 60
+    for bits, pos in ((0, base), (1, base - 1 - window)):  # entry, position that it does not see
+        c, table, lengths = filled(dev, 1, 2, 64, 16, [base + 1], dtype, fmt)
+        q = queries(dev, 1, 4, 1, 64, dtype)
+        tree = torch.tensor([[bits]])
+        want = tc.cached_attention(q, c, table, lengths, window, tree=tree.to(dev))
+        check_attention(want, q, c, table, [base + 1], [1], seen_by(1, 1, [base + 1], [1], window, 0, tree))
+        for x in (c.k, c.v) if fmt is None else (c.k_scale, c.v_scale):
+            x[table[0, pos // 16].long(), :, pos % 16] = NAN
+        assert torch.equal(tc.cached_attention(q, c, table, lengths, window, tree=tree.to(dev)), want)

@@ -60,12 +60,15 @@ struct Piece {
 //
 // fp32 on codes of 8 bits runs on the 16-bit matrix cores all the same: a code is exact in bfloat16, and an fp32 value is
 // the sum of three bfloat16 numbers (8 bits each of its 24), so three products give what an fp32 one gives, in a fifth
-// of its time.
+// of its time. fp16 probabilities times a value's scale leave fp16's range (a small row's where a large one is also
+// held), so those are two bfloat16 numbers, which have fp32's.
 template <int DT, int FMT, int DP>
 struct Shape {
   static constexpr bool kF32 = DT == TMAC_F32 && FMT == kCacheSame;  // fp32 products
   static constexpr int kType = DT == TMAC_F32 ? TMAC_BF16 : DT;      // of the others
   static constexpr int kParts = DT == TMAC_F32 && FMT != kCacheSame ? 3 : 1;
+  static constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
+  static constexpr int kProbType = kScaled16 ? TMAC_BF16 : kType;    // of the second product
   static constexpr int kElem = FMT != kCacheSame ? 1 : DT == TMAC_F32 ? 4 : 2;  // bytes of a stored value
   static constexpr int kRun = 16 / kElem;           // values in 16 bytes: a lane's piece of a key
   static constexpr int kPieces = DP / (4 * kRun);   // of each key, per lane; piece c of group g: 4 kRun c + kRun g ..
@@ -297,29 +300,6 @@ __device__ __forceinline__ float soft_join(Soft& s) {
   return s.lim == -kInf && s.l == s.l ? -kInf : s.mu;
 }
 
-// A power of two above every scale vs so far, for fp16 probabilities times a scale (v_ref); what was summed up before
-// moves to it, and vs becomes relative to it.
-template <int RT, int NJ>
-__device__ __forceinline__ void relate_scales(float& v_ref, float (&vs)[8], f32x4 (&acc)[RT][NJ]) {
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(vs[i]));
-  if (__any(top > v_ref)) {
-    top = fmaxf(top, lane_xor<16>(top));
-    top = fmaxf(top, lane_xor<32>(top));
-    const float to = __uint_as_float(((__float_as_uint(top) >> 23) + (top < 0x1p126f)) << 23);
-    const float f = v_ref / to;
-    v_ref = to;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
-  }
-  const float inv = 1.f / v_ref;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] *= inv;
-}
-
 // o / sum; zeros for a row that sees nothing or is none, NaN where the sequence's numbers do not fit
 template <int N>
 __device__ __forceinline__ void row_finish(const Seq& s, int t, float sum, float (&o)[N]) {
@@ -354,7 +334,6 @@ template <int DT, int FMT, int DP, int RT, int WAVES, bool ROWS>
 __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 1 : 2)) void cached_attn_kernel(AttnArgs a) {
   using S = Shape<DT, FMT, DP>;
   constexpr int NJ = S::NJ, kRows = 16 * RT, NB = NJ * S::kElem;
-  constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
   extern __shared__ float sh[];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -377,6 +356,7 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
   const Keys<5> keys = keys_of(a, s, t_lo, t_end < s.n - 1 ? t_end : s.n - 1);
   const int base = s.len - s.n, len = s.len;
   const bool tree = a.tree != nullptr;
+  const bool mixed = a.c.T > 1 || tree;  // some rows may not see all of [lo, hi]
   int tile0 = 0, tile1 = keys.n_tiles;
   if (a.splits > 1) {
     const int per = (keys.n_tiles + a.splits - 1u) / static_cast<unsigned>(a.splits);
@@ -528,10 +508,9 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
   // of them), which leaves the result's own rounding as the only one of its size; with more rows they are rounded once.
   // The second number may be 0 or below it, which times an infinite value is NaN where the probability's product is
   // infinite: a wave that finds its sums not finite starts again with two equal halves, and takes those sums' results.
-  constexpr int kProbs = S::kParts > 1 ? S::kParts : RT == 1 ? 2 : 1;
+  constexpr int kProbs = S::kF32 ? 1 : S::kParts > 1 ? S::kParts : RT == 1 || S::kScaled16 ? 2 : 1;
   constexpr bool kAgain = kProbs == 2 && FMT == kCacheSame;
   bool halves_only = false, cleaned;
-  float v_ref;
   // This wave's place in LDS: row_cap rows of kPitchO floats, so that 16 rows begin at different banks.
   constexpr int kPitchO = DP + 4;
   const int cap = a.row_cap;
@@ -567,7 +546,6 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
   first_tile();
   for (;;) {
     cleaned = false;
-    v_ref = 0x1p-126f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       soft[rt] = Soft{-kInf, 0.f, 0.f};
@@ -652,7 +630,7 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
           for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
           if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
         }
-        if (FMT == kCacheSame && a.c.T > 1) {
+        if (FMT == kCacheSame && mixed) {
           uint32_t changed = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -665,14 +643,13 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
           if (__any(changed != 0)) cleaned = true;
         }
       }
-      if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         soften(soft[rt], x[rt], acc[rt], a);
         if constexpr (FMT != kCacheSame) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
-          if (!full && a.c.T > 1) {  // 0 times a scale of NaN
+          if (!full && mixed) {  // 0 times a scale of NaN
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
           }
@@ -686,9 +663,9 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
           for (int u = 0; u < 4; ++u) {
             uint32_t w[kProbs];
             if (kAgain && halves_only)
-              w[0] = w[kProbs - 1] = Mfma<S::kType>::pack2(0.5f * x[rt][2 * u], 0.5f * x[rt][2 * u + 1]);
+              w[0] = w[kProbs - 1] = Mfma<S::kProbType>::pack2(0.5f * x[rt][2 * u], 0.5f * x[rt][2 * u + 1]);
             else
-              split2<S::kType, kProbs>(x[rt][2 * u], x[rt][2 * u + 1], w);
+              split2<S::kProbType, kProbs>(x[rt][2 * u], x[rt][2 * u + 1], w);
 #pragma unroll
             for (int i = 0; i < kProbs; ++i) pw[rt][i][u] = w[i];
           }
@@ -704,11 +681,11 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
               acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
           }
         } else {
-          const u32x4 v = value_operand<S::kType, FMT, NB>(vp, j);
+          const u32x4 v = value_operand<S::kProbType, FMT, NB>(vp, j);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<S::kType>(v, pw[rt][i], acc[rt][j]);
+            for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<S::kProbType>(v, pw[rt][i], acc[rt][j]);
         }
       }
       if (more) load_values();
@@ -738,12 +715,6 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
           if (__builtin_isfinite(first)) acc[rt][j][i] = first;
         }
     }
-  }
-  if constexpr (kScaled16) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[rt][j] *= v_ref;
   }
   if (FMT == kCacheSame && cleaned) {
     // What was taken for zeros and is not finite, to the rows that see it.
@@ -860,8 +831,9 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
 template <int DT, int FMT, int DP>
 __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
   constexpr int RT = 2, kWaves = 4, kRows = 16 * RT, NJ = DP / 16, kPieces = DP / 32, kHalves = DP / 64;
+  using S = Shape<DT, FMT, DP>;
+  constexpr int kProbType = S::kProbType, kProbs = S::kScaled16 ? 2 : 1;
   constexpr int kKeys = 64, kHalfTile = kKeys * 64, kTile = kHalves * kHalfTile;  // of 16-bit values
-  constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
   // a thread's share of a stage: kLoads pieces of 16 bytes of keys and as many of values
   constexpr int kElem = FMT == kCacheSame ? 2 : 1, kChunks = DP * kElem / 16, kLoads = kKeys * kChunks / 256;
   static_assert(kLoads >= 1, "a stage gives every thread a piece");
@@ -986,8 +958,8 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
           for (int w = 0; w < 2; ++w) {
             x[2 * w] = code2<DT, FMT, false>(rk[u][2 * h + w]);
             x[2 * w + 1] = code2<DT, FMT, true>(rk[u][2 * h + w]);
-            y[2 * w] = code2<DT, FMT, false>(rv[u][2 * h + w]);
-            y[2 * w + 1] = code2<DT, FMT, true>(rv[u][2 * h + w]);
+            y[2 * w] = code2<kProbType, FMT, false>(rv[u][2 * h + w]);
+            y[2 * w + 1] = code2<kProbType, FMT, true>(rv[u][2 * h + w]);
           }
           if (bad[u]) x = u32x4{kNan2, kNan2, kNan2, kNan2};
           const int chunk = 2 * piece + h, to = (chunk >> 3) * kHalfTile + swz64(r, chunk & 7);
@@ -1039,7 +1011,6 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  float v_ref = 0x1p-126f;
 
   if (threadIdx.x == 0) s_cleaned = 0;
   __syncthreads();
@@ -1110,8 +1081,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
             if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
         }
       }
-      if constexpr (kScaled16) relate_scales(v_ref, vs, acc);
-      u32x4 pw[RT];
+      u32x4 pw[RT][kProbs];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         soften(soft[rt], x[rt], acc[rt], a);
@@ -1124,22 +1094,23 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
           }
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) pw[rt][w] = Mfma<DT>::pack2(x[rt][2 * w], x[rt][2 * w + 1]);
+        for (int w = 0; w < 4; ++w) {
+          uint32_t y[kProbs];
+          split2<kProbType, kProbs>(x[rt][2 * w], x[rt][2 * w + 1], y);
+#pragma unroll
+          for (int i = 0; i < kProbs; ++i) pw[rt][i][w] = y[i];
+        }
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const u32x4 v = lds_read_tr4x2_swz64(&sv[st][(j >> 2) * kHalfTile], sub + 4 * g, sub + 16 + 4 * g, 16 * (j & 3), lane);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16<DT>(v, pw[rt], acc[rt][j]);
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<kProbType>(v, pw[rt][i], acc[rt][j]);
       }
     }
     __syncthreads();
-  }
-  if constexpr (kScaled16) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[rt][j] *= v_ref;
   }
   if (FMT == kCacheSame && s_cleaned) {
     // What was taken for zeros and is not finite, to the rows that see it.
