@@ -151,3 +151,22 @@ def test_captured_steps(dev):
         torch.cuda.synchronize()
         assert torch.equal(out, m.decode(ids[:, t:t + 1], eager)), t
         assert torch.equal(held.lengths, eager.lengths)
+
+
+def test_a_draft_s_counts_are_the_state_s(dev):
+    """The counts of a draft may be in a buffer that is used again; a path longer than a sequence's draft keeps no more."""
+    m = model(dev)
+    ids = torch.randint(0, 211, (2, 30), device=dev)
+    tree = torch.tensor([0b1, 0b11, 0b111], device=dev)
+    counts = torch.tensor([3, 2], dtype=torch.int32, device=dev)
+    state = m.new_decode_state(2, 64)
+    m.decode(ids[:, :20], state)
+    m.decode(ids[:, 20:23], state, counts=counts, tree=tree)
+    counts.fill_(1)
+    state.keep(torch.tensor([[0, 1, 2], [0, 1, 2]], dtype=torch.int32, device=dev))
+    assert state.lengths.tolist() == [5 + 23, 5 + 22]
+    rest = torch.stack([ids[0, 23:28], ids[1, 22:27]])
+    got = m.decode(rest, state)
+    with torch.no_grad():
+        want = m(ids)["logits"]
+    assert close(got[0], want[0, 23:28], torch.float32) and close(got[1], want[1, 22:27], torch.float32)

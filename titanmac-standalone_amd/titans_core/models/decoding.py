@@ -35,10 +35,10 @@ class DecodeState:
             raise RuntimeError("DecodeState: the last call's draft was not settled: call keep()")
         if self.used + T > self.room:
             raise ValueError(f"DecodeState: {self.used} tokens are held and {T} more do not fit in {self.room}")
-        self.used += T
         self.lengths.add_(T if counts is None else counts)
+        self.used += T
         if draft:
-            self._draft = T if counts is None else counts
+            self._draft = T if counts is None else counts.clone()  # the caller's may be a buffer that changes
             self._draft_rows = T
 
     def keep(self, path: torch.Tensor) -> None:
@@ -53,6 +53,8 @@ class DecodeState:
             for cache in self.caches:
                 cache_keep(cache, self.table, self.lengths, path, self._draft)
             kept = (path >= 0).sum(1, dtype=torch.int32)
+            if isinstance(self._draft, torch.Tensor):
+                kept = torch.minimum(kept, self._draft)  # places behind a shorter draft are none
             self.lengths.add_(kept - self._draft)
         self.used += path.shape[1] - self._draft_rows
         self._draft = None

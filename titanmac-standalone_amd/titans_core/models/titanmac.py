@@ -475,8 +475,8 @@ class TitanMAC(nn.Module):
                              f"{tuple(tree.shape)}")
         place = torch.arange(T, device=input_ids.device) if tree is None else draft_depths(tree)
         positions = (state.lengths - state.n_persistent).unsqueeze(1) + place
-        state._advance(T, counts, tree is not None)
         x = self._embed_at(input_ids, positions)
+        state._advance(T, counts, tree is not None)
         for layer, cache in zip(self.layers, state.caches):
             x = layer.forward_cached(x, cache, state.table, state.lengths, counts=counts, tree=tree)
         if last:
@@ -499,7 +499,7 @@ class TitanMAC(nn.Module):
     def generate(self, input_ids: torch.Tensor, n_tokens: int, *, counts: Optional[torch.Tensor] = None,
                  fmt: Optional[str] = None) -> torch.Tensor:
         """The n_tokens [B, n_tokens] that follow the prompts input_ids [B, T] if each is the likeliest (ties: the lower
-        id). counts (int32 [B]): the prompts' lengths; fmt: how keys and values are held (``new_decode_state``)."""
+        id). counts (int32 [B]): the prompts' lengths, at least 1; fmt: how keys and values are held (``new_decode_state``)."""
         B, T = input_ids.shape
         if T < 1 or n_tokens < 0:
             raise ValueError(f"generate: needs prompts and n_tokens >= 0, got {tuple(input_ids.shape)}, {n_tokens}")
