@@ -276,3 +276,14 @@ def test_decoding_refusals():
     block = tc.TitanBlock(config(use_block_sparse=True))
     with pytest.raises(ValueError, match="use_block_sparse"):
         block.forward_cached(torch.zeros(1, 1, 32), None, None, None)
+
+
+def test_pools_without_versions():
+    """Pools made in inference mode have no version to move on; those beside them do."""
+    with torch.inference_mode():
+        a = torch.zeros(2, H, 16, 48, dtype=torch.bfloat16)
+    b = torch.zeros(2, H, 16, 48, dtype=torch.bfloat16)
+    for k, v in ((a, a.clone()), (a, b), (b, a)):
+        at = b._version
+        kc._changed(tc.KVCache(k, v, D))
+        assert b._version == at + (k is b or v is b)

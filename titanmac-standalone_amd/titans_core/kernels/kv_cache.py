@@ -89,7 +89,8 @@ class KVCache(tuple):
             k_scale = v_scale = None
             changing = (k, v)
         return tuple.__new__(cls, (k, v, k_scale, v_scale, d, fmt, heads, shape, device, changing,
-                                   dtype if fmt == SAME else None, (1 << 30) // page))
+                                   dtype if fmt == SAME else None, (1 << 30) // page,
+                                   tuple(t for t in changing if not t.is_inference())))  # those have no version
 
     def __getnewargs__(self):
         return self.k, self.v, self.d_head, self.k_scale, self.v_scale
@@ -190,10 +191,7 @@ def _arg(cache: KVCache, table, pitch: int, lengths, counts, dtype: torch.dtype)
 
 def _changed(cache: KVCache) -> None:
     """What autograd (or a caller's own cache) keeps of the pools is out of date."""
-    tensors = cache[9]
-    if tensors[0].is_inference():
-        tensors = [t for t in tensors if not t.is_inference()]
-    torch.autograd.graph.increment_version(tensors)
+    torch.autograd.graph.increment_version(cache[12])
 
 
 # ------------------------------------------------------------------ write
