@@ -543,6 +543,145 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
     load_values();
     look_up(tile0 + kStep);
   };
+  // One tile; `more`: the next one's loads are issued on the way. The last tile is code of its own: as a condition in one loop
+  // the loads' registers were copied at its end, which waited for them there.
+  auto one_tile = [&](int it, auto more) {
+    const int key0 = key_now;
+    bool bad[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) bad[hf] = static_cast<unsigned>(page[hf]) >= static_cast<unsigned>(a.c.n_pages);
+    // every row sees the whole tile (rows that are none see it too: their results are not used)
+    const bool full = !bad[0] && !bad[1] && keys.all_see(key0);
+
+    if (narrow) {
+#pragma unroll
+      for (int c = 0; c < S::kPieces; ++c)
+        if (S::kRun * (4 * c + g) >= a.c.pitch) kp[0][c].clear(), kp[1][c].clear();
+    }
+    f32x4 sc[RT][2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sc[rt][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < S::kPieces; ++c)
+#pragma unroll
+        for (int e = 0; e < S::kOps; ++e) {
+          const auto key = key_operand<DT, FMT, DP>(kp[hf][c], e);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            if constexpr (S::kF32) {
+              sc[rt][hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key, q32[rt][c * S::kRun + e], sc[rt][hf], 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int i = 0; i < S::kParts; ++i)
+                sc[rt][hf] = mfma16<S::kType>(key, q16[rt][i][c * S::kOps + e], sc[rt][hf]);
+            }
+          }
+        }
+    }
+    float x[RT][8];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[rt][i] = sc[rt][i >> 2][i & 3];
+        if constexpr (FMT != kCacheSame) x[rt][i] *= ks[i];
+      }
+    if constexpr (decltype(more)::value) {
+      key_now = key_next;
+      place();
+      load_keys();
+      look_up(it + 2 * kStep);
+    }
+
+    uint32_t vis[RT];  // bit i: the row sees key i of this lane's eight
+    if (!full) {
+      const int kb = key0 + 4 * g;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        vis[rt] = row_sees(row[rt], kb, base, tree);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
+        if (bad[0] || bad[1]) {  // a page that is none: NaN for the rows that see it
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (bad[i >> 2] && (vis[rt] >> i & 1)) x[rt][i] = __builtin_nanf("");
+        }
+      }
+      // Values of keys that no row sees may be anything: zeros in their place. So may be those that some rows see
+      // and others do not (0 times infinity): zeros here, added after the loop for the rows that see them.
+      const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
+      const int lo = keys.hi >= keys.lo ? keys.lo : kNowhere;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = kb + 16 * (i >> 2) + (i & 3);
+        const uint32_t on = (((key < keys.np) | in_span(key, lo, span)) & !bad[i >> 2]) ? ~0u : 0u;
+#pragma unroll
+        for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
+        if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
+      }
+      if (FMT == kCacheSame && mixed) {
+        uint32_t changed = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int w = 0; w < NB / 4; ++w) {
+            const uint32_t y = finite_only<DT>(vp[i].w[w]);
+            changed |= y ^ vp[i].w[w];
+            vp[i].w[w] = y;
+          }
+        if (__any(changed != 0)) cleaned = true;
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      soften(soft[rt], x[rt], acc[rt], a);
+      if constexpr (FMT != kCacheSame) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
+        if (!full && mixed) {  // 0 times a scale of NaN
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
+        }
+      }
+    }
+    u32x4 pw[RT][kProbs];
+    if constexpr (!S::kF32) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w[kProbs];
+          if (kAgain && halves_only)
+            w[0] = w[kProbs - 1] = Mfma<S::kProbType>::pack2(0.5f * x[rt][2 * u], 0.5f * x[rt][2 * u + 1]);
+          else
+            split2<S::kProbType, kProbs>(x[rt][2 * u], x[rt][2 * u + 1], w);
+#pragma unroll
+          for (int i = 0; i < kProbs; ++i) pw[rt][i][u] = w[i];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if constexpr (S::kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = __uint_as_float(vp[i].w[j]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
+        }
+      } else {
+        const u32x4 v = value_operand<S::kProbType, FMT, NB>(vp, j);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<S::kProbType>(v, pw[rt][i], acc[rt][j]);
+      }
+    }
+    if constexpr (decltype(more)::value) load_values();
+  };
   first_tile();
   for (;;) {
     cleaned = false;
@@ -552,143 +691,10 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int it = tile0; it < tile1; it += kStep) {
-      const int key0 = key_now;
-      bool bad[2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) bad[hf] = static_cast<unsigned>(page[hf]) >= static_cast<unsigned>(a.c.n_pages);
-      const bool more = it + kStep < tile1;
-      // every row sees the whole tile (rows that are none see it too: their results are not used)
-      const bool full = !bad[0] && !bad[1] && keys.all_see(key0);
-
-      if (narrow) {
-#pragma unroll
-        for (int c = 0; c < S::kPieces; ++c)
-          if (S::kRun * (4 * c + g) >= a.c.pitch) kp[0][c].clear(), kp[1][c].clear();
-      }
-      f32x4 sc[RT][2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sc[rt][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < S::kPieces; ++c)
-#pragma unroll
-          for (int e = 0; e < S::kOps; ++e) {
-            const auto key = key_operand<DT, FMT, DP>(kp[hf][c], e);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              if constexpr (S::kF32) {
-                sc[rt][hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(key, q32[rt][c * S::kRun + e], sc[rt][hf], 0, 0, 0);
-              } else {
-#pragma unroll
-                for (int i = 0; i < S::kParts; ++i)
-                  sc[rt][hf] = mfma16<S::kType>(key, q16[rt][i][c * S::kOps + e], sc[rt][hf]);
-              }
-            }
-          }
-      }
-      float x[RT][8];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[rt][i] = sc[rt][i >> 2][i & 3];
-          if constexpr (FMT != kCacheSame) x[rt][i] *= ks[i];
-        }
-      if (more) {
-        key_now = key_next;
-        place();
-        load_keys();
-        look_up(it + 2 * kStep);
-      }
-
-      uint32_t vis[RT];  // bit i: the row sees key i of this lane's eight
-      if (!full) {
-        const int kb = key0 + 4 * g;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          vis[rt] = row_sees(row[rt], kb, base, tree);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (!(vis[rt] >> i & 1)) x[rt][i] = -kInf;
-          if (bad[0] || bad[1]) {  // a page that is none: NaN for the rows that see it
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (bad[i >> 2] && (vis[rt] >> i & 1)) x[rt][i] = __builtin_nanf("");
-          }
-        }
-        // Values of keys that no row sees may be anything: zeros in their place. So may be those that some rows see
-        // and others do not (0 times infinity): zeros here, added after the loop for the rows that see them.
-        const uint32_t span = keys.hi >= keys.lo ? keys.hi - keys.lo : 0;
-        const int lo = keys.hi >= keys.lo ? keys.lo : kNowhere;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = kb + 16 * (i >> 2) + (i & 3);
-          const uint32_t on = (((key < keys.np) | in_span(key, lo, span)) & !bad[i >> 2]) ? ~0u : 0u;
-#pragma unroll
-          for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
-          if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
-        }
-        if (FMT == kCacheSame && mixed) {
-          uint32_t changed = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int w = 0; w < NB / 4; ++w) {
-              const uint32_t y = finite_only<DT>(vp[i].w[w]);
-              changed |= y ^ vp[i].w[w];
-              vp[i].w[w] = y;
-            }
-          if (__any(changed != 0)) cleaned = true;
-        }
-      }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        soften(soft[rt], x[rt], acc[rt], a);
-        if constexpr (FMT != kCacheSame) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
-          if (!full && mixed) {  // 0 times a scale of NaN
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[rt][i] = vis[rt] >> i & 1 ? x[rt][i] : 0.f;
-          }
-        }
-      }
-      u32x4 pw[RT][kProbs];
-      if constexpr (!S::kF32) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w[kProbs];
-            if (kAgain && halves_only)
-              w[0] = w[kProbs - 1] = Mfma<S::kProbType>::pack2(0.5f * x[rt][2 * u], 0.5f * x[rt][2 * u + 1]);
-            else
-              split2<S::kProbType, kProbs>(x[rt][2 * u], x[rt][2 * u + 1], w);
-#pragma unroll
-            for (int i = 0; i < kProbs; ++i) pw[rt][i][u] = w[i];
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if constexpr (S::kF32) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = __uint_as_float(vp[i].w[j]);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              acc[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, x[rt][i], acc[rt][j], 0, 0, 0);
-          }
-        } else {
-          const u32x4 v = value_operand<S::kProbType, FMT, NB>(vp, j);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<S::kProbType>(v, pw[rt][i], acc[rt][j]);
-        }
-      }
-      if (more) load_values();
+    if (tile0 < tile1) {
+      int it = tile0;
+      for (; it + kStep < tile1; it += kStep) one_tile(it, std::true_type{});
+      one_tile(it, std::false_type{});
     }
     if (!kAgain || halves_only) break;
     float t = 0.f;
@@ -1001,6 +1007,8 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
         for (int u = 0; u < 4; ++u) w[u] = Mfma<DT>::pack2(x[2 * u], x[2 * u + 1]);
       }
       q[rt][c] = w;
+      // in registers before the loop: a wait for them inside would be one for the stages on their way
+      asm volatile("" : "+v"(q[rt][c]));
     }
   }
   f32x4 acc[RT][NJ];
@@ -1271,8 +1279,8 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
   // Waves with rows of their own, where there are many: 1280 tiles of 16 rows on 130 of keys 56, with the keys shared
   // out 75; 15680 on 9 43 and 71; 1024 on 130 67 and 92; 780 on 36 23.7 and 15.0; 160 on 66 17.2 and 15.4.
   p.rows = rows > 64 && n16 >= 1000;
-  // 32 rows a workgroup, 16 where those are few and the keys as well: 640 tiles of rows on 19 of keys 13.5 with 16, 15.6
-  // with 32; 320 on 7 7.4 and 8.5; 108 on 29 10.2 and 13.3; 1280 on 19 22.4 and 20.6; 2560 60 and 40; 128 on 130 28.8 and
+  // 32 rows a workgroup, 16 where those are few and the keys as well: 640 tiles of rows on 19 of keys 14.5 with 16, 15.6
+  // with 32; 320 on 7 7.6 and 9.0; 108 on 29 10.6 and 13.5; 1280 on 19 23.5 and 20.7; 2560 62 and 40; 128 on 130 31 and
   // 24. Wide fp32 rows: 690 on 48 188 and 150.
   p.rt = rows <= 16 || (tiles <= 48 && n16 <= (wide(dtype, same, dp, 1) ? 256 : 704)) ? 1 : 2;
   const int cap = 16 * p.rt;
@@ -1291,7 +1299,7 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     const int64_t blocks = heads * p.n_rb;
     // Four waves a workgroup instead of eight where the tiles are few, or the workgroups many: eight waves with 32 rows
     // fill a CU's registers alone (320 blocks of 19 tiles 21.6, with four waves 16.7; 20 blocks 10.6 and 11.5); with 16
-    // rows 640 blocks of 17 tiles 16.6 and 14.3, 504 17.2 and 12.0, 160 8.9 and 9.4, 640 of 33 34 and 37.
+    // rows 640 blocks of 17 tiles 16.6 and 14.3, 504 17.2 and 12.0, 160 9.6 and 10.9, 640 of 33 37.0 and 38.4.
     p.waves = tiles <= 8 || wide(dtype, same, dp, p.rt) || (blocks > 256 && (p.rt == 2 || tiles <= 24)) ? 4 : 8;
     // Few blocks with long axes in parts, until each CU has a workgroup of four waves (two in 8 bits, whose tiles are
     // half as large). 10 blocks of 512 tiles 88 whole, 14 in 25 parts; 80 of 130 tiles 25.7 and 19.4 in three; 96 of 130
