@@ -170,3 +170,20 @@ def test_a_draft_s_counts_are_the_state_s(dev):
     with torch.no_grad():
         want = m(ids)["logits"]
     assert close(got[0], want[0, 23:28], torch.float32) and close(got[1], want[1, 22:27], torch.float32)
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_inside_autocast(dev, fmt):
+    """As forward inside it: projections and caches in bfloat16 (or codes of it), the rest as the parameters are."""
+    m = model(dev)
+    ids = torch.randint(0, 211, (2, 40), device=dev)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        want = m(ids)["logits"]
+        state = m.new_decode_state(2, fmt=fmt)
+        got = torch.cat([m.decode(ids[:, a:b], state) for a, b in ((0, 25), (25, 26), (26, 40))], 1)
+        assert m.generate(ids, 3, fmt=fmt).shape == (2, 3)
+    assert state.caches[0].k.dtype == (torch.bfloat16 if fmt is None else torch.int8) and got.dtype == want.dtype
+    if fmt is None:
+        assert close(got, want, torch.bfloat16)
+    else:  # int8 rows are off by half of a 127th of the row's largest value, a bfloat16 step's size
+        assert (got.float() - want.float()).norm() <= (33 * 2.0 ** -8 + 3 * 11 / 254) * want.float().norm()

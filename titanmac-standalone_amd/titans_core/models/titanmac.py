@@ -426,9 +426,9 @@ class TitanMAC(nn.Module):
     def new_decode_state(self, batch: int, max_tokens: Optional[int] = None, *, fmt: Optional[str] = None,
                          page: int = 64) -> DecodeState:
         """Empty caches for ``batch`` sequences of up to max_tokens (default: max_seq_len) tokens, with the persistent rows
-        already in them. fmt: None holds keys and values in the model's type, "int8" and "e4m3" in 8 bits with a
-        scale per row (``KVCache``). For models of causal WindowedAttention (use_block_sparse=False) without a neural
-        memory."""
+        already in them. fmt: None holds keys and values in the model's type (made inside ``torch.autocast``: in
+        autocast's; decode inside it then too), "int8" and "e4m3" in 8 bits with a scale per row (``KVCache``). For models
+        of causal WindowedAttention (use_block_sparse=False) without a neural memory."""
         cfg = self.config
         if self.neural_memory is not None:
             raise ValueError("new_decode_state: a neural memory's tokens depend on whole segments; there is no cache of it")
@@ -441,7 +441,9 @@ class TitanMAC(nn.Module):
                              f"{room}")
         w, Np = self.embed_tokens.weight, self._n_persistent()
         per = -(-(Np + room) // page)
-        caches = [KVCache.new(batch * per, cfg.n_heads, cfg.d_head, page=page, dtype=w.dtype, fmt=fmt, device=w.device)
+        dev = w.device.type
+        dtype = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else w.dtype  # the projections' outputs
+        caches = [KVCache.new(batch * per, cfg.n_heads, cfg.d_head, page=page, dtype=dtype, fmt=fmt, device=w.device)
                   for _ in self.layers]
         table = torch.arange(batch * per, dtype=torch.int32, device=w.device).view(batch, per)
         state = DecodeState(caches, table, torch.full((batch,), Np, dtype=torch.int32, device=w.device), Np, room)
