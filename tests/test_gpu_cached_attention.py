@@ -446,3 +446,23 @@ def test_a_draft_of_one(dev, dtype, fmt):
         for x in (c.k, c.v) if fmt is None else (c.k_scale, c.v_scale):
             x[table[0, pos // 16].long(), :, pos % 16] = NAN
         assert torch.equal(tc.cached_attention(q, c, table, lengths, window, tree=tree.to(dev)), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H,heads", [(9, 2, 2), (40, 2, 2), (200, 128, 32)])
+def test_codes_that_are_none(dev, T, H, heads, dtype):
+    """e4m3 codes of NaN in pools that cache_write has not filled: NaN in their column for the rows that see them, nothing to
+    the others."""
+    lens = [T + 100]
+    c, table, lengths = filled(dev, 1, heads, 64, 32, lens, dtype, "e4m3")
+    q = queries(dev, 1, H, T, 64, dtype)
+    want = tc.cached_attention(q, c, table, lengths, 50, 4)
+    mask = seen_by(1, T, lens, [T], 50, 4)[0].to(dev)
+    spots = [lens[0] - 4, lens[0] - T + 2, lens[0] - T - 50]  # row 1 sees none of them
+    for pos, code in zip(spots, (0x7f, 0xff, 0x7f)):
+        c.v.view(torch.uint8)[table[0, pos // 32].long(), :, pos % 32, 3] = code
+    got = tc.cached_attention(q, c, table, lengths, 50, 4)
+    hit = mask[:, spots].any(-1)
+    assert hit.any() and (~hit).any()
+    assert torch.isnan(got[0][:, hit][..., 3]).all() and torch.equal(got[0][:, hit][..., 4:], want[0][:, hit][..., 4:])
+    assert torch.equal(got[0][:, ~hit], want[0][:, ~hit])

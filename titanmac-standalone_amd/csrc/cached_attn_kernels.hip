@@ -237,13 +237,30 @@ __device__ __forceinline__ Keys<SH> keys_of(const AttnArgs& a, const Seq& s, int
   return k;
 }
 
-// w with what is not finite in it (two 16-bit values, or one fp32) replaced by zeros
-template <int DT>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-  if constexpr (DT == TMAC_F32) return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+// Two 16-bit values, one fp32, or four codes: the top bit of each that is not finite (any bit for fp32), and w with
+// zeros in their place.
+template <int DT, int FMT>
+__device__ __forceinline__ uint32_t not_finite_bits(uint32_t w) {
+  if constexpr (FMT == kCacheE4m3) return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  if constexpr (DT == TMAC_F32) return (w & 0x7f800000u) == 0x7f800000u;
   constexpr uint32_t kExp = DT == TMAC_BF16 ? 0x7f807f80u : 0x7c007c00u, kLow = DT == TMAC_BF16 ? 0x00800080u : 0x04000400u;
-  const uint32_t top = ((w & kExp) + kLow) & 0x80008000u;  // the top bit of a half whose exponent is all ones
-  return w & ~((top >> 15) * 0xffffu);
+  return ((w & kExp) + kLow) & 0x80008000u;
+}
+template <int DT, int FMT>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  const uint32_t t = not_finite_bits<DT, FMT>(w);
+  if constexpr (FMT == kCacheE4m3) return w & ~((t >> 7) * 0xffu);
+  if constexpr (DT == TMAC_F32) return t ? 0u : w;
+  return w & ~((t >> 15) * 0xffffu);
+}
+
+// What finite_only takes from a stored value: the value, if it is not finite, or 0.
+template <int DT, int FMT>
+__device__ __forceinline__ float not_finite(const uint8_t* p) {
+  if constexpr (FMT == kCacheE4m3) return (*p & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f;
+  float v[1];
+  row_load<DT, 1>(p, v);
+  return __builtin_isfinite(v[0]) ? 0.f : v[0];
 }
 
 // Bit i: the row sees the i-th of this lane's eight keys kb, kb + 1, .. kb + 3, kb + 16, .. kb + 19.
@@ -622,17 +639,19 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
         for (int w = 0; w < NB / 4; ++w) vp[i].w[w] &= on;
         if constexpr (FMT != kCacheSame) vs[i] = on ? vs[i] : 0.f;
       }
-      if (FMT == kCacheSame && mixed) {
-        uint32_t changed = 0;
+      if (FMT != kCacheInt8 && mixed) {
+        uint32_t found = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int w = 0; w < NB / 4; ++w) {
-            const uint32_t y = finite_only<DT>(vp[i].w[w]);
-            changed |= y ^ vp[i].w[w];
-            vp[i].w[w] = y;
-          }
-        if (__any(changed != 0)) cleaned = true;
+          for (int w = 0; w < NB / 4; ++w) found |= not_finite_bits<DT, FMT>(vp[i].w[w]);
+        if (__any(found != 0)) {
+          cleaned = true;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int w = 0; w < NB / 4; ++w) vp[i].w[w] = finite_only<DT, FMT>(vp[i].w[w]);
+        }
       }
     }
 #pragma unroll
@@ -722,7 +741,7 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
         }
     }
   }
-  if (FMT == kCacheSame && cleaned) {
+  if (FMT != kCacheInt8 && cleaned) {
     // What was taken for zeros and is not finite, to the rows that see it.
     for (int it = tile0; it < tile1; it += kStep) {
       const int key0 = keys.first(it);
@@ -736,12 +755,10 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             const int col = (4 * g + i) * NJ + j;
-            float v[1] = {0.f};
-            if (col < a.c.d) row_load<DT, 1>(vb + col * S::kElem, v);
-            if (__builtin_isfinite(v[0])) continue;
+            const float v = col < a.c.d ? not_finite<DT, FMT>(vb + col * S::kElem) : 0.f;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-              if (sees(row[rt], key, base)) acc[rt][j][i] += v[0];
+              if (v != 0.f && sees(row[rt], key, base)) acc[rt][j][i] += v;
           }
       }
     }
@@ -939,15 +956,15 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
         const uint32_t on = ((key < keys.np) | in_span(key, span_lo, span)) ? ~0u : 0u;
 #pragma unroll
         for (int w = 0; w < 4; ++w) rv[u][w] &= on;
-        if constexpr (FMT == kCacheSame) {  // rows that do not see a value must not meet what is not finite: see below
-          uint32_t changed = 0;
+        if constexpr (FMT != kCacheInt8) {  // rows that do not see a value must not meet what is not finite: see below
+          uint32_t found = 0;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t y = finite_only<DT>(rv[u][w]);
-            changed |= y ^ rv[u][w];
-            rv[u][w] = y;
+          for (int w = 0; w < 4; ++w) found |= not_finite_bits<DT, FMT>(rv[u][w]);
+          if (found) {
+            s_cleaned = 1;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) rv[u][w] = finite_only<DT, FMT>(rv[u][w]);
           }
-          if (changed) s_cleaned = 1;
         }
       }
       constexpr uint32_t kNan2 = 0x7fff7fffu;
@@ -1120,7 +1137,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
     }
     __syncthreads();
   }
-  if (FMT == kCacheSame && s_cleaned) {
+  if (FMT != kCacheInt8 && s_cleaned) {
     // What was taken for zeros and is not finite, to the rows that see it.
     for (int it = tile0; it < tile1; ++it) {
       const int key0 = keys.first(it);
@@ -1135,12 +1152,10 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int c = 16 * j + 4 * g + i;
-            float v[1] = {0.f};
-            if (c < a.c.d) row_load<DT, 1>(vb + c * 2, v);
-            if (__builtin_isfinite(v[0])) continue;
+            const float v = c < a.c.d ? not_finite<DT, FMT>(vb + c * kElem) : 0.f;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-              if (sees(row[rt], key, base)) acc[rt][j][i] += v[0];
+              if (v != 0.f && sees(row[rt], key, base)) acc[rt][j][i] += v;
           }
       }
     }
