@@ -816,8 +816,8 @@ int tmac_cache_keep(const tmac_cache* cache, const int32_t* d_path, int64_t path
  * positions j < base as above, and drafted row s if also its place is at least its own minus window (or it is stored
  * below n_persistent). Rows that see nothing, and rows t >= count, are zeros. What a row does not see does not reach
  * it, whatever is stored there.
- * Scores, sums and the accumulation are fp32; in 16 bit the probabilities are two numbers of dtype, or rounded to it where
- * the rows are many. window >= 0.
+ * Scores, sums and the accumulation are fp32; in 16 bit the probabilities are two numbers of dtype (fp16 on 8-bit codes: of
+ * bfloat16). window >= 0.
  * d_ws: tmac_cached_attn_workspace bytes (0: none), 16-byte aligned. */
 int tmac_cached_attn_workspace(const tmac_cache* cache, int B, int T, int n_q_heads, int64_t window, int n_persistent,
                                size_t* ws_bytes);

@@ -140,3 +140,35 @@ def filled(dev, B, H, d, page, lens, dtype, fmt, seed=0, spread=1.0, fill=None, 
     v = torch.randn(B, H, n, d, generator=g, device=dev).to(dtype)
     tc.cache_write(k, v, c, table, lengths, counts=lengths)
     return c, table, lengths
+
+
+def check_two_numbers(out, q, cache, table, lens, news, masks, least=2.0 ** -25):
+    """check_attention for probabilities that are held in two numbers in 16 bit: what both leave over is at most 2^-15 of a
+    probability where the numbers are bfloat16 (whose step is 2^-7: the second is below 2^-6 and off by 2^-15), 2^-21 in
+    fp16, and in fp16 `least` of the row's largest."""
+    B, H, T, d = out.shape
+    G = H // cache.k.shape[1]
+    half = {torch.float32: 2 * E, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[out.dtype]
+    of_fp16 = out.dtype == torch.float16 and cache.k_scale is None
+    up = 0.0 if out.dtype == torch.float32 else 2.0 ** -21 if of_fp16 else 2.0 ** -15
+    for b in range(B):
+        n, new = lens[b], news[b]
+        assert torch.all(out[b, :, new:] == 0), b
+        if new == 0:
+            continue
+        mask = masks[b].to(out.device)
+        any_sees = mask.any(0)[None, :, None]
+        k, v = (torch.where(any_sees, pool_rows(cache, table, b, n, name), 0.0).repeat_interleave(G, 0) for name in "kv")
+        x, scale = q[b, :, :new].double(), d ** -0.5
+        z = ((x @ k.transpose(1, 2)) * scale).masked_fill(~mask, -math.inf)
+        size = (x.abs() @ k.abs().transpose(1, 2)) * scale
+        dz = ((d * E * size + 4 * E * z.abs().nan_to_num(0.0, 0.0)) * mask).amax(-1, keepdim=True)
+        p = torch.softmax(z, -1).nan_to_num(0.0)
+        want, A = p @ v, p @ v.abs()
+        tol = A * (up + 2 * dz + 2 * (n + 200) * E) + half * want.abs() + 1e-30
+        if out.dtype == torch.float16:  # the results' own least number, and that of the probabilities
+            tol += 2.0 ** -25
+            if of_fp16:
+                tol += least * n * p.amax(-1, keepdim=True) * v.abs().amax(-2, keepdim=True)
+        off = (out[b, :, :new].double() - want).abs()
+        assert torch.all(off <= tol), (b, int((off > tol).sum()), float((off / tol).max()))

@@ -69,6 +69,9 @@ struct Shape {
   static constexpr int kParts = DT == TMAC_F32 && FMT != kCacheSame ? 3 : 1;
   static constexpr bool kScaled16 = DT == TMAC_F16 && FMT != kCacheSame;
   static constexpr int kProbType = kScaled16 ? TMAC_BF16 : kType;    // of the second product
+  // Probabilities in 16 bit are two numbers, whoever shares the launch: the result's rounding is then the only one of its
+  // size. With one, the error over 8192 positions was 0.0023 of the result in bfloat16, with two 0.0017, its rounding's.
+  static constexpr int kProbs = kF32 ? 1 : kParts > 1 ? kParts : 2;
   static constexpr int kElem = FMT != kCacheSame ? 1 : DT == TMAC_F32 ? 4 : 2;  // bytes of a stored value
   static constexpr int kRun = 16 / kElem;           // values in 16 bytes: a lane's piece of a key
   static constexpr int kPieces = DP / (4 * kRun);   // of each key, per lane; piece c of group g: 4 kRun c + kRun g ..
@@ -88,6 +91,33 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&w)[P]) {
     x -= Mfma<TYPE>::to_f32(static_cast<uint16_t>(w[i]));
     y -= Mfma<TYPE>::to_f32(static_cast<uint16_t>(w[i] >> 16));
   }
+}
+
+// Probabilities x, y as the sum of two pairs of TYPE that are both above 0 where x, y are (a number below 0, or 0, times an
+// infinite value would be NaN beside the other's infinity): the first is the number below the leading bits of x, so the
+// second has one to two of its last places. 2^-15 of x at most are left over in bfloat16, 2^-21 (or half of the least
+// number) in fp16.
+template <int TYPE>
+__device__ __forceinline__ void split_positive2(float x, float y, uint32_t (&w)[2]) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  uint32_t lead;
+  if constexpr (TYPE == TMAC_BF16)
+    lead = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+  else
+    lead = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, lead), u16x2{1, 1}));
+  w[1] = Mfma<TYPE>::pack2(x - Mfma<TYPE>::to_f32(static_cast<uint16_t>(w[0])),
+                           y - Mfma<TYPE>::to_f32(static_cast<uint16_t>(w[0] >> 16)));
+}
+
+// Probabilities (times the values' scales in 8 bits, which may be of any sign) as the sum of kProbs pairs of kProbType.
+template <int DT, int FMT, int DP>
+__device__ __forceinline__ void split_probs(float x, float y, uint32_t (&w)[Shape<DT, FMT, DP>::kProbs]) {
+  using S = Shape<DT, FMT, DP>;
+  if constexpr (FMT == kCacheSame && !S::kF32)
+    split_positive2<S::kProbType>(x, y, w);
+  else
+    split2<S::kProbType, S::kProbs>(x, y, w);
 }
 
 // operand e of a key's piece
@@ -521,45 +551,12 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
       }
     }
   };
-  // With 16 rows a wave, whose time goes into the cache's reading, 16-bit probabilities are two numbers (16 bits and more
-  // of them), which leaves the result's own rounding as the only one of its size; with more rows they are rounded once.
-  // The second number may be 0 or below it, which times an infinite value is NaN where the probability's product is
-  // infinite: a wave that finds its sums not finite starts again with two equal halves, and takes those sums' results.
-  constexpr int kProbs = S::kF32 ? 1 : S::kParts > 1 ? S::kParts : RT == 1 || S::kScaled16 ? 2 : 1;
-  constexpr bool kAgain = kProbs == 2 && FMT == kCacheSame;
-  bool halves_only = false, cleaned;
+  bool cleaned = false;
   // This wave's place in LDS: row_cap rows of kPitchO floats, so that 16 rows begin at different banks.
   constexpr int kPitchO = DP + 4;
   const int cap = a.row_cap;
   float* const so = sh + wave * cap * kPitchO;
-  auto put_sums = [&](auto factor) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = 16 * rt + n;
-      if (r >= cap) continue;
-      float f;
-      if constexpr (std::is_same_v<decltype(factor), float>)
-        f = factor;
-      else
-        f = factor(rt);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; j += 4)
-          *reinterpret_cast<f32x4*>(so + r * kPitchO + (4 * g + i) * NJ + j) =
-              f32x4{acc[rt][j][i] * f, acc[rt][j + 1][i] * f, acc[rt][j + 2][i] * f, acc[rt][j + 3][i] * f};
-    }
-  };
   int key_now = 0;
-  auto first_tile = [&]() {
-    if (tile0 >= tile1) return;
-    look_up(tile0);
-    key_now = key_next;
-    place();
-    load_keys();
-    load_values();
-    look_up(tile0 + kStep);
-  };
   // One tile; `more`: the next one's loads are issued on the way. The last tile is code of its own: as a condition in one loop
   // the loads' registers were copied at its end, which waited for them there.
   auto one_tile = [&](int it, auto more) {
@@ -666,19 +663,16 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
         }
       }
     }
-    u32x4 pw[RT][kProbs];
+    u32x4 pw[RT][S::kProbs];
     if constexpr (!S::kF32) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          uint32_t w[kProbs];
-          if (kAgain && halves_only)
-            w[0] = w[kProbs - 1] = Mfma<S::kProbType>::pack2(0.5f * x[rt][2 * u], 0.5f * x[rt][2 * u + 1]);
-          else
-            split2<S::kProbType, kProbs>(x[rt][2 * u], x[rt][2 * u + 1], w);
+          uint32_t w[S::kProbs];
+          split_probs<DT, FMT, DP>(x[rt][2 * u], x[rt][2 * u + 1], w);
 #pragma unroll
-          for (int i = 0; i < kProbs; ++i) pw[rt][i][u] = w[i];
+          for (int i = 0; i < S::kProbs; ++i) pw[rt][i][u] = w[i];
         }
     }
 #pragma unroll
@@ -696,50 +690,29 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int i = 0; i < kProbs; ++i) acc[rt][j] = mfma16<S::kProbType>(v, pw[rt][i], acc[rt][j]);
+          for (int i = 0; i < S::kProbs; ++i) acc[rt][j] = mfma16<S::kProbType>(v, pw[rt][i], acc[rt][j]);
       }
     }
     if constexpr (decltype(more)::value) load_values();
   };
-  first_tile();
-  for (;;) {
-    cleaned = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      soft[rt] = Soft{-kInf, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    if (tile0 < tile1) {
-      int it = tile0;
-      for (; it + kStep < tile1; it += kStep) one_tile(it, std::true_type{});
-      one_tile(it, std::false_type{});
-    }
-    if (!kAgain || halves_only) break;
-    float t = 0.f;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t = fmaf(acc[rt][j][i], 0.f, t);
-    if (!__any(t != t)) break;
-    halves_only = true;
-    put_sums(1.f);
-    first_tile();
+  if (tile0 < tile1) {
+    look_up(tile0);
+    key_now = key_next;
+    place();
+    load_keys();
+    load_values();
+    look_up(tile0 + kStep);
   }
-  if (kAgain && halves_only) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (16 * rt + n >= a.row_cap) continue;
+  for (int rt = 0; rt < RT; ++rt) {
+    soft[rt] = Soft{-kInf, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const float first = so[(16 * rt + n) * kPitchO + (4 * g + i) * NJ + j];
-          if (__builtin_isfinite(first)) acc[rt][j][i] = first;
-        }
-    }
+    for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (tile0 < tile1) {
+    int it = tile0;
+    for (; it + kStep < tile1; it += kStep) one_tile(it, std::true_type{});
+    one_tile(it, std::false_type{});
   }
   if (FMT != kCacheInt8 && cleaned) {
     // What was taken for zeros and is not finite, to the rows that see it.
@@ -809,12 +782,21 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
     if (r < cap && g == 0) sm[wave * cap + r] = float2{m[rt], soft[rt].l};
   }
   __syncthreads();
-  put_sums([&](int rt) {
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = 16 * rt + n;
+    if (r >= cap) continue;
     float top = -kInf;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + 16 * rt + n].x);
-    return m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
-  });
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w * cap + r].x);
+    const float f = m[rt] == top ? 1.f : __builtin_amdgcn_exp2f(m[rt] - top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; j += 4)
+        *reinterpret_cast<f32x4*>(so + r * kPitchO + (4 * g + i) * NJ + j) =
+            f32x4{acc[rt][j][i] * f, acc[rt][j + 1][i] * f, acc[rt][j + 2][i] * f, acc[rt][j + 3][i] * f};
+  }
   __syncthreads();
   const int live = rows_all - row0 < cap ? rows_all - row0 : cap;
   for (int u = threadIdx.x; u < live * (DP / 4); u += 64 * WAVES) {
@@ -855,7 +837,7 @@ template <int DT, int FMT, int DP>
 __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
   constexpr int RT = 2, kWaves = 4, kRows = 16 * RT, NJ = DP / 16, kPieces = DP / 32, kHalves = DP / 64;
   using S = Shape<DT, FMT, DP>;
-  constexpr int kProbType = S::kProbType, kProbs = S::kScaled16 ? 2 : 1;
+  constexpr int kProbType = S::kProbType, kProbs = S::kProbs;
   constexpr int kKeys = 64, kHalfTile = kKeys * 64, kTile = kHalves * kHalfTile;  // of 16-bit values
   // a thread's share of a stage: kLoads pieces of 16 bytes of keys and as many of values
   constexpr int kElem = FMT == kCacheSame ? 2 : 1, kChunks = DP * kElem / 16, kLoads = kKeys * kChunks / 256;
@@ -1121,7 +1103,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t y[kProbs];
-          split2<kProbType, kProbs>(x[rt][2 * w], x[rt][2 * w + 1], y);
+          split_probs<DT, FMT, DP>(x[rt][2 * w], x[rt][2 * w + 1], y);
 #pragma unroll
           for (int i = 0; i < kProbs; ++i) pw[rt][i][w] = y[i];
         }

@@ -414,9 +414,8 @@ def cached_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengt
     its drafted rows inside its window. A row that sees nothing, and rows t ≥ count, give zeros.
 
     What a row does not see never reaches its result, whatever is stored there. Scores, sums and the accumulation are in
-    fp32; in 16 bit the probabilities meet the values as two numbers of q's type, or rounded to it where the rows are many.
-    scale defaults to
-    1/sqrt(d_head). No gradient."""
+    fp32; in 16 bit the probabilities meet the values as two numbers of q's type (of bfloat16 for float16 on a cache in
+    8 bits), which together keep 16 bits of them and more. scale defaults to 1/sqrt(d_head). No gradient."""
     shape = q.shape
     if len(shape) != 4:
         raise ValueError(f"cached_attention: q must be [B, H, T, d_head], got {tuple(shape)}")
