@@ -25,3 +25,28 @@ def test_probabilities_keep_their_bits(dev, B, T, H, heads, d, n, dtype, fmt):
     out = tc.cached_attention(q, c, table, lengths, None, 4)
     news = [min(T, length) for length in lens]
     check_two_numbers(out, q, c, table, lens, news, seen_by(B, T, lens, news, None, 4))
+
+
+@pytest.mark.parametrize("T,H,heads,d,high", [(1, 4, 4, 64, 8), (1, 4, 4, 128, 8), (40, 4, 4, 64, 8), (100, 8, 1, 64, 1),
+                                              (100, 8, 1, 128, 1)])
+def test_small_probabilities_of_long_axes_in_fp16(dev, T, H, heads, d, high):
+    """2^18 keys that have e^-17.5 of the likeliest ones' probability each, which is below half of fp16's least number,
+    and together 0.0065 of one's. The likeliest (the first of each of the first tiles) have values of 0, the others of 1.
+
+    Each probability may be off by half of fp16's least number times 2^-7 (they are held times 2^7) of the likeliest, the
+    result by half a step."""
+    n, page, B = 1 << 18, 256, 64  # all sequences read the same pages
+    c = tc.KVCache.new(n // page, heads, d, page=page, dtype=torch.float16, device=dev)
+    c.v.fill_(1)
+    at = torch.arange(high, device=dev) * 32
+    c.k[at // page, :, at % page, 0] = 17.5
+    c.v[at // page, :, at % page] = 0
+    table = torch.arange(n // page, dtype=torch.int32, device=dev).expand(B, -1).contiguous()
+    lengths = torch.full((B,), n, dtype=torch.int32, device=dev)
+    q = torch.ones(B, H, T, d, dtype=torch.float16, device=dev)
+    out = tc.cached_attention(q, c, table, lengths, scale=1.0)
+    seen = torch.arange(n - T, n, device=dev, dtype=torch.float64) + 1 - high  # of the small ones, by row
+    small = seen * 2.718281828459045 ** -17.5
+    want = (small / (small + high))[:, None]
+    tol = 2.0 ** -11 * want + 2.0 ** -25 + n * 2.0 ** -32 / high + 2 * (n + 200) * 2.0 ** -24 * want
+    assert torch.all((out.double() - want).abs() <= tol), (float(out.amin()), float(out.amax()), float(want[0]))

@@ -72,6 +72,9 @@ struct Shape {
   // Probabilities in 16 bit are two numbers, whoever shares the launch: the result's rounding is then the only one of its
   // size. With one, the error over 8192 positions was 0.0023 of the result in bfloat16, with two 0.0017, its rounding's.
   static constexpr int kProbs = kF32 ? 1 : kParts > 1 ? kParts : 2;
+  // fp16's least number is 2^-24, and so much is lost of each of a long axis' small probabilities: they are taken times
+  // 2^kLift (with kSlack, up to 2^15).
+  static constexpr int kLift = DT == TMAC_F16 && FMT == kCacheSame ? 7 : 0;
   static constexpr int kElem = FMT != kCacheSame ? 1 : DT == TMAC_F32 ? 4 : 2;  // bytes of a stored value
   static constexpr int kRun = 16 / kElem;           // values in 16 bytes: a lane's piece of a key
   static constexpr int kPieces = DP / (4 * kRun);   // of each key, per lane; piece c of group g: 4 kRun c + kRun g ..
@@ -306,7 +309,7 @@ __device__ __forceinline__ uint32_t row_sees(const Row& r, int kb, int base, boo
 }
 
 // The running softmax of a row, as the lanes that hold it have it. Exponents are taken relative to mu, which is a score
-// times scale2 (0 while there is none) and moves only for one that is more than kSlack above it: up to then
+// times scale2, less LIFT (0 while there is none) and moves only for one that is more than kSlack above it: up to then
 // exponentials stay below 2^kSlack, where the sums in fp32 and the probabilities in 16 bit are as good. Moving costs as
 // much as a tile's exponentials, and a wave's 16 rows have a new largest score in two of three tiles of 40. lim: that
 // bound, not scaled; l: this lane's part of the sum.
@@ -315,8 +318,8 @@ struct Soft {
   float lim, mu, l;
 };
 
-// Scores x (−inf where masked) become exponentials; what was summed up before moves with mu.
-template <int NJ>
+// Scores x (−inf where masked) become exponentials times 2^LIFT; what was summed up before moves with mu.
+template <int LIFT, int NJ>
 __device__ __forceinline__ void soften(Soft& s, float (&x)[8], f32x4 (&acc)[NJ], const AttnArgs& a) {
   float mx = x[0];
 #pragma unroll
@@ -325,7 +328,7 @@ __device__ __forceinline__ void soften(Soft& s, float (&x)[8], f32x4 (&acc)[NJ],
     mx = fmaxf(mx, lane_xor<16>(mx));
     mx = fmaxf(mx, lane_xor<32>(mx));
     if (mx > s.lim) {  // the same in the row's four lanes
-      const float to = mx * a.scale2, f = s.lim == -kInf ? 1.f : __builtin_amdgcn_exp2f(s.mu - to);
+      const float to = fmaf(mx, a.scale2, -static_cast<float>(LIFT)), f = s.lim == -kInf ? 1.f : __builtin_amdgcn_exp2f(s.mu - to);
       s.lim = mx + a.slack;
       s.mu = to;
       s.l *= f;
@@ -653,7 +656,7 @@ __global__ __launch_bounds__(64 * WAVES, (wide(DT, FMT == kCacheSame, DP, RT) ? 
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      soften(soft[rt], x[rt], acc[rt], a);
+      soften<S::kLift>(soft[rt], x[rt], acc[rt], a);
       if constexpr (FMT != kCacheSame) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
@@ -1091,7 +1094,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_rows_kernel(AttnArgs a) {
       u32x4 pw[RT][kProbs];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        soften(soft[rt], x[rt], acc[rt], a);
+        soften<S::kLift>(soft[rt], x[rt], acc[rt], a);
         if constexpr (FMT != kCacheSame) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[rt][i] *= vs[i];
