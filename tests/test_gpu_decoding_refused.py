@@ -1,0 +1,39 @@
+"""A call of TitanMAC.decode that is refused, and the same call again."""
+import pytest
+import torch
+
+from test_gpu_decoding import close, model
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("why", ["dropout", "autocast", "type"])
+@pytest.mark.parametrize("draft", [False, True])
+def test_again_after_a_refusal(dev, why, draft):
+    m = model(dev, attention_dropout=0.1)
+    ids = torch.randint(0, 211, (2, 40), device=dev)
+    with torch.no_grad():
+        want = m(ids)["logits"]
+    state = m.new_decode_state(2, 64)
+    m.decode(ids[:, :20], state)
+    tree = torch.tensor([(1 << t + 1) - 1 for t in range(6)], device=dev) if draft else None
+    args = (ids[:, 20:26], state)
+    if why == "dropout":
+        m.train()
+        with pytest.raises(ValueError, match="dropout"):
+            m.decode(*args, tree=tree)
+        m.eval()
+    elif why == "autocast":
+        with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(TypeError, match="does not hold"):
+            m.decode(*args, tree=tree)
+    else:
+        m.double()
+        with pytest.raises((TypeError, RuntimeError, ValueError)):
+            m.decode(*args, tree=tree)
+        m.float()
+    assert state.lengths.tolist() == [25, 25] and state.used == 20
+    got = [m.decode(*args, tree=tree)]
+    if draft:
+        state.keep(torch.arange(6, dtype=torch.int32, device=dev).expand(2, 6))
+    got.append(m.decode(ids[:, 26:], state))
+    assert close(torch.cat(got, 1), want[:, 20:], torch.float32) and state.used == 40

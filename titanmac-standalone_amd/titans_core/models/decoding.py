@@ -29,12 +29,17 @@ class DecodeState:
         self.used = 0             # at most so many are held
         self._draft: Optional[Union[int, torch.Tensor]] = None
 
-    def _advance(self, T: int, counts: Optional[torch.Tensor], draft: bool) -> None:
-        """T new rows for each sequence (counts of them, if given)."""
+    def _ahead(self, T: int, counts: Optional[torch.Tensor]) -> torch.Tensor:
+        """The lengths with T new rows for each sequence (counts of them, if given). Nothing here changes before the
+        logits are made (``_advance``): a call that is refused on the way leaves the state as it was."""
         if self._draft is not None:
             raise RuntimeError("DecodeState: the last call's draft was not settled: call keep()")
         if self.used + T > self.room:
             raise ValueError(f"DecodeState: {self.used} tokens are held and {T} more do not fit in {self.room}")
+        return self.lengths + (T if counts is None else counts)
+
+    def _advance(self, T: int, counts: Optional[torch.Tensor], draft: bool) -> None:
+        """The caches hold the rows of ``_ahead``."""
         self.lengths.add_(T if counts is None else counts)
         self.used += T
         if draft:

@@ -463,7 +463,8 @@ class TitanMAC(nn.Module):
 
         counts (int32 [B]): how many of the T are tokens; the rest is padding, whose logits say nothing. tree (int64
         [B, T] or [T], T up to 64): the tokens are a draft, as in ``cached_attention``; ``state.keep`` then says
-        which of them stay. Hooks of the blocks and their attention are not run."""
+        which of them stay. Hooks of the blocks and their attention are not run. A call that raises an error leaves
+        ``state`` as it was."""
         B, T = input_ids.shape
         if B != state.lengths.shape[0]:
             raise ValueError(f"decode: the state has {state.lengths.shape[0]} sequences, input_ids is "
@@ -477,17 +478,19 @@ class TitanMAC(nn.Module):
                              f"{tuple(tree.shape)}")
         place = torch.arange(T, device=input_ids.device) if tree is None else draft_depths(tree)
         positions = (state.lengths - state.n_persistent).unsqueeze(1) + place
+        lengths = state._ahead(T, counts)
         x = self._embed_at(input_ids, positions)
-        state._advance(T, counts, tree is not None)
         for layer, cache in zip(self.layers, state.caches):
-            x = layer.forward_cached(x, cache, state.table, state.lengths, counts=counts, tree=tree)
+            x = layer.forward_cached(x, cache, state.table, lengths, counts=counts, tree=tree)
         if last:
             if counts is None:
                 x = x[:, -1:]
             else:
                 at = (counts.long() - 1).clamp(min=0)
                 x = x.gather(1, at.view(B, 1, 1).expand(B, 1, x.shape[-1]))
-        return self.lm_head(self.norm(x))
+        logits = self.lm_head(self.norm(x))
+        state._advance(T, counts, tree is not None)
+        return logits
 
     def _embed_at(self, input_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Token plus position rows [B, T, d] at given positions; padding may be past the table's last."""
