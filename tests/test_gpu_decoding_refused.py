@@ -1,4 +1,4 @@
-"""A call of TitanMAC.decode that is refused, and the same call again."""
+"""Calls of TitanMAC.decode that are refused, the same calls again, and calls that are not to be refused."""
 import pytest
 import torch
 
@@ -37,3 +37,24 @@ def test_again_after_a_refusal(dev, why, draft):
         state.keep(torch.arange(6, dtype=torch.int32, device=dev).expand(2, 6))
     got.append(m.decode(ids[:, 26:], state))
     assert close(torch.cat(got, 1), want[:, 20:], torch.float32) and state.used == 40
+
+
+def test_many_drafts_in_a_small_room(dev):
+    """Drafts of six tokens of which two stay, by paths as wide as the drafts: the room holds what is kept."""
+    m = model(dev)
+    ids = torch.randint(0, 211, (2, 40), device=dev)
+    with torch.no_grad():
+        want = m(ids)["logits"]
+    state = m.new_decode_state(2, 40, page=16)
+    got = [m.decode(ids[:, :20], state)]
+    tree = torch.tensor([0b1, 0b10, 0b101, 0b1010, 0b10, 0b10001], device=dev)
+    path = torch.tensor([[0, 2, -1, -1, -1, -1]], dtype=torch.int32, device=dev).expand(2, 6)
+    for at in range(20, 36, 2):
+        draft = torch.randint(0, 211, (2, 6), device=dev)
+        draft[:, 0], draft[:, 2] = ids[:, at], ids[:, at + 1]
+        got.append(m.decode(draft, state, tree=tree)[:, [0, 2]])
+        state.keep(path)
+    with pytest.raises(ValueError, match="42 tokens do not fit in 40"):
+        m.decode(draft, state, tree=tree)
+    got.append(m.decode(ids[:, 36:], state))
+    assert close(torch.cat(got, 1), want, torch.float32) and state.used == 40

@@ -478,7 +478,7 @@ class TitanMAC(nn.Module):
                              f"{tuple(tree.shape)}")
         place = torch.arange(T, device=input_ids.device) if tree is None else draft_depths(tree)
         positions = (state.lengths - state.n_persistent).unsqueeze(1) + place
-        lengths = state._ahead(T, counts)
+        lengths, *bounds = state._ahead(T, counts)
         x = self._embed_at(input_ids, positions)
         for layer, cache in zip(self.layers, state.caches):
             x = layer.forward_cached(x, cache, state.table, lengths, counts=counts, tree=tree)
@@ -489,7 +489,7 @@ class TitanMAC(nn.Module):
                 at = (counts.long() - 1).clamp(min=0)
                 x = x.gather(1, at.view(B, 1, 1).expand(B, 1, x.shape[-1]))
         logits = self.lm_head(self.norm(x))
-        state._advance(T, counts, tree is not None)
+        state._advance(T, counts, tree is not None, *bounds)
         return logits
 
     def _embed_at(self, input_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
