@@ -817,7 +817,7 @@ int tmac_cache_keep(const tmac_cache* cache, const int32_t* d_path, int64_t path
  * below n_persistent). Rows that see nothing, and rows t >= count, are zeros. What a row does not see does not reach
  * it, whatever is stored there.
  * Scores, sums and the accumulation are fp32; in 16 bit the probabilities are two numbers of dtype (fp16 on 8-bit codes: of
- * bfloat16). window >= 0.
+ * bfloat16). window >= 0, from 2^30 on none.
  * d_ws: tmac_cached_attn_workspace bytes (0: none), 16-byte aligned. */
 int tmac_cached_attn_workspace(const tmac_cache* cache, int B, int T, int n_q_heads, int64_t window, int n_persistent,
                                size_t* ws_bytes);

@@ -164,7 +164,7 @@ struct AttnArgs {
   uint8_t* out;
   float* ws;
   int B, Hq, G, g_shift, n_rb, splits, np, row_cap, per_xcd, n_blocks;  // g_shift: log2 of G, or -1
-  int window;  // INT_MAX / 2 and above: none
+  int window;  // up to kNowhere: none
   float scale2, slack, q_sign;  // slack: kSlack / scale2; scale2: |scale| · log2 e (1 for scale 0); the queries are taken times q_sign, the scale's sign
   bool q_vec, out_vec;
 };
@@ -1273,7 +1273,7 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
   const bool same = !c.ks;
   const int dp = c.pitch <= 64 ? 64 : 128;
   const int64_t len = static_cast<int64_t>(c.max_pages) << c.page_shift;
-  int64_t keys = window + c.T + np;
+  int64_t keys = (window < kNowhere ? window : kNowhere) + c.T + np;
   if (keys > len) keys = len;
   const int64_t tiles = keys / 32 + 2, heads = static_cast<int64_t>(B) * c.n_heads, n16 = heads * ((rows + 15) / 16);
   // Waves with rows of their own, where there are many: 1280 tiles of 16 rows on 130 of keys 56, with the keys shared
@@ -1406,9 +1406,8 @@ extern "C" int tmac_cached_attn(const tmac_cache* cache, const void* d_q, const 
   a.ws = static_cast<float*>(d_ws);
   a.B = B, a.Hq = n_q_heads, a.G = G, a.g_shift = G & (G - 1) ? -1 : __builtin_ctz(G), a.n_rb = p.n_rb;
   a.splits = p.splits, a.row_cap = p.row_cap, a.n_blocks = static_cast<int>(blocks), a.per_xcd = (a.n_blocks + 7) / 8;
-  constexpr int kMost = 1 << 30;
-  a.np = n_persistent < kMost ? n_persistent : kMost;
-  a.window = window < kMost ? static_cast<int>(window) : kMost;
+  a.np = n_persistent < kNowhere ? n_persistent : kNowhere;
+  a.window = window < kNowhere ? static_cast<int>(window) : kNowhere;
   a.scale2 = scale == 0.f ? 1.f : fabsf(scale) * kLog2e;
   a.slack = kSlack / a.scale2;
   a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : scale;
