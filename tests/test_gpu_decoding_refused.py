@@ -58,3 +58,27 @@ def test_many_drafts_in_a_small_room(dev):
         m.decode(draft, state, tree=tree)
     got.append(m.decode(ids[:, 36:], state))
     assert close(torch.cat(got, 1), want, torch.float32) and state.used == 40
+
+
+@pytest.mark.parametrize("narrow", [("embed_positions",), ("embed_tokens",), ("embed_tokens", "embed_positions"), ("rows",),
+                                    ("embed_tokens", "embed_positions", "rows")])
+def test_tables_of_several_types(dev, narrow):
+    """Tables in bfloat16 beside layers in fp32, as forward takes them: what a row is embedded as is of the widest."""
+    m = model(dev, tie_weights=False)
+    for name in narrow:
+        if name == "rows":
+            m.persistent_tokens.data = m.persistent_tokens.data.bfloat16()
+        else:
+            getattr(m, name).bfloat16()
+    ids = torch.randint(0, 211, (2, 40), device=dev)
+    if len(narrow) == 3:  # then all of a text's rows are bfloat16, which the layers refuse
+        with torch.no_grad(), pytest.raises((RuntimeError, TypeError, ValueError)):
+            m(ids)
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            m.decode(ids, m.new_decode_state(2))
+        return
+    with torch.no_grad():
+        want = m(ids)["logits"]
+    state = m.new_decode_state(2)
+    got = torch.cat([m.decode(ids[:, a:b], state) for a, b in ((0, 25), (25, 26), (26, 40))], 1)
+    assert close(got, want, torch.float32)

@@ -442,7 +442,10 @@ class TitanMAC(nn.Module):
         w, Np = self.embed_tokens.weight, self._n_persistent()
         per = -(-(Np + room) // page)
         dev = w.device.type
-        dtype = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else w.dtype  # the projections' outputs
+        if torch.is_autocast_enabled(dev):  # the projections' outputs
+            dtype = torch.get_autocast_dtype(dev)
+        else:
+            dtype = self.layers[0].attention.qkv_proj.weight.dtype if self.layers else w.dtype
         caches = [KVCache.new(batch * per, cfg.n_heads, cfg.d_head, page=page, dtype=dtype, fmt=fmt, device=w.device)
                   for _ in self.layers]
         table = torch.arange(batch * per, dtype=torch.int32, device=w.device).view(batch, per)
@@ -450,6 +453,8 @@ class TitanMAC(nn.Module):
         if Np:
             with torch.no_grad():
                 x = self.persistent_tokens.unsqueeze(0).expand(batch, -1, -1)
+                for table_of in (self.embed_tokens, self.embed_positions):  # as behind the tokens' rows
+                    x = x.to(torch.promote_types(x.dtype, table_of.weight.dtype))
                 for layer, cache in zip(self.layers, caches):
                     x = layer.forward_cached(x, cache, table, state.lengths)
         return state
@@ -496,9 +501,13 @@ class TitanMAC(nn.Module):
         """Token plus position rows [B, T, d] at given positions; padding may be past the table's last."""
         tok, pos = self.embed_tokens, self.embed_positions
         if (_plain_lookup(tok) and _plain_lookup(pos) and input_ids.dtype in (torch.int64, torch.int32)
-                and tok.weight.is_cuda and _lib.eager_native(input_ids, tok.weight, pos.weight)):
-            return token_embedding(input_ids, tok.weight, pos.weight, positions=positions)
-        return tok(input_ids) + pos(positions.clamp(0, pos.num_embeddings - 1))
+                and tok.weight.is_cuda and tok.weight.dtype == pos.weight.dtype and tok.weight.dtype in _lib._DTYPE_CODE
+                and _lib.eager_native(input_ids, tok.weight, pos.weight)):
+            x = token_embedding(input_ids, tok.weight, pos.weight, positions=positions)
+        else:
+            x = tok(input_ids) + pos(positions.clamp(0, pos.num_embeddings - 1))
+        rows = self.persistent_tokens  # forward's rows have a type for both
+        return x if rows is None else x.to(torch.promote_types(x.dtype, rows.dtype))
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, n_tokens: int, *, counts: Optional[torch.Tensor] = None,
