@@ -172,3 +172,20 @@ def check_two_numbers(out, q, cache, table, lens, news, masks, least=2.0 ** -25)
                 tol += least * n * p.amax(-1, keepdim=True) * v.abs().amax(-2, keepdim=True)
         off = (out[b, :, :new].double() - want).abs()
         assert torch.all(off <= tol), (b, int((off > tol).sum()), float((off / tol).max()))
+
+
+# B, T, H, heads, d, positions, page: between them, and over types and formats, every kernel of the attention is launched
+SHAPES = [
+    (10, 1, 20, 10, 64, 300, 16), (10, 1, 10, 10, 128, 300, 16),      # 16 rows, the keys over eight waves
+    (30, 1, 10, 10, 64, 300, 64), (30, 1, 10, 10, 128, 300, 64),      # over four
+    (6, 40, 10, 10, 128, 300, 32),
+    (3, 1, 2, 2, 64, 5000, 64), (3, 1, 2, 2, 128, 5000, 64),          # in many parts
+    (3, 1, 24, 24, 64, 5000, 64), (3, 1, 48, 24, 128, 5000, 64),      # in a few
+    (18, 20, 10, 10, 64, 1700, 64), (18, 10, 20, 10, 128, 1700, 64),  # 32 rows, eight waves
+    (27, 20, 10, 10, 64, 1700, 64), (27, 20, 10, 10, 128, 1700, 64),  # four waves
+    (3, 30, 2, 2, 64, 5000, 64), (3, 30, 2, 2, 128, 5000, 64),        # in parts
+    (4, 30, 16, 16, 64, 3000, 128), (4, 30, 16, 16, 128, 3000, 128),
+    (15, 40, 8, 8, 96, 300, 16),                                      # fp32: 360 tiles of 16 rows
+    (20, 200, 5, 5, 40, 300, 32), (12, 200, 8, 8, 128, 260, 32),      # rows over the waves
+    (2, 320, 32, 4, 64, 1000, 32), (2, 320, 32, 4, 128, 1000, 256),   # in parts
+]

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import titans_core as tc
-from cache_cases import FORMATS, check_two_numbers, filled, gen, seen_by
+from cache_cases import FORMATS, SHAPES, check_two_numbers, filled, gen, seen_by
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,51 @@ def test_small_probabilities_of_long_axes_in_fp16(dev, T, H, heads, d, high):
     want = (small / (small + high))[:, None]
     tol = 2.0 ** -11 * want + 2.0 ** -25 + n * 2.0 ** -32 / high + 2 * (n + 200) * 2.0 ** -24 * want
     assert torch.all((out.double() - want).abs() <= tol), (float(out.amin()), float(out.amax()), float(want[0]))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,T,H,heads,d,n,page", SHAPES)
+def test_every_kernel(dev, B, T, H, heads, d, n, page, dtype, fmt):
+    """Ragged sequences, some with fewer new rows than others; drafts where they are as short. That these shapes launch every
+    kernel is tested on the CPU (test_cached_attention_host.py)."""
+    lens = [n - 13 * (b % 16) for b in range(B)]
+    news = [min(T - T // 3 if b % 3 == 2 else T, lens[b]) for b in range(B)]
+    c, table, lengths = filled(dev, B, heads, d, page, lens, dtype, fmt, fill=float("nan"))
+    assert table.shape[1] == -(-n // page)
+    q = queries(dev, B, H, T, d, dtype)
+    counts = torch.tensor(news, dtype=torch.int32, device=dev)
+    trees = [None]
+    if 1 < T <= 64:
+        g = torch.Generator().manual_seed(T)
+        bits = [1]
+        for t in range(1, T):
+            bits.append(bits[int(torch.randint(0, t, (1,), generator=g))] | 1 << t)
+        trees.append(torch.tensor([x - (1 << 64) if x >> 63 else x for x in bits], device=dev))
+    for tree in trees:
+        out = tc.cached_attention(q, c, table, lengths, None, 4, counts=counts, tree=tree)
+        check_two_numbers(out, q, c, table, lens, news, seen_by(B, T, lens, news, None, 4, None if tree is None else tree.cpu()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,T,H,heads,d,n,page", SHAPES)
+def test_values_that_are_not_finite(dev, B, T, H, heads, d, n, page, dtype):
+    """An infinite value that every row sees and one that is NaN and only some see: they reach their columns, and nothing
+    else changes."""
+    lens = [n - 13 * (b % 16) for b in range(B)]
+    news = [min(T, length) for length in lens]
+    c, table, lengths = filled(dev, B, heads, d, page, lens, dtype, None)
+    q = queries(dev, B, H, T, d, dtype)
+    want = tc.cached_attention(q, c, table, lengths, None, 4)
+    for b in range(B):
+        for pos, col, value in ((1, 3, float("inf")), (lens[b] - news[b] // 2 - 1, 5, float("nan"))):
+            c.v[table[b, pos // page].long(), :, pos % page, col] = value
+    got = tc.cached_attention(q, c, table, lengths, None, 4)
+    for b in range(B):
+        sees = torch.arange(T, device=dev) >= news[b] - news[b] // 2 - 1
+        real = torch.arange(T, device=dev) < news[b]
+        assert torch.all(got[b][:, real, 3] == float("inf")) and torch.all(got[b][:, ~real] == 0)
+        assert torch.equal(got[b][..., 5].isnan(), (sees & real).expand(H, T))
+        want[b][:, real, 3] = float("inf")
+        want[b][:, real & sees, 5] = 0
+        assert torch.equal(got[b].nan_to_num(0.0, float("inf")), want[b])
