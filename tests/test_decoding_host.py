@@ -118,3 +118,19 @@ def test_a_capture_does_not_wait(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     m.decode(ids, state)
     assert state.used == 9
+
+
+def test_inference_mode(monkeypatch):
+    """A state that was made inside inference mode goes on outside it, and the other way round."""
+    m = model(monkeypatch)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    for made, used in ((True, False), (False, True), (True, True)):
+        with torch.inference_mode(made):
+            state = m.new_decode_state(2, 20)
+        with torch.inference_mode(used):
+            m.decode(ids, state, counts=torch.tensor([3, 1], dtype=torch.int32))
+        with torch.inference_mode(made):
+            m.decode(ids, state, tree=torch.tensor([1, 3, 7]))
+        with torch.inference_mode(used):
+            state.keep(torch.tensor([[0], [1]], dtype=torch.int32))
+        assert state.lengths.tolist() == [4, 2]

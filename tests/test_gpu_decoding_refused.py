@@ -82,3 +82,17 @@ def test_tables_of_several_types(dev, narrow):
     state = m.new_decode_state(2)
     got = torch.cat([m.decode(ids[:, a:b], state) for a, b in ((0, 25), (25, 26), (26, 40))], 1)
     assert close(got, want, torch.float32)
+
+
+def test_inference_mode(dev):
+    """A state made inside inference mode, used outside it and inside."""
+    m = model(dev)
+    ids = torch.randint(0, 211, (2, 40), device=dev)
+    with torch.inference_mode():
+        want = m(ids)["logits"]
+        state = m.new_decode_state(2)
+    got = [m.decode(ids[:, :20], state)]
+    with torch.inference_mode():
+        got.append(m.decode(ids[:, 20:21], state))
+    got.append(m.decode(ids[:, 21:], state))
+    assert close(torch.cat(got, 1), want, torch.float32)

@@ -446,12 +446,13 @@ class TitanMAC(nn.Module):
             dtype = torch.get_autocast_dtype(dev)
         else:
             dtype = self.layers[0].attention.qkv_proj.weight.dtype if self.layers else w.dtype
-        caches = [KVCache.new(batch * per, cfg.n_heads, cfg.d_head, page=page, dtype=dtype, fmt=fmt, device=w.device)
-                  for _ in self.layers]
-        table = torch.arange(batch * per, dtype=torch.int32, device=w.device).view(batch, per)
-        state = DecodeState(caches, table, torch.full((batch,), Np, dtype=torch.int32, device=w.device), Np, room)
-        if Np:
-            with torch.no_grad():
+        # what changes from call to call is not an inference tensor, which could be written inside inference mode only
+        with torch.inference_mode(False), torch.no_grad():
+            caches = [KVCache.new(batch * per, cfg.n_heads, cfg.d_head, page=page, dtype=dtype, fmt=fmt, device=w.device)
+                      for _ in self.layers]
+            table = torch.arange(batch * per, dtype=torch.int32, device=w.device).view(batch, per)
+            state = DecodeState(caches, table, torch.full((batch,), Np, dtype=torch.int32, device=w.device), Np, room)
+            if Np:
                 x = self.persistent_tokens.unsqueeze(0).expand(batch, -1, -1)
                 for table_of in (self.embed_tokens, self.embed_positions):  # as behind the tokens' rows
                     x = x.to(torch.promote_types(x.dtype, table_of.weight.dtype))
