@@ -98,3 +98,17 @@ def test_values_that_are_not_finite(dev, B, T, H, heads, d, n, page, dtype):
         want[b][:, real, 3] = float("inf")
         want[b][:, real & sees, 5] = 0
         assert torch.equal(got[b].nan_to_num(0.0, float("inf")), want[b])
+
+
+@pytest.mark.parametrize("window", [61, 62, 63, 64, 65, 127])
+def test_windows_of_a_draft_s_length(dev, window):
+    """Places of a draft's rows are up to 64 apart: that of an entry without bits and that of one with all."""
+    B, T, lens = 3, 64, [64, 100, 300]
+    c, table, lengths = filled(dev, B, 2, 64, 16, lens, torch.float32, None, fill=float("nan"))
+    q = queries(dev, B, 4, T, 64, torch.float32)
+    chain = [(1 << t + 1) - 1 for t in range(T)]
+    trees = [chain, [0] + [-1] * 63, [-1 if t % 3 else t & 1 for t in range(T)]]
+    trees = torch.tensor([[x - (1 << 64) if x >> 63 == 1 else x for x in row] for row in trees])
+    for n_persistent in (0, 5):
+        out = tc.cached_attention(q, c, table, lengths, window, n_persistent, tree=trees.to(dev))
+        check_two_numbers(out, q, c, table, lens, [T] * B, seen_by(B, T, lens, [T] * B, window, n_persistent, trees))

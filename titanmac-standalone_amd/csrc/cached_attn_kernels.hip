@@ -214,7 +214,7 @@ __device__ __forceinline__ Row row_of(const AttnArgs& a, const Seq& s, int b, in
     r.span = base - 1 - lo;
   }
   r.bits = static_cast<uint64_t>(tree[t]) & have;
-  if (a.window < 2 * TMAC_CACHE_MAX_TREE) {  // drafted rows may be behind the window: their places differ by up to 64
+  if (a.window < TMAC_CACHE_MAX_TREE) {  // drafted rows may be behind the window: their places differ by up to 64
     for (int u = 0; u < s.n; ++u)
       if (base + bits_set(tree[u]) - 1 < p - a.window && base + u >= a.np) r.bits &= ~(1ull << u);
   }
