@@ -1276,12 +1276,12 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
   int64_t keys = (window < kNowhere ? window : kNowhere) + c.T + np;
   if (keys > len) keys = len;
   const int64_t tiles = keys / 32 + 2, heads = static_cast<int64_t>(B) * c.n_heads, n16 = heads * ((rows + 15) / 16);
-  // Waves with rows of their own, where there are many: 1280 tiles of 16 rows on 130 of keys 56, with the keys shared
-  // out 75; 15680 on 9 43 and 71; 1024 on 130 67 and 92; 780 on 36 23.7 and 15.0; 160 on 66 17.2 and 15.4.
+  // Waves with rows of their own, where there are many: 1280 tiles of 16 rows on 162 of keys 68, with the keys shared
+  // out 79; 15680 on 10 49 and 76; 1024 on 130 82 and 97; 780 on 36 26.0 and 15.2; 160 on 66 18.9 and 15.5.
   p.rows = rows > 64 && n16 >= 1000;
-  // 32 rows a workgroup, 16 where those are few and the keys as well: 640 tiles of rows on 19 of keys 14.5 with 16, 15.6
-  // with 32; 320 on 7 7.6 and 9.0; 108 on 29 10.6 and 13.5; 1280 on 19 23.5 and 20.7; 2560 62 and 40; 128 on 130 31 and
-  // 24. Wide fp32 rows: 690 on 48 188 and 150.
+  // 32 rows a workgroup, 16 where those are few and the keys as well: 640 tiles of rows on 20 of keys 14.4 with 16, 16.2
+  // with 32; 320 on 8 7.8 and 9.3; 108 on 29 10.4 and 13.9; 1280 on 20 22.3 and 21.4; 2560 63 and 40; 128 on 130 30 and
+  // 24. Wide fp32 rows: 690 on 49 192 and 165.
   p.rt = rows <= 16 || (tiles <= 48 && n16 <= (wide(dtype, same, dp, 1) ? 256 : 704)) ? 1 : 2;
   const int cap = 16 * p.rt;
   int64_t s = 1;
@@ -1289,7 +1289,7 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     p.rt = 2;
     p.waves = 4;
     p.n_rb = (rows + 127) / 128;
-    // two workgroups for every CU, each with 8 tiles at least: 160 blocks of 130 tiles 121 whole, 65 in three parts
+    // two workgroups for every CU, each with 8 tiles at least: 160 blocks of 162 tiles 115 whole, 65-68 in three parts
     const int64_t blocks = heads * p.n_rb;
     s = 512 / blocks;
     if (s > tiles / 8) s = tiles / 8;
@@ -1298,13 +1298,13 @@ Plan plan(const CacheArgs& c, int dtype, int B, int rows, int64_t window, int np
     p.row_cap = rows < cap ? rows : cap;
     const int64_t blocks = heads * p.n_rb;
     // Four waves a workgroup instead of eight where the tiles are few, or the workgroups many: eight waves with 32 rows
-    // fill a CU's registers alone (320 blocks of 19 tiles 21.6, with four waves 16.7; 20 blocks 10.6 and 11.5); with 16
-    // rows 640 blocks of 17 tiles 16.6 and 14.3, 504 17.2 and 12.0, 160 9.6 and 10.9, 640 of 33 37.0 and 38.4.
+    // fill a CU's registers alone (320 blocks of 20 tiles 21.1, with four waves 16.3; 20 blocks 10.4 and 10.9); with 16
+    // rows 640 blocks of 18 tiles 15.9 and 13.8, 480 13.8 and 13.7, 160 9.1 and 9.8, 640 of 34 36.8 and 37.4.
     p.waves = tiles <= 8 || wide(dtype, same, dp, p.rt) || (blocks > 256 && (p.rt == 2 || tiles <= 24)) ? 4 : 8;
     // Few blocks with long axes in parts, until each CU has a workgroup of four waves (two in 8 bits, whose tiles are
-    // half as large). 10 blocks of 512 tiles 88 whole, 14 in 25 parts; 80 of 130 tiles 25.7 and 19.4 in three; 96 of 130
-    // with d = 128 56 and 41 in two; 160 33 and 35 in three; in 8 bits 40 of 130 23.8 and 11.9 in 12, 160 26.0 and 23.5
-    // in three, 240 30 and 35 in two. Shorter axes gain less than the second launch costs the host (10 blocks of 34 tiles
+    // half as large). 10 blocks of 512 tiles 87 whole, 14 in 25 parts; 80 of 130 tiles 27.3 and 19.3 in three; 96 of 130
+    // with d = 128 55 and 41 in two; 160 33-38 and 36 in three; in 8 bits 40 of 130 22.2 and 11.9 in 12, 160 23.9 and 22.7
+    // in three, 240 30 and 34 in two. Shorter axes gain less than the second launch costs the host (10 blocks of 34 tiles
     // 9.5 and 7.9).
     if (tiles > 48) {
       s = same ? 256 / blocks : 512 / blocks >= 3 ? 512 / blocks : 1;
