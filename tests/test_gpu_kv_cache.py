@@ -282,3 +282,17 @@ def test_streams_graph_and_versions(dev):
         tc.cache_write(k, v, e, table, lengths)
         assert same_bits(e.k, c.k) and same_bits(e.k_scale, c.k_scale)
         assert all(same_bits(a, b) for a, b in zip(held, tc.cache_read(e, table, lengths, 128)))
+
+
+def test_what_e4m3_rounds_up_past_fp16(dev):
+    """Above 57344 = 448 · 2^7 a row's scale is 2^8, where e4m3 goes by 16 · 2^8 from 128 · 2^8 on: 63456 is nearer to 240 · 2^8
+    than to 2^16, 63488 is a tie, which goes to 2^16."""
+    c, table = empty_cache(dev, 1, 1, 16, 16, torch.float16, "e4m3"), torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    n = torch.tensor([4], dtype=torch.int32, device=dev)
+    x = torch.zeros(1, 1, 4, 16, dtype=torch.float16, device=dev)
+    x[0, 0, :, 0] = torch.tensor([57344.0, 63456.0, 63488.0, -65504.0])
+    tc.cache_write(x, x, c, table, n)
+    for y in tc.cache_read(c, table, n, 4, dtype=torch.float16):
+        assert y[0, 0, :, 0].tolist() == [57344.0, 61440.0, math.inf, -math.inf] and torch.all(y[..., 1:] == 0)
+    for y in tc.cache_read(c, table, n, 4):
+        assert y[0, 0, :, 0].tolist() == [57344.0, 61440.0, 65536.0, -65536.0]

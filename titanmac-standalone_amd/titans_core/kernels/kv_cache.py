@@ -276,7 +276,8 @@ def _(k, v, ks, vs, table, lengths, T, d, dtype):
 def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, n_positions: int, *,
                dtype: Optional[torch.dtype] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Positions 0 .. n_positions − 1 of every sequence as k, v [B, n_heads, n_positions, d_head]: zeros behind a
-    sequence's length. dtype: the values' type (default: the cache's, bfloat16 for one in 8 bits)."""
+    sequence's length. dtype: the values' type (default: the cache's, bfloat16 for one in 8 bits). A value that e4m3 rounded
+    up to more than dtype holds (one of 63488 or more in float16) is infinite."""
     if dtype is None:
         dtype = cache[10] or torch.bfloat16
     T = int(n_positions)
